@@ -444,6 +444,69 @@ int mtp_scene_neighbors_f32(const float *last, const double *speed_angle, const 
 int mtp_soft_labels_f64(const int64_t *offsets, const int64_t *ids, const int32_t *labels, int64_t n, int k,
                         double *dense, void *stream);
 
+/* ---- routing of agents to modalities, and the layers behind it ----
+ *
+ * What PCCSNet.forward does between the classifier's scores and the candidates (classifier -> k most probable modalities ->
+ * one pass of the following layers per candidate, PCCSNet/models/components.py:116-131), as operators with gradients.  Element
+ * types (`dtype`): float, bfloat16, half; sums, softmax statistics and weights are float.  Row distances (ld) count elements;
+ * pointers need the alignment of their elements only.  No call reads its workspace before writing it. */
+#define MTP_FLOAT 0
+#define MTP_BFLOAT16 1
+#define MTP_HALF 2
+
+/* The k largest scores of each row, largest first, equal scores by the lower index: ids[n][k] and weights[n][k] = softmax over
+ * all e scores at the chosen (normalize = 0) or over the chosen alone (normalize = 1).  -inf: the modality is not allowed; where
+ * fewer than k are left, ids are -1 and weights 0.  A row with a NaN has NaN weights (and ids of its other scores).
+ * stats [n][2] (may be NULL): the largest score and 1 / sum, for the gradient.  e <= 4096, k <= min(e, 128). */
+int mtp_route_topk(int dtype, const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights,
+                   float *stats, void *stream);
+/* Gradient towards the scores, out [n][e], from the gradient g [n][k] of the weights. */
+int mtp_route_topk_grad(int dtype, const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, const int32_t *ids,
+                        const float *weights, const float *stats, const float *g, void *out, void *stream);
+
+/* Stable sort of `pairs` modality ids: order[row] = pair, position[pair] = row, offsets[e + 1] = first row of each modality.
+ * Ids outside [0, e) come behind the last modality: rows [offsets[e], pairs).  e <= 4096. */
+int64_t mtp_sort_pairs_workspace_bytes(int64_t pairs, int e);
+int mtp_sort_pairs(const int32_t *ids, int64_t pairs, int e, int32_t *offsets, int32_t *order, int32_t *position, void *ws,
+                   size_t ws_bytes, void *stream);
+
+/* rows[position[t * k + j]] = x[t], zero for rows >= *held (a device int32: offsets + e).  rows [n * k][d]. */
+int mtp_dispatch_rows(int dtype, const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held,
+                      void *rows, void *stream);
+/* y[t] = sum_j weights[t][j] rows[position[t * k + j]] over rows < *held, in the order of j; weights NULL: all one. */
+int mtp_combine_rows(int dtype, const void *rows, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
+                     const float *weights, void *y, void *stream);
+/* From the gradient g [n][d] of y: grad_rows [n * k][d] (zero for rows >= *held) and grad_weights [n][k]; either may be NULL. */
+int mtp_combine_rows_grad(int dtype, const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position,
+                          const int32_t *held, const float *weights, void *grad_rows, float *grad_weights, void *stream);
+
+/* y = act(x W^T + bias) + residual, act 0 none, 1 relu, 2 gelu (erf), 3 silu.  x [rows][in] (ldx), residual [rows][out] (ldr),
+ * y [rows][out].  offsets NULL: w [out][in], bias [out].  Else rows are sorted by set: rows [offsets[s], offsets[s + 1]) use
+ * w[s] and bias[s] of w [n_sets][out][in], bias [n_sets][out]; rows behind offsets[n_sets] become zero.  bias, residual and pre may
+ * be NULL; pre [rows][out] receives x W^T + bias.  in, out, n_sets <= 65536.
+ * mtp_linear_workspace_bytes: a, lda = the first matrix of the step (x; dz; dz), b, ldb = the second (w; w; x).  Operands whose
+ * rows do not start on 4 bytes (odd sizes of 16-bit types) are laid out anew in it, and a weight gradient over many rows is
+ * summed in parts. */
+#define MTP_LINEAR_FORWARD 0
+#define MTP_LINEAR_GRAD_INPUT 1
+#define MTP_LINEAR_GRAD_WEIGHT 2
+int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows, int in, int out, int n_sets, const void *a, int64_t lda,
+                                   const void *b, int64_t ldb);
+int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias, int act,
+               const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre, void *ws, size_t ws_bytes,
+               void *stream);
+/* dz = g * act'(pre), rows at the distance lddz; rows behind offsets[n_sets] are not written. */
+int mtp_linear_act_grad(int dtype, const void *g, const void *pre, int64_t rows, int out, int act, const int32_t *offsets,
+                        int n_sets, void *dz, int64_t lddz, void *stream);
+/* dst = g, zero behind offsets[n_sets]: the gradient of the residual. */
+int mtp_linear_mask_rows(int dtype, const void *g, int64_t rows, int out, const int32_t *offsets, int n_sets, void *dst,
+                         void *stream);
+/* dx = dz W [rows][in]; dw = dz^T x [n_sets][out][in] and db [n_sets][out] (may be NULL), summed per set. */
+int mtp_linear_grad_input(int dtype, const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in,
+                          const int32_t *offsets, int n_sets, void *dx, void *ws, size_t ws_bytes, void *stream);
+int mtp_linear_grad_weight(int dtype, const void *dz, int64_t rows, int out, int64_t lddz, const void *x, int in, int64_t ldx,
+                           const int32_t *offsets, int n_sets, void *dw, void *db, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

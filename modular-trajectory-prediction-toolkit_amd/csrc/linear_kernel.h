@@ -1,0 +1,573 @@
+// The tiled product of the linear layers (included by linear.hip).
+//
+//   out[r][c] = sum_k Q(r, k) P(c, k)
+//
+// P runs along the contiguous axis of the output, Q along its rows.  Forward: P = W, Q = x; input gradient: P = W taken
+// along its rows, Q = dz; weight gradient: P = x, Q = dz, the sum running over the tokens.  Each operand is either "KC"
+// (the summed index is contiguous in memory) or "RC" (the output's index is).
+//
+// One workgroup owns a BC x BR tile.  Tiles of 128 bytes of k (64 halves or 32 floats) go from memory straight into LDS,
+// 16 bytes a lane, into one of two buffers while the other feeds the matrix cores.  The loads are buffer loads: what lies
+// behind the operand's last element arrives as zero, so ragged rows and ragged sums need no code in the loop.  A KC row
+// whose length is no multiple of 16 bytes has its last piece cleared in LDS before it is used.
+//
+// LDS layouts (16-byte pieces; 64 banks of 4 bytes):
+//   KC: row i holds its 8 pieces at p ^ ((i >> 1) & 7): the 16 rows that one step of a ds_read_b128 touches fall on 16
+//       different pieces of the 256-byte bank line.
+//   RC: k row after k row; 16-bit operands are read with the transposing ds_read_b64_tr_b16 (a group of 16 lanes reads four
+//       k rows of 16 columns), pieces placed at p ^ 4 * (row bits) so that the four rows fall on different banks; floats
+//       are read one by one, the two lane halves (k and k + 4) on different halves of the bank line.
+#pragma once
+#include <type_traits>
+
+#include "mtp_internal.h"
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+typedef short s16x4v __attribute__((ext_vector_type(4)));
+typedef short s16x8v __attribute__((ext_vector_type(8)));
+typedef int i32x4v __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+    return (float)v;
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+    return (T)v;  // round to nearest even
+}
+
+// LDS-DMA of 16 bytes a lane: LDS destination = uniform byte address + lane * 16, source = buffer + voff, zero where voff is
+// outside the buffer.  Inline asm so that the compiler does not wait for it in front of the next ds_read; the caller waits
+// (dma_wait_all) before the barrier that publishes the tile.  M0 is kept.
+__device__ __forceinline__ void buffer_lds16(i32x4v rsrc, unsigned voff, unsigned lds_uniform) {
+    unsigned keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(voff), "s"(rsrc), "s"(lds_uniform)
+        : "memory");
+}
+__device__ __forceinline__ void dma_wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Buffer descriptor of [p, p + bytes), raw; p and bytes are the same in every lane.
+__device__ __forceinline__ i32x4v make_rsrc(const void *p, int64_t bytes) {
+    // the range check works on 4 bytes: a last lone half has to be inside (its neighbour is in the same aligned 4 bytes)
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    const int64_t n = bytes <= 0 ? 0 : (bytes > 0x7ffffffc ? 0x7ffffffc : (bytes + 3) & ~(int64_t)3);
+    i32x4v r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)((a >> 32) & 0xffff));
+    r[2] = __builtin_amdgcn_readfirstlane((int)n);
+    r[3] = 0x00020000;
+    return r;
+}
+
+// One operand: the matrix, its leading dimension, and how many of its elements count.
+struct LinOperand {
+    const void *base;
+    int64_t ld;     // elements from row to row
+    int64_t group;  // elements from one set to the next (weights), 0 where all sets share the matrix
+};
+
+constexpr unsigned LIN_OUTSIDE = 0x80000000u;  // a buffer offset that no descriptor above reaches
+
+// Loads and reads R x 128 bytes of one operand.  SZ: element size.
+template <typename T, bool KC, int R, int NT>
+struct LinTile {
+    static constexpr int SZ = sizeof(T);
+    static constexpr int EPC = 16 / SZ;             // elements per piece
+    static constexpr int BK = 128 / SZ;             // k per tile
+    static constexpr int PIECES = R * 8;            // the same for both layouts
+    static constexpr int PER = PIECES / NT;         // pieces per thread
+    static constexpr int RB = R * SZ;               // RC: bytes of a k row
+    static constexpr int CPR = RB / 16;             // RC: pieces of a k row
+    static_assert(PIECES % NT == 0, "tile");
+
+    // RC: what is added to a piece's place in its k row
+    static __device__ __forceinline__ int twist(int k) {
+        if constexpr (SZ == 4) return 8 * ((k >> 2) & 1);
+        else if constexpr (RB == 128) return 4 * ((k >> 1) & 1);
+        else return 4 * (k & 3);
+    }
+
+    unsigned voff[PER];
+    int piece_k[KC ? PER : 1];  // KC: first k of the piece
+
+    __device__ __forceinline__ void init(int64_t ld, int tid) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int q = i * NT + tid;
+            if constexpr (KC) {
+                const int row = q >> 3, p = (q & 7) ^ ((row >> 1) & 7);
+                voff[i] = (unsigned)(row * (int)ld * SZ + p * 16);
+                piece_k[i] = p * EPC;
+            } else {
+                const int k = q / CPR, p = (q % CPR) ^ twist(k);
+                voff[i] = (unsigned)(k * (int)ld * SZ + p * 16);
+            }
+        }
+    }
+    // k_left: how much of the summed axis this and the later tiles hold
+    __device__ __forceinline__ void load(i32x4v rsrc, int64_t k_left, unsigned lds, int wave) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            unsigned v = voff[i];
+            if constexpr (KC) v = piece_k[i] < k_left ? v : LIN_OUTSIDE;
+            buffer_lds16(rsrc, v, lds + (unsigned)((i * NT + wave * 64) * 16));
+        }
+    }
+    // KC, last tile, k_left no multiple of a piece: the elements behind the end of each row become zero
+    static __device__ __forceinline__ void clear_tail(char *lds, int k_left, int tid) {
+        const int p = k_left / EPC, e0 = k_left % EPC;
+        for (int row = tid; row < R; row += NT) {
+            T *at = reinterpret_cast<T *>(lds + row * 128 + (p ^ ((row >> 1) & 7)) * 16);
+            for (int e = e0; e < EPC; ++e) at[e] = (T)0.f;
+        }
+    }
+};
+
+template <typename T>
+struct LinMfma;
+template <>
+struct LinMfma<__bf16> {
+    typedef bf16x8v frag;
+    static __device__ __forceinline__ f32x16v mul(frag p, frag q, f32x16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(p, q, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ frag ones() {
+        frag f;
+        for (int i = 0; i < 8; ++i) f[i] = (__bf16)1.f;
+        return f;
+    }
+};
+template <>
+struct LinMfma<_Float16> {
+    typedef f16x8v frag;
+    static __device__ __forceinline__ f32x16v mul(frag p, frag q, f32x16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(p, q, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ frag ones() {
+        frag f;
+        for (int i = 0; i < 8; ++i) f[i] = (_Float16)1.f;
+        return f;
+    }
+};
+// float: a "fragment" is the four floats a lane half holds of eight consecutive k; four matrix instructions consume it
+template <>
+struct LinMfma<float> {
+    typedef f32x4v frag;
+    static __device__ __forceinline__ f32x16v mul(frag p, frag q, f32x16v c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(p[e], q[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ frag ones() { return frag{1.f, 1.f, 1.f, 1.f}; }
+};
+
+// Reads the 32-row fragments of one operand out of an LDS tile.  A tile holds 128 bytes of k = STEPS fragments (of 16 halves
+// or 8 floats).
+template <typename T, bool KC, int R>
+struct LinReader {
+    static constexpr int SZ = sizeof(T);
+    static constexpr int STEPS = 4;
+    static constexpr int RB = R * SZ;
+    typedef typename LinMfma<T>::frag frag;
+    const char *at;  // this lane's place for fragment row 0 of the wave
+    int k_off[STEPS];
+    int lane_, col0_;
+
+    // row0: first row of the wave within the tile (a multiple of 32)
+    __device__ __forceinline__ void init(int row0, int lane) {
+        const int i = lane & 31, h = lane >> 5;
+        lane_ = lane;
+        col0_ = row0;
+        if constexpr (KC) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) k_off[s] = (row0 + i) * 128 + (((s * 2 + h) ^ ((i >> 1) & 7)) * 16);
+        }
+    }
+    __device__ __forceinline__ frag read(const char *lds, int f, int s) const {
+        if constexpr (KC) {
+            return *reinterpret_cast<const frag *>(lds + k_off[s] + f * 32 * 128);
+        } else if constexpr (SZ == 2) {
+            const int g = lane_ >> 4, i = lane_ & 15;
+            const int col = col0_ + f * 32 + 16 * (g & 1) + 4 * (i & 3);
+            const int kr = i >> 2;
+            const int piece = (col >> 3) ^ LinTile<T, false, R, 64>::twist(kr);
+            const char *p = lds + (s * 16 + 8 * (g >> 1) + kr) * RB + piece * 16 + (col & 7) * 2;
+            typedef __attribute__((address_space(3))) s16x4v lds_s4;
+            const s16x4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+            const s16x4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 4 * RB));
+            s16x8v v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = lo[e];
+                v[4 + e] = hi[e];
+            }
+            return __builtin_bit_cast(frag, v);
+        } else {
+            const int i = lane_ & 31, h = lane_ >> 5;
+            const int col = col0_ + f * 32 + i;
+            const int piece = (col >> 2) ^ (8 * h);
+            const char *p = lds + (s * 8 + 4 * h) * RB + piece * 16 + (col & 3) * 4;
+            frag v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float *>(p + e * RB);
+            return v;
+        }
+    }
+};
+
+// ---- sets (experts): rows [offsets[e], offsets[e+1]) belong to set e ----
+__device__ __forceinline__ void lin_bounds(const int32_t *offsets, int e, int n_sets, int64_t rows, int64_t *lo, int64_t *hi) {
+    // what the caller hands over is kept inside the matrix whatever it says
+    int64_t a = offsets[e], b = e < n_sets ? (int64_t)offsets[e + 1] : rows;
+    a = a < 0 ? 0 : (a > rows ? rows : a);
+    b = b < a ? a : (b > rows ? rows : b);
+    *lo = a;
+    *hi = b;
+}
+
+__device__ __forceinline__ int64_t lin_uniform(int64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// The set and the rows of row tile `tile`, tiles of BR rows counted set after set; the rows behind the last set come last,
+// as "set" n_sets.  Every wave finds it for itself: 64 sets at a time, a prefix sum over the lanes.
+template <int BR>
+__device__ __forceinline__ bool lin_find_tile(const int32_t *offsets, int n_sets, int64_t rows, int64_t tile, int *set, int64_t *row0,
+                                              int64_t *row_end) {
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0;
+    for (int e0 = 0; e0 <= n_sets; e0 += 64) {
+        const int e = e0 + lane;
+        int64_t lo = 0, hi = 0;
+        if (e <= n_sets) lin_bounds(offsets, e, n_sets, rows, &lo, &hi);
+        const int mine = (int)((hi - lo + BR - 1) / BR);
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(sum, d);
+            if (lane >= d) sum += up;
+        }
+        const int64_t first = before + sum - mine;
+        const uint64_t hit = __ballot(mine > 0 && tile >= first && tile < first + mine);
+        if (hit != 0) {
+            const int src = __ffsll((unsigned long long)hit) - 1;
+            const int64_t f = __shfl((long long)first, src), l = __shfl((long long)lo, src), h = __shfl((long long)hi, src);
+            *set = e0 + src;
+            *row0 = lin_uniform(l + (tile - f) * BR);
+            *row_end = lin_uniform(h);
+            return true;
+        }
+        before += __shfl(sum, 63);
+    }
+    return false;
+}
+
+enum { LIN_NONE = 0, LIN_RELU = 1, LIN_GELU = 2, LIN_SILU = 3 };
+
+__device__ __forceinline__ float lin_act(float z, int act) {
+    if (act == LIN_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    if (act == LIN_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (act == LIN_SILU) return z / (1.f + expf(-z));
+    return z;
+}
+__device__ __forceinline__ float lin_slope(float z, int act) {
+    if (act == LIN_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
+    if (act == LIN_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    if (act == LIN_SILU) {
+        const float q = 1.f / (1.f + expf(-z));
+        return q * (1.f + z * (1.f - q));
+    }
+    return 1.f;
+}
+
+struct LinArgs {
+    LinOperand P, Q;
+    int64_t rows;      // rows of x
+    int cols, k;       // contiguous size of the output; length of the summed axis (forward, input gradient)
+    const int32_t *offsets;  // [n_sets + 1] or NULL
+    int n_sets;
+    int64_t row_tiles;
+    int col_tiles, out_rows, splits;  // weight gradient: rows of the output, parts of the summed axis
+    const void *bias;
+    const void *residual;
+    int64_t ld_res;
+    int act;
+    void *out;
+    void *pre;
+    void *bias_out;
+    float *partial;  // weight gradient with splits > 1: [splits][n_sets][out_rows][cols] then [splits][n_sets][out_rows]
+};
+
+// four consecutive columns of one output row
+template <typename T>
+__device__ __forceinline__ void lin_store4(T *p, const float *v, int n, bool whole) {
+    if (whole) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(v[e]);
+        *reinterpret_cast<t4 *>(p) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < n) p[e] = from_f32<T>(v[e]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void lin_load4(const T *p, float *v, int n, bool whole) {
+    if (whole) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        const t4 w = *reinterpret_cast<const t4 *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_f32(w[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(p[e]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ bool lin_aligned4(const void *p, int64_t ld) {
+    return ((uintptr_t)p % (4 * sizeof(T)) == 0) && (ld % 4 == 0);
+}
+
+// Consecutive workgroups go to different XCDs in turn: each XCD gets one contiguous run of tiles, so that the tiles that share
+// an operand meet in one L2.
+__device__ __forceinline__ int64_t lin_xcd_order(int64_t id, int64_t n) {
+    const int64_t per = n / 8;
+    return id < per * 8 ? (id % 8) * per + id / 8 : id;
+}
+
+enum { LIN_FORWARD = 0, LIN_GRAD_INPUT = 1, LIN_GRAD_WEIGHT = 2 };
+
+template <typename T, int MODE, int BC, int BR, int WC, int WR>
+__global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinArgs a) {
+    constexpr int NT = 64 * (BC / WC) * (BR / WR);
+    constexpr bool PKC = MODE == LIN_FORWARD, QKC = MODE != LIN_GRAD_WEIGHT;
+    constexpr int SZ = sizeof(T), BK = 128 / SZ;
+    constexpr int FC = WC / 32, FR = WR / 32;
+    constexpr int P_BYTES = BC * 128, STAGE = (BC + BR) * 128;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 * STAGE
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wc = wave % (BC / WC), wr = wave / (BC / WC);
+
+    int64_t id = lin_xcd_order(blockIdx.x, gridDim.x);
+    int64_t row0 = 0, row_end = 0, k_lo = 0, k_len = a.k;
+    int set = 0, split = 0;
+    const int ct = (int)(id % a.col_tiles);
+    id /= a.col_tiles;
+    const int64_t c0 = (int64_t)ct * BC;
+    if constexpr (MODE == LIN_GRAD_WEIGHT) {
+        const int rt = (int)(id % a.row_tiles);
+        id /= a.row_tiles;
+        split = (int)(id % a.splits);
+        set = (int)(id / a.splits);
+        row0 = (int64_t)rt * BR;
+        row_end = a.out_rows;
+        int64_t lo = 0, hi = a.rows;
+        if (a.offsets != nullptr) lin_bounds(a.offsets, set, a.n_sets, a.rows, &lo, &hi);
+        const int64_t part = ((hi - lo + a.splits - 1) / a.splits + BK - 1) / BK * BK;
+        k_lo = lo + part * split;
+        k_lo = k_lo < hi ? k_lo : hi;
+        k_len = hi - k_lo < part ? hi - k_lo : part;
+    } else if (a.offsets != nullptr) {
+        if (!lin_find_tile<BR>(a.offsets, a.n_sets, a.rows, id, &set, &row0, &row_end)) return;
+    } else {
+        row0 = id * BR;
+        row_end = a.rows;
+    }
+    T *out = reinterpret_cast<T *>(a.out);
+    if (MODE != LIN_GRAD_WEIGHT && set == a.n_sets) {  // rows behind the last set
+        for (int64_t i = tid; i < (int64_t)BR * BC; i += NT) {
+            const int64_t r = row0 + i / BC, c = c0 + i % BC;
+            if (r < row_end && c < a.cols) {
+                out[r * a.cols + c] = (T)0.f;
+                if (MODE == LIN_FORWARD && a.pre != nullptr) reinterpret_cast<T *>(a.pre)[r * a.cols + c] = (T)0.f;
+            }
+        }
+        return;
+    }
+
+    // operand windows: first element, bytes to the last element that counts, bytes per step along k
+    const T *p_at = reinterpret_cast<const T *>(a.P.base) + set * a.P.group;
+    const T *q_at = reinterpret_cast<const T *>(a.Q.base) + set * a.Q.group;
+    int64_t p_left, q_left, p_step, q_step;
+    if constexpr (PKC) {
+        const int64_t n = a.cols - c0 < BC ? a.cols - c0 : BC;
+        p_at += c0 * a.P.ld;
+        p_left = ((n - 1) * a.P.ld + k_len) * SZ;
+        p_step = 128;
+    } else {
+        p_at += k_lo * a.P.ld + c0;
+        p_left = k_len > 0 ? ((k_len - 1) * a.P.ld + a.cols - c0) * SZ : 0;
+        p_step = (int64_t)BK * a.P.ld * SZ;
+    }
+    const int64_t n_rows = row_end - row0 < BR ? row_end - row0 : BR;
+    if constexpr (QKC) {
+        q_at += row0 * a.Q.ld;
+        q_left = ((n_rows - 1) * a.Q.ld + k_len) * SZ;
+        q_step = 128;
+    } else {
+        q_at += k_lo * a.Q.ld + row0;
+        q_left = k_len > 0 ? ((k_len - 1) * a.Q.ld + row_end - row0) * SZ : 0;
+        q_step = (int64_t)BK * a.Q.ld * SZ;
+    }
+    LinTile<T, PKC, BC, NT> tp;
+    LinTile<T, QKC, BR, NT> tq;
+    tp.init(a.P.ld, tid);
+    tq.init(a.Q.ld, tid);
+    LinReader<T, PKC, BC> rp;
+    LinReader<T, QKC, BR> rq;
+    rp.init(wc * WC, lane);
+    rq.init(wr * WR, lane);
+
+    f32x16v acc[FC][FR];
+    f32x16v acc_ones[MODE == LIN_GRAD_WEIGHT ? FR : 1];
+#pragma unroll
+    for (int c = 0; c < FC; ++c)
+#pragma unroll
+        for (int r = 0; r < FR; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[c][r][e] = 0.f;
+    const bool sum_q = MODE == LIN_GRAD_WEIGHT && a.bias_out != nullptr && ct == 0 && wc == 0;
+    if constexpr (MODE == LIN_GRAD_WEIGHT) {
+#pragma unroll
+        for (int r = 0; r < FR; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc_ones[r][e] = 0.f;
+    }
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+    const int64_t n_steps = (k_len + BK - 1) / BK;
+    int64_t k_left = k_len;
+    auto fetch = [&](int buf) {
+        const unsigned l = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(buf * STAGE));
+        tp.load(make_rsrc(p_at, p_left), k_left, l, wave);
+        tq.load(make_rsrc(q_at, q_left), k_left, l + P_BYTES, wave);
+        p_at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(p_at) + p_step);
+        q_at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(q_at) + q_step);
+        p_left -= p_step;
+        q_left -= q_step;
+        k_left -= BK;
+    };
+    if (n_steps > 0) fetch(0);
+    for (int64_t t = 0; t < n_steps; ++t) {
+        dma_wait_all();
+        __syncthreads();  // tile t has landed, and nobody reads the other buffer any more
+        char *buf = smem + (t & 1) * STAGE;
+        const int64_t left = k_len - t * BK;
+        if constexpr (PKC || QKC) {
+            if (left < BK && left % (16 / SZ) != 0) {
+                if constexpr (PKC) LinTile<T, true, BC, NT>::clear_tail(buf, (int)left, tid);
+                if constexpr (QKC) LinTile<T, true, BR, NT>::clear_tail(buf + P_BYTES, (int)left, tid);
+                __syncthreads();
+            }
+        }
+        if (t + 1 < n_steps) fetch((int)((t + 1) & 1));
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            typename LinMfma<T>::frag fp[FC], fq[FR];
+#pragma unroll
+            for (int c = 0; c < FC; ++c) fp[c] = rp.read(buf, c, s);
+#pragma unroll
+            for (int r = 0; r < FR; ++r) fq[r] = rq.read(buf + P_BYTES, r, s);
+#pragma unroll
+            for (int c = 0; c < FC; ++c)
+#pragma unroll
+                for (int r = 0; r < FR; ++r) acc[c][r] = LinMfma<T>::mul(fp[c], fq[r], acc[c][r]);
+            if constexpr (MODE == LIN_GRAD_WEIGHT) {
+                if (sum_q) {
+#pragma unroll
+                    for (int r = 0; r < FR; ++r) acc_ones[r] = LinMfma<T>::mul(LinMfma<T>::ones(), fq[r], acc_ones[r]);
+                }
+            }
+        }
+    }
+
+    // ---- epilogue: lane (i, h) holds row i of a fragment, columns 8 g + 4 h + 0..3 for g = 0..3 ----
+    const int i = lane & 31, h = lane >> 5;
+    const bool vec = lin_aligned4<T>(out, a.cols);
+    const bool vec_res = MODE == LIN_FORWARD && a.residual != nullptr && lin_aligned4<T>(a.residual, a.ld_res);
+    const bool vec_pre = MODE == LIN_FORWARD && a.pre != nullptr && lin_aligned4<T>(a.pre, a.cols);
+#pragma unroll
+    for (int c = 0; c < FC; ++c) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int64_t col = c0 + wc * WC + c * 32 + 8 * g + 4 * h;
+            const int n = (int)(a.cols - col < 4 ? a.cols - col : 4);
+            if (n <= 0) continue;
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (MODE == LIN_FORWARD) {
+                if (a.bias != nullptr) {
+                    const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols + col;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < n) bias[e] = to_f32(b[e]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < FR; ++r) {
+                const int64_t row = row0 + wr * WR + r * 32 + i;
+                if (row >= row_end) continue;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[c][r][4 * g + e];
+                if constexpr (MODE == LIN_FORWARD) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += bias[e];
+                    if (a.pre != nullptr)
+                        lin_store4(reinterpret_cast<T *>(a.pre) + row * a.cols + col, v, n, vec_pre && n == 4);
+                    if (a.act != LIN_NONE) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = lin_act(v[e], a.act);
+                    }
+                    if (a.residual != nullptr) {
+                        float res[4];
+                        lin_load4(reinterpret_cast<const T *>(a.residual) + row * a.ld_res + col, res, n, vec_res && n == 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += res[e];
+                    }
+                }
+                if constexpr (MODE == LIN_GRAD_WEIGHT) {
+                    const int64_t at = ((int64_t)set * a.out_rows + row) * a.cols + col;
+                    if (a.splits > 1) {
+                        lin_store4(a.partial + (int64_t)split * a.n_sets * a.out_rows * a.cols + at, v, n,
+                                   a.cols % 4 == 0 && n == 4);
+                    } else {
+                        lin_store4(out + at, v, n, vec && n == 4);
+                    }
+                } else {
+                    lin_store4(out + row * a.cols + col, v, n, vec && n == 4);
+                }
+            }
+        }
+    }
+    if constexpr (MODE == LIN_GRAD_WEIGHT) {
+        if (sum_q && h == 0) {
+#pragma unroll
+            for (int r = 0; r < FR; ++r) {
+                const int64_t row = row0 + wr * WR + r * 32 + i;
+                if (row < row_end) {
+                    const int64_t at = (int64_t)set * a.out_rows + row;
+                    if (a.splits > 1)
+                        a.partial[(int64_t)a.splits * a.n_sets * a.out_rows * a.cols +
+                                  (int64_t)split * a.n_sets * a.out_rows + at] = acc_ones[r][0];
+                    else
+                        reinterpret_cast<T *>(a.bias_out)[at] = from_f32<T>(acc_ones[r][0]);
+                }
+            }
+        }
+    }
+}

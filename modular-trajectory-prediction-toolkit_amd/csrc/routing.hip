@@ -1,0 +1,693 @@
+// Routing of agents to modalities on gfx950: the k most probable modalities of each agent, the (agent, modality) pairs sorted
+// by modality, the agents' rows copied to their pairs and the pairs' answers summed back with their weights; and the gradients.
+//
+// Everything here moves data: each kernel reads its inputs and writes its outputs once (the sort reads the ids twice).
+// No result depends on the order in which workgroups run: sums go over a token's own pairs in their order, and the sort is
+// stable.  Types float, bfloat16, half; softmax statistics, weights and sums are float.
+#include "mtp_internal.h"
+
+namespace {
+
+constexpr int ROUTE_MAX_E = 4096;  // index bits of a sort key; registers of a lane
+constexpr int ROUTE_MAX_K = 128;
+
+template <typename T>
+__device__ __forceinline__ float up(T v) {
+    return (float)v;
+}
+
+// ---- top k ----
+// A key orders like (score, -index): the score's bits made monotonous, then 4095 - index, put into the mantissa of a double
+// with a fixed exponent, so that one v_max_f64 / v_min_f64 pair is a compare-exchange of value and index at once.
+__device__ __forceinline__ double route_key(float s, int index) {
+    s = s + 0.0f;  // -0 equals +0
+    uint32_t b = __float_as_uint(s);
+    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    const uint64_t m = ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - index);
+    return __longlong_as_double((long long)(0x4000000000000000ull | m));
+}
+__device__ __forceinline__ float route_key_score(double key) {
+    uint32_t b = (uint32_t)((uint64_t)__double_as_longlong(key) >> 12);
+    b = (b & 0x80000000u) ? (b & 0x7fffffffu) : ~b;
+    return __uint_as_float(b);
+}
+__device__ __forceinline__ int route_key_index(double key) {
+    return ROUTE_MAX_E - 1 - (int)((uint64_t)__double_as_longlong(key) & (ROUTE_MAX_E - 1));
+}
+constexpr double ROUTE_NO_KEY = 2.0;  // mantissa 0: below every score's key, -inf's included
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
+    return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+constexpr int ROW_ROR = 0x120;  // rotation within 16 lanes
+
+// over the L lanes (16 or 64) that share a row, the same result in each
+template <int L>
+__device__ __forceinline__ double group_max(double v) {
+    v = fmax(v, dpp_f64<ROW_ROR + 8>(v));
+    v = fmax(v, dpp_f64<ROW_ROR + 4>(v));
+    v = fmax(v, dpp_f64<ROW_ROR + 2>(v));
+    v = fmax(v, dpp_f64<ROW_ROR + 1>(v));
+    if constexpr (L == 64) {
+        v = fmax(v, __shfl_xor(v, 16));
+        v = fmax(v, __shfl_xor(v, 32));
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+    v += dpp_f32<ROW_ROR + 8>(v);
+    v += dpp_f32<ROW_ROR + 4>(v);
+    v += dpp_f32<ROW_ROR + 2>(v);
+    v += dpp_f32<ROW_ROR + 1>(v);
+    if constexpr (L == 64) {
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+    }
+    return v;
+}
+
+// Batcher's odd-even merge sort of V registers, largest first
+template <int V>
+__device__ __forceinline__ void sort_registers(double (&a)[V]) {
+#pragma unroll
+    for (int p = 1; p < V; p *= 2) {
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2) {
+#pragma unroll
+            for (int j = q % p; j + q < V; j += 2 * q) {
+#pragma unroll
+                for (int i = 0; i < q; ++i) {
+                    if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const double x = a[i + j], y = a[i + j + q];
+                        a[i + j] = fmax(x, y);
+                        a[i + j + q] = fmin(x, y);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// L lanes share a row, lane `sub` holds the scores sub, sub + L, ...  Each lane sorts its own V keys and lays the first
+// min(V, k) of them into LDS; k times the largest head is taken (a maximum over the L lanes), and the lane it came from moves on
+// to its next key.
+template <typename T, int L, int V, int KB>
+__global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores, int64_t n, int e, int64_t ld, int k, int normalize,
+                                                    int32_t *__restrict__ ids, float *__restrict__ weights,
+                                                    float *__restrict__ stats) {
+    extern __shared__ __attribute__((aligned(16))) double lists[];  // [min(V, k)][256]
+    const int tid = threadIdx.x, sub = tid % L;
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + tid / L;
+    const bool live = row < n;
+    const T *s = scores + (live ? row : n - 1) * ld;
+
+    double key[V];
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int i = j * L + sub;
+        key[j] = ROUTE_NO_KEY;
+        if (i < e) {
+            const float v = up(s[i]);
+            bad |= v != v;
+            key[j] = route_key(v != v ? -__builtin_inff() : v, i);
+        }
+    }
+    float total = 0.f, top = 0.f;
+    if (!normalize) {  // the softmax over all modalities
+        double m = ROUTE_NO_KEY;
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmax(m, key[j]);
+        top = route_key_score(group_max<L>(m));
+        if (top == -__builtin_inff()) top = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (key[j] != ROUTE_NO_KEY) total += expf(route_key_score(key[j]) - top);
+        total = group_sum<L>(total);
+    }
+    const uint64_t any_bad = __ballot(bad);
+    const bool row_bad = ((any_bad >> ((tid & 63) / L * L)) & (L == 64 ? ~0ull : 0xffffull)) != 0;
+
+    sort_registers<V>(key);
+    const int depth = V < k ? V : k;
+    double *mine = lists + tid;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < depth) mine[j * 256] = key[j];
+    int at = 0;
+    double head = key[0];
+    double chosen[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        chosen[b] = ROUTE_NO_KEY;
+        const int most = k - b * L < L ? k - b * L : L;
+        for (int i = 0; i < most; ++i) {
+            const double best = group_max<L>(head);
+            if (sub == i) chosen[b] = best;
+            if (head == best) {  // keys differ by their index: one lane; where nothing is left, no matter
+                ++at;
+                head = at < depth ? mine[at * 256] : ROUTE_NO_KEY;
+            }
+        }
+    }
+    float w[KB];
+    if (normalize) {
+        // lane 0 of the first batch has the largest score
+        const double first = __shfl(chosen[0], (tid & 63) / L * L);
+        top = first == ROUTE_NO_KEY ? 0.f : route_key_score(first);
+        if (top == -__builtin_inff()) top = 0.f;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        const float v = route_key_score(chosen[b]);
+        const bool none = chosen[b] == ROUTE_NO_KEY || v == -__builtin_inff();
+        if (none) chosen[b] = ROUTE_NO_KEY;
+        w[b] = none ? 0.f : expf(v - top);
+        sum += w[b];
+    }
+    if (normalize) total = group_sum<L>(sum);
+    const float scale = total != 0.f ? 1.f / total : (total != total ? total : 0.f);
+    if (!live) return;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        const int i = b * L + sub;
+        if (i < k) {
+            const bool none = chosen[b] == ROUTE_NO_KEY;
+            ids[row * k + i] = none ? -1 : route_key_index(chosen[b]);
+            weights[row * k + i] = row_bad ? __builtin_nanf("") : w[b] * scale;
+        }
+    }
+    if (stats != nullptr && sub == 0) {
+        stats[row * 2] = top;
+        stats[row * 2 + 1] = row_bad ? __builtin_nanf("") : scale;
+    }
+}
+
+// Gradient towards the scores, a few rows per workgroup:
+//   normalised: w_j (g_j - sum g w) at the chosen, zero elsewhere;  else: p_j (g_j [chosen] - sum g w) everywhere
+template <typename T>
+__global__ __launch_bounds__(256) void k_route_grad(const T *__restrict__ scores, int64_t n, int e, int64_t ld, int k, int normalize,
+                                                    const int32_t *__restrict__ ids, const float *__restrict__ weights,
+                                                    const float *__restrict__ stats, const float *__restrict__ g,
+                                                    T *__restrict__ out, int rows_per) {
+    extern __shared__ __attribute__((aligned(16))) float tile[];  // [rows_per][e], then [rows_per] dots
+    float *dots = tile + rows_per * e;
+    const int tid = threadIdx.x;
+    const int64_t row0 = (int64_t)blockIdx.x * rows_per;
+    const int rows = (int)(n - row0 < rows_per ? n - row0 : rows_per);
+    for (int i = tid; i < rows * e; i += 256) tile[i] = 0.f;
+    __syncthreads();
+    const int sub = tid & 15;
+    for (int r = tid >> 4; r < rows; r += 16) {
+        const int64_t at = (row0 + r) * k;
+        float dot = 0.f;
+        for (int j = sub; j < k; j += 16) dot += weights[at + j] * g[at + j];
+        dot = group_sum<16>(dot);
+        for (int j = sub; j < k; j += 16) {
+            const int id = ids[at + j];
+            const float w = weights[at + j];
+            if (id >= 0 && id < e) tile[r * e + id] = normalize ? w * (g[at + j] - dot) : w * g[at + j];
+        }
+        if (sub == 0) dots[r] = dot;
+    }
+    __syncthreads();
+    T *o = out + row0 * e;
+    for (int i = tid; i < rows * e; i += 256) {
+        float v = tile[i];
+        if (!normalize) {
+            const int r = i / e, c = i - r * e;
+            const float top = stats[(row0 + r) * 2], scale = stats[(row0 + r) * 2 + 1];
+            v -= expf(up(scores[(row0 + r) * ld + c]) - top) * scale * dots[r];
+        }
+        o[i] = (T)v;
+    }
+}
+
+// ---- pairs sorted by modality ----
+// Stable counting sort.  A wave owns a run of pairs and goes through it 64 at a time; lanes with the same modality find each
+// other by ballots over the modality's bits, so a pair's place is (pairs of its modality before this round) + (lanes below).
+__device__ __forceinline__ int pair_key(int id, int e) { return id >= 0 && id < e ? id : e; }
+
+__device__ __forceinline__ uint64_t same_key_lanes(int key, int bits, bool valid) {
+    uint64_t mask = __ballot(valid);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t ones = __ballot((key >> b) & 1);
+        mask &= ((key >> b) & 1) ? ones : ~ones;
+    }
+    return mask;
+}
+
+// counts[b * (e + 1) + x] = pairs of modality x in workgroup b's run
+__global__ __launch_bounds__(256) void k_pairs_count(const int32_t *__restrict__ ids, int64_t pairs, int e, int run,
+                                                     int32_t *__restrict__ counts) {
+    extern __shared__ int hist[];
+    for (int i = threadIdx.x; i <= e; i += 256) hist[i] = 0;
+    __syncthreads();
+    const int64_t lo = (int64_t)blockIdx.x * run, hi = lo + run < pairs ? lo + run : pairs;
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 256) atomicAdd(&hist[pair_key(ids[i], e)], 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i <= e; i += 256) counts[(int64_t)blockIdx.x * (e + 1) + i] = hist[i];
+}
+
+// counts -> the exclusive prefix over the workgroups, and the modality's total.  64 modalities and 16 parts a workgroup.
+__global__ __launch_bounds__(1024) void k_pairs_scan(int32_t *__restrict__ counts, int blocks, int e, int32_t *__restrict__ totals) {
+    __shared__ int part[16][64];
+    const int x = blockIdx.x * 64 + (threadIdx.x & 63), p = threadIdx.x >> 6;
+    const int per = (blocks + 15) / 16;
+    const int lo = p * per, hi = lo + per < blocks ? lo + per : blocks;
+    int sum = 0;
+    if (x <= e)
+        for (int b = lo; b < hi; ++b) sum += counts[(int64_t)b * (e + 1) + x];
+    part[p][threadIdx.x & 63] = sum;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < 16; ++i) {
+        const int v = part[i][threadIdx.x & 63];
+        if (i < p) before += v;
+        all += v;
+    }
+    if (x <= e) {
+        for (int b = lo; b < hi; ++b) {
+            const int v = counts[(int64_t)b * (e + 1) + x];
+            counts[(int64_t)b * (e + 1) + x] = before;
+            before += v;
+        }
+        if (p == 0) totals[x] = all;
+    }
+}
+
+// exclusive prefix sum of v[0 .. m) in LDS, by the whole workgroup of W waves; scratch: W ints
+template <int W>
+__device__ __forceinline__ void scan_lds(int *v, int m, int *scratch) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int base = 0;
+    for (int i0 = 0; i0 < m; i0 += W * 64) {
+        const int i = i0 + tid;
+        const int mine = i < m ? v[i] : 0;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(sum, d);
+            if (lane >= d) sum += u;
+        }
+        if (lane == 63) scratch[wave] = sum;
+        __syncthreads();
+        int before = base, all = 0;
+        for (int w = 0; w < W; ++w) {
+            if (w < wave) before += scratch[w];
+            all += scratch[w];
+        }
+        if (i < m) v[i] = before + sum - mine;
+        base += all;
+        __syncthreads();
+    }
+}
+
+// W waves; run: pairs per workgroup, a multiple of 64 * W.  counts / totals NULL: one workgroup has all the pairs.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_pairs_place(const int32_t *__restrict__ ids, int64_t pairs, int e, int bits, int run,
+                                                        const int32_t *__restrict__ counts, const int32_t *__restrict__ totals,
+                                                        int32_t *__restrict__ offsets, int32_t *__restrict__ order,
+                                                        int32_t *__restrict__ position) {
+    extern __shared__ int lds[];  // start[e + 1], next[W][e + 1], scratch[W]
+    int *start = lds, *next = lds + (e + 1), *scratch = next + W * (e + 1);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t lo = (int64_t)blockIdx.x * run + (int64_t)wave * (run / W);
+    const int64_t end = lo + run / W < pairs ? lo + run / W : pairs;
+    for (int i = tid; i < W * (e + 1); i += 64 * W) next[i] = 0;
+    __syncthreads();
+    int *here = next + wave * (e + 1);
+    for (int64_t i = lo + lane; i < end; i += 64) atomicAdd(&here[pair_key(ids[i], e)], 1);
+    __syncthreads();
+    for (int x = tid; x <= e; x += 64 * W) {
+        int all = 0;
+        for (int w = 0; w < W; ++w) {  // the waves' shares of this modality, one behind the other
+            const int v = next[w * (e + 1) + x];
+            next[w * (e + 1) + x] = all;
+            all += v;
+        }
+        start[x] = totals != nullptr ? totals[x] : all;
+    }
+    __syncthreads();
+    scan_lds<W>(start, e + 1, scratch);
+    if (blockIdx.x == 0)
+        for (int x = tid; x <= e; x += 64 * W) offsets[x] = start[x];
+    for (int x = tid; x <= e; x += 64 * W) {
+        const int at = start[x] + (counts != nullptr ? counts[(int64_t)blockIdx.x * (e + 1) + x] : 0);
+        for (int w = 0; w < W; ++w) next[w * (e + 1) + x] += at;
+    }
+    __syncthreads();
+    volatile int *mine = here;
+    for (int64_t i0 = lo; i0 < end; i0 += 64) {
+        const int64_t i = i0 + lane;
+        const bool valid = i < end;
+        const int key = valid ? pair_key(ids[i], e) : e;
+        const uint64_t peers = same_key_lanes(key, bits, valid);
+        const uint64_t below = peers & ((1ull << lane) - 1);
+        const int at = valid ? mine[key] + __popcll(below) : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (valid && below == 0) mine[key] = at + __popcll(peers);
+        __builtin_amdgcn_wave_barrier();
+        if (valid) {
+            position[i] = at;
+            order[at] = (int32_t)i;
+        }
+    }
+}
+
+// ---- rows to their pairs and back ----
+template <typename T, int N>
+struct Pack {
+    typedef T type __attribute__((ext_vector_type(N)));
+};
+template <typename T>
+struct Pack<T, 1> {
+    typedef T type;
+};
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const typename Pack<T, N>::type &v, float *f) {
+    if constexpr (N == 1) f[0] = up(v);
+    else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = up(v[e]);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ typename Pack<T, N>::type pack(const float *f) {
+    if constexpr (N == 1) return (T)f[0];
+    else {
+        typename Pack<T, N>::type v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = (T)f[e];
+        return v;
+    }
+}
+
+// rows[position[t][j]] = x[t], zero where the pair has no modality; one thread per N elements of a token
+template <typename T, int N>
+__global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64_t n, int d, int64_t ld, int k,
+                                                  const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
+                                                  T *__restrict__ rows) {
+    typedef typename Pack<T, N>::type vec;
+    const int per = d / N;
+    const int64_t total = n * per;
+    const int held = *held_at;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per, c = i - t * per;
+        const vec v = *reinterpret_cast<const vec *>(x + t * ld + c * N);
+        const vec zero = {};
+        for (int j = 0; j < k; ++j) {
+            const int64_t p = position[t * k + j];
+            *reinterpret_cast<vec *>(rows + p * d + c * N) = p < held ? v : zero;
+        }
+    }
+}
+
+// y[t] = sum_j weights[t][j] rows[position[t][j]] (weights NULL: all one), pairs without a modality left out
+template <typename T, int N>
+__global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int64_t n, int d, int k,
+                                                 const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
+                                                 const float *__restrict__ weights, T *__restrict__ y) {
+    typedef typename Pack<T, N>::type vec;
+    const int per = d / N;
+    const int64_t total = n * per;
+    const int held = *held_at;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per, c = i - t * per;
+        float sum[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] = 0.f;
+#pragma unroll 4
+        for (int j = 0; j < k; ++j) {
+            const int64_t p = position[t * k + j];
+            if (p < held) {
+                float f[N];
+                unpack<T, N>(*reinterpret_cast<const vec *>(rows + p * d + c * N), f);
+                const float w = weights != nullptr ? weights[t * k + j] : 1.f;
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] = fmaf(w, f[e], sum[e]);
+            }
+        }
+        *reinterpret_cast<vec *>(y + t * d + c * N) = pack<T, N>(sum);
+    }
+}
+
+// grad_rows[position[t][j]] = weights[t][j] g[t] (zero behind the last modality); grad_weights[t][j] = <rows[...], g[t]>.
+// L lanes share a token.
+template <typename T, int N, int L>
+__global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows, const T *__restrict__ g, int64_t n, int d, int k,
+                                                      const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
+                                                      const float *__restrict__ weights, T *__restrict__ grad_rows,
+                                                      float *__restrict__ grad_weights) {
+    typedef typename Pack<T, N>::type vec;
+    const int per = d / N, sub = threadIdx.x % L;
+    const int held = *held_at;
+    for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L; t < n; t += (int64_t)gridDim.x * (256 / L)) {
+        for (int j = 0; j < k; ++j) {
+            const int64_t p = position[t * k + j];
+            const bool in = p < held;
+            const float w = in ? weights[t * k + j] : 0.f;
+            float dot = 0.f;
+            for (int c = sub; c < per; c += L) {
+                float gv[N], rv[N];
+                unpack<T, N>(*reinterpret_cast<const vec *>(g + t * d + c * N), gv);
+                if (in && grad_weights != nullptr) {
+                    unpack<T, N>(*reinterpret_cast<const vec *>(rows + p * d + c * N), rv);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) dot = fmaf(rv[e], gv[e], dot);
+                }
+                if (grad_rows != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) gv[e] = in ? w * gv[e] : 0.f;
+                    *reinterpret_cast<vec *>(grad_rows + p * d + c * N) = pack<T, N>(gv);
+                }
+            }
+            if (grad_weights != nullptr) {
+#pragma unroll
+                for (int m = L / 2; m > 0; m >>= 1) dot += __shfl_xor(dot, m);
+                if (sub == 0) grad_weights[t * k + j] = dot;
+            }
+        }
+    }
+}
+
+unsigned blocks_of(int64_t items, int per_block) {
+    const int64_t b = (items + per_block - 1) / per_block;
+    return (unsigned)(b < 1 ? 1 : (b > 256 * 32 ? 256 * 32 : b));
+}
+
+template <typename T, int L, int V, int KB>
+int launch_topk(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights, float *stats,
+                hipStream_t s) {
+    const int lds = (V < k ? V : k) * 256 * 8;
+    const int64_t blocks = (n + 256 / L - 1) / (256 / L);
+    MTP_SET_MAX_LDS_ONCE((k_route_topk<T, L, V, KB>), V * 256 * 8);
+    hipLaunchKernelGGL((k_route_topk<T, L, V, KB>), dim3((unsigned)blocks), dim3(256), lds, s, reinterpret_cast<const T *>(scores), n,
+                       e, ld, k, normalize, ids, weights, stats);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+template <typename T, int L, int V>
+int route_by_k(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights, float *stats,
+               hipStream_t s) {
+    if (k <= L) return launch_topk<T, L, V, 1>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    if (k <= 2 * L) return launch_topk<T, L, V, 2>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    if constexpr (L == 16) return launch_topk<T, L, V, 8>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    mtp_set_error("mtp_route_topk: k=%d", k);
+    return MTP_E_ARG;
+}
+
+template <typename T>
+int route(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights, float *stats,
+          hipStream_t s) {
+    if (e <= 1024 && n >= 1024) {
+        if (e <= 64) return route_by_k<T, 16, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 256) return route_by_k<T, 16, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 512) return route_by_k<T, 16, 32>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        return route_by_k<T, 16, 64>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    }
+    if (e <= 256) return route_by_k<T, 64, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    if (e <= 1024) return route_by_k<T, 64, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    return route_by_k<T, 64, 64>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+}
+
+constexpr int PAIRS_RUN = 2048;      // pairs of a workgroup
+constexpr int PAIRS_ALONE = 16384;   // up to here one workgroup sorts them all
+
+int64_t pairs_blocks(int64_t pairs) { return (pairs + PAIRS_RUN - 1) / PAIRS_RUN; }
+bool pairs_alone(int64_t pairs, int e) { return pairs <= PAIRS_ALONE && (int64_t)17 * (e + 1) * 4 + 64 <= 128 * 1024; }
+
+template <typename T>
+int dispatch(const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held, void *rows,
+             hipStream_t s) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool vec = d % N == 0 && ld % N == 0 && ((uintptr_t)x | (uintptr_t)rows) % 16 == 0;
+    if (vec)
+        hipLaunchKernelGGL((k_dispatch<T, N>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(x), n,
+                           d, ld, k, position, held, reinterpret_cast<T *>(rows));
+    else
+        hipLaunchKernelGGL((k_dispatch<T, 1>), dim3(blocks_of(n * d, 256)), dim3(256), 0, s, reinterpret_cast<const T *>(x), n, d, ld,
+                           k, position, held, reinterpret_cast<T *>(rows));
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+template <typename T>
+int combine(const void *rows, int64_t n, int d, int k, const int32_t *position, const int32_t *held, const float *weights, void *y,
+            hipStream_t s) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)y) % 16 == 0;
+    if (vec)
+        hipLaunchKernelGGL((k_combine<T, N>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
+                           n, d, k, position, held, weights, reinterpret_cast<T *>(y));
+    else
+        hipLaunchKernelGGL((k_combine<T, 1>), dim3(blocks_of(n * d, 256)), dim3(256), 0, s, reinterpret_cast<const T *>(rows), n, d,
+                           k, position, held, weights, reinterpret_cast<T *>(y));
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+template <typename T, int N, int L>
+int launch_combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
+                        const float *weights, void *grad_rows, float *grad_weights, hipStream_t s) {
+    hipLaunchKernelGGL((k_combine_grad<T, N, L>), dim3(blocks_of(n, 256 / L)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
+                       reinterpret_cast<const T *>(g), n, d, k, position, held, weights, reinterpret_cast<T *>(grad_rows),
+                       grad_weights);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+template <typename T>
+int combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
+                 const float *weights, void *grad_rows, float *grad_weights, hipStream_t s) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)g | (uintptr_t)grad_rows) % 16 == 0;
+    if (!vec)
+        return launch_combine_grad<T, 1, 64>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (d / N <= 8) return launch_combine_grad<T, N, 8>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (d / N <= 16) return launch_combine_grad<T, N, 16>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    return launch_combine_grad<T, N, 32>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+}
+
+bool known_type(int dtype) { return dtype == MTP_FLOAT || dtype == MTP_BFLOAT16 || dtype == MTP_HALF; }
+
+}  // namespace
+
+#define ROUTE_BY_TYPE(dtype, call) ((dtype) == MTP_FLOAT ? call<float> : (dtype) == MTP_BFLOAT16 ? call<__bf16> : call<_Float16>)
+
+extern "C" int mtp_route_topk(int dtype, const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids,
+                              float *weights, float *stats, void *stream) {
+    MTP_REQUIRE(known_type(dtype), "mtp_route_topk: unknown type %d", dtype);
+    MTP_REQUIRE(n >= 0 && n <= 0x7fffffff && e >= 1 && e <= ROUTE_MAX_E && k >= 1 && k <= e && k <= ROUTE_MAX_K && ld >= e,
+                "mtp_route_topk: bad shape n=%lld e=%d k=%d ld=%lld", (long long)n, e, k, (long long)ld);
+    if (n == 0) return MTP_OK;
+    MTP_REQUIRE(scores && ids && weights, "mtp_route_topk: null pointer");
+    return ROUTE_BY_TYPE(dtype, route)(scores, n, e, ld, k, normalize != 0, ids, weights, stats, mtp_stream(stream));
+}
+
+extern "C" int mtp_route_topk_grad(int dtype, const void *scores, int64_t n, int e, int64_t ld, int k, int normalize,
+                                   const int32_t *ids, const float *weights, const float *stats, const float *g, void *out,
+                                   void *stream) {
+    MTP_REQUIRE(known_type(dtype), "mtp_route_topk_grad: unknown type %d", dtype);
+    MTP_REQUIRE(n >= 0 && n <= 0x7fffffff && e >= 1 && e <= ROUTE_MAX_E && k >= 1 && k <= e && k <= ROUTE_MAX_K && ld >= e,
+                "mtp_route_topk_grad: bad shape n=%lld e=%d k=%d ld=%lld", (long long)n, e, k, (long long)ld);
+    if (n == 0) return MTP_OK;
+    MTP_REQUIRE(scores && ids && weights && stats && g && out, "mtp_route_topk_grad: null pointer");
+    int rows_per = 8192 / e;
+    if (rows_per < 1) rows_per = 1;
+    if (rows_per > 64) rows_per = 64;
+    const int lds = rows_per * (e + 1) * 4;
+    const dim3 grid((unsigned)((n + rows_per - 1) / rows_per));
+    hipStream_t s = mtp_stream(stream);
+    if (dtype == MTP_FLOAT)
+        hipLaunchKernelGGL(k_route_grad<float>, grid, dim3(256), lds, s, (const float *)scores, n, e, ld, k, normalize, ids, weights,
+                           stats, g, (float *)out, rows_per);
+    else if (dtype == MTP_BFLOAT16)
+        hipLaunchKernelGGL(k_route_grad<__bf16>, grid, dim3(256), lds, s, (const __bf16 *)scores, n, e, ld, k, normalize, ids,
+                           weights, stats, g, (__bf16 *)out, rows_per);
+    else
+        hipLaunchKernelGGL(k_route_grad<_Float16>, grid, dim3(256), lds, s, (const _Float16 *)scores, n, e, ld, k, normalize, ids,
+                           weights, stats, g, (_Float16 *)out, rows_per);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+extern "C" int64_t mtp_sort_pairs_workspace_bytes(int64_t pairs, int e) {
+    if (pairs < 0 || e < 1 || pairs_alone(pairs, e)) return 0;
+    return (pairs_blocks(pairs) + 1) * (int64_t)(e + 1) * 4;
+}
+
+extern "C" int mtp_sort_pairs(const int32_t *ids, int64_t pairs, int e, int32_t *offsets, int32_t *order, int32_t *position, void *ws,
+                              size_t ws_bytes, void *stream) {
+    MTP_REQUIRE(pairs >= 0 && pairs <= 0x7fffffff && e >= 1 && e <= ROUTE_MAX_E, "mtp_sort_pairs: bad shape pairs=%lld e=%d",
+                (long long)pairs, e);
+    MTP_REQUIRE(offsets && (pairs == 0 || (ids && order && position)), "mtp_sort_pairs: null pointer");
+    int bits = 1;
+    while ((1 << bits) <= e) ++bits;
+    hipStream_t s = mtp_stream(stream);
+    if (pairs_alone(pairs, e)) {
+        const int run = pairs == 0 ? 1024 : (int)((pairs + 1023) / 1024 * 1024);
+        const int lds = (17 * (e + 1) + 16) * 4;
+        MTP_SET_MAX_LDS_ONCE(k_pairs_place<16>, 128 * 1024);
+        hipLaunchKernelGGL(k_pairs_place<16>, dim3(1), dim3(1024), lds, s, ids, pairs, e, bits, run, (const int32_t *)nullptr,
+                           (const int32_t *)nullptr, offsets, order, position);
+        MTP_LAUNCH_CHECK();
+        return MTP_OK;
+    }
+    if ((int64_t)ws_bytes < mtp_sort_pairs_workspace_bytes(pairs, e) || ws == nullptr) {
+        mtp_set_error("mtp_sort_pairs: workspace of %zu bytes, needs %lld", ws_bytes,
+                      (long long)mtp_sort_pairs_workspace_bytes(pairs, e));
+        return MTP_E_WORKSPACE;
+    }
+    const int blocks = (int)pairs_blocks(pairs);
+    int32_t *counts = reinterpret_cast<int32_t *>(ws), *totals = counts + (int64_t)blocks * (e + 1);
+    hipLaunchKernelGGL(k_pairs_count, dim3(blocks), dim3(256), (e + 1) * 4, s, ids, pairs, e, PAIRS_RUN, counts);
+    MTP_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_pairs_scan, dim3((e + 64) / 64), dim3(1024), 0, s, counts, blocks, e, totals);
+    MTP_LAUNCH_CHECK();
+    MTP_SET_MAX_LDS_ONCE(k_pairs_place<4>, (5 * (ROUTE_MAX_E + 1) + 4) * 4);
+    hipLaunchKernelGGL(k_pairs_place<4>, dim3(blocks), dim3(256), (5 * (e + 1) + 4) * 4, s, ids, pairs, e, bits, PAIRS_RUN, counts,
+                       totals, offsets, order, position);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+#define CHECK_ROWS(who)                                                                                                     \
+    MTP_REQUIRE(known_type(dtype), who ": unknown type %d", dtype);                                                         \
+    MTP_REQUIRE(n >= 0 && k >= 1 && d >= 1 && d <= (1 << 20) && n * (int64_t)k <= 0x7fffffff, who ": bad shape n=%lld k=%d d=%d", \
+                (long long)n, k, d);                                                                                        \
+    if (n == 0) return MTP_OK
+
+extern "C" int mtp_dispatch_rows(int dtype, const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position,
+                                 const int32_t *held, void *rows, void *stream) {
+    CHECK_ROWS("mtp_dispatch_rows");
+    MTP_REQUIRE(ld >= d, "mtp_dispatch_rows: row distance below the row's length");
+    MTP_REQUIRE(x && position && held && rows, "mtp_dispatch_rows: null pointer");
+    return ROUTE_BY_TYPE(dtype, dispatch)(x, n, d, ld, k, position, held, rows, mtp_stream(stream));
+}
+
+extern "C" int mtp_combine_rows(int dtype, const void *rows, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
+                                const float *weights, void *y, void *stream) {
+    CHECK_ROWS("mtp_combine_rows");
+    MTP_REQUIRE(rows && position && held && y, "mtp_combine_rows: null pointer");
+    return ROUTE_BY_TYPE(dtype, combine)(rows, n, d, k, position, held, weights, y, mtp_stream(stream));
+}
+
+extern "C" int mtp_combine_rows_grad(int dtype, const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position,
+                                     const int32_t *held, const float *weights, void *grad_rows, float *grad_weights, void *stream) {
+    CHECK_ROWS("mtp_combine_rows_grad");
+    MTP_REQUIRE(rows && g && position && held && weights && (grad_rows || grad_weights), "mtp_combine_rows_grad: null pointer");
+    return ROUTE_BY_TYPE(dtype, combine_grad)(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights,
+                                              mtp_stream(stream));
+}

@@ -13,6 +13,8 @@ FLAG_STATE, FLAG_N_ITER, FLAG_N_EMPTY, FLAG_WORDS = 0, 1, 2, 8
 POT_F64, POT_OPENBLAS = 0, 1  # mtp_accel.h MTP_POT_*
 LLOYD_NO_FINAL_ESTEP = 1
 LLOYD_SUMS_SKLEARN_1T = 2
+FLOAT, BFLOAT16, HALF = 0, 1, 2  # element types of the routing and layer entry points
+LINEAR_FORWARD, LINEAR_GRAD_INPUT, LINEAR_GRAD_WEIGHT = 0, 1, 2
 
 _vp, _i64, _i32, _f32, _f64, _sz = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_double,
                                     ctypes.c_size_t)
@@ -88,6 +90,19 @@ SIGNATURES = {
                                           _vp, _vp]),
     "mtp_best_of_k_reranked_f64": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _f64, _i32, _vp, _vp, _vp, _vp,
                                           _vp, _vp]),
+    "mtp_route_topk": (_i32, [_i32, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "mtp_route_topk_grad": (_i32, [_i32, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mtp_sort_pairs_workspace_bytes": (_i64, [_i64, _i32]),
+    "mtp_sort_pairs": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mtp_dispatch_rows": (_i32, [_i32, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "mtp_combine_rows": (_i32, [_i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "mtp_combine_rows_grad": (_i32, [_i32, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mtp_linear_workspace_bytes": (_i64, [_i32, _i32, _i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64]),
+    "mtp_linear": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _i32, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "mtp_linear_act_grad": (_i32, [_i32, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp, _i64, _vp]),
+    "mtp_linear_mask_rows": (_i32, [_i32, _vp, _i64, _i32, _vp, _i32, _vp, _vp]),
+    "mtp_linear_grad_input": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _sz, _vp]),
+    "mtp_linear_grad_weight": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _LIB = None

@@ -411,3 +411,302 @@ def best_of_k_reranked(pred, gt, order, mode=0, ade_div=None, best_of=None):
         check(fn(ptr(pred), ptr(gt), ptr(order), order.shape[1], n, k, ktot, t, float(ade_div), int(mode), ptr(min_ade),
                  ptr(min_fde), ptr(idx), ptr(idx2), ptr(sums), stream_ptr()), "mtp_best_of_k_reranked")
     return dict(min_ade=min_ade, min_fde=min_fde, idx=idx, idx2=idx2, sums=sums)
+
+
+# ------------------------------------------------------------------------------------------
+# Routing of agents to modalities, and the layers behind it
+# ------------------------------------------------------------------------------------------
+_TYPE_CODE = {torch.float32: _lib.FLOAT, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.HALF}
+_ACT_CODE = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
+MAX_MODALITIES, MAX_TOPK = 4096, 128  # mtp_accel.h
+
+
+def _device_tensor(t, name, ndim):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise _lib.MtpError(f"{name}: pccs_accel kernels need a HIP device tensor (got device={t.device}); "
+                            "there is no CPU path")
+    if t.dim() != ndim:
+        raise ValueError(f"{name}: expected {ndim} dimensions, got shape {tuple(t.shape)}")
+    return t
+
+
+def _type_code(t, name):
+    code = _TYPE_CODE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _like(t, name, ndim, ref, ref_name, dtype=None, shape=None):
+    """A contiguous tensor on ref's device, of ref's type (or ``dtype``) and of ``shape``."""
+    _device_tensor(t, name, ndim)
+    want = ref.dtype if dtype is None else dtype
+    if t.dtype != want:
+        raise TypeError(f"{name}: expected dtype {want}, got {t.dtype}")
+    if t.device != ref.device:
+        raise ValueError(f"{name}: on {t.device}, {ref_name} on {ref.device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    return t
+
+
+def _row_distance(t, name):
+    """Elements from row to row of a matrix whose rows are contiguous (a slice of columns of a contiguous one is)."""
+    rows, cols = t.shape
+    if rows <= 1 and (cols <= 1 or t.stride(1) == 1):
+        return max(cols, 1)
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name}: rows must be contiguous and must not overlap (strides {t.stride()})")
+    return t.stride(0)
+
+
+def route_topk(scores, k, normalize=True, want_stats=False):
+    """(ids int32 [N, k], weights float32 [N, k], stats float32 [N, 2] or None) -- ``mtp_route_topk``."""
+    _device_tensor(scores, "scores", 2)
+    code = _type_code(scores, "scores")
+    n, e = scores.shape
+    k = int(k)
+    if not 1 <= e <= MAX_MODALITIES:
+        raise ValueError(f"scores: {e} modalities, expected 1 to {MAX_MODALITIES}")
+    if not 1 <= k <= min(e, MAX_TOPK):
+        raise ValueError(f"k={k} must be in [1, {min(e, MAX_TOPK)}]")
+    ld = _row_distance(scores, "scores")
+    dev = scores.device
+    ids = torch.empty((n, k), dtype=torch.int32, device=dev)
+    weights = torch.empty((n, k), dtype=torch.float32, device=dev)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if want_stats else None
+    with torch.cuda.device(dev):
+        check(lib().mtp_route_topk(code, ptr(scores), n, e, ld, k, int(bool(normalize)), ptr(ids), ptr(weights), ptr(stats),
+                                   stream_ptr()), "mtp_route_topk")
+    return ids, weights, stats
+
+
+def route_topk_grad(scores, ids, weights, stats, grad, normalize=True):
+    """Gradient of the scores [N, E] from that of the weights [N, k] -- ``mtp_route_topk_grad``."""
+    _device_tensor(scores, "scores", 2)
+    code = _type_code(scores, "scores")
+    n, e = scores.shape
+    _like(ids, "ids", 2, scores, "scores", torch.int32)
+    k = ids.shape[1]
+    _like(ids, "ids", 2, scores, "scores", torch.int32, (n, k))
+    _like(weights, "weights", 2, scores, "scores", torch.float32, (n, k))
+    _like(stats, "stats", 2, scores, "scores", torch.float32, (n, 2))
+    _like(grad, "grad", 2, scores, "scores", torch.float32, (n, k))
+    ld = _row_distance(scores, "scores")
+    out = torch.empty((n, e), dtype=scores.dtype, device=scores.device)
+    with torch.cuda.device(scores.device):
+        check(lib().mtp_route_topk_grad(code, ptr(scores), n, e, ld, k, int(bool(normalize)), ptr(ids), ptr(weights),
+                                        ptr(stats), ptr(grad), ptr(out), stream_ptr()), "mtp_route_topk_grad")
+    return out
+
+
+def sort_pairs(ids, n_modalities):
+    """(offsets int32 [E + 1], order int32 [P], position int32 of ids' shape) -- ``mtp_sort_pairs``."""
+    if not isinstance(ids, torch.Tensor):
+        raise TypeError(f"ids: expected a torch.Tensor, got {type(ids).__name__}")
+    _req(ids, "ids", torch.int32, align=4)
+    e = int(n_modalities)
+    if not 1 <= e <= MAX_MODALITIES:
+        raise ValueError(f"n_modalities={e} must be in [1, {MAX_MODALITIES}]")
+    pairs, dev = ids.numel(), ids.device
+    if pairs > 0x7fffffff:
+        raise ValueError(f"{pairs} pairs are more than 32-bit positions hold")
+    offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
+    order = torch.empty(pairs, dtype=torch.int32, device=dev)
+    position = torch.empty(ids.shape, dtype=torch.int32, device=dev)
+    ws_bytes = int(lib().mtp_sort_pairs_workspace_bytes(pairs, e))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with torch.cuda.device(dev):
+        check(lib().mtp_sort_pairs(ptr(ids), pairs, e, ptr(offsets), ptr(order), ptr(position), ptr(ws), ws_bytes,
+                                   stream_ptr()), "mtp_sort_pairs")
+    return offsets, order, position
+
+
+def _held(offsets):
+    return ctypes.c_void_p(offsets.data_ptr() + 4 * (offsets.numel() - 1))
+
+
+def dispatch_rows(x, position, offsets):
+    """rows [N * k, D]: x's rows at their pairs' places -- ``mtp_dispatch_rows``."""
+    _device_tensor(x, "x", 2)
+    code = _type_code(x, "x")
+    n, d = x.shape
+    _like(position, "position", 2, x, "x", torch.int32)
+    _like(offsets, "offsets", 1, x, "x", torch.int32)
+    if position.shape[0] != n:
+        raise ValueError(f"x has {n} rows, the pairs have {position.shape[0]}")
+    ld, k = _row_distance(x, "x"), position.shape[1]
+    rows = torch.empty((n * k, d), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        check(lib().mtp_dispatch_rows(code, ptr(x), n, d, ld, k, ptr(position), _held(offsets), ptr(rows), stream_ptr()),
+              "mtp_dispatch_rows")
+    return rows
+
+
+def combine_rows(rows, position, offsets, weights=None):
+    """[N, D]: each agent's rows summed with its weights (None: all one) -- ``mtp_combine_rows``."""
+    _device_tensor(rows, "rows", 2)
+    code = _type_code(rows, "rows")
+    _like(position, "position", 2, rows, "rows", torch.int32)
+    _like(offsets, "offsets", 1, rows, "rows", torch.int32)
+    n, k = position.shape
+    d = rows.shape[1]
+    _like(rows, "rows", 2, rows, "rows", shape=(n * k, d))
+    if weights is not None:
+        _like(weights, "weights", 2, rows, "rows", torch.float32, (n, k))
+    y = torch.empty((n, d), dtype=rows.dtype, device=rows.device)
+    with torch.cuda.device(rows.device):
+        check(lib().mtp_combine_rows(code, ptr(rows), n, d, k, ptr(position), _held(offsets), ptr(weights), ptr(y),
+                                     stream_ptr()), "mtp_combine_rows")
+    return y
+
+
+def combine_rows_grad(rows, grad, position, offsets, weights, want_rows=True, want_weights=True):
+    """(gradient of rows or None, of weights or None) from that of ``combine_rows``' result -- ``mtp_combine_rows_grad``."""
+    _device_tensor(rows, "rows", 2)
+    code = _type_code(rows, "rows")
+    _like(position, "position", 2, rows, "rows", torch.int32)
+    _like(offsets, "offsets", 1, rows, "rows", torch.int32)
+    n, k = position.shape
+    d = rows.shape[1]
+    _like(rows, "rows", 2, rows, "rows", shape=(n * k, d))
+    _like(grad, "grad", 2, rows, "rows", shape=(n, d))
+    _like(weights, "weights", 2, rows, "rows", torch.float32, (n, k))
+    grad_rows = torch.empty_like(rows) if want_rows else None
+    grad_weights = torch.empty_like(weights) if want_weights else None
+    with torch.cuda.device(rows.device):
+        check(lib().mtp_combine_rows_grad(code, ptr(rows), ptr(grad), n, d, k, ptr(position), _held(offsets), ptr(weights),
+                                          ptr(grad_rows), ptr(grad_weights), stream_ptr()), "mtp_combine_rows_grad")
+    return grad_rows, grad_weights
+
+
+def _act_code(activation):
+    code = _ACT_CODE.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be None, 'none', 'relu', 'gelu' or 'silu', got {activation!r}")
+    return code
+
+
+def _sets(weight, x, offsets):
+    """(number of weight matrices, out, in) of a weight [out, in], or [S, out, in] with offsets [S + 1]."""
+    _like(weight, "weight", 2 if offsets is None else 3, x, "x")
+    if offsets is None:
+        return 1, weight.shape[0], weight.shape[1]
+    _like(offsets, "offsets", 1, x, "x", torch.int32, (weight.shape[0] + 1,))
+    return weight.shape
+
+
+def _workspace(n_bytes, device):
+    return torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
+
+
+def linear(x, weight, bias=None, activation=None, residual=None, offsets=None, want_pre=False):
+    """(act(x weight^T + bias) + residual, x weight^T + bias or None) -- ``mtp_linear``."""
+    _device_tensor(x, "x", 2)
+    code, act = _type_code(x, "x"), _act_code(activation)
+    s, out, i = _sets(weight, x, offsets)
+    rows = x.shape[0]
+    if x.shape[1] != i:
+        raise ValueError(f"x has {x.shape[1]} features, weight takes {i}")
+    if not (1 <= i <= 65536 and 1 <= out <= 65536 and 1 <= s <= 65536):
+        raise ValueError(f"weight: sizes must be in [1, 65536], got shape {tuple(weight.shape)}")
+    ldx, ldr = _row_distance(x, "x"), 0
+    if bias is not None:
+        _like(bias, "bias", weight.dim() - 1, x, "x", shape=tuple(weight.shape[:-1]))
+    if residual is not None:
+        _device_tensor(residual, "residual", 2)
+        if residual.dtype != x.dtype or residual.device != x.device or tuple(residual.shape) != (rows, out):
+            raise ValueError(f"residual: expected {x.dtype} {(rows, out)} on {x.device}, got {residual.dtype} "
+                             f"{tuple(residual.shape)} on {residual.device}")
+        ldr = _row_distance(residual, "residual")
+    dev = x.device
+    y = torch.empty((rows, out), dtype=x.dtype, device=dev)
+    pre = torch.empty((rows, out), dtype=x.dtype, device=dev) if want_pre else None
+    px, pw = ptr(x), ptr(weight)
+    ws_bytes = int(lib().mtp_linear_workspace_bytes(code, _lib.LINEAR_FORWARD, rows, i, out, s, px, ldx, pw, i))
+    ws = _workspace(ws_bytes, dev)
+    with torch.cuda.device(dev):
+        check(lib().mtp_linear(code, px, rows, i, ldx, pw, out, ptr(bias), act, ptr(residual), ldr, ptr(offsets), s, ptr(y),
+                               ptr(pre), ptr(ws), ws_bytes, stream_ptr()), "mtp_linear")
+    return y, pre
+
+
+def linear_act_grad(grad, pre, activation, offsets=None):
+    """grad * act'(pre) [rows, out]; with a 16-bit type and an odd ``out`` a slice of rows padded to 16 bytes."""
+    _device_tensor(grad, "grad", 2)
+    code, act = _type_code(grad, "grad"), _act_code(activation)
+    rows, out = grad.shape
+    _like(grad, "grad", 2, grad, "grad")
+    _like(pre, "pre", 2, grad, "grad", shape=(rows, out))
+    s = 1
+    if offsets is not None:
+        _like(offsets, "offsets", 1, grad, "grad", torch.int32)
+        s = offsets.numel() - 1
+    ld = out if grad.element_size() == 4 or out % 2 == 0 else -(-out // 8) * 8
+    dz = torch.empty((rows, ld), dtype=grad.dtype, device=grad.device)
+    with torch.cuda.device(grad.device):
+        check(lib().mtp_linear_act_grad(code, ptr(grad), ptr(pre), rows, out, act, ptr(offsets), s, ptr(dz), ld, stream_ptr()),
+              "mtp_linear_act_grad")
+    return dz[:, :out]
+
+
+def linear_mask_rows(grad, offsets):
+    """A copy of grad [rows, out] with zeros behind the last set's rows."""
+    _device_tensor(grad, "grad", 2)
+    code = _type_code(grad, "grad")
+    _like(grad, "grad", 2, grad, "grad")
+    _like(offsets, "offsets", 1, grad, "grad", torch.int32)
+    dst = torch.empty_like(grad)
+    with torch.cuda.device(grad.device):
+        check(lib().mtp_linear_mask_rows(code, ptr(grad), grad.shape[0], grad.shape[1], ptr(offsets), offsets.numel() - 1,
+                                         ptr(dst), stream_ptr()), "mtp_linear_mask_rows")
+    return dst
+
+
+def linear_grad_input(dz, weight, offsets=None):
+    """dz weight [rows, in] -- ``mtp_linear_grad_input``."""
+    _device_tensor(dz, "dz", 2)
+    code = _type_code(dz, "dz")
+    s, out, i = _sets(weight, dz, offsets)
+    rows = dz.shape[0]
+    if dz.shape[1] != out:
+        raise ValueError(f"dz has {dz.shape[1]} columns, weight gives {out}")
+    ld = _row_distance(dz, "dz")
+    dx = torch.empty((rows, i), dtype=dz.dtype, device=dz.device)
+    pz, pw = ptr(dz), ptr(weight)
+    ws_bytes = int(lib().mtp_linear_workspace_bytes(code, _lib.LINEAR_GRAD_INPUT, rows, i, out, s, pz, ld, pw, i))
+    ws = _workspace(ws_bytes, dz.device)
+    with torch.cuda.device(dz.device):
+        check(lib().mtp_linear_grad_input(code, pz, rows, out, ld, pw, i, ptr(offsets), s, ptr(dx), ptr(ws), ws_bytes,
+                                          stream_ptr()), "mtp_linear_grad_input")
+    return dx
+
+
+def linear_grad_weight(dz, x, offsets=None, want_bias=False):
+    """(dz^T x [out, in] or [S, out, in], the column sums of dz or None) -- ``mtp_linear_grad_weight``."""
+    _device_tensor(dz, "dz", 2)
+    _device_tensor(x, "x", 2)
+    code = _type_code(dz, "dz")
+    rows, out = dz.shape
+    if x.dtype != dz.dtype or x.device != dz.device or x.shape[0] != rows:
+        raise ValueError(f"x: expected {dz.dtype} with {rows} rows on {dz.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    i = x.shape[1]
+    lead, s = (), 1
+    if offsets is not None:
+        _like(offsets, "offsets", 1, dz, "dz", torch.int32)
+        s = offsets.numel() - 1
+        lead = (s,)
+    ldz, ldx = _row_distance(dz, "dz"), _row_distance(x, "x")
+    dw = torch.empty(lead + (out, i), dtype=dz.dtype, device=dz.device)
+    db = torch.empty(lead + (out,), dtype=dz.dtype, device=dz.device) if want_bias else None
+    pz, px = ptr(dz), ptr(x)
+    ws_bytes = int(lib().mtp_linear_workspace_bytes(code, _lib.LINEAR_GRAD_WEIGHT, rows, i, out, s, pz, ldz, px, ldx))
+    ws = _workspace(ws_bytes, dz.device)
+    with torch.cuda.device(dz.device):
+        check(lib().mtp_linear_grad_weight(code, pz, rows, out, ldz, px, i, ldx, ptr(offsets), s, ptr(dw), ptr(db), ptr(ws),
+                                           ws_bytes, stream_ptr()), "mtp_linear_grad_weight")
+    return dw, db

@@ -1,0 +1,350 @@
+"""``pccs_accel.routing`` on the GPU against float64 formulas (routing_reference.py), and the routed layers as they run together."""
+import math
+
+import pytest
+import torch
+
+import routing_reference as R
+from pccs_accel import kernels as K
+from pccs_accel.layers import modality_linear
+from pccs_accel.routing import PairPlan, combine, dispatch, route_topk, sort_pairs
+
+pytestmark = pytest.mark.gpu
+
+# rows, modalities, k: one agent, every width of the kernel (64, 256, 512, 1024, 4096), few and many rows, k up to all
+ROUTES = [(1, 1, 1), (1, 200, 20), (3, 7, 7), (5, 64, 1), (1030, 5, 3), (1500, 64, 64), (1025, 65, 17), (1200, 200, 20), (900, 256, 128),
+          (1100, 257, 33), (1050, 400, 7), (1040, 1024, 128), (30, 1024, 8), (7, 1025, 5), (2, 4096, 128), (1024, 33, 32), (1026, 999, 16)]
+
+
+def _scores(seed, n, e, dtype):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, e, generator=g) * 2).to(dtype)
+
+
+def _route(dev, scores, k, normalize, g):
+    leaf = scores.to(dev).requires_grad_()
+    ids, w = route_topk(leaf, k, normalize=normalize)
+    assert ids.dtype == torch.int32 and w.dtype == torch.float32
+    ds, = torch.autograd.grad(w, leaf, g.to(dev))
+    plain_ids, plain_w = route_topk(scores.to(dev), k, normalize=normalize)
+    assert torch.equal(plain_ids, ids) and torch.equal(plain_w.nan_to_num(7), w.detach().nan_to_num(7))
+    return ids, w, ds
+
+
+def _check_route(dev, scores, k, normalize, seed=0):
+    g = torch.randn(scores.shape[0], k, generator=torch.Generator().manual_seed(seed))
+    want = R.route(scores, k, normalize, g)
+    ids, w, ds = _route(dev, scores, k, normalize, g)
+    assert torch.equal(ids.cpu(), want["ids"])
+    R.check("w", w, want["w"])
+    assert ds.dtype == scores.dtype
+    R.check("ds", ds, want["ds"])
+
+
+@pytest.mark.parametrize("dtype", R.TYPES, ids=str)
+@pytest.mark.parametrize("size", ROUTES, ids=str)
+def test_route_and_gradient(gpu_device, size, dtype):
+    n, e, k = size
+    for normalize in (False, True):
+        _check_route(gpu_device, _scores(n + e, n, e, dtype), k, normalize)
+
+
+@pytest.mark.parametrize("n", [3, 1100])
+def test_route_ties_go_to_the_lowest_index(gpu_device, n):
+    for dtype in R.TYPES:
+        g = torch.Generator().manual_seed(1)
+        scores = torch.randint(-2, 3, (n, 150), generator=g).to(dtype)
+        scores[0] = 0
+        scores[1, ::2] = -0.0  # equals +0
+        scores[1, 1::2] = 0.0
+        _check_route(gpu_device, scores, 40, True)
+        _check_route(gpu_device, scores, 40, False)
+
+
+@pytest.mark.parametrize("n", [6, 1200])
+def test_route_masked_rows(gpu_device, n):
+    for dtype in R.TYPES:
+        for normalize in (False, True):
+            scores = _scores(3, n, 90, dtype)
+            scores[0] = -math.inf                     # nothing allowed
+            scores[1, 5:] = -math.inf                 # fewer than k
+            scores[2] = torch.finfo(dtype).min        # lowest value: allowed, and a tie
+            scores[3, :] = -math.inf
+            scores[3, 77] = torch.finfo(dtype).max
+            _check_route(gpu_device, scores, 9, normalize)
+            ids, w = route_topk(scores.to(gpu_device), 9, normalize=normalize)
+            assert (ids[0] == -1).all() and (w[0] == 0).all() and (ids[1, 5:] == -1).all()
+            assert ids[3].tolist() == [77] + [-1] * 8 and w[3, 0] == 1
+
+
+def test_route_nan_and_infinity(gpu_device):
+    for n in (4, 1100):
+        for normalize in (False, True):
+            scores = _scores(4, n, 70, torch.float32)
+            scores[1, 3] = math.nan
+            scores[2, 8] = math.inf
+            ids, w = route_topk(scores.to(gpu_device), 70, normalize=normalize)
+            assert torch.isnan(w[1]).all() and 3 not in ids[1, :69].tolist() and ids[1, 69] == -1
+            assert ids[2, 0] == 8 and torch.isnan(w[2, 0])
+            keep = [0, 3]
+            assert torch.isfinite(w[keep]).all()
+
+
+def test_route_large_scores_keep_their_precision(gpu_device):
+    """Differences count, not sizes: scores around 30 000 in float32."""
+    scores = _scores(5, 40, 60, torch.float32) + 30000.0
+    for normalize in (False, True):
+        _check_route(gpu_device, scores, 12, normalize)
+
+
+def test_route_takes_a_slice_of_columns(gpu_device):
+    for dtype in R.TYPES:
+        wide = _scores(6, 1100, 131, dtype)
+        want = R.route(wide[:, 7:97], 5, True)
+        ids, w = route_topk(wide.to(gpu_device)[:, 7:97], 5)
+        assert torch.equal(ids.cpu(), want["ids"])
+        R.check("w", w, want["w"])
+
+
+def test_route_gradient_against_differences(gpu_device):
+    scores = _scores(8, 6, 30, torch.float32)
+    g = torch.randn(6, 4, generator=torch.Generator().manual_seed(2))
+    for normalize in (False, True):
+        ids, w, ds = _route(gpu_device, scores, 4, normalize, g)
+        ids = ids.cpu().long()
+        d = torch.randn(6, 30, generator=torch.Generator().manual_seed(3), dtype=torch.float64)
+
+        def value(h):
+            s = scores.double() + h * d
+            top = s.gather(1, ids)
+            return float((g.double() * torch.exp(top - torch.logsumexp(top if normalize else s, 1, keepdim=True))).sum())
+        slope = (value(1e-4) - value(-1e-4)) / 2e-4
+        err = float((R.route(scores, 4, normalize, g)["ds"][1] * d.abs()).sum())
+        # central differences: h^2 / 6 times the third derivative of a softmax along d (at most some 6 max|d|^3 sum|g|)
+        err += 1e-8 * float(d.abs().max()) ** 3 * float(g.abs().sum()) + 1e-10
+        assert abs(float((ds.cpu().double() * d).sum()) - slope) <= err
+
+
+PAIRS = [(0, 3, 5), (1, 1, 1), (1, 20, 200), (5, 3, 2), (63, 1, 4), (64, 1, 4), (65, 2, 7), (1000, 4, 300), (3000, 5, 200), (900, 8, 4096),
+         (5000, 4, 1), (17970, 4, 400), (40000, 3, 1024), (9000, 2, 4096)]
+
+
+@pytest.mark.parametrize("size", PAIRS, ids=str)
+def test_sort_pairs(gpu_device, size):
+    n, k, e = size
+    g = torch.Generator().manual_seed(n + e)
+    for low in (0, -1):
+        ids = torch.randint(low, e, (n, k), generator=g, dtype=torch.int32)
+        if low < 0 and n:
+            ids[n // 2] = e + 3  # out of range counts as none
+        key = ids.reshape(-1).long()
+        key = torch.where((key < 0) | (key >= e), torch.full_like(key, e), key)
+        order = torch.sort(key, stable=True).indices
+        position = torch.empty_like(order)
+        position[order] = torch.arange(n * k)
+        plan = sort_pairs(ids.to(gpu_device), e)
+        offsets = torch.cat([torch.zeros(1).long(), torch.bincount(key, minlength=e + 1)[:e].cumsum(0)])
+        assert torch.equal(plan.offsets.cpu().long(), offsets)
+        assert torch.equal(plan.order.cpu().long(), order)
+        assert torch.equal(plan.position.cpu().long(), position.view(n, k))
+
+
+def _plan(seed, n, k, e, none=0.0):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, e, (n, k), generator=g, dtype=torch.int32)
+    ids[torch.rand(n, k, generator=g) < none] = -1
+    return ids
+
+
+@pytest.mark.parametrize("dtype", R.TYPES, ids=str)
+@pytest.mark.parametrize("size", [(1, 1, 1, 3), (1, 20, 96, 200), (7, 3, 33, 5), (50, 2, 8, 4), (129, 4, 96, 30), (40, 5, 130, 9),
+                                  (700, 20, 48, 200), (33, 2, 1024, 6), (2000, 1, 64, 50), (3, 4, 520, 7)], ids=str)
+def test_rows_there_and_back(gpu_device, size, dtype):
+    n, k, d, e = size
+    u = R.half_step(dtype)
+    for none in (0.0, 0.3):
+        ids = _plan(n + d, n, k, e, none)
+        plan = sort_pairs(ids.to(gpu_device), e)
+        g = torch.Generator().manual_seed(d)
+        x = torch.randn(n, d, generator=g).to(dtype)
+        rows = torch.randn(n * k, d, generator=g).to(dtype)
+        w = torch.rand(n, k, generator=g)
+        g_rows, g_y = torch.randn(n * k, d, generator=g).to(dtype), torch.randn(n, d, generator=g).to(dtype)
+        here = plan.position.cpu().long()
+        there = ((ids >= 0) & (ids < e)).double()
+
+        xd = x.to(gpu_device).requires_grad_()
+        out = dispatch(xd, plan)
+        want = torch.zeros(n * k, d, dtype=dtype)
+        want[here.reshape(-1)] = (x.double()[:, None, :] * there[:, :, None]).reshape(-1, d).to(dtype)
+        assert torch.equal(out.cpu(), want)
+        dx, = torch.autograd.grad(out, xd, g_rows.to(gpu_device))
+        terms = g_rows.double()[here] * there[:, :, None]
+        v, e32 = terms.sum(1), (k + 2) * R.U32 * terms.abs().sum(1)
+        R.check("dx", dx, (v, e32 + u * (v.abs() + e32) + R.floor_of(dtype)))
+
+        rd, wd = rows.to(gpu_device).requires_grad_(), w.to(gpu_device).requires_grad_()
+        y = combine(rd, plan, wd)
+        terms = rows.double()[here] * (w.double() * there)[:, :, None]
+        v, e32 = terms.sum(1), (k + 2) * R.U32 * terms.abs().sum(1)
+        R.check("y", y, (v, e32 + u * (v.abs() + e32) + R.floor_of(dtype)))
+        dr, dw = torch.autograd.grad(y, [rd, wd], g_y.to(gpu_device))
+        back = torch.zeros(n * k, d, dtype=torch.float64)
+        back[here.reshape(-1)] = ((w.double() * there)[:, :, None] * g_y.double()[:, None, :]).reshape(-1, d)
+        R.check("drows", dr, (back, (u + 2 * R.U32) * back.abs() + R.floor_of(dtype)))
+        prod = rows.double()[here] * g_y.double()[:, None, :] * there[:, :, None]
+        R.check("dw", dw, (prod.sum(2), (d + 2) * R.U32 * prod.abs().sum(2)))
+
+        rd = rows.to(gpu_device).requires_grad_()
+        y = combine(rd, plan)
+        terms = rows.double()[here] * there[:, :, None]
+        v, e32 = terms.sum(1), (k + 2) * R.U32 * terms.abs().sum(1)
+        R.check("sum", y, (v, e32 + u * (v.abs() + e32) + R.floor_of(dtype)))
+        dr, = torch.autograd.grad(y, rd, g_y.to(gpu_device))
+        back = torch.zeros(n * k, d, dtype=dtype)
+        back[here.reshape(-1)] = (g_y.double()[:, None, :] * there[:, :, None]).reshape(-1, d).to(dtype)
+        assert torch.equal(dr.cpu(), back)
+
+
+def test_rows_from_a_slice_and_without_agents(gpu_device):
+    plan = sort_pairs(_plan(1, 40, 3, 6).to(gpu_device), 6)
+    wide = torch.randn(40, 70, generator=torch.Generator().manual_seed(1)).to(gpu_device)
+    for start in (0, 1, 4):
+        assert torch.equal(dispatch(wide[:, start:start + 48], plan), dispatch(wide[:, start:start + 48].contiguous(), plan))
+    empty = sort_pairs(torch.empty(0, 3, dtype=torch.int32, device=gpu_device), 6)
+    assert dispatch(wide[:0], empty).shape == (0, 70) and combine(wide[:0], empty, wide[:0, :3].contiguous()).shape == (0, 70)
+
+
+def test_rows_that_nobody_answers_may_hold_anything(gpu_device):
+    """NaN behind the last modality's rows does not reach a sum or a gradient."""
+    ids = _plan(2, 30, 4, 5, none=0.5)
+    plan = sort_pairs(ids.to(gpu_device), 5)
+    rows = torch.randn(120, 24, generator=torch.Generator().manual_seed(2)).to(gpu_device)
+    held = int(plan.offsets[-1])
+    clean = combine(rows, plan, torch.ones(30, 4, device=gpu_device))
+    rows[held:] = math.nan
+    w = torch.ones(30, 4, device=gpu_device, requires_grad=True)
+    leaf = rows.clone().requires_grad_()
+    y = combine(leaf, plan, w)
+    assert torch.equal(y, clean)
+    dr, dw = torch.autograd.grad(y, [leaf, w], torch.ones_like(y))
+    assert torch.isfinite(dr).all() and torch.isfinite(dw).all() and not dr[held:].any()
+
+
+def _layer(scores, x, w1, b1, w2, b2, k):
+    """Two layers per modality over each agent's k modalities, averaged with the router's weights."""
+    ids, w = route_topk(scores, k)
+    plan = sort_pairs(ids, scores.shape[1])
+    hidden = modality_linear(dispatch(x, plan), plan.offsets, w1, b1, activation="gelu")
+    return combine(modality_linear(hidden, plan.offsets, w2, b2), plan, w)
+
+
+def _layer_inputs(n, e, d, h, o, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(n, e, generator=g) * 2).to(dtype), torch.tanh(torch.randn(n, d, generator=g)).to(dtype),
+            (torch.randn(e, h, d, generator=g) / d ** 0.5).to(dtype), (torch.randn(e, h, generator=g) * 0.1).to(dtype),
+            (torch.randn(e, o, h, generator=g) / h ** 0.5).to(dtype), (torch.randn(e, o, generator=g) * 0.1).to(dtype)]
+
+
+@pytest.mark.parametrize("dtype", R.TYPES, ids=str)
+@pytest.mark.parametrize("size", [(1, 200, 4, 96, 64, 24), (37, 12, 3, 17, 33, 5), (500, 20, 6, 48, 64, 24)], ids=str)
+def test_routed_layers_together(gpu_device, size, dtype):
+    n, e, k, d, h, o = size
+    inputs = _layer_inputs(n, e, d, h, o, dtype)
+    inputs[0][n // 2, 2:] = -math.inf  # an agent with two modalities left
+    gy = torch.randn(n, o, generator=torch.Generator().manual_seed(5)).to(dtype)
+    exact = [t.double().requires_grad_() for t in inputs]
+    s, x, w1, b1, w2, b2 = exact
+    ids = R.route(inputs[0], k, True)["ids"].long()
+    y = 0
+    top = s.gather(1, ids.clamp_min(0)).masked_fill(ids < 0, -math.inf)
+    weight = torch.softmax(top, 1)
+    for j in range(k):
+        e_j = ids[:, j].clamp_min(0)
+        hidden = R.act(torch.einsum("nd,nhd->nh", x, w1[e_j]) + b1[e_j], "gelu")
+        y = y + (weight[:, j] * (ids[:, j] >= 0))[:, None] * (torch.einsum("nh,noh->no", hidden, w2[e_j]) + b2[e_j])
+    want = torch.autograd.grad(y, exact, gy.double())
+    leaves = [t.to(gpu_device).requires_grad_() for t in inputs]
+    out = _layer(*leaves, k)
+    got = torch.autograd.grad(out, leaves, gy.to(gpu_device))
+    # each of the (at most ten) tensors between the inputs and a gradient is rounded to the type once, float32 sums of at most
+    # n * k terms on the way: 2-norm of the error against the 2-norm of the result, roundings added up, twice over for cancellation
+    most = 2 * (10 * R.half_step(dtype) + 4 * (n * k + d + h) * R.U32)
+    for name, a, c in zip(("y", "scores", "x", "w1", "b1", "w2", "b2"), (out,) + got, (y,) + want):
+        a, c = a.detach().cpu().double(), c.detach()
+        assert float((a - c).norm()) <= most * float(c.norm()), (name, float((a - c).norm() / c.norm()), most)
+
+
+def test_routed_layers_in_graphs_and_streams(gpu_device):
+    """Two captured graphs replayed in turn with eager work between, and two streams at once."""
+    base = [t.to(gpu_device) for t in _layer_inputs(300, 50, 32, 40, 24, torch.bfloat16)]
+    gy = torch.randn(300, 24, generator=torch.Generator().manual_seed(5)).to(gpu_device).to(torch.bfloat16)
+
+    def step(inputs):
+        leaves = [t.detach().requires_grad_() for t in inputs]
+        y = _layer(*leaves, 5)
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, gy))
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        static = [t.clone() for t in base]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(static)
+        graphs.append((graph, static, outs))
+    for turn in range(4):
+        for graph, static, outs in graphs:
+            for t, src in zip(static, base):
+                t.copy_(src * (1 - 0.2 * turn))
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, c in zip(outs, step([t.clone() for t in static])):
+                assert torch.equal(a, c)
+    want = step(base)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(step(base))
+    torch.cuda.synchronize()
+    for outs in got:
+        for a, c in zip(outs, want):
+            assert torch.equal(a, c)
+
+
+def test_refusals(gpu_device):
+    d = gpu_device
+    s = torch.zeros(4, 9, device=d)
+    ids = torch.zeros(4, 2, dtype=torch.int32, device=d)
+    plan = sort_pairs(ids, 9)
+    for call, error in [
+        (lambda: route_topk(s.cpu(), 2), K._lib.MtpError),
+        (lambda: route_topk(s.double(), 2), TypeError),
+        (lambda: route_topk(s[0], 2), ValueError),
+        (lambda: route_topk(s, 0), ValueError),
+        (lambda: route_topk(s, 10), ValueError),
+        (lambda: route_topk(torch.zeros(2, 300, device=d), 129), ValueError),
+        (lambda: route_topk(torch.zeros(2, 4097, device=d), 2), ValueError),
+        (lambda: route_topk(s.T, 2), ValueError),
+        (lambda: route_topk(s[:1].expand(4, 9), 2), ValueError),
+        (lambda: sort_pairs(ids.long(), 9), TypeError),
+        (lambda: sort_pairs(ids.cpu(), 9), K._lib.MtpError),
+        (lambda: sort_pairs(ids[:, :1], 9), ValueError),
+        (lambda: sort_pairs(ids.view(-1), 9), ValueError),
+        (lambda: sort_pairs(ids, 0), ValueError),
+        (lambda: sort_pairs(ids, 4097), ValueError),
+        (lambda: dispatch(s[:3], plan), ValueError),
+        (lambda: dispatch(s.long(), plan), TypeError),
+        (lambda: combine(s, plan), ValueError),
+        (lambda: combine(torch.zeros(8, 9, device=d), plan, torch.zeros(4, 3, device=d)), ValueError),
+        (lambda: combine(torch.zeros(8, 9, device=d), plan, torch.zeros(4, 2, device=d).half()), TypeError),
+        (lambda: combine(torch.zeros(9, 8, device=d).T, plan), ValueError),
+        (lambda: combine(torch.zeros(8, 9, device=d), PairPlan(plan.offsets.long(), plan.order, plan.position)), TypeError),
+    ]:
+        with pytest.raises(error):
+            call()
