@@ -176,6 +176,24 @@ int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int
     return launch_product<T, LIN_FORWARD>(a, s);
 }
 
+// where the parts of a backward pass lie in the workspace: dz, then what the products need one after the other
+struct BackwardPlan {
+    int64_t lddz, dz_bytes, input_bytes, weight_bytes;
+    int64_t total() const { return dz_bytes + (input_bytes > weight_bytes ? input_bytes : weight_bytes); }
+};
+BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g, const void *w, const void *x,
+                           int64_t ldx, bool want_x, bool want_w) {
+    BackwardPlan p{};
+    // dz has rows of its own, so they can start where the loads want them
+    const bool own = act != LIN_NONE;
+    p.lddz = own && elem_size(dtype) == 2 && out % 2 != 0 ? round_up(out, 8) : out;
+    p.dz_bytes = own ? round_up(rows * p.lddz * elem_size(dtype), 256) : 0;
+    const void *dz = own ? nullptr : g;
+    if (want_x) p.input_bytes = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_GRAD_INPUT, rows, in, out, n_sets, dz, p.lddz, w, in);
+    if (want_w) p.weight_bytes = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_GRAD_WEIGHT, rows, in, out, n_sets, dz, p.lddz, x, ldx);
+    return p;
+}
+
 template <typename T>
 int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, const int32_t *offsets, int n_sets,
                void *dx, char *ws, hipStream_t s) {
@@ -337,4 +355,39 @@ extern "C" int mtp_linear_grad_weight(int dtype, const void *dz, int64_t rows, i
     }
     return MTP_BY_TYPE(dtype, grad_weight)(dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db,
                                            reinterpret_cast<char *>(ws), mtp_stream(stream));
+}
+
+extern "C" int64_t mtp_linear_backward_workspace_bytes(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g,
+                                                       const void *w, const void *x, int64_t ldx, int want_x, int want_w) {
+    if (rows < 0 || in < 1 || out < 1 || n_sets < 1) return 0;
+    return plan_backward(dtype, rows, in, out, n_sets, act, g, w, x, ldx, want_x != 0, want_w != 0).total();
+}
+
+extern "C" int mtp_linear_backward(int dtype, const void *g, const void *pre, int act, const void *x, int64_t rows, int in,
+                                   int64_t ldx, const void *w, int out, const int32_t *offsets, int n_sets, void *dx, void *dw,
+                                   void *db, void *ws, size_t ws_bytes, void *stream) {
+    int rc = check_sizes("mtp_linear_backward", dtype, rows, in, out, offsets, n_sets);
+    if (rc != MTP_OK) return rc;
+    MTP_REQUIRE(dx || dw, "mtp_linear_backward: nothing is asked for");
+    MTP_REQUIRE(db == nullptr || dw != nullptr, "mtp_linear_backward: the bias' gradient comes with the weight's");
+    const BackwardPlan p = plan_backward(dtype, rows, in, out, n_sets, act, g, w, x, ldx, dx != nullptr, dw != nullptr);
+    if ((int64_t)ws_bytes < p.total() || (p.total() > 0 && ws == nullptr)) {
+        mtp_set_error("mtp_linear_backward: workspace of %zu bytes, needs %lld", ws_bytes, (long long)p.total());
+        return MTP_E_WORKSPACE;
+    }
+    char *rest = reinterpret_cast<char *>(ws) + p.dz_bytes;
+    const void *dz = g;
+    if (act != LIN_NONE) {
+        rc = mtp_linear_act_grad(dtype, g, pre, rows, out, act, offsets, n_sets, ws, p.lddz, stream);
+        if (rc != MTP_OK) return rc;
+        dz = ws;
+    }
+    if (dx != nullptr) {
+        rc = mtp_linear_grad_input(dtype, dz, rows, out, p.lddz, w, in, offsets, n_sets, dx, rest, (size_t)p.input_bytes, stream);
+        if (rc != MTP_OK) return rc;
+    }
+    if (dw != nullptr)
+        rc = mtp_linear_grad_weight(dtype, dz, rows, out, p.lddz, x, in, ldx, offsets, n_sets, dw, db, rest, (size_t)p.weight_bytes,
+                                    stream);
+    return rc;
 }

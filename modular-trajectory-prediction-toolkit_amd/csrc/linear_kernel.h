@@ -276,18 +276,47 @@ __device__ __forceinline__ bool lin_find_tile(const int32_t *offsets, int n_sets
 
 enum { LIN_NONE = 0, LIN_RELU = 1, LIN_GELU = 2, LIN_SILU = 3 };
 
+// 0.5 erfc(|z| / sqrt 2) = 0.5 exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.4 |z| / sqrt 2): the form of Hastings' approximations
+// (Abramowitz and Stegun 7.1.26), P of degree 5 fitted here to 3e-8; evaluated in float it is off by at most 2e-7.  *e
+// receives exp(-z^2 / 2), which the slope needs too.
+__device__ __forceinline__ float lin_gauss_tail(float z, float *e) {
+    *e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.28284271247461901f, 1.f));
+    float p = fmaf(t, -0.20033471286296844f, 0.7094687819480896f);
+    p = fmaf(t, p, -0.37145283818244934f);
+    p = fmaf(t, p, 0.46873366832733154f);
+    p = fmaf(t, p, 0.16163088381290436f);
+    p = fmaf(t, p, 0.23195423185825348f);
+    return 0.5f * *e * t * p;
+}
+// the standard normal distribution function
+__device__ __forceinline__ float lin_gauss(float z, float *e) {
+    const float tail = lin_gauss_tail(z, e);
+    return z < 0.f ? tail : 1.f - tail;
+}
+__device__ __forceinline__ float lin_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+
 __device__ __forceinline__ float lin_act(float z, int act) {
     if (act == LIN_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-    if (act == LIN_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    if (act == LIN_SILU) return z / (1.f + expf(-z));
+    if (act == LIN_GELU) {
+        float e;
+        return z * lin_gauss(z, &e);
+    }
+    if (act == LIN_SILU) return z * lin_sigmoid(z);
     return z;
 }
 __device__ __forceinline__ float lin_slope(float z, int act) {
     if (act == LIN_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
-    if (act == LIN_GELU) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    if (act == LIN_GELU) {
+        float e;
+        const float c = lin_gauss(z, &e);
+        return fmaf(z * 0.39894228040143268f, e, c);
+    }
     if (act == LIN_SILU) {
-        const float q = 1.f / (1.f + expf(-z));
-        return q * (1.f + z * (1.f - q));
+        const float q = lin_sigmoid(z);
+        return q * fmaf(z, 1.f - q, 1.f);
     }
     return 1.f;
 }
@@ -310,36 +339,32 @@ struct LinArgs {
     float *partial;  // weight gradient with splits > 1: [splits][n_sets][out_rows][cols] then [splits][n_sets][out_rows]
 };
 
-// four consecutive columns of one output row
-template <typename T>
-__device__ __forceinline__ void lin_store4(T *p, const float *v, int n, bool whole) {
-    if (whole) {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 w;
+// N consecutive elements
+template <typename T, int N>
+__device__ __forceinline__ void lin_store(T *p, const float *v) {
+    if constexpr (N == 1) *p = from_f32<T>(v[0]);
+    else {
+        typedef T tn __attribute__((ext_vector_type(N)));
+        tn w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(v[e]);
-        *reinterpret_cast<t4 *>(p) = w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < n) p[e] = from_f32<T>(v[e]);
+        for (int e = 0; e < N; ++e) w[e] = from_f32<T>(v[e]);
+        *reinterpret_cast<tn *>(p) = w;
     }
 }
-template <typename T>
-__device__ __forceinline__ void lin_load4(const T *p, float *v, int n, bool whole) {
-    if (whole) {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        const t4 w = *reinterpret_cast<const t4 *>(p);
+template <typename T, int N>
+__device__ __forceinline__ void lin_load(const T *p, float *v) {
+    if constexpr (N == 1) v[0] = to_f32(*p);
+    else {
+        typedef T tn __attribute__((ext_vector_type(N)));
+        const tn w = *reinterpret_cast<const tn *>(p);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = to_f32(w[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(p[e]) : 0.f;
+        for (int e = 0; e < N; ++e) v[e] = to_f32(w[e]);
     }
 }
+// 16-byte pieces: the address and the row distance allow them
 template <typename T>
-__device__ __forceinline__ bool lin_aligned4(const void *p, int64_t ld) {
-    return ((uintptr_t)p % (4 * sizeof(T)) == 0) && (ld % 4 == 0);
+__device__ __forceinline__ bool lin_aligned16(const void *p, int64_t ld) {
+    return (uintptr_t)p % 16 == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
 }
 
 // Consecutive workgroups go to different XCDs in turn: each XCD gets one contiguous run of tiles, so that the tiles that share
@@ -350,6 +375,65 @@ __device__ __forceinline__ int64_t lin_xcd_order(int64_t id, int64_t n) {
 }
 
 enum { LIN_FORWARD = 0, LIN_GRAD_INPUT = 1, LIN_GRAD_WEIGHT = 2 };
+
+// A tile's rows on their way out of LDS, N columns a thread; U is the type they leave in.
+template <typename T, typename U, int MODE, int BC, int ER, int NT, int N>
+__device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, U *to, int set, int64_t r0, int64_t row_end, int64_t c0,
+                                          int tid) {
+    constexpr int ITEMS = BC / N, STEP = NT / ITEMS;  // items of a row; rows that the workgroup takes at a time
+    constexpr int PM = (BC / 4 < 32 ? BC / 4 : 32) - 1;
+    const int item = tid % ITEMS;
+    const int64_t col = c0 + item * N;
+    if (col >= a.cols) return;  // (16-byte pieces: cols is a multiple of N)
+    float bias[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) bias[e] = 0.f;
+    if constexpr (MODE == LIN_FORWARD) {
+        if (a.bias != nullptr) {
+            const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols + col;
+#pragma unroll
+            for (int e = 0; e < N; ++e) bias[e] = to_f32(b[e]);
+        }
+    }
+    for (int row = tid / ITEMS; row < ER; row += STEP) {
+        const int64_t r = r0 + row;
+        if (r >= row_end) break;
+        float v[N];
+        if constexpr (N == 1) {
+            v[0] = z[row * BC + (((item >> 2) ^ (row & PM)) << 2) + (item & 3)];
+        } else {
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q) {
+                const f32x4v w = *reinterpret_cast<const f32x4v *>(z + row * BC + (((item * (N / 4) + q) ^ (row & PM)) << 2));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[q * 4 + e] = w[e];
+            }
+        }
+        const int64_t at = r * a.cols + col;
+        if constexpr (MODE == LIN_FORWARD) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] += bias[e];
+            if (a.pre != nullptr) lin_store<T, N>(reinterpret_cast<T *>(a.pre) + at, v);
+            if (a.act == LIN_GELU) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = lin_act(v[e], LIN_GELU);
+            } else if (a.act == LIN_SILU) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = lin_act(v[e], LIN_SILU);
+            } else if (a.act == LIN_RELU) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = lin_act(v[e], LIN_RELU);
+            }
+            if (a.residual != nullptr) {
+                float res[N];
+                lin_load<T, N>(reinterpret_cast<const T *>(a.residual) + r * a.ld_res + col, res);
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] += res[e];
+            }
+        }
+        lin_store<U, N>(to + at, v);
+    }
+}
 
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
 __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinArgs a) {
@@ -496,62 +580,49 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
         }
     }
 
-    // ---- epilogue: lane (i, h) holds row i of a fragment, columns 8 g + 4 h + 0..3 for g = 0..3 ----
+    // ---- epilogue ----
+    // lane (i, h) holds row i of a fragment, columns 8 g + 4 h + 0..3 for g = 0..3: stored from there a wave would touch 32 rows
+    // with 16 bytes each.  The sums go through LDS (as floats, pieces of 16 bytes placed at p ^ row so that neither side
+    // conflicts), and whole rows of the tile leave in 16-byte pieces; bias, activation and residual are applied on the way.
     const int i = lane & 31, h = lane >> 5;
-    const bool vec = lin_aligned4<T>(out, a.cols);
-    const bool vec_res = MODE == LIN_FORWARD && a.residual != nullptr && lin_aligned4<T>(a.residual, a.ld_res);
-    const bool vec_pre = MODE == LIN_FORWARD && a.pre != nullptr && lin_aligned4<T>(a.pre, a.cols);
+    constexpr int ER = 2 * STAGE / (BC * 4) < BR ? 2 * STAGE / (BC * 4) : BR;  // rows per pass
+    constexpr int PM = (BC / 4 < 32 ? BC / 4 : 32) - 1;
+    static_assert(BR % ER == 0 && ER % WR == 0, "a wave's rows are in one pass");
+    float *z = reinterpret_cast<float *>(smem);
+    const bool to_partial = MODE == LIN_GRAD_WEIGHT && a.splits > 1;
+    bool vec = lin_aligned16<T>(a.out, a.cols);
+    if constexpr (MODE == LIN_FORWARD) {
+        if (a.residual != nullptr) vec = vec && lin_aligned16<T>(a.residual, a.ld_res);
+        if (a.pre != nullptr) vec = vec && lin_aligned16<T>(a.pre, a.cols);
+    }
+    if (to_partial) vec = a.cols % 4 == 0;
+    for (int p0 = 0; p0 < BR; p0 += ER) {
+        __syncthreads();
+        if (wr * WR >= p0 && wr * WR < p0 + ER) {
 #pragma unroll
-    for (int c = 0; c < FC; ++c) {
+            for (int c = 0; c < FC; ++c)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int64_t col = c0 + wc * WC + c * 32 + 8 * g + 4 * h;
-            const int n = (int)(a.cols - col < 4 ? a.cols - col : 4);
-            if (n <= 0) continue;
-            float bias[4] = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (MODE == LIN_FORWARD) {
-                if (a.bias != nullptr) {
-                    const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols + col;
+                for (int r = 0; r < FR; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < n) bias[e] = to_f32(b[e]);
-                }
-            }
+                    for (int g = 0; g < 4; ++g) {
+                        const int row = wr * WR - p0 + r * 32 + i;
+                        const int piece = (wc * WC + c * 32 + 8 * g + 4 * h) >> 2;
+                        f32x4v v;
 #pragma unroll
-            for (int r = 0; r < FR; ++r) {
-                const int64_t row = row0 + wr * WR + r * 32 + i;
-                if (row >= row_end) continue;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[c][r][4 * g + e];
-                if constexpr (MODE == LIN_FORWARD) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += bias[e];
-                    if (a.pre != nullptr)
-                        lin_store4(reinterpret_cast<T *>(a.pre) + row * a.cols + col, v, n, vec_pre && n == 4);
-                    if (a.act != LIN_NONE) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = lin_act(v[e], a.act);
+                        for (int e = 0; e < 4; ++e) v[e] = acc[c][r][4 * g + e];
+                        *reinterpret_cast<f32x4v *>(z + row * BC + ((piece ^ (row & PM)) << 2)) = v;
                     }
-                    if (a.residual != nullptr) {
-                        float res[4];
-                        lin_load4(reinterpret_cast<const T *>(a.residual) + row * a.ld_res + col, res, n, vec_res && n == 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += res[e];
-                    }
-                }
-                if constexpr (MODE == LIN_GRAD_WEIGHT) {
-                    const int64_t at = ((int64_t)set * a.out_rows + row) * a.cols + col;
-                    if (a.splits > 1) {
-                        lin_store4(a.partial + (int64_t)split * a.n_sets * a.out_rows * a.cols + at, v, n,
-                                   a.cols % 4 == 0 && n == 4);
-                    } else {
-                        lin_store4(out + at, v, n, vec && n == 4);
-                    }
-                } else {
-                    lin_store4(out + row * a.cols + col, v, n, vec && n == 4);
-                }
-            }
+        }
+        __syncthreads();
+        const int64_t r0 = row0 + p0;
+        if (to_partial) {
+            float *part = a.partial + ((int64_t)split * a.n_sets + set) * a.out_rows * a.cols;
+            if (vec) lin_leave<T, float, MODE, BC, ER, NT, 4>(a, z, part, set, r0, row_end, c0, tid);
+            else lin_leave<T, float, MODE, BC, ER, NT, 1>(a, z, part, set, r0, row_end, c0, tid);
+        } else {
+            T *to = out + (MODE == LIN_GRAD_WEIGHT ? (int64_t)set * a.out_rows * a.cols : 0);
+            if (vec) lin_leave<T, T, MODE, BC, ER, NT, 16 / SZ>(a, z, to, set, r0, row_end, c0, tid);
+            else lin_leave<T, T, MODE, BC, ER, NT, 1>(a, z, to, set, r0, row_end, c0, tid);
         }
     }
     if constexpr (MODE == LIN_GRAD_WEIGHT) {

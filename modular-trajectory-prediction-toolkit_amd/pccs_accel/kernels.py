@@ -421,6 +421,26 @@ _ACT_CODE = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 MAX_MODALITIES, MAX_TOPK = 4096, 128  # mtp_accel.h
 
 
+# The stream's handle without a Stream object around it: these calls are a few microseconds long in all.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _call(device, name, *args):
+    """Entry point ``name`` on ``device``'s current stream; raises on an error code."""
+    fn, i = getattr(lib(), name), device.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc != 0:
+        check(rc, name)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def _device_tensor(t, name, ndim):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
@@ -479,9 +499,7 @@ def route_topk(scores, k, normalize=True, want_stats=False):
     ids = torch.empty((n, k), dtype=torch.int32, device=dev)
     weights = torch.empty((n, k), dtype=torch.float32, device=dev)
     stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if want_stats else None
-    with torch.cuda.device(dev):
-        check(lib().mtp_route_topk(code, ptr(scores), n, e, ld, k, int(bool(normalize)), ptr(ids), ptr(weights), ptr(stats),
-                                   stream_ptr()), "mtp_route_topk")
+    _call(dev, "mtp_route_topk", code, _at(scores), n, e, ld, k, int(bool(normalize)), _at(ids), _at(weights), _at(stats))
     return ids, weights, stats
 
 
@@ -498,9 +516,8 @@ def route_topk_grad(scores, ids, weights, stats, grad, normalize=True):
     _like(grad, "grad", 2, scores, "scores", torch.float32, (n, k))
     ld = _row_distance(scores, "scores")
     out = torch.empty((n, e), dtype=scores.dtype, device=scores.device)
-    with torch.cuda.device(scores.device):
-        check(lib().mtp_route_topk_grad(code, ptr(scores), n, e, ld, k, int(bool(normalize)), ptr(ids), ptr(weights),
-                                        ptr(stats), ptr(grad), ptr(out), stream_ptr()), "mtp_route_topk_grad")
+    _call(scores.device, "mtp_route_topk_grad", code, _at(scores), n, e, ld, k, int(bool(normalize)), _at(ids), _at(weights),
+          _at(stats), _at(grad), _at(out))
     return out
 
 
@@ -520,14 +537,12 @@ def sort_pairs(ids, n_modalities):
     position = torch.empty(ids.shape, dtype=torch.int32, device=dev)
     ws_bytes = int(lib().mtp_sort_pairs_workspace_bytes(pairs, e))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with torch.cuda.device(dev):
-        check(lib().mtp_sort_pairs(ptr(ids), pairs, e, ptr(offsets), ptr(order), ptr(position), ptr(ws), ws_bytes,
-                                   stream_ptr()), "mtp_sort_pairs")
+    _call(dev, "mtp_sort_pairs", _at(ids), pairs, e, _at(offsets), _at(order), _at(position), _at(ws), ws_bytes)
     return offsets, order, position
 
 
 def _held(offsets):
-    return ctypes.c_void_p(offsets.data_ptr() + 4 * (offsets.numel() - 1))
+    return offsets.data_ptr() + 4 * (offsets.numel() - 1)
 
 
 def dispatch_rows(x, position, offsets):
@@ -541,9 +556,7 @@ def dispatch_rows(x, position, offsets):
         raise ValueError(f"x has {n} rows, the pairs have {position.shape[0]}")
     ld, k = _row_distance(x, "x"), position.shape[1]
     rows = torch.empty((n * k, d), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().mtp_dispatch_rows(code, ptr(x), n, d, ld, k, ptr(position), _held(offsets), ptr(rows), stream_ptr()),
-              "mtp_dispatch_rows")
+    _call(x.device, "mtp_dispatch_rows", code, _at(x), n, d, ld, k, _at(position), _held(offsets), _at(rows))
     return rows
 
 
@@ -559,9 +572,7 @@ def combine_rows(rows, position, offsets, weights=None):
     if weights is not None:
         _like(weights, "weights", 2, rows, "rows", torch.float32, (n, k))
     y = torch.empty((n, d), dtype=rows.dtype, device=rows.device)
-    with torch.cuda.device(rows.device):
-        check(lib().mtp_combine_rows(code, ptr(rows), n, d, k, ptr(position), _held(offsets), ptr(weights), ptr(y),
-                                     stream_ptr()), "mtp_combine_rows")
+    _call(rows.device, "mtp_combine_rows", code, _at(rows), n, d, k, _at(position), _held(offsets), _at(weights), _at(y))
     return y
 
 
@@ -578,9 +589,8 @@ def combine_rows_grad(rows, grad, position, offsets, weights, want_rows=True, wa
     _like(weights, "weights", 2, rows, "rows", torch.float32, (n, k))
     grad_rows = torch.empty_like(rows) if want_rows else None
     grad_weights = torch.empty_like(weights) if want_weights else None
-    with torch.cuda.device(rows.device):
-        check(lib().mtp_combine_rows_grad(code, ptr(rows), ptr(grad), n, d, k, ptr(position), _held(offsets), ptr(weights),
-                                          ptr(grad_rows), ptr(grad_weights), stream_ptr()), "mtp_combine_rows_grad")
+    _call(rows.device, "mtp_combine_rows_grad", code, _at(rows), _at(grad), n, d, k, _at(position), _held(offsets),
+          _at(weights), _at(grad_rows), _at(grad_weights))
     return grad_rows, grad_weights
 
 
@@ -626,12 +636,11 @@ def linear(x, weight, bias=None, activation=None, residual=None, offsets=None, w
     dev = x.device
     y = torch.empty((rows, out), dtype=x.dtype, device=dev)
     pre = torch.empty((rows, out), dtype=x.dtype, device=dev) if want_pre else None
-    px, pw = ptr(x), ptr(weight)
+    px, pw = _at(x), _at(weight)
     ws_bytes = int(lib().mtp_linear_workspace_bytes(code, _lib.LINEAR_FORWARD, rows, i, out, s, px, ldx, pw, i))
     ws = _workspace(ws_bytes, dev)
-    with torch.cuda.device(dev):
-        check(lib().mtp_linear(code, px, rows, i, ldx, pw, out, ptr(bias), act, ptr(residual), ldr, ptr(offsets), s, ptr(y),
-                               ptr(pre), ptr(ws), ws_bytes, stream_ptr()), "mtp_linear")
+    _call(dev, "mtp_linear", code, px, rows, i, ldx, pw, out, _at(bias), act, _at(residual), ldr, _at(offsets), s, _at(y),
+          _at(pre), _at(ws), ws_bytes)
     return y, pre
 
 
@@ -648,9 +657,7 @@ def linear_act_grad(grad, pre, activation, offsets=None):
         s = offsets.numel() - 1
     ld = out if grad.element_size() == 4 or out % 2 == 0 else -(-out // 8) * 8
     dz = torch.empty((rows, ld), dtype=grad.dtype, device=grad.device)
-    with torch.cuda.device(grad.device):
-        check(lib().mtp_linear_act_grad(code, ptr(grad), ptr(pre), rows, out, act, ptr(offsets), s, ptr(dz), ld, stream_ptr()),
-              "mtp_linear_act_grad")
+    _call(grad.device, "mtp_linear_act_grad", code, _at(grad), _at(pre), rows, out, act, _at(offsets), s, _at(dz), ld)
     return dz[:, :out]
 
 
@@ -661,9 +668,8 @@ def linear_mask_rows(grad, offsets):
     _like(grad, "grad", 2, grad, "grad")
     _like(offsets, "offsets", 1, grad, "grad", torch.int32)
     dst = torch.empty_like(grad)
-    with torch.cuda.device(grad.device):
-        check(lib().mtp_linear_mask_rows(code, ptr(grad), grad.shape[0], grad.shape[1], ptr(offsets), offsets.numel() - 1,
-                                         ptr(dst), stream_ptr()), "mtp_linear_mask_rows")
+    _call(grad.device, "mtp_linear_mask_rows", code, _at(grad), grad.shape[0], grad.shape[1], _at(offsets),
+          offsets.numel() - 1, _at(dst))
     return dst
 
 
@@ -677,12 +683,10 @@ def linear_grad_input(dz, weight, offsets=None):
         raise ValueError(f"dz has {dz.shape[1]} columns, weight gives {out}")
     ld = _row_distance(dz, "dz")
     dx = torch.empty((rows, i), dtype=dz.dtype, device=dz.device)
-    pz, pw = ptr(dz), ptr(weight)
+    pz, pw = _at(dz), _at(weight)
     ws_bytes = int(lib().mtp_linear_workspace_bytes(code, _lib.LINEAR_GRAD_INPUT, rows, i, out, s, pz, ld, pw, i))
     ws = _workspace(ws_bytes, dz.device)
-    with torch.cuda.device(dz.device):
-        check(lib().mtp_linear_grad_input(code, pz, rows, out, ld, pw, i, ptr(offsets), s, ptr(dx), ptr(ws), ws_bytes,
-                                          stream_ptr()), "mtp_linear_grad_input")
+    _call(dz.device, "mtp_linear_grad_input", code, pz, rows, out, ld, pw, i, _at(offsets), s, _at(dx), _at(ws), ws_bytes)
     return dx
 
 
@@ -703,10 +707,36 @@ def linear_grad_weight(dz, x, offsets=None, want_bias=False):
     ldz, ldx = _row_distance(dz, "dz"), _row_distance(x, "x")
     dw = torch.empty(lead + (out, i), dtype=dz.dtype, device=dz.device)
     db = torch.empty(lead + (out,), dtype=dz.dtype, device=dz.device) if want_bias else None
-    pz, px = ptr(dz), ptr(x)
+    pz, px = _at(dz), _at(x)
     ws_bytes = int(lib().mtp_linear_workspace_bytes(code, _lib.LINEAR_GRAD_WEIGHT, rows, i, out, s, pz, ldz, px, ldx))
     ws = _workspace(ws_bytes, dz.device)
-    with torch.cuda.device(dz.device):
-        check(lib().mtp_linear_grad_weight(code, pz, rows, out, ldz, px, i, ldx, ptr(offsets), s, ptr(dw), ptr(db), ptr(ws),
-                                           ws_bytes, stream_ptr()), "mtp_linear_grad_weight")
+    _call(dz.device, "mtp_linear_grad_weight", code, pz, rows, out, ldz, px, i, ldx, _at(offsets), s, _at(dw), _at(db),
+          _at(ws), ws_bytes)
     return dw, db
+
+
+def linear_backward(grad, pre, activation, x, weight, offsets=None, want_x=True, want_weight=True, want_bias=True):
+    """(dx, dweight, dbias), None for what is not wanted, from the gradient of ``linear``'s result (contiguous) and the
+    ``pre`` it gave (None without an activation) -- ``mtp_linear_backward``: one call for the whole backward pass."""
+    _device_tensor(x, "x", 2)
+    code, act = _type_code(x, "x"), _act_code(activation)
+    s, out, i = _sets(weight, x, offsets)
+    rows = x.shape[0]
+    if x.shape[1] != i:
+        raise ValueError(f"x has {x.shape[1]} features, weight takes {i}")
+    _like(grad, "grad", 2, x, "x", shape=(rows, out))
+    if act:
+        _like(pre, "pre", 2, x, "x", shape=(rows, out))
+    want_weight = want_weight or want_bias
+    if not (want_x or want_weight):
+        return None, None, None
+    ldx, dev = _row_distance(x, "x"), x.device
+    dx = torch.empty((rows, i), dtype=x.dtype, device=dev) if want_x else None
+    dw = torch.empty_like(weight) if want_weight else None
+    db = torch.empty(weight.shape[:-1], dtype=x.dtype, device=dev) if want_bias else None
+    pg, px, pw = grad.data_ptr(), x.data_ptr(), weight.data_ptr()
+    ws_bytes = lib().mtp_linear_backward_workspace_bytes(code, rows, i, out, s, act, pg, pw, px, ldx, want_x, want_weight)
+    ws = _workspace(ws_bytes, dev)
+    _call(dev, "mtp_linear_backward", code, pg, _at(pre) if act else None, act, px, rows, i, ldx, pw, out, _at(offsets), s,
+          _at(dx), _at(dw), _at(db), _at(ws), ws_bytes)
+    return dx, dw, db

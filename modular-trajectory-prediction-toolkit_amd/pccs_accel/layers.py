@@ -18,9 +18,10 @@ from . import kernels as K
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, offsets):
-        curved = K._act_code(activation) != 0
-        y, pre = K.linear(x, weight, bias, activation, residual, offsets, want_pre=curved)
-        ctx.save_for_backward(x, weight, pre, offsets)
+        # relu's slope can be read off y where nothing was added to it
+        from_y = activation == "relu" and residual is None
+        y, pre = K.linear(x, weight, bias, activation, residual, offsets, want_pre=activation not in (None, "none") and not from_y)
+        ctx.save_for_backward(x, weight, y if from_y else pre, offsets)
         ctx.activation = activation
         return y
 
@@ -30,17 +31,11 @@ class _Linear(torch.autograd.Function):
         x, weight, pre, offsets = ctx.saved_tensors
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
         grad = grad.contiguous()
-        dx = dw = db = dr = None
-        if want_x or want_w or want_b:
-            dz = grad if pre is None else K.linear_act_grad(grad, pre, ctx.activation, offsets)
-            if want_x:
-                dx = K.linear_grad_input(dz, weight, offsets)
-            if want_w or want_b:
-                dw, db = K.linear_grad_weight(dz, x, offsets, want_bias=want_b)
-                dw = dw if want_w else None
+        dx, dw, db = K.linear_backward(grad, pre, ctx.activation, x, weight, offsets, want_x, want_w, want_b)
+        dr = None
         if want_r:  # rows behind the last set have none
             dr = grad if offsets is None else K.linear_mask_rows(grad, offsets)
-        return dx, dw, db, dr, None, None
+        return dx, dw if want_w else None, db, dr, None, None
 
 
 def _apply(x, weight, bias, activation, residual, offsets):
