@@ -4,6 +4,8 @@
 // Everything here moves data: each kernel reads its inputs and writes its outputs once (the sort reads the ids twice).
 // No result depends on the order in which workgroups run: sums go over a token's own pairs in their order, and the sort is
 // stable.  Types float, bfloat16, half; softmax statistics, weights and sums are float.
+#include <type_traits>
+
 #include "mtp_internal.h"
 
 namespace {
@@ -17,57 +19,99 @@ __device__ __forceinline__ float up(T v) {
 }
 
 // ---- top k ----
-// A key orders like (score, -index): the score's bits made monotonous, then 4095 - index, put into the mantissa of a double
-// with a fixed exponent, so that one v_max_f64 / v_min_f64 pair is a compare-exchange of value and index at once.
-__device__ __forceinline__ double route_key(float s, int index) {
-    s = s + 0.0f;  // -0 equals +0
-    uint32_t b = __float_as_uint(s);
-    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    const uint64_t m = ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - index);
-    return __longlong_as_double((long long)(0x4000000000000000ull | m));
-}
-__device__ __forceinline__ float route_key_score(double key) {
-    uint32_t b = (uint32_t)((uint64_t)__double_as_longlong(key) >> 12);
-    b = (b & 0x80000000u) ? (b & 0x7fffffffu) : ~b;
-    return __uint_as_float(b);
-}
-__device__ __forceinline__ int route_key_index(double key) {
-    return ROUTE_MAX_E - 1 - (int)((uint64_t)__double_as_longlong(key) & (ROUTE_MAX_E - 1));
-}
-constexpr double ROUTE_NO_KEY = 2.0;  // mantissa 0: below every score's key, -inf's included
+// A key orders like (score, -index), so that a maximum finds value and index at once and equal scores go to the lower index.
+// 16-bit scores: the bits made monotonous in the upper half of 32, 65535 - index in the lower.  float: 32 + 12 bits in the mantissa of
+// a double with a fixed exponent, which v_max_f64 / v_min_f64 compare.  NONE is below every key, that of -inf included.
+template <typename T>
+struct RouteKey {
+    typedef uint32_t type;
+    static constexpr type NONE = 0;
+    static constexpr uint32_t INF = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
+    static __device__ __forceinline__ type make(T v, int index, bool *bad) {
+        uint32_t b = __builtin_bit_cast(uint16_t, v);
+        if ((b & 0x7fffu) > INF) {
+            *bad = true;
+            b = 0x8000u | INF;  // NaN: as -inf
+        }
+        b = b == 0x8000u ? 0u : b;  // -0 equals +0
+        b = (b & 0x8000u) ? (b ^ 0xffffu) : (b | 0x8000u);
+        return (b << 16) | (uint32_t)(0xffff - index);
+    }
+    static __device__ __forceinline__ float score(type k) {
+        uint32_t b = k >> 16;
+        b = (b & 0x8000u) ? (b ^ 0x8000u) : (b ^ 0xffffu);
+        return (float)__builtin_bit_cast(T, (uint16_t)b);
+    }
+    static __device__ __forceinline__ int index(type k) { return 0xffff - (int)(k & 0xffffu); }
+    static __device__ __forceinline__ type more(type a, type b) { return a > b ? a : b; }
+    static __device__ __forceinline__ type less(type a, type b) { return a > b ? b : a; }
+    template <int CTRL>
+    static __device__ __forceinline__ type turn(type v) {
+        return (type)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+    }
+    static __device__ __forceinline__ type lane(type v, int l) { return (type)__builtin_amdgcn_readlane((int)v, l); }
+};
+template <>
+struct RouteKey<float> {
+    typedef double type;
+    static constexpr type NONE = 2.0;
+    static __device__ __forceinline__ type make(float v, int index, bool *bad) {
+        if (v != v) {
+            *bad = true;
+            v = -__builtin_inff();
+        }
+        uint32_t b = __float_as_uint(v + 0.0f);  // -0 equals +0
+        b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+        return __longlong_as_double((long long)(0x4000000000000000ull | ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - index)));
+    }
+    static __device__ __forceinline__ float score(type k) {
+        const uint32_t b = (uint32_t)((uint64_t)__double_as_longlong(k) >> 12);
+        return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
+    }
+    static __device__ __forceinline__ int index(type k) {
+        return ROUTE_MAX_E - 1 - (int)((uint64_t)__double_as_longlong(k) & (ROUTE_MAX_E - 1));
+    }
+    static __device__ __forceinline__ type more(type a, type b) { return fmax(a, b); }
+    static __device__ __forceinline__ type less(type a, type b) { return fmin(a, b); }
+    template <int CTRL>
+    static __device__ __forceinline__ type turn(type v) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xf, 0xf, true);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
+        return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+    }
+    static __device__ __forceinline__ type lane(type v, int l) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
+        return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+    }
+};
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_f32(float v) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-template <int CTRL>
-__device__ __forceinline__ double dpp_f64(double v) {
-    const uint64_t b = (uint64_t)__double_as_longlong(v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xf, 0xf, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
-    return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
-}
 constexpr int ROW_ROR = 0x120;  // rotation within 16 lanes
 
 // over the L lanes (16 or 64) that share a row, the same result in each
-template <int L>
-__device__ __forceinline__ double group_max(double v) {
-    v = fmax(v, dpp_f64<ROW_ROR + 8>(v));
-    v = fmax(v, dpp_f64<ROW_ROR + 4>(v));
-    v = fmax(v, dpp_f64<ROW_ROR + 2>(v));
-    v = fmax(v, dpp_f64<ROW_ROR + 1>(v));
-    if constexpr (L == 64) {
-        v = fmax(v, __shfl_xor(v, 16));
-        v = fmax(v, __shfl_xor(v, 32));
-    }
+template <typename T, int L>
+__device__ __forceinline__ typename RouteKey<T>::type group_max(typename RouteKey<T>::type v) {
+    typedef RouteKey<T> R;
+    v = R::more(v, R::template turn<ROW_ROR + 8>(v));
+    v = R::more(v, R::template turn<ROW_ROR + 4>(v));
+    v = R::more(v, R::template turn<ROW_ROR + 2>(v));
+    v = R::more(v, R::template turn<ROW_ROR + 1>(v));
+    if constexpr (L == 64)
+        v = R::more(R::more(R::lane(v, 0), R::lane(v, 16)), R::more(R::lane(v, 32), R::lane(v, 48)));
     return v;
+}
+template <int CTRL>
+__device__ __forceinline__ float turn_f32(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
-    v += dpp_f32<ROW_ROR + 8>(v);
-    v += dpp_f32<ROW_ROR + 4>(v);
-    v += dpp_f32<ROW_ROR + 2>(v);
-    v += dpp_f32<ROW_ROR + 1>(v);
+    v += turn_f32<ROW_ROR + 8>(v);
+    v += turn_f32<ROW_ROR + 4>(v);
+    v += turn_f32<ROW_ROR + 2>(v);
+    v += turn_f32<ROW_ROR + 1>(v);
     if constexpr (L == 64) {
         v += __shfl_xor(v, 16);
         v += __shfl_xor(v, 32);
@@ -76,8 +120,8 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 // Batcher's odd-even merge sort of V registers, largest first
-template <int V>
-__device__ __forceinline__ void sort_registers(double (&a)[V]) {
+template <typename T, int V>
+__device__ __forceinline__ void sort_registers(typename RouteKey<T>::type (&a)[V]) {
 #pragma unroll
     for (int p = 1; p < V; p *= 2) {
 #pragma unroll
@@ -87,9 +131,9 @@ __device__ __forceinline__ void sort_registers(double (&a)[V]) {
 #pragma unroll
                 for (int i = 0; i < q; ++i) {
                     if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
-                        const double x = a[i + j], y = a[i + j + q];
-                        a[i + j] = fmax(x, y);
-                        a[i + j + q] = fmin(x, y);
+                        const typename RouteKey<T>::type x = a[i + j], y = a[i + j + q];
+                        a[i + j] = RouteKey<T>::more(x, y);
+                        a[i + j + q] = RouteKey<T>::less(x, y);
                     }
                 }
             }
@@ -97,82 +141,96 @@ __device__ __forceinline__ void sort_registers(double (&a)[V]) {
     }
 }
 
-// L lanes share a row, lane `sub` holds the scores sub, sub + L, ...  Each lane sorts its own V keys and lays the first
-// min(V, k) of them into LDS; k times the largest head is taken (a maximum over the L lanes), and the lane it came from moves on
-// to its next key.
+// L lanes share a row, lane `sub` holds the scores sub * V to sub * V + V - 1 (loaded in pieces of up to 16 bytes where the rows
+// allow it).  Each lane sorts its keys and lays them into LDS, as many as could be chosen; k times the largest head is taken (a
+// maximum over the L lanes), and the lane it came from moves on to its next key.
 template <typename T, int L, int V, int KB>
 __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores, int64_t n, int e, int64_t ld, int k, int normalize,
-                                                    int32_t *__restrict__ ids, float *__restrict__ weights,
+                                                    int pieces, int32_t *__restrict__ ids, float *__restrict__ weights,
                                                     float *__restrict__ stats) {
-    extern __shared__ __attribute__((aligned(16))) double lists[];  // [min(V, k)][256]
+    typedef RouteKey<T> R;
+    typedef typename R::type key_t;
+    extern __shared__ __attribute__((aligned(16))) char route_lds[];  // key_t [min(V, k) + 1][256]
+    key_t *lists = reinterpret_cast<key_t *>(route_lds);
+    constexpr int W = V * (int)sizeof(T) < 16 ? V : 16 / (int)sizeof(T);  // elements of a piece
     const int tid = threadIdx.x, sub = tid % L;
     const int64_t row = (int64_t)blockIdx.x * (256 / L) + tid / L;
     const bool live = row < n;
     const T *s = scores + (live ? row : n - 1) * ld;
 
-    double key[V];
+    T v[V];
+    if (pieces) {  // e is a multiple of W
+        typedef T piece_t __attribute__((ext_vector_type(W)));
+#pragma unroll
+        for (int q = 0; q < V / W; ++q) {
+            const int i = sub * V + q * W;
+            const piece_t p = *reinterpret_cast<const piece_t *>(s + (i < e ? i : 0));
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[q * W + j] = p[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = s[sub * V + j < e ? sub * V + j : 0];
+    }
+    key_t key[V];
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int i = j * L + sub;
-        key[j] = ROUTE_NO_KEY;
-        if (i < e) {
-            const float v = up(s[i]);
-            bad |= v != v;
-            key[j] = route_key(v != v ? -__builtin_inff() : v, i);
-        }
+        const int i = sub * V + j;
+        bool is_bad = false;
+        const key_t made = R::make(v[j], i, &is_bad);
+        key[j] = i < e ? made : R::NONE;
+        bad |= is_bad && i < e;
     }
     float total = 0.f, top = 0.f;
     if (!normalize) {  // the softmax over all modalities
-        double m = ROUTE_NO_KEY;
+        key_t m = key[0];
 #pragma unroll
-        for (int j = 0; j < V; ++j) m = fmax(m, key[j]);
-        top = route_key_score(group_max<L>(m));
+        for (int j = 1; j < V; ++j) m = R::more(m, key[j]);
+        top = R::score(group_max<T, L>(m));
         if (top == -__builtin_inff()) top = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (key[j] != ROUTE_NO_KEY) total += expf(route_key_score(key[j]) - top);
+        for (int j = 0; j < V; ++j) total += key[j] != R::NONE ? expf(R::score(key[j]) - top) : 0.f;
         total = group_sum<L>(total);
     }
     const uint64_t any_bad = __ballot(bad);
     const bool row_bad = ((any_bad >> ((tid & 63) / L * L)) & (L == 64 ? ~0ull : 0xffffull)) != 0;
 
-    sort_registers<V>(key);
+    sort_registers<T, V>(key);
     const int depth = V < k ? V : k;
-    double *mine = lists + tid;
+    key_t *next = lists + tid;
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        if (j < depth) mine[j * 256] = key[j];
-    int at = 0;
-    double head = key[0];
-    double chosen[KB];
+        if (j < depth) next[j * 256] = key[j];
+    next[depth * 256] = R::NONE;
+    key_t head = key[0];
+    key_t chosen[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-        chosen[b] = ROUTE_NO_KEY;
+        chosen[b] = R::NONE;
         const int most = k - b * L < L ? k - b * L : L;
         for (int i = 0; i < most; ++i) {
-            const double best = group_max<L>(head);
+            const key_t best = group_max<T, L>(head);
             if (sub == i) chosen[b] = best;
-            if (head == best) {  // keys differ by their index: one lane; where nothing is left, no matter
-                ++at;
-                head = at < depth ? mine[at * 256] : ROUTE_NO_KEY;
-            }
+            // keys differ by their index, so one lane moves on; a lane that has given its last key stays at NONE
+            next += head == best && best != R::NONE ? 256 : 0;
+            head = *next;
         }
     }
     float w[KB];
     if (normalize) {
         // lane 0 of the first batch has the largest score
-        const double first = __shfl(chosen[0], (tid & 63) / L * L);
-        top = first == ROUTE_NO_KEY ? 0.f : route_key_score(first);
+        const key_t first = __shfl(chosen[0], (tid & 63) / L * L);
+        top = first == R::NONE ? 0.f : R::score(first);
         if (top == -__builtin_inff()) top = 0.f;
     }
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-        const float v = route_key_score(chosen[b]);
-        const bool none = chosen[b] == ROUTE_NO_KEY || v == -__builtin_inff();
-        if (none) chosen[b] = ROUTE_NO_KEY;
-        w[b] = none ? 0.f : expf(v - top);
+        const float x = R::score(chosen[b]);
+        const bool none = chosen[b] == R::NONE || x == -__builtin_inff();
+        if (none) chosen[b] = R::NONE;
+        w[b] = none ? 0.f : expf(x - top);
         sum += w[b];
     }
     if (normalize) total = group_sum<L>(sum);
@@ -182,8 +240,8 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
     for (int b = 0; b < KB; ++b) {
         const int i = b * L + sub;
         if (i < k) {
-            const bool none = chosen[b] == ROUTE_NO_KEY;
-            ids[row * k + i] = none ? -1 : route_key_index(chosen[b]);
+            const bool none = chosen[b] == R::NONE;
+            ids[row * k + i] = none ? -1 : R::index(chosen[b]);
             weights[row * k + i] = row_bad ? __builtin_nanf("") : w[b] * scale;
         }
     }
@@ -193,43 +251,56 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
     }
 }
 
-// Gradient towards the scores, a few rows per workgroup:
-//   normalised: w_j (g_j - sum g w) at the chosen, zero elsewhere;  else: p_j (g_j [chosen] - sum g w) everywhere
+// Gradient towards the scores, a few rows per workgroup, put together in LDS and written in whole 16-byte pieces:
+//   w_j (g_j - sum g w) at the chosen;  elsewhere zero (normalised) or -p_j sum g w, p the softmax over all
 template <typename T>
 __global__ __launch_bounds__(256) void k_route_grad(const T *__restrict__ scores, int64_t n, int e, int64_t ld, int k, int normalize,
                                                     const int32_t *__restrict__ ids, const float *__restrict__ weights,
                                                     const float *__restrict__ stats, const float *__restrict__ g,
-                                                    T *__restrict__ out, int rows_per) {
-    extern __shared__ __attribute__((aligned(16))) float tile[];  // [rows_per][e], then [rows_per] dots
-    float *dots = tile + rows_per * e;
-    const int tid = threadIdx.x;
+                                                    T *__restrict__ out, int rows_per, int pieces) {
+    extern __shared__ __attribute__((aligned(16))) char grad_lds[];  // float dots[rows_per], then T tile[rows_per][e]
+    float *dots = reinterpret_cast<float *>(grad_lds);
+    char *tile_at = grad_lds + (rows_per * 4 + 15) / 16 * 16;
+    T *tile = reinterpret_cast<T *>(tile_at);
+    const int tid = threadIdx.x, sub = tid & 15;
     const int64_t row0 = (int64_t)blockIdx.x * rows_per;
     const int rows = (int)(n - row0 < rows_per ? n - row0 : rows_per);
-    for (int i = tid; i < rows * e; i += 256) tile[i] = 0.f;
-    __syncthreads();
-    const int sub = tid & 15;
     for (int r = tid >> 4; r < rows; r += 16) {
         const int64_t at = (row0 + r) * k;
         float dot = 0.f;
         for (int j = sub; j < k; j += 16) dot += weights[at + j] * g[at + j];
         dot = group_sum<16>(dot);
+        if (sub == 0) dots[r] = dot;
+    }
+    const int held = rows * e, whole = (held * (int)sizeof(T) + 15) / 16;
+    if (normalize) {
+        for (int i = tid; i < whole; i += 256) reinterpret_cast<float4 *>(tile_at)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+    } else {
+        __syncthreads();
+        for (int r = tid >> 6; r < rows; r += 4) {
+            const float top = stats[(row0 + r) * 2], scale = stats[(row0 + r) * 2 + 1] * -dots[r];
+            const T *s = scores + (row0 + r) * ld;
+            for (int c = tid & 63; c < e; c += 64) tile[r * e + c] = (T)(expf(up(s[c]) - top) * scale);
+        }
+        __syncthreads();
+    }
+    for (int r = tid >> 4; r < rows; r += 16) {
+        const int64_t at = (row0 + r) * k;
+        const float dot = dots[r];
         for (int j = sub; j < k; j += 16) {
             const int id = ids[at + j];
-            const float w = weights[at + j];
-            if (id >= 0 && id < e) tile[r * e + id] = normalize ? w * (g[at + j] - dot) : w * g[at + j];
+            if (id >= 0 && id < e) tile[r * e + id] = (T)(weights[at + j] * (g[at + j] - dot));
         }
-        if (sub == 0) dots[r] = dot;
     }
     __syncthreads();
     T *o = out + row0 * e;
-    for (int i = tid; i < rows * e; i += 256) {
-        float v = tile[i];
-        if (!normalize) {
-            const int r = i / e, c = i - r * e;
-            const float top = stats[(row0 + r) * 2], scale = stats[(row0 + r) * 2 + 1];
-            v -= expf(up(scores[(row0 + r) * ld + c]) - top) * scale * dots[r];
-        }
-        o[i] = (T)v;
+    if (pieces) {  // every workgroup's rows start on 16 bytes
+        const int full = held * (int)sizeof(T) / 16;
+        for (int i = tid; i < full; i += 256) reinterpret_cast<float4 *>(o)[i] = reinterpret_cast<const float4 *>(tile_at)[i];
+        for (int i = full * 16 / (int)sizeof(T) + tid; i < held; i += 256) o[i] = tile[i];
+    } else {
+        for (int i = tid; i < held; i += 256) o[i] = tile[i];
     }
 }
 
@@ -259,20 +330,20 @@ __global__ __launch_bounds__(256) void k_pairs_count(const int32_t *__restrict__
     for (int i = threadIdx.x; i <= e; i += 256) counts[(int64_t)blockIdx.x * (e + 1) + i] = hist[i];
 }
 
-// counts -> the exclusive prefix over the workgroups, and the modality's total.  64 modalities and 16 parts a workgroup.
+// counts -> the exclusive prefix over the workgroups, and the modality's total.  16 modalities and 64 parts a workgroup.
 __global__ __launch_bounds__(1024) void k_pairs_scan(int32_t *__restrict__ counts, int blocks, int e, int32_t *__restrict__ totals) {
-    __shared__ int part[16][64];
-    const int x = blockIdx.x * 64 + (threadIdx.x & 63), p = threadIdx.x >> 6;
-    const int per = (blocks + 15) / 16;
-    const int lo = p * per, hi = lo + per < blocks ? lo + per : blocks;
+    __shared__ int part[64][16];
+    const int m = threadIdx.x & 15, x = blockIdx.x * 16 + m, p = threadIdx.x >> 4;
+    const int per = (blocks + 63) / 64;
+    const int lo = p * per < blocks ? p * per : blocks, hi = lo + per < blocks ? lo + per : blocks;
     int sum = 0;
     if (x <= e)
         for (int b = lo; b < hi; ++b) sum += counts[(int64_t)b * (e + 1) + x];
-    part[p][threadIdx.x & 63] = sum;
+    part[p][m] = sum;
     __syncthreads();
     int before = 0, all = 0;
-    for (int i = 0; i < 16; ++i) {
-        const int v = part[i][threadIdx.x & 63];
+    for (int i = 0; i < 64; ++i) {
+        const int v = part[i][m];
         if (i < p) before += v;
         all += v;
     }
@@ -413,7 +484,9 @@ __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64
     }
 }
 
-// y[t] = sum_j weights[t][j] rows[position[t][j]] (weights NULL: all one), pairs without a modality left out
+// y[t] = sum_j weights[t][j] rows[position[t][j]] (weights NULL: all one), pairs without a modality left out.  One thread per N
+// elements of a token; four rows are in flight at a time (their places are all valid, what does not count is dropped after
+// the load).
 template <typename T, int N>
 __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int64_t n, int d, int k,
                                                  const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
@@ -424,58 +497,117 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
     const int held = *held_at;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t t = i / per, c = i - t * per;
+        const int32_t *at = position + t * k;
+        const float *wt = weights + t * k;
         float sum[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) sum[e] = 0.f;
-#pragma unroll 4
-        for (int j = 0; j < k; ++j) {
-            const int64_t p = position[t * k + j];
-            if (p < held) {
-                float f[N];
-                unpack<T, N>(*reinterpret_cast<const vec *>(rows + p * d + c * N), f);
-                const float w = weights != nullptr ? weights[t * k + j] : 1.f;
+        for (int j0 = 0; j0 < k; j0 += 4) {
+            vec v[4];
+            float w[4];
+            bool in[4];
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum[e] = fmaf(w, f[e], sum[e]);
+            for (int q = 0; q < 4; ++q) {
+                const int j = j0 + q < k ? j0 + q : k - 1;
+                const int64_t p = at[j];
+                in[q] = p < held && j0 + q < k;
+                v[q] = *reinterpret_cast<const vec *>(rows + p * d + c * N);
+                w[q] = weights != nullptr ? wt[j] : 1.f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float f[N];
+                unpack<T, N>(v[q], f);
+                if (in[q]) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum[e] = fmaf(w[q], f[e], sum[e]);
+                }
             }
         }
         *reinterpret_cast<vec *>(y + t * d + c * N) = pack<T, N>(sum);
     }
 }
 
+// the sum over L neighbouring lanes, the same in each
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += turn_f32<0xB1>(v);                          // lane ^ 1
+    v += turn_f32<0x4E>(v);                          // lane ^ 2
+    v += turn_f32<0x141>(v);                         // the other four of eight
+    if constexpr (L >= 16) v += turn_f32<0x140>(v);  // the other eight of sixteen
+    if constexpr (L >= 32) v += __shfl_xor(v, 16);
+    if constexpr (L >= 64) v += __shfl_xor(v, 32);
+    return v;
+}
+
 // grad_rows[position[t][j]] = weights[t][j] g[t] (zero behind the last modality); grad_weights[t][j] = <rows[...], g[t]>.
-// L lanes share a token.
-template <typename T, int N, int L>
+// L lanes share a token and hold C pieces of N elements of its gradient each; four rows are in flight at a time.
+template <typename T, int N, int L, int C>
 __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows, const T *__restrict__ g, int64_t n, int d, int k,
                                                       const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
                                                       const float *__restrict__ weights, T *__restrict__ grad_rows,
                                                       float *__restrict__ grad_weights) {
     typedef typename Pack<T, N>::type vec;
+    constexpr int Q = C == 1 ? 4 : 1;
     const int per = d / N, sub = threadIdx.x % L;
     const int held = *held_at;
     for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L; t < n; t += (int64_t)gridDim.x * (256 / L)) {
-        for (int j = 0; j < k; ++j) {
-            const int64_t p = position[t * k + j];
-            const bool in = p < held;
-            const float w = in ? weights[t * k + j] : 0.f;
-            float dot = 0.f;
-            for (int c = sub; c < per; c += L) {
-                float gv[N], rv[N];
-                unpack<T, N>(*reinterpret_cast<const vec *>(g + t * d + c * N), gv);
-                if (in && grad_weights != nullptr) {
-                    unpack<T, N>(*reinterpret_cast<const vec *>(rows + p * d + c * N), rv);
+        const int32_t *at = position + t * k;
+        for (int c0 = 0; c0 < per; c0 += L * C) {
+            float gv[C][N];
 #pragma unroll
-                    for (int e = 0; e < N; ++e) dot = fmaf(rv[e], gv[e], dot);
-                }
-                if (grad_rows != nullptr) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) gv[e] = in ? w * gv[e] : 0.f;
-                    *reinterpret_cast<vec *>(grad_rows + p * d + c * N) = pack<T, N>(gv);
-                }
+            for (int c = 0; c < C; ++c) {
+                const int x = c0 + c * L + sub;
+                vec v = {};
+                if (x < per) v = *reinterpret_cast<const vec *>(g + t * d + (int64_t)x * N);
+                unpack<T, N>(v, gv[c]);
             }
-            if (grad_weights != nullptr) {
+            for (int j0 = 0; j0 < k; j0 += Q) {
+                int64_t p[Q];
+                vec v[Q][C];
 #pragma unroll
-                for (int m = L / 2; m > 0; m >>= 1) dot += __shfl_xor(dot, m);
-                if (sub == 0) grad_weights[t * k + j] = dot;
+                for (int q = 0; q < Q; ++q) {
+                    p[q] = at[j0 + q < k ? j0 + q : k - 1];
+                    if (grad_weights != nullptr) {
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const int x = c0 + c * L + sub;
+                            v[q][c] = *reinterpret_cast<const vec *>(rows + p[q] * d + (int64_t)(x < per ? x : 0) * N);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    const int j = j0 + q;
+                    if (j >= k) break;
+                    const bool in = p[q] < held;
+                    if (grad_rows != nullptr) {
+                        const float w = in ? weights[t * k + j] : 0.f;
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const int x = c0 + c * L + sub;
+                            float o[N];
+#pragma unroll
+                            for (int e = 0; e < N; ++e) o[e] = in ? w * gv[c][e] : 0.f;
+                            if (x < per) *reinterpret_cast<vec *>(grad_rows + p[q] * d + (int64_t)x * N) = pack<T, N>(o);
+                        }
+                    }
+                    if (grad_weights != nullptr) {
+                        float dot = 0.f;
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            float rv[N];
+                            unpack<T, N>(v[q][c], rv);
+                            if (in && c0 + c * L + sub < per) {
+#pragma unroll
+                                for (int e = 0; e < N; ++e) dot = fmaf(rv[e], gv[c][e], dot);
+                            }
+                        }
+                        dot = lanes_sum<L>(dot);
+                        // a row longer than L * C pieces comes in parts, added in their order
+                        if (sub == 0) grad_weights[t * k + j] = c0 == 0 ? dot : grad_weights[t * k + j] + dot;
+                    }
+                }
             }
         }
     }
@@ -489,11 +621,13 @@ unsigned blocks_of(int64_t items, int per_block) {
 template <typename T, int L, int V, int KB>
 int launch_topk(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights, float *stats,
                 hipStream_t s) {
-    const int lds = (V < k ? V : k) * 256 * 8;
+    constexpr int KEY = (int)sizeof(typename RouteKey<T>::type), W = V * (int)sizeof(T) < 16 ? V : 16 / (int)sizeof(T);
+    const int lds = ((V < k ? V : k) + 1) * 256 * KEY;
     const int64_t blocks = (n + 256 / L - 1) / (256 / L);
-    MTP_SET_MAX_LDS_ONCE((k_route_topk<T, L, V, KB>), V * 256 * 8);
+    const int pieces = e % W == 0 && ld % W == 0 && (uintptr_t)scores % (W * sizeof(T)) == 0;
+    MTP_SET_MAX_LDS_ONCE((k_route_topk<T, L, V, KB>), (V + 1) * 256 * KEY);
     hipLaunchKernelGGL((k_route_topk<T, L, V, KB>), dim3((unsigned)blocks), dim3(256), lds, s, reinterpret_cast<const T *>(scores), n,
-                       e, ld, k, normalize, ids, weights, stats);
+                       e, ld, k, normalize, pieces, ids, weights, stats);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -558,10 +692,10 @@ int combine(const void *rows, int64_t n, int d, int k, const int32_t *position, 
     return MTP_OK;
 }
 
-template <typename T, int N, int L>
+template <typename T, int N, int L, int C>
 int launch_combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
                         const float *weights, void *grad_rows, float *grad_weights, hipStream_t s) {
-    hipLaunchKernelGGL((k_combine_grad<T, N, L>), dim3(blocks_of(n, 256 / L)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
+    hipLaunchKernelGGL((k_combine_grad<T, N, L, C>), dim3(blocks_of(n, 256 / L)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
                        reinterpret_cast<const T *>(g), n, d, k, position, held, weights, reinterpret_cast<T *>(grad_rows),
                        grad_weights);
     MTP_LAUNCH_CHECK();
@@ -574,10 +708,11 @@ int combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const
     constexpr int N = 16 / (int)sizeof(T);
     const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)g | (uintptr_t)grad_rows) % 16 == 0;
     if (!vec)
-        return launch_combine_grad<T, 1, 64>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    if (d / N <= 8) return launch_combine_grad<T, N, 8>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    if (d / N <= 16) return launch_combine_grad<T, N, 16>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    return launch_combine_grad<T, N, 32>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+        return launch_combine_grad<T, 1, 64, 4>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (d / N <= 8) return launch_combine_grad<T, N, 8, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (d / N <= 16) return launch_combine_grad<T, N, 16, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (d / N <= 32) return launch_combine_grad<T, N, 32, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    return launch_combine_grad<T, N, 64, 2>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
 }
 
 bool known_type(int dtype) { return dtype == MTP_FLOAT || dtype == MTP_BFLOAT16 || dtype == MTP_HALF; }
@@ -604,21 +739,24 @@ extern "C" int mtp_route_topk_grad(int dtype, const void *scores, int64_t n, int
                 "mtp_route_topk_grad: bad shape n=%lld e=%d k=%d ld=%lld", (long long)n, e, k, (long long)ld);
     if (n == 0) return MTP_OK;
     MTP_REQUIRE(scores && ids && weights && stats && g && out, "mtp_route_topk_grad: null pointer");
-    int rows_per = 8192 / e;
-    if (rows_per < 1) rows_per = 1;
+    // 16 KB of rows; eight rows of any length start on 16 bytes
+    const int sz = dtype == MTP_FLOAT ? 4 : 2;
+    int rows_per = 16384 / (e * sz) / 8 * 8;
+    if (rows_per == 0) rows_per = 8 * e * sz <= 56 * 1024 ? 8 : 1;
     if (rows_per > 64) rows_per = 64;
-    const int lds = rows_per * (e + 1) * 4;
+    const int pieces = (uintptr_t)out % 16 == 0 && (int64_t)rows_per * e * sz % 16 == 0;
+    const int lds = (rows_per * 4 + 15) / 16 * 16 + (rows_per * e * sz + 15) / 16 * 16;
     const dim3 grid((unsigned)((n + rows_per - 1) / rows_per));
     hipStream_t s = mtp_stream(stream);
     if (dtype == MTP_FLOAT)
         hipLaunchKernelGGL(k_route_grad<float>, grid, dim3(256), lds, s, (const float *)scores, n, e, ld, k, normalize, ids, weights,
-                           stats, g, (float *)out, rows_per);
+                           stats, g, (float *)out, rows_per, pieces);
     else if (dtype == MTP_BFLOAT16)
         hipLaunchKernelGGL(k_route_grad<__bf16>, grid, dim3(256), lds, s, (const __bf16 *)scores, n, e, ld, k, normalize, ids,
-                           weights, stats, g, (__bf16 *)out, rows_per);
+                           weights, stats, g, (__bf16 *)out, rows_per, pieces);
     else
         hipLaunchKernelGGL(k_route_grad<_Float16>, grid, dim3(256), lds, s, (const _Float16 *)scores, n, e, ld, k, normalize, ids,
-                           weights, stats, g, (_Float16 *)out, rows_per);
+                           weights, stats, g, (_Float16 *)out, rows_per, pieces);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -654,7 +792,7 @@ extern "C" int mtp_sort_pairs(const int32_t *ids, int64_t pairs, int e, int32_t 
     int32_t *counts = reinterpret_cast<int32_t *>(ws), *totals = counts + (int64_t)blocks * (e + 1);
     hipLaunchKernelGGL(k_pairs_count, dim3(blocks), dim3(256), (e + 1) * 4, s, ids, pairs, e, PAIRS_RUN, counts);
     MTP_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_pairs_scan, dim3((e + 64) / 64), dim3(1024), 0, s, counts, blocks, e, totals);
+    hipLaunchKernelGGL(k_pairs_scan, dim3((e + 16) / 16), dim3(1024), 0, s, counts, blocks, e, totals);
     MTP_LAUNCH_CHECK();
     MTP_SET_MAX_LDS_ONCE(k_pairs_place<4>, (5 * (ROUTE_MAX_E + 1) + 4) * 4);
     hipLaunchKernelGGL(k_pairs_place<4>, dim3(blocks), dim3(256), (5 * (e + 1) + 4) * 4, s, ids, pairs, e, bits, PAIRS_RUN, counts,
