@@ -464,8 +464,23 @@ __device__ __forceinline__ typename Pack<T, N>::type pack(const float *f) {
     }
 }
 
+// Rows of pairs are read and written once.  More of them than the 256 MB memory-side cache holds go past the caches (ONCE: there
+// and back with gradients over 1.47 M rows of 384 bytes 637 us, 745 us without); fewer are likely still there for the next kernel
+// (143 760 rows of 192 bytes: the two sums 13 us, 17 us past the caches).
+template <bool ONCE, typename V>
+__device__ __forceinline__ V load_row(const V *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+
+template <bool ONCE, typename V>
+__device__ __forceinline__ void store_row(V *p, V v) {
+    if constexpr (ONCE) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+
 // rows[position[t][j]] = x[t], zero where the pair has no modality; one thread per N elements of a token
-template <typename T, int N>
+template <typename T, int N, bool ONCE>
 __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64_t n, int d, int64_t ld, int k,
                                                   const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
                                                   T *__restrict__ rows) {
@@ -479,7 +494,7 @@ __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64
         const vec zero = {};
         for (int j = 0; j < k; ++j) {
             const int64_t p = position[t * k + j];
-            *reinterpret_cast<vec *>(rows + p * d + c * N) = p < held ? v : zero;
+            store_row<ONCE>(reinterpret_cast<vec *>(rows + p * d + c * N), p < held ? v : zero);
         }
     }
 }
@@ -487,7 +502,7 @@ __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64
 // y[t] = sum_j weights[t][j] rows[position[t][j]] (weights NULL: all one), pairs without a modality left out.  One thread per N
 // elements of a token; four rows are in flight at a time (their places are all valid, what does not count is dropped after
 // the load).
-template <typename T, int N>
+template <typename T, int N, bool ONCE>
 __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int64_t n, int d, int k,
                                                  const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
                                                  const float *__restrict__ weights, T *__restrict__ y) {
@@ -511,7 +526,7 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
                 const int j = j0 + q < k ? j0 + q : k - 1;
                 const int64_t p = at[j];
                 in[q] = p < held && j0 + q < k;
-                v[q] = *reinterpret_cast<const vec *>(rows + p * d + c * N);
+                v[q] = load_row<ONCE>(reinterpret_cast<const vec *>(rows + p * d + c * N));
                 w[q] = weights != nullptr ? wt[j] : 1.f;
             }
 #pragma unroll
@@ -524,7 +539,7 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
                 }
             }
         }
-        *reinterpret_cast<vec *>(y + t * d + c * N) = pack<T, N>(sum);
+        store_row<ONCE>(reinterpret_cast<vec *>(y + t * d + c * N), pack<T, N>(sum));
     }
 }
 
@@ -542,7 +557,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 
 // grad_rows[position[t][j]] = weights[t][j] g[t] (zero behind the last modality); grad_weights[t][j] = <rows[...], g[t]>.
 // L lanes share a token and hold C pieces of N elements of its gradient each; four rows are in flight at a time.
-template <typename T, int N, int L, int C>
+template <typename T, int N, int L, int C, bool ONCE>
 __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows, const T *__restrict__ g, int64_t n, int d, int k,
                                                       const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
                                                       const float *__restrict__ weights, T *__restrict__ grad_rows,
@@ -572,7 +587,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
 #pragma unroll
                         for (int c = 0; c < C; ++c) {
                             const int x = c0 + c * L + sub;
-                            v[q][c] = *reinterpret_cast<const vec *>(rows + p[q] * d + (int64_t)(x < per ? x : 0) * N);
+                            v[q][c] = load_row<ONCE>(reinterpret_cast<const vec *>(rows + p[q] * d + (int64_t)(x < per ? x : 0) * N));
                         }
                     }
                 }
@@ -589,7 +604,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                             float o[N];
 #pragma unroll
                             for (int e = 0; e < N; ++e) o[e] = in ? w * gv[c][e] : 0.f;
-                            if (x < per) *reinterpret_cast<vec *>(grad_rows + p[q] * d + (int64_t)x * N) = pack<T, N>(o);
+                            if (x < per) store_row<ONCE>(reinterpret_cast<vec *>(grad_rows + p[q] * d + (int64_t)x * N), pack<T, N>(o));
                         }
                     }
                     if (grad_weights != nullptr) {
@@ -662,17 +677,32 @@ constexpr int PAIRS_ALONE = 16384;   // up to here one workgroup sorts them all
 int64_t pairs_blocks(int64_t pairs) { return (pairs + PAIRS_RUN - 1) / PAIRS_RUN; }
 bool pairs_alone(int64_t pairs, int e) { return pairs <= PAIRS_ALONE && (int64_t)17 * (e + 1) * 4 + 64 <= 128 * 1024; }
 
+constexpr int64_t CACHE_BYTES = 256ll << 20;
+
+template <typename T, int N, bool ONCE>
+int launch_dispatch(const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held, void *rows,
+                    hipStream_t s) {
+    hipLaunchKernelGGL((k_dispatch<T, N, ONCE>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(x),
+                       n, d, ld, k, position, held, reinterpret_cast<T *>(rows));
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
 template <typename T>
 int dispatch(const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held, void *rows,
              hipStream_t s) {
     constexpr int N = 16 / (int)sizeof(T);
     const bool vec = d % N == 0 && ld % N == 0 && ((uintptr_t)x | (uintptr_t)rows) % 16 == 0;
-    if (vec)
-        hipLaunchKernelGGL((k_dispatch<T, N>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(x), n,
-                           d, ld, k, position, held, reinterpret_cast<T *>(rows));
-    else
-        hipLaunchKernelGGL((k_dispatch<T, 1>), dim3(blocks_of(n * d, 256)), dim3(256), 0, s, reinterpret_cast<const T *>(x), n, d, ld,
-                           k, position, held, reinterpret_cast<T *>(rows));
+    if (!vec) return launch_dispatch<T, 1, false>(x, n, d, ld, k, position, held, rows, s);
+    if (n * k * d * (int64_t)sizeof(T) > CACHE_BYTES) return launch_dispatch<T, N, true>(x, n, d, ld, k, position, held, rows, s);
+    return launch_dispatch<T, N, false>(x, n, d, ld, k, position, held, rows, s);
+}
+
+template <typename T, int N, bool ONCE>
+int launch_combine(const void *rows, int64_t n, int d, int k, const int32_t *position, const int32_t *held, const float *weights,
+                   void *y, hipStream_t s) {
+    hipLaunchKernelGGL((k_combine<T, N, ONCE>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
+                       n, d, k, position, held, weights, reinterpret_cast<T *>(y));
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -682,22 +712,17 @@ int combine(const void *rows, int64_t n, int d, int k, const int32_t *position, 
             hipStream_t s) {
     constexpr int N = 16 / (int)sizeof(T);
     const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)y) % 16 == 0;
-    if (vec)
-        hipLaunchKernelGGL((k_combine<T, N>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
-                           n, d, k, position, held, weights, reinterpret_cast<T *>(y));
-    else
-        hipLaunchKernelGGL((k_combine<T, 1>), dim3(blocks_of(n * d, 256)), dim3(256), 0, s, reinterpret_cast<const T *>(rows), n, d,
-                           k, position, held, weights, reinterpret_cast<T *>(y));
-    MTP_LAUNCH_CHECK();
-    return MTP_OK;
+    if (!vec) return launch_combine<T, 1, false>(rows, n, d, k, position, held, weights, y, s);
+    if (n * k * d * (int64_t)sizeof(T) > CACHE_BYTES) return launch_combine<T, N, true>(rows, n, d, k, position, held, weights, y, s);
+    return launch_combine<T, N, false>(rows, n, d, k, position, held, weights, y, s);
 }
 
-template <typename T, int N, int L, int C>
+template <typename T, int N, int L, int C, bool ONCE = false>
 int launch_combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
                         const float *weights, void *grad_rows, float *grad_weights, hipStream_t s) {
-    hipLaunchKernelGGL((k_combine_grad<T, N, L, C>), dim3(blocks_of(n, 256 / L)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
-                       reinterpret_cast<const T *>(g), n, d, k, position, held, weights, reinterpret_cast<T *>(grad_rows),
-                       grad_weights);
+    hipLaunchKernelGGL((k_combine_grad<T, N, L, C, ONCE>), dim3(blocks_of(n, 256 / L)), dim3(256), 0, s,
+                       reinterpret_cast<const T *>(rows), reinterpret_cast<const T *>(g), n, d, k, position, held, weights,
+                       reinterpret_cast<T *>(grad_rows), grad_weights);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -707,11 +732,18 @@ int combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const
                  const float *weights, void *grad_rows, float *grad_weights, hipStream_t s) {
     constexpr int N = 16 / (int)sizeof(T);
     const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)g | (uintptr_t)grad_rows) % 16 == 0;
-    if (!vec)
-        return launch_combine_grad<T, 1, 64, 4>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    const bool once = n * k * d * (int64_t)sizeof(T) > CACHE_BYTES;
+    if (!vec) return launch_combine_grad<T, 1, 64, 4>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
     if (d / N <= 8) return launch_combine_grad<T, N, 8, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    if (d / N <= 16) return launch_combine_grad<T, N, 16, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    if (d / N <= 32) return launch_combine_grad<T, N, 32, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (d / N <= 16) {
+        if (once) return launch_combine_grad<T, N, 16, 1, true>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+        return launch_combine_grad<T, N, 16, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    }
+    if (d / N <= 32) {
+        if (once) return launch_combine_grad<T, N, 32, 1, true>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+        return launch_combine_grad<T, N, 32, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    }
+    if (once) return launch_combine_grad<T, N, 64, 2, true>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
     return launch_combine_grad<T, N, 64, 2>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
 }
 
