@@ -483,7 +483,7 @@ int mtp_combine_rows_grad(int dtype, const void *rows, const void *g, int64_t n,
 /* y = act(x W^T + bias) + residual, act 0 none, 1 relu, 2 gelu (erf), 3 silu.  x [rows][in] (ldx), residual [rows][out] (ldr),
  * y [rows][out].  offsets NULL: w [out][in], bias [out].  Else rows are sorted by set: rows [offsets[s], offsets[s + 1]) use
  * w[s] and bias[s] of w [n_sets][out][in], bias [n_sets][out]; rows behind offsets[n_sets] become zero.  bias, residual and pre may
- * be NULL; pre [rows][out] receives x W^T + bias.  in, out, n_sets <= 65536.
+ * be NULL; pre [rows][out] receives x W^T + bias.  in, out <= 65536, n_sets <= 65535.
  * mtp_linear_workspace_bytes: a, lda = the first matrix of the step (x; dz; dz), b, ldb = the second (w; w; x).  Operands whose
  * rows do not start on 4 bytes (odd sizes of 16-bit types) are laid out anew in it, and a weight gradient over many rows is
  * summed in parts. */

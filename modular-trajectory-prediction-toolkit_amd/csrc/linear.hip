@@ -50,13 +50,50 @@ __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g
     }
 }
 
-// the parts of a split weight gradient, added in their order
-template <typename T>
-__global__ __launch_bounds__(256) void k_linear_join(const float *__restrict__ partial, int splits, int64_t n, T *__restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float s = 0.f;
-        for (int p = 0; p < splits; ++p) s += partial[(int64_t)p * n + i];
-        out[i] = from_f32<T>(s);
+// The parts of a cut weight gradient, added in a fixed order: G groups of parts side by side, then the groups.  A workgroup takes
+// 1024 / G elements of one set; sets in one part are done already.
+template <typename T, int G>
+__global__ __launch_bounds__(256) void k_linear_join(LinArgs a) {
+    constexpr int E = 256 / G;  // threads of a group, four elements each
+    __shared__ f32x4v sums[256];
+    const int mine = threadIdx.x % E, group = threadIdx.x / E, set = blockIdx.y;
+    int64_t first = 0;
+    int count = lin_pieces(a.rows, a.part_bits, 1);
+    if (a.offsets != nullptr) {
+        int64_t lo, hi;
+        lin_bounds(a.offsets, set, a.n_sets, a.rows, &lo, &hi);
+        count = lin_pieces(hi - lo, a.part_bits, 1);
+        if (count <= 1) return;
+        first = lin_parts_before(a.offsets, a.n_sets, set, a.rows, a.part_bits);
+    }
+    if (count <= 1 || first + count > a.parts) return;
+    const int64_t weights = (int64_t)a.out_rows * a.cols, all = weights + (a.bias_out != nullptr ? a.out_rows : 0);
+    // the weights' sums, then the bias', are one row of `all` elements; four neighbours may span the border
+    const int64_t i0 = ((int64_t)blockIdx.x * E + mine) * 4;
+    f32x4v s = {0.f, 0.f, 0.f, 0.f};
+    if (i0 + 4 <= weights && weights % 4 == 0) {
+        const float *at = a.partial + first * weights + i0;
+#pragma unroll 4
+        for (int p = group; p < count; p += G) s += *reinterpret_cast<const f32x4v *>(at + p * weights);
+    } else {
+        for (int e = 0; e < 4; ++e) {
+            const int64_t i = i0 + e;
+            if (i >= all) break;
+            const float *at = i < weights ? a.partial + first * weights + i : a.partial_bias + first * a.out_rows + (i - weights);
+            const int64_t step = i < weights ? weights : a.out_rows;
+            for (int p = group; p < count; p += G) s[e] += at[p * step];
+        }
+    }
+    if constexpr (G > 1) {
+        sums[threadIdx.x] = s;
+        __syncthreads();
+        if (group != 0) return;
+        for (int g = 1; g < G; ++g) s += sums[g * E + mine];
+    }
+    for (int e = 0; e < 4; ++e) {
+        const int64_t i = i0 + e;
+        if (i < weights) reinterpret_cast<T *>(a.out)[set * weights + i] = from_f32<T>(s[e]);
+        else if (i < all) reinterpret_cast<T *>(a.bias_out)[(int64_t)set * a.out_rows + (i - weights)] = from_f32<T>(s[e]);
     }
 }
 
@@ -104,13 +141,63 @@ int relayout(const void **p, int64_t *ld, int64_t rows, int cols, char **ws, hip
     return MTP_OK;
 }
 
-int splits_for(int64_t rows, int in, int out, int n_sets, int dtype) {
-    const int64_t tiles = (int64_t)n_sets * ((out + 127) / 128) * ((in + 127) / 128);
-    const int64_t mean = rows / n_sets;
-    int64_t s = (512 + tiles - 1) / tiles;
-    const int64_t most = mean / (4 * 128 / elem_size(dtype));
-    if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s);
+// Which tile: columns x rows of the output a workgroup owns.  Measured on the card, microseconds of one product:
+//   TILE_32x128   few columns (143 760 rows, 256 -> 24, bfloat16: 20, 24 with 64x64, 29 with 128x128), few tiles in all
+//                 (1024 rows, 256 -> 200: 5.1, 6.9 with 128x128), float with up to 96 columns (73 568 rows, 512 -> 96: 72,
+//                 82 with 96x128, 113 with 128x128)
+//   TILE_64x64    few tiles and few rows; weight gradients of float (8192 rows, 512 x 512: 65, 75 with 128x64)
+//   TILE_64x128   up to 64 columns (300 000 rows, 96 -> 64: 18, 25 with 128x64)
+//   TILE_96x128   up to 96 columns of 16-bit types (143 760 rows, 256 -> 96: 30, 31 with 128x64, 37 with 32x128)
+//   TILE_128x64   most others: three workgroups a CU (143 760 rows, 96 -> 256 with gelu: 62, 67 with 128x128)
+//   TILE_128x128  input and weight gradients of 16-bit types, whose products are longer than their way out (143 760 rows,
+//                 24 -> 256: 33, 37 with 128x64)
+//   TILE_256x256  long sums of 16-bit types that fill the card with such tiles (32 768 rows, 2048 -> 2048: 276, 337 with
+//                 128x128): half the LDS traffic a product
+enum LinTileShape { TILE_32x128, TILE_64x64, TILE_64x128, TILE_96x128, TILE_128x64, TILE_128x128, TILE_256x256 };
+
+int64_t tiles_of(int64_t rows, int64_t cols, int bc, int br) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); }
+
+LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, bool grouped) {
+    if (mode == MTP_LINEAR_GRAD_WEIGHT) {  // rows, cols: of the gradient
+        if (!half) return cols <= 96 ? TILE_32x128 : TILE_64x64;
+        if (cols <= 32) return TILE_32x128;
+        if (rows <= 64) return cols <= 64 ? TILE_64x64 : TILE_128x64;
+        if (cols <= 64) return TILE_64x128;
+        if (cols <= 96) return TILE_96x128;
+        return tiles_of(rows, cols, 128, 128) >= 64 ? TILE_128x128 : TILE_128x64;
+    }
+    if (cols <= 32) return TILE_32x128;
+    if (tiles_of(rows, cols, 64, 64) < 512) return rows < 128 ? TILE_64x64 : TILE_32x128;
+    if (cols <= 64) return TILE_64x128;
+    if (cols <= 96) return half ? TILE_96x128 : TILE_32x128;
+    if (half && !grouped && k >= 512 && tiles_of(rows, cols, 256, 256) >= 192) return TILE_256x256;
+    if (half && mode == MTP_LINEAR_GRAD_INPUT) return TILE_128x128;
+    return TILE_128x64;
+}
+
+// Rows of x that one workgroup of the weight gradient sums, as a power of two.  One matrix: some 1024 workgroups, 2048 of big
+// tiles (32 768 rows, 2048 x 2048: 374 us with 2048 workgroups, 455 with 1024, 617 with 512).  Many: sets differ in size by a
+// factor of ten, and the longest one is what the others wait for.
+int part_bits_for(int64_t rows, int in, int out, int n_sets, bool half) {
+    int64_t tiles;
+    int64_t most = 1024;
+    switch (pick_tile(MTP_LINEAR_GRAD_WEIGHT, half, out, in, rows, n_sets > 1)) {
+        case TILE_32x128: tiles = tiles_of(out, in, 32, 128); break;
+        case TILE_64x64: tiles = tiles_of(out, in, 64, 64); break;
+        case TILE_64x128: tiles = tiles_of(out, in, 64, 128); break;
+        case TILE_96x128: tiles = tiles_of(out, in, 96, 128); break;
+        case TILE_128x64: tiles = tiles_of(out, in, 128, 64); break;
+        default: tiles = tiles_of(out, in, 128, 128), most = 2048;
+    }
+    const int64_t part = rows * tiles / most;
+    int bits = 9;
+    while (bits < 30 && ((int64_t)1 << bits) < part) ++bits;
+    return bits;
+}
+// parts of the sets that have more than one: such a set has more rows than `part`, so fewer parts than twice its rows / part
+int64_t most_parts(int64_t rows, int n_sets, int bits) {
+    if (n_sets == 1) return (rows >> bits) == 0 ? 0 : (rows + ((int64_t)1 << bits) - 1) >> bits;
+    return (2 * rows) >> bits;
 }
 
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
@@ -121,7 +208,7 @@ int launch_tile(LinArgs a, hipStream_t s) {
     int64_t blocks;
     if (MODE == LIN_GRAD_WEIGHT) {
         a.row_tiles = (a.out_rows + BR - 1) / BR;
-        blocks = a.row_tiles * a.col_tiles * a.splits * a.n_sets;
+        blocks = a.row_tiles * a.col_tiles * ((a.rows >> a.part_bits) + a.n_sets);
     } else {
         // a set's last tile may be ragged, and so may the one behind the last set
         a.row_tiles = a.offsets == nullptr ? (a.rows + BR - 1) / BR : (a.rows + (int64_t)(a.n_sets + 1) * (BR - 1)) / BR;
@@ -137,18 +224,28 @@ int launch_tile(LinArgs a, hipStream_t s) {
 
 template <typename T, int MODE>
 int launch_product(const LinArgs &a, hipStream_t s) {
-    const int64_t r = MODE == LIN_GRAD_WEIGHT ? (int64_t)a.out_rows * a.n_sets * a.splits : a.rows;
-    const int64_t big = ((r + 127) / 128) * ((a.cols + 127) / 128);
-    if (big >= 256 && (a.offsets == nullptr || MODE == LIN_GRAD_WEIGHT || a.rows / a.n_sets >= 128))
-        return launch_tile<T, MODE, 128, 128, 64, 64>(a, s);
-    return launch_tile<T, MODE, 64, 64, 32, 32>(a, s);
+    const bool half = sizeof(T) == 2;
+    switch (pick_tile(MODE, half, MODE == LIN_GRAD_WEIGHT ? a.out_rows : a.rows, a.cols, a.k, a.offsets != nullptr)) {
+        case TILE_32x128: return launch_tile<T, MODE, 32, 128, 32, 32>(a, s);
+        case TILE_64x64: return launch_tile<T, MODE, 64, 64, 32, 32>(a, s);
+        case TILE_64x128: return launch_tile<T, MODE, 64, 128, 32, 64>(a, s);
+        case TILE_128x64: return launch_tile<T, MODE, 128, 64, 64, 32>(a, s);
+        case TILE_96x128:
+            if constexpr (sizeof(T) == 2) return launch_tile<T, MODE, 96, 128, 96, 32>(a, s);
+        case TILE_128x128:
+            if constexpr (sizeof(T) == 2 && MODE != LIN_FORWARD) return launch_tile<T, MODE, 128, 128, 64, 64>(a, s);
+        case TILE_256x256:
+            if constexpr (sizeof(T) == 2 && MODE != LIN_GRAD_WEIGHT) return launch_tile<T, MODE, 256, 256, 128, 64>(a, s);
+    }
+    mtp_set_error("mtp_linear: no kernel of this shape");
+    return MTP_E_ARG;
 }
 
 int check_sizes(const char *who, int dtype, int64_t rows, int in, int out, const int32_t *offsets, int n_sets) {
     MTP_REQUIRE(dtype == MTP_FLOAT || dtype == MTP_BFLOAT16 || dtype == MTP_HALF, "%s: unknown type %d", who, dtype);
     MTP_REQUIRE(rows >= 0 && rows <= 0x7fffffff && in >= 1 && out >= 1 && in <= 65536 && out <= 65536,
                 "%s: bad shape rows=%lld in=%d out=%d", who, (long long)rows, in, out);
-    MTP_REQUIRE(n_sets >= 1 && n_sets <= 65536 && (offsets != nullptr || n_sets == 1), "%s: bad number of sets %d", who, n_sets);
+    MTP_REQUIRE(n_sets >= 1 && n_sets <= 65535 && (offsets != nullptr || n_sets == 1), "%s: bad number of sets %d", who, n_sets);
     return MTP_OK;
 }
 
@@ -228,21 +325,23 @@ int grad_weight(const void *dz, int64_t rows, int out, int64_t lddz, const void 
     a.offsets = offsets;
     a.n_sets = n_sets;
     a.k = (int)rows;
-    a.splits = splits_for(rows, in, out, n_sets, sizeof(T) == 4 ? MTP_FLOAT : MTP_BFLOAT16);
+    a.part_bits = part_bits_for(rows, in, out, n_sets, sizeof(T) == 2);
+    const int64_t parts = most_parts(rows, n_sets, a.part_bits);
     a.out = dw;
     a.bias_out = db;
     a.partial = reinterpret_cast<float *>(ws);
+    a.partial_bias = a.partial + parts * out * in;
+    a.parts = parts;
     rc = launch_product<T, LIN_GRAD_WEIGHT>(a, s);
-    if (rc != MTP_OK || a.splits == 1) return rc;
-    const int64_t n = (int64_t)n_sets * out * in;
-    hipLaunchKernelGGL(k_linear_join<T>, dim3(grid_for(n)), dim3(256), 0, s, a.partial, a.splits, n, reinterpret_cast<T *>(dw));
+    if (rc != MTP_OK || parts == 0) return rc;
+    const int64_t all = (int64_t)out * (in + 1);
+    if (n_sets == 1 && parts >= 32)
+        hipLaunchKernelGGL((k_linear_join<T, 16>), dim3((unsigned)((all + 63) / 64), 1), dim3(256), 0, s, a);
+    else if (n_sets == 1 && parts >= 8)
+        hipLaunchKernelGGL((k_linear_join<T, 4>), dim3((unsigned)((all + 255) / 256), 1), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_linear_join<T, 1>), dim3((unsigned)((all + 1023) / 1024), (unsigned)n_sets), dim3(256), 0, s, a);
     MTP_LAUNCH_CHECK();
-    if (db != nullptr) {
-        const int64_t m = (int64_t)n_sets * out;
-        hipLaunchKernelGGL(k_linear_join<T>, dim3(grid_for(m)), dim3(256), 0, s, a.partial + (int64_t)a.splits * n, a.splits, m,
-                           reinterpret_cast<T *>(db));
-        MTP_LAUNCH_CHECK();
-    }
     return MTP_OK;
 }
 
@@ -258,9 +357,7 @@ extern "C" int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows,
     if (step == MTP_LINEAR_FORWARD) return relayout_bytes(dtype, a, lda, rows, in) + relayout_bytes(dtype, b, in, w_rows, in);
     if (step == MTP_LINEAR_GRAD_INPUT) return relayout_bytes(dtype, a, lda, rows, out) + relayout_bytes(dtype, b, in, w_rows, in);
     int64_t n = relayout_bytes(dtype, a, lda, rows, out) + relayout_bytes(dtype, b, ldb, rows, in);
-    const int s = splits_for(rows, in, out, n_sets, dtype);
-    if (s > 1) n += (int64_t)s * w_rows * (in + 1) * 4;
-    return n;
+    return n + most_parts(rows, n_sets, part_bits_for(rows, in, out, n_sets, elem_size(dtype) == 2)) * out * (in + 1) * 4;
 }
 
 extern "C" int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias,

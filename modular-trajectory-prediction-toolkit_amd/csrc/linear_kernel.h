@@ -55,6 +55,11 @@ __device__ __forceinline__ void buffer_lds16(i32x4v rsrc, unsigned voff, unsigne
         : "memory");
 }
 __device__ __forceinline__ void dma_wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until at most N of this wave's loads are in flight (they land in their order)
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // Buffer descriptor of [p, p + bytes), raw; p and bytes are the same in every lane.
 __device__ __forceinline__ i32x4v make_rsrc(const void *p, int64_t bytes) {
@@ -92,7 +97,8 @@ struct LinTile {
 
     // RC: what is added to a piece's place in its k row
     static __device__ __forceinline__ int twist(int k) {
-        if constexpr (SZ == 4) return 8 * ((k >> 2) & 1);
+        if constexpr (SZ == 4) return RB % 256 == 0 ? 8 * ((k >> 2) & 1) : 0;
+        else if constexpr (RB % 128 == 64) return 0;  // four rows fall on four different quarters of the bank line by themselves
         else if constexpr (RB == 128) return 4 * ((k >> 1) & 1);
         else return 4 * (k & 3);
     }
@@ -215,7 +221,7 @@ struct LinReader {
         } else {
             const int i = lane_ & 31, h = lane_ >> 5;
             const int col = col0_ + f * 32 + i;
-            const int piece = (col >> 2) ^ (8 * h);
+            const int piece = (col >> 2) ^ LinTile<T, false, R, 64>::twist(4 * h);
             const char *p = lds + (s * 8 + 4 * h) * RB + piece * 16 + (col & 3) * 4;
             frag v;
 #pragma unroll
@@ -235,43 +241,105 @@ __device__ __forceinline__ void lin_bounds(const int32_t *offsets, int e, int n_
     *hi = b;
 }
 
-__device__ __forceinline__ int64_t lin_uniform(int64_t v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
-    return (int64_t)(((uint64_t)hi << 32) | lo);
+constexpr int lin_log2(int v) { return v <= 1 ? 0 : 1 + lin_log2(v / 2); }
+
+// prefix sum over the 64 lanes
+__device__ __forceinline__ int lin_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 to the second 16, lane 47 to the fourth
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 to the upper 32
+    return v;
 }
 
-// The set and the rows of row tile `tile`, tiles of BR rows counted set after set; the rows behind the last set come last,
-// as "set" n_sets.  Every wave finds it for itself: 64 sets at a time, a prefix sum over the lanes.
-template <int BR>
-__device__ __forceinline__ bool lin_find_tile(const int32_t *offsets, int n_sets, int64_t rows, int64_t tile, int *set, int64_t *row0,
-                                              int64_t *row_end) {
-    const int lane = threadIdx.x & 63;
-    int64_t before = 0;
-    for (int e0 = 0; e0 <= n_sets; e0 += 64) {
-        const int e = e0 + lane;
-        int64_t lo = 0, hi = 0;
-        if (e <= n_sets) lin_bounds(offsets, e, n_sets, rows, &lo, &hi);
-        const int mine = (int)((hi - lo + BR - 1) / BR);
-        int sum = mine;
+// What a set's rows are cut into: row tiles of BR rows, or for the weight gradient parts of `part` rows, one at least (a set
+// without rows has a gradient of zero).
+// What a piece is: 1 << part_bits rows.
+__device__ __forceinline__ int lin_pieces(int64_t len, int part_bits, int least) {
+    const int n = (int)(((uint32_t)len + (1u << part_bits) - 1) >> part_bits);
+    return n < least ? least : n;
+}
+
+struct LinPiece {
+    int set, count;     // the set and the number of its pieces
+    int64_t index;      // which of them
+    int64_t lo, hi;     // the set's rows
+    int64_t split_at;   // CUT: pieces of sets with more than one piece before this set
+};
+
+// Eight neighbouring sets a lane, 512 a wave: the numbers of pieces of the sets from e0 + 8 * lane on (0 beyond `last`).
+__device__ __forceinline__ void lin_count(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least, int e0,
+                                          int (&lo)[8], int (&len)[8], int (&n)[8]) {
+    const int first = e0 + (int)(threadIdx.x & 63) * 8;
+    int at[9];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int up = __shfl_up(sum, d);
-            if (lane >= d) sum += up;
+    for (int u = 0; u < 9; ++u) at[u] = offsets[first + u < n_sets ? first + u : n_sets];  // all on their way at once
+    const int top = (int)rows;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int a = min(max(at[u], 0), top);
+        const int b = first + u < n_sets ? min(max(at[u + 1], a), top) : top;
+        lo[u] = a;
+        len[u] = b - a;
+        n[u] = first + u <= last ? lin_pieces(b - a, part_bits, least) : 0;
+    }
+}
+
+// Piece number `piece`, counted set after set (`last`: number of the last set; the rows behind the sets are "set" n_sets).  Every
+// wave finds it for itself: a prefix sum over the lanes finds the eight sets, and their counts are read across.
+template <bool CUT>
+__device__ __forceinline__ bool lin_find(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least, int64_t piece,
+                                         LinPiece *out) {
+    int64_t before = 0, split_before = 0;
+    for (int e0 = 0; e0 <= last; e0 += 512) {
+        int lo[8], len[8], n[8], mine = 0, many = 0;
+        lin_count(offsets, n_sets, last, rows, part_bits, least, e0, lo, len, n);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            mine += n[u];
+            if (CUT) many += n[u] > 1 ? n[u] : 0;
         }
-        const int64_t first = before + sum - mine;
-        const uint64_t hit = __ballot(mine > 0 && tile >= first && tile < first + mine);
+        const int upto = lin_scan(mine), many_upto = CUT ? lin_scan(many) : 0;
+        const int64_t want = piece - before;
+        const uint64_t hit = __ballot(want >= upto - mine && want < upto);
         if (hit != 0) {
-            const int src = __ffsll((unsigned long long)hit) - 1;
-            const int64_t f = __shfl((long long)first, src), l = __shfl((long long)lo, src), h = __shfl((long long)hi, src);
-            *set = e0 + src;
-            *row0 = lin_uniform(l + (tile - f) * BR);
-            *row_end = lin_uniform(h);
-            return true;
+            const int src = __builtin_ctzll(hit);
+            int at = __builtin_amdgcn_readlane(upto - mine, src), split_at = __builtin_amdgcn_readlane(many_upto - many, src);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int c = __builtin_amdgcn_readlane(n[u], src);
+                if (want < at + c) {
+                    out->set = e0 + src * 8 + u;
+                    out->count = c;
+                    out->index = want - at;
+                    out->lo = __builtin_amdgcn_readlane(lo[u], src);
+                    out->hi = out->lo + __builtin_amdgcn_readlane(len[u], src);
+                    out->split_at = split_before + split_at;
+                    return true;
+                }
+                at += c;
+                split_at += c > 1 ? c : 0;
+            }
         }
-        before += __shfl(sum, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
+        split_before += __builtin_amdgcn_readlane(many_upto, 63);
     }
     return false;
+}
+
+// parts of the sets before `set` that are cut into more than one
+__device__ __forceinline__ int64_t lin_parts_before(const int32_t *offsets, int n_sets, int set, int64_t rows, int part_bits) {
+    int64_t before = 0;
+    for (int e0 = 0; e0 < set; e0 += 512) {
+        int lo[8], len[8], n[8], many = 0;
+        lin_count(offsets, n_sets, set - 1, rows, part_bits, 1, e0, lo, len, n);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) many += n[u] > 1 ? n[u] : 0;
+        before += __builtin_amdgcn_readlane(lin_scan(many), 63);
+    }
+    return before;
 }
 
 enum { LIN_NONE = 0, LIN_RELU = 1, LIN_GELU = 2, LIN_SILU = 3 };
@@ -328,7 +396,8 @@ struct LinArgs {
     const int32_t *offsets;  // [n_sets + 1] or NULL
     int n_sets;
     int64_t row_tiles;
-    int col_tiles, out_rows, splits;  // weight gradient: rows of the output, parts of the summed axis
+    int col_tiles;
+    int out_rows, part_bits;  // weight gradient: rows of the output; a workgroup sums 1 << part_bits rows of x
     const void *bias;
     const void *residual;
     int64_t ld_res;
@@ -336,7 +405,9 @@ struct LinArgs {
     void *out;
     void *pre;
     void *bias_out;
-    float *partial;  // weight gradient with splits > 1: [splits][n_sets][out_rows][cols] then [splits][n_sets][out_rows]
+    float *partial;  // weight gradient: the sums of sets that are cut into parts, [parts][out_rows][cols], ...
+    float *partial_bias;  // ... and [parts][out_rows]
+    int64_t parts;        // room for so many
 };
 
 // N consecutive elements
@@ -374,69 +445,100 @@ __device__ __forceinline__ int64_t lin_xcd_order(int64_t id, int64_t n) {
     return id < per * 8 ? (id % 8) * per + id / 8 : id;
 }
 
+// a piece's place in a row of `pieces` may be twisted by these bits of the row's number
+constexpr int lin_twist_mask(int pieces) { return (pieces & -pieces) < 32 ? (pieces & -pieces) - 1 : 31; }
+// the largest power of two that is at most `room` and `rows`
+constexpr int lin_pass_rows(int room, int rows) {
+    int n = 1;
+    while (n * 2 <= room && n * 2 <= rows) n *= 2;
+    return n;
+}
+
 enum { LIN_FORWARD = 0, LIN_GRAD_INPUT = 1, LIN_GRAD_WEIGHT = 2 };
 
-// A tile's rows on their way out of LDS, N columns a thread; U is the type they leave in.
+// A tile's rows on their way out of LDS, N columns a thread; U is the type they leave in.  Four rows are on their way at a time.
 template <typename T, typename U, int MODE, int BC, int ER, int NT, int N>
-__device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, U *to, int set, int64_t r0, int64_t row_end, int64_t c0,
-                                          int tid) {
+__device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, const float *bias, U *to, int64_t r0, int64_t row_end,
+                                          int64_t c0, int tid) {
     constexpr int ITEMS = BC / N, STEP = NT / ITEMS;  // items of a row; rows that the workgroup takes at a time
-    constexpr int PM = (BC / 4 < 32 ? BC / 4 : 32) - 1;
+    constexpr int PM = lin_twist_mask(BC / 4), AT_ONCE = ER / STEP < 4 ? (ER / STEP < 1 ? 1 : ER / STEP) : 4;
     const int item = tid % ITEMS;
     const int64_t col = c0 + item * N;
-    if (col >= a.cols) return;  // (16-byte pieces: cols is a multiple of N)
-    float bias[N];
+    if (col >= a.cols || tid >= ITEMS * STEP) return;  // (16-byte pieces: cols is a multiple of N)
+    const int rows = (int)(row_end - r0 < ER ? row_end - r0 : ER);
+    for (int row0 = tid / ITEMS; row0 < rows; row0 += STEP * AT_ONCE) {
+        float v[AT_ONCE][N], res[AT_ONCE][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) bias[e] = 0.f;
-    if constexpr (MODE == LIN_FORWARD) {
-        if (a.bias != nullptr) {
-            const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols + col;
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int row = row0 + u * STEP < rows ? row0 + u * STEP : row0;
+            if constexpr (N == 1) {
+                v[u][0] = z[row * BC + (((item >> 2) ^ (row & PM)) << 2) + (item & 3)];
+            } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) bias[e] = to_f32(b[e]);
-        }
-    }
-    for (int row = tid / ITEMS; row < ER; row += STEP) {
-        const int64_t r = r0 + row;
-        if (r >= row_end) break;
-        float v[N];
-        if constexpr (N == 1) {
-            v[0] = z[row * BC + (((item >> 2) ^ (row & PM)) << 2) + (item & 3)];
-        } else {
+                for (int q = 0; q < N / 4; ++q) {
+                    const f32x4v w = *reinterpret_cast<const f32x4v *>(z + row * BC + (((item * (N / 4) + q) ^ (row & PM)) << 2));
 #pragma unroll
-            for (int q = 0; q < N / 4; ++q) {
-                const f32x4v w = *reinterpret_cast<const f32x4v *>(z + row * BC + (((item * (N / 4) + q) ^ (row & PM)) << 2));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[q * 4 + e] = w[e];
+                    for (int e = 0; e < 4; ++e) v[u][q * 4 + e] = w[e];
+                }
+            }
+            if constexpr (MODE == LIN_FORWARD) {
+                if (a.residual != nullptr)
+                    lin_load<T, N>(reinterpret_cast<const T *>(a.residual) + (r0 + row) * a.ld_res + col, res[u]);
             }
         }
-        const int64_t at = r * a.cols + col;
         if constexpr (MODE == LIN_FORWARD) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] += bias[e];
-            if (a.pre != nullptr) lin_store<T, N>(reinterpret_cast<T *>(a.pre) + at, v);
-            if (a.act == LIN_GELU) {
+            for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[e] = lin_act(v[e], LIN_GELU);
-            } else if (a.act == LIN_SILU) {
+                for (int e = 0; e < N; ++e) v[u][e] += bias[e];
+            if (a.pre != nullptr) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[e] = lin_act(v[e], LIN_SILU);
-            } else if (a.act == LIN_RELU) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[e] = lin_act(v[e], LIN_RELU);
+                for (int u = 0; u < AT_ONCE; ++u)
+                    if (row0 + u * STEP < rows)
+                        lin_store<T, N>(reinterpret_cast<T *>(a.pre) + (r0 + row0 + u * STEP) * a.cols + col, v[u]);
             }
-            if (a.residual != nullptr) {
-                float res[N];
-                lin_load<T, N>(reinterpret_cast<const T *>(a.residual) + r * a.ld_res + col, res);
+            auto bend = [&](auto kind) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[e] += res[e];
+                for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[u][e] = lin_act(v[u][e], decltype(kind)::value);
+            };
+            if (a.act == LIN_GELU) bend(std::integral_constant<int, LIN_GELU>{});
+            else if (a.act == LIN_SILU) bend(std::integral_constant<int, LIN_SILU>{});
+            else if (a.act == LIN_RELU) bend(std::integral_constant<int, LIN_RELU>{});
+            if (a.residual != nullptr) {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[u][e] += res[u][e];
             }
         }
-        lin_store<U, N>(to + at, v);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            if (row0 + u * STEP < rows) lin_store<U, N>(to + (r0 + row0 + u * STEP) * a.cols + col, v[u]);
     }
+}
+// the bias of the columns that lin_leave gives this thread
+template <typename T, int BC, int N>
+__device__ __forceinline__ void lin_bias(const LinArgs &a, int set, int64_t c0, int tid, float *bias) {
+    const int64_t col = c0 + tid % (BC / N) * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) bias[e] = 0.f;
+    if (a.bias == nullptr || col >= a.cols) return;
+    const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols + col;
+#pragma unroll
+    for (int e = 0; e < N; ++e) bias[e] = to_f32(b[e]);
+}
+
+// waves a SIMD that a tile's 2 * (BC + BR) * 128 bytes of LDS leave room for (160 KB a CU): what the registers have to allow
+constexpr int lin_waves(int bc, int br, int threads) {
+    const int groups = 160 * 1024 / (2 * (bc + br) * 128);
+    const int waves = groups * threads / 256;
+    return waves < 1 ? 1 : waves > 4 ? 4 : waves;
 }
 
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
-__global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinArgs a) {
+__global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * (BC / WC) * (BR / WR))) void k_linear_tile(LinArgs a) {
     constexpr int NT = 64 * (BC / WC) * (BR / WR);
     constexpr bool PKC = MODE == LIN_FORWARD, QKC = MODE != LIN_GRAD_WEIGHT;
     constexpr int SZ = sizeof(T), BK = 128 / SZ;
@@ -448,33 +550,37 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
     const int wc = wave % (BC / WC), wr = wave / (BC / WC);
 
     int64_t id = lin_xcd_order(blockIdx.x, gridDim.x);
-    int64_t row0 = 0, row_end = 0, k_lo = 0, k_len = a.k;
-    int set = 0, split = 0;
+    int64_t row0 = 0, row_end = 0, k_lo = 0, k_len = a.k, part_at = -1;
+    int set = 0;
     const int ct = (int)(id % a.col_tiles);
     id /= a.col_tiles;
     const int64_t c0 = (int64_t)ct * BC;
     if constexpr (MODE == LIN_GRAD_WEIGHT) {
-        const int rt = (int)(id % a.row_tiles);
+        row0 = (int64_t)(id % a.row_tiles) * BR;
         id /= a.row_tiles;
-        split = (int)(id % a.splits);
-        set = (int)(id / a.splits);
-        row0 = (int64_t)rt * BR;
         row_end = a.out_rows;
-        int64_t lo = 0, hi = a.rows;
-        if (a.offsets != nullptr) lin_bounds(a.offsets, set, a.n_sets, a.rows, &lo, &hi);
-        const int64_t part = ((hi - lo + a.splits - 1) / a.splits + BK - 1) / BK * BK;
-        k_lo = lo + part * split;
-        k_lo = k_lo < hi ? k_lo : hi;
-        k_len = hi - k_lo < part ? hi - k_lo : part;
+        LinPiece p{0, lin_pieces(a.rows, a.part_bits, 1), id, 0, a.rows, 0};
+        if (a.offsets == nullptr ? id >= p.count : !lin_find<true>(a.offsets, a.n_sets, a.n_sets - 1, a.rows, a.part_bits, 1, id, &p)) return;
+        set = p.set;
+        k_lo = p.lo + (p.index << a.part_bits);
+        k_len = p.hi - k_lo < (1 << a.part_bits) ? p.hi - k_lo : (int64_t)1 << a.part_bits;
+        if (p.count > 1) {
+            part_at = p.split_at + p.index;
+            if (part_at >= a.parts) return;  // offsets that overlap: more parts than there can be
+        }
     } else if (a.offsets != nullptr) {
-        if (!lin_find_tile<BR>(a.offsets, a.n_sets, a.rows, id, &set, &row0, &row_end)) return;
+        LinPiece p;
+        if (!lin_find<false>(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, id, &p)) return;
+        set = p.set;
+        row0 = p.lo + p.index * BR;
+        row_end = p.hi;
     } else {
         row0 = id * BR;
         row_end = a.rows;
     }
     T *out = reinterpret_cast<T *>(a.out);
     if (MODE != LIN_GRAD_WEIGHT && set == a.n_sets) {  // rows behind the last set
-        for (int64_t i = tid; i < (int64_t)BR * BC; i += NT) {
+        for (int i = tid; i < BR * BC; i += NT) {
             const int64_t r = row0 + i / BC, c = c0 + i % BC;
             if (r < row_end && c < a.cols) {
                 out[r * a.cols + c] = (T)0.f;
@@ -546,10 +652,15 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
         q_left -= q_step;
         k_left -= BK;
     };
+    // both buffers are on their way before the first is used; later tiles are fetched one ahead
+    constexpr int IN_FLIGHT = LinTile<T, PKC, BC, NT>::PER + LinTile<T, QKC, BR, NT>::PER;
     if (n_steps > 0) fetch(0);
+    if (n_steps > 1) fetch(1);
     for (int64_t t = 0; t < n_steps; ++t) {
-        dma_wait_all();
-        __syncthreads();  // tile t has landed, and nobody reads the other buffer any more
+        if (t == 0 && n_steps > 1) dma_wait<IN_FLIGHT>();
+        else dma_wait_all();
+        __syncthreads();  // tile t has landed for every wave, and nobody reads the other buffer any more
+        if (t > 0 && t + 1 < n_steps) fetch((int)((t + 1) & 1));
         char *buf = smem + (t & 1) * STAGE;
         const int64_t left = k_len - t * BK;
         if constexpr (PKC || QKC) {
@@ -559,7 +670,6 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
                 __syncthreads();
             }
         }
-        if (t + 1 < n_steps) fetch((int)((t + 1) & 1));
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             typename LinMfma<T>::frag fp[FC], fq[FR];
@@ -585,17 +695,22 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
     // with 16 bytes each.  The sums go through LDS (as floats, pieces of 16 bytes placed at p ^ row so that neither side
     // conflicts), and whole rows of the tile leave in 16-byte pieces; bias, activation and residual are applied on the way.
     const int i = lane & 31, h = lane >> 5;
-    constexpr int ER = 2 * STAGE / (BC * 4) < BR ? 2 * STAGE / (BC * 4) : BR;  // rows per pass
-    constexpr int PM = (BC / 4 < 32 ? BC / 4 : 32) - 1;
+    constexpr int ER = lin_pass_rows(2 * STAGE / (BC * 4), BR);  // rows per pass
+    constexpr int PM = lin_twist_mask(BC / 4);
     static_assert(BR % ER == 0 && ER % WR == 0, "a wave's rows are in one pass");
     float *z = reinterpret_cast<float *>(smem);
-    const bool to_partial = MODE == LIN_GRAD_WEIGHT && a.splits > 1;
+    const bool to_partial = MODE == LIN_GRAD_WEIGHT && part_at >= 0;
     bool vec = lin_aligned16<T>(a.out, a.cols);
     if constexpr (MODE == LIN_FORWARD) {
         if (a.residual != nullptr) vec = vec && lin_aligned16<T>(a.residual, a.ld_res);
         if (a.pre != nullptr) vec = vec && lin_aligned16<T>(a.pre, a.cols);
     }
     if (to_partial) vec = a.cols % 4 == 0;
+    float bias[16 / SZ];
+    if constexpr (MODE == LIN_FORWARD) {
+        if (vec) lin_bias<T, BC, 16 / SZ>(a, set, c0, tid, bias);
+        else lin_bias<T, BC, 1>(a, set, c0, tid, bias);
+    }
     for (int p0 = 0; p0 < BR; p0 += ER) {
         __syncthreads();
         if (wr * WR >= p0 && wr * WR < p0 + ER) {
@@ -616,13 +731,13 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
         __syncthreads();
         const int64_t r0 = row0 + p0;
         if (to_partial) {
-            float *part = a.partial + ((int64_t)split * a.n_sets + set) * a.out_rows * a.cols;
-            if (vec) lin_leave<T, float, MODE, BC, ER, NT, 4>(a, z, part, set, r0, row_end, c0, tid);
-            else lin_leave<T, float, MODE, BC, ER, NT, 1>(a, z, part, set, r0, row_end, c0, tid);
+            float *part = a.partial + part_at * a.out_rows * a.cols;
+            if (vec) lin_leave<T, float, MODE, BC, ER, NT, 4>(a, z, bias, part, r0, row_end, c0, tid);
+            else lin_leave<T, float, MODE, BC, ER, NT, 1>(a, z, bias, part, r0, row_end, c0, tid);
         } else {
             T *to = out + (MODE == LIN_GRAD_WEIGHT ? (int64_t)set * a.out_rows * a.cols : 0);
-            if (vec) lin_leave<T, T, MODE, BC, ER, NT, 16 / SZ>(a, z, to, set, r0, row_end, c0, tid);
-            else lin_leave<T, T, MODE, BC, ER, NT, 1>(a, z, to, set, r0, row_end, c0, tid);
+            if (vec) lin_leave<T, T, MODE, BC, ER, NT, 16 / SZ>(a, z, bias, to, r0, row_end, c0, tid);
+            else lin_leave<T, T, MODE, BC, ER, NT, 1>(a, z, bias, to, r0, row_end, c0, tid);
         }
     }
     if constexpr (MODE == LIN_GRAD_WEIGHT) {
@@ -631,12 +746,8 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR)) void k_linear_tile(LinA
             for (int r = 0; r < FR; ++r) {
                 const int64_t row = row0 + wr * WR + r * 32 + i;
                 if (row < row_end) {
-                    const int64_t at = (int64_t)set * a.out_rows + row;
-                    if (a.splits > 1)
-                        a.partial[(int64_t)a.splits * a.n_sets * a.out_rows * a.cols +
-                                  (int64_t)split * a.n_sets * a.out_rows + at] = acc_ones[r][0];
-                    else
-                        reinterpret_cast<T *>(a.bias_out)[at] = from_f32<T>(acc_ones[r][0]);
+                    if (part_at >= 0) a.partial_bias[part_at * a.out_rows + row] = acc_ones[r][0];
+                    else reinterpret_cast<T *>(a.bias_out)[(int64_t)set * a.out_rows + row] = from_f32<T>(acc_ones[r][0]);
                 }
             }
         }

@@ -622,8 +622,8 @@ def linear(x, weight, bias=None, activation=None, residual=None, offsets=None, w
     rows = x.shape[0]
     if x.shape[1] != i:
         raise ValueError(f"x has {x.shape[1]} features, weight takes {i}")
-    if not (1 <= i <= 65536 and 1 <= out <= 65536 and 1 <= s <= 65536):
-        raise ValueError(f"weight: sizes must be in [1, 65536], got shape {tuple(weight.shape)}")
+    if not (1 <= i <= 65536 and 1 <= out <= 65536 and 1 <= s <= 65535):
+        raise ValueError(f"weight: sizes must be in [1, 65536] ([1, 65535] matrices), got shape {tuple(weight.shape)}")
     ldx, ldr = _row_distance(x, "x"), 0
     if bias is not None:
         _like(bias, "bias", weight.dim() - 1, x, "x", shape=tuple(weight.shape[:-1]))
