@@ -117,6 +117,12 @@ unsigned grid_for(int64_t items) {
     return (unsigned)(b < 1 ? 1 : (b > 256 * 16 ? 256 * 16 : b));
 }
 
+// Tiles of 16 rows that k_linear_few works on at a time, 0: the rows are too many for it.
+int few_rows(int64_t rows, int n_sets) {
+    const int64_t mean = n_sets > 1 ? (rows + n_sets - 1) / n_sets : rows;
+    return mean <= 16 ? 1 : mean <= 32 ? 2 : mean <= 64 ? 4 : 0;
+}
+
 // rows of a 16-bit operand have to start on 4 bytes; a row distance beyond 2^20 elements would leave the loads' 32-bit offsets
 bool needs_relayout(int dtype, const void *p, int64_t ld) {
     return ld > (1 << 20) || (elem_size(dtype) == 2 && (ld % 2 != 0 || (uintptr_t)p % 4 != 0));
@@ -241,6 +247,20 @@ int launch_product(const LinArgs &a, hipStream_t s) {
     return MTP_E_ARG;
 }
 
+// Few rows (of each set): see k_linear_few.  RT tiles of 16 rows share a reading of W.
+template <typename T, int RT>
+int launch_few(LinArgs a, hipStream_t s) {
+    a.col_tiles = (a.cols + 15) / 16;
+    a.row_tiles = a.offsets == nullptr ? (a.rows + 16 * RT - 1) / (16 * RT)
+                                       : (a.rows + (int64_t)(a.n_sets + 1) * (16 * RT - 1)) / (16 * RT);
+    const int64_t most = a.offsets == nullptr ? a.row_tiles : a.row_tiles < a.rows ? a.row_tiles : a.rows;  // a tile has a row
+    const int64_t blocks = most * a.col_tiles;
+    MTP_REQUIRE(blocks <= 0x7fffffff, "mtp_linear: %lld workgroups are too many", (long long)blocks);
+    hipLaunchKernelGGL((k_linear_few<T, RT>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
 int check_sizes(const char *who, int dtype, int64_t rows, int in, int out, const int32_t *offsets, int n_sets) {
     MTP_REQUIRE(dtype == MTP_FLOAT || dtype == MTP_BFLOAT16 || dtype == MTP_HALF, "%s: unknown type %d", who, dtype);
     MTP_REQUIRE(rows >= 0 && rows <= 0x7fffffff && in >= 1 && out >= 1 && in <= 65536 && out <= 65536,
@@ -253,9 +273,12 @@ template <typename T>
 int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias, int act,
             const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre, char *ws, hipStream_t s) {
     int64_t ldw = in;
-    int rc = relayout<T>(&x, &ldx, rows, in, &ws, s);
-    if (rc == MTP_OK) rc = relayout<T>(&w, &ldw, (int64_t)n_sets * out, in, &ws, s);
-    if (rc != MTP_OK) return rc;
+    const int few = few_rows(rows, n_sets);
+    if (few == 0) {
+        int rc = relayout<T>(&x, &ldx, rows, in, &ws, s);
+        if (rc == MTP_OK) rc = relayout<T>(&w, &ldw, (int64_t)n_sets * out, in, &ws, s);
+        if (rc != MTP_OK) return rc;
+    }
     LinArgs a{};
     a.P = LinOperand{w, ldw, (int64_t)out * ldw};
     a.Q = LinOperand{x, ldx, 0};
@@ -270,6 +293,9 @@ int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int
     a.act = act;
     a.out = y;
     a.pre = pre;
+    if (few == 1) return launch_few<T, 1>(a, s);
+    if (few == 2) return launch_few<T, 2>(a, s);
+    if (few == 4) return launch_few<T, 4>(a, s);
     return launch_product<T, LIN_FORWARD>(a, s);
 }
 
@@ -354,6 +380,7 @@ extern "C" int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows,
                                               int64_t lda, const void *b, int64_t ldb) {
     if (rows < 0 || in < 1 || out < 1 || n_sets < 1) return 0;
     const int64_t w_rows = (int64_t)n_sets * out;
+    if (step == MTP_LINEAR_FORWARD && few_rows(rows, n_sets) != 0) return 0;
     if (step == MTP_LINEAR_FORWARD) return relayout_bytes(dtype, a, lda, rows, in) + relayout_bytes(dtype, b, in, w_rows, in);
     if (step == MTP_LINEAR_GRAD_INPUT) return relayout_bytes(dtype, a, lda, rows, out) + relayout_bytes(dtype, b, in, w_rows, in);
     int64_t n = relayout_bytes(dtype, a, lda, rows, out) + relayout_bytes(dtype, b, ldb, rows, in);

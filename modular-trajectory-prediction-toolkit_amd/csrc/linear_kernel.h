@@ -684,7 +684,14 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
             if constexpr (MODE == LIN_GRAD_WEIGHT) {
                 if (sum_q) {
 #pragma unroll
-                    for (int r = 0; r < FR; ++r) acc_ones[r] = LinMfma<T>::mul(LinMfma<T>::ones(), fq[r], acc_ones[r]);
+                    for (int r = 0; r < FR; ++r) {
+                        if constexpr (SZ == 4) {  // a matrix instruction would cost as much as one of the product's
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc_ones[r][0] += fq[r][e];
+                        } else {
+                            acc_ones[r] = LinMfma<T>::mul(LinMfma<T>::ones(), fq[r], acc_ones[r]);
+                        }
+                    }
                 }
             }
         }
@@ -740,6 +747,12 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
             else lin_leave<T, T, MODE, BC, ER, NT, 1>(a, z, bias, to, r0, row_end, c0, tid);
         }
     }
+    if constexpr (MODE == LIN_GRAD_WEIGHT && SZ == 4) {  // the two halves of a wave hold different k
+        if (sum_q) {
+#pragma unroll
+            for (int r = 0; r < FR; ++r) acc_ones[r][0] += __shfl_xor(acc_ones[r][0], 32);
+        }
+    }
     if constexpr (MODE == LIN_GRAD_WEIGHT) {
         if (sum_q && h == 0) {
 #pragma unroll
@@ -750,6 +763,145 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
                     else reinterpret_cast<T *>(a.bias_out)[(int64_t)set * a.out_rows + row] = from_f32<T>(acc_ones[r][0]);
                 }
             }
+        }
+    }
+}
+
+// ---- few rows ----
+// Up to 16 * RT rows of x against 16 columns of the output: W is read once, straight from memory into the operands of the 16 x 16
+// matrix instructions (a lane holds 16 bytes of k of one row of W and of x), the four waves share the sum over k and are
+// added through LDS.  What bounds it is reading W: each wave has UNROLL pieces of it in flight.
+template <typename T>
+struct LinMfma16;
+template <>
+struct LinMfma16<__bf16> {
+    static __device__ __forceinline__ f32x4v mul(bf16x8v p, bf16x8v q, f32x4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, q, c, 0, 0, 0);
+    }
+};
+template <>
+struct LinMfma16<_Float16> {
+    static __device__ __forceinline__ f32x4v mul(f16x8v p, f16x8v q, f32x4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, c, 0, 0, 0);
+    }
+};
+template <>
+struct LinMfma16<float> {
+    static __device__ __forceinline__ f32x4v mul(f32x4v p, f32x4v q, f32x4v c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[e], q[e], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// 16 bytes of a row; rows need the alignment of their elements only
+template <typename T>
+__device__ __forceinline__ typename LinMfma<T>::frag lin_piece(const T *at) {
+    constexpr int N = 16 / sizeof(T);
+    typedef T loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    return *reinterpret_cast<const loose *>(at);
+}
+// the same from k0 on, elements from k on are zero
+template <typename T>
+__device__ __forceinline__ typename LinMfma<T>::frag lin_piece_to(const T *row, int k0, int k) {
+    constexpr int N = 16 / sizeof(T);
+    if (k0 + N <= k) return lin_piece<T>(row + k0);
+    typename LinMfma<T>::frag f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = k0 + e < k ? row[k0 + e] : (T)0.f;
+    return f;
+}
+
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void k_linear_few(LinArgs a) {
+    constexpr int N = 16 / (int)sizeof(T), STEP = 4 * N, UNROLL = RT == 1 ? 4 : 2;  // k of a step: four lane groups
+    typedef typename LinMfma<T>::frag frag;
+    __shared__ f32x4v sums[3][RT][64];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ct = (int)(blockIdx.x % a.col_tiles);
+    const int64_t c0 = (int64_t)ct * 16, id = blockIdx.x / a.col_tiles;
+    int64_t row0 = 0, row_end = a.rows;
+    int set = 0;
+    if (a.offsets != nullptr) {
+        LinPiece p;
+        if (!lin_find<false>(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(16 * RT), 0, id, &p)) return;
+        set = p.set;
+        row0 = p.lo + p.index * (16 * RT);
+        row_end = p.hi;
+    } else {
+        row0 = id * (16 * RT);
+    }
+    T *out = reinterpret_cast<T *>(a.out);
+    if (set == a.n_sets) {  // rows behind the last set
+        const int64_t r = row0 + tid / 16, c = c0 + tid % 16;
+        for (int64_t x = r; x < row_end && x < row0 + 16 * RT; x += 16)
+            if (c < a.cols) {
+                out[x * a.cols + c] = (T)0.f;
+                if (a.pre != nullptr) reinterpret_cast<T *>(a.pre)[x * a.cols + c] = (T)0.f;
+            }
+        return;
+    }
+    const int k = a.k, steps = (k + STEP - 1) / STEP;
+    const int64_t wc = c0 + i < a.cols ? c0 + i : a.cols - 1;  // rows and columns that are not there are computed and dropped
+    const T *w = reinterpret_cast<const T *>(a.P.base) + set * a.P.group + wc * a.P.ld;
+    const T *x[RT];
+    f32x4v acc[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int64_t at = row0 + r * 16 + i < row_end ? row0 + r * 16 + i : row_end - 1;
+        x[r] = reinterpret_cast<const T *>(a.Q.base) + at * a.Q.ld;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
+    }
+    // wave w takes the steps w, w + 4, ...; the last one may reach beyond k
+    const int whole = k / STEP;
+    int s0 = wave;
+    for (; s0 + 4 * (UNROLL - 1) < whole; s0 += 4 * UNROLL) {
+        frag fw[UNROLL], fx[UNROLL][RT];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k0 = (s0 + 4 * u) * STEP + g * N;
+            fw[u] = lin_piece<T>(w + k0);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) fx[u][r] = lin_piece<T>(x[r] + k0);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[r] = LinMfma16<T>::mul(fw[u], fx[u][r], acc[r]);
+    }
+    for (; s0 < steps; s0 += 4) {
+        const int k0 = s0 * STEP + g * N;
+        const frag fw = lin_piece_to<T>(w, k0, k);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r] = LinMfma16<T>::mul(fw, lin_piece_to<T>(x[r], k0, k), acc[r]);
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) sums[wave - 1][r][lane] = acc[r];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    // lane (i, g): row i, columns 4 g to 4 g + 3
+    const int64_t col = c0 + 4 * g;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        f32x4v v = acc[r];
+#pragma unroll
+        for (int o = 0; o < 3; ++o) v += sums[o][r][lane];
+        const int64_t row = row0 + r * 16 + i;
+        if (row >= row_end) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (col + e >= a.cols) break;
+            const int64_t at = row * a.cols + col + e;
+            float z = v[e];
+            if (a.bias != nullptr) z += to_f32(reinterpret_cast<const T *>(a.bias)[(int64_t)set * a.cols + col + e]);
+            if (a.pre != nullptr) reinterpret_cast<T *>(a.pre)[at] = from_f32<T>(z);
+            z = lin_act(z, a.act);
+            if (a.residual != nullptr) z += to_f32(reinterpret_cast<const T *>(a.residual)[row * a.ld_res + col + e]);
+            out[at] = from_f32<T>(z);
         }
     }
 }

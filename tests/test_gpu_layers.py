@@ -72,6 +72,23 @@ def test_linear_many_rows(gpu_device, size, dtype):
     _compare(_run(gpu_device, x, w, b, r, gy, "gelu"), R.linear(x, w, b, "gelu", r, gy), dtype)
 
 
+@pytest.mark.parametrize("dtype", R.TYPES, ids=str)
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 32, 33, 64, 65])
+def test_linear_few_rows(gpu_device, rows, dtype):
+    """The kernels for few rows and their borders: long sums, sizes and row starts of every alignment."""
+    for i, o, start in ((1024, 1024, 0), (511, 33, 0), (130, 7, 1), (31, 16, 3), (2048, 40, 5)):
+        x, w, b, r, _ = _inputs(rows + i, rows, i + 8, o, dtype)
+        x, w = x[:, start:start + i], w[:, :i].contiguous()
+        y = linear(_strided(x, gpu_device), w.to(gpu_device), b.to(gpu_device), "gelu", r.to(gpu_device))
+        R.check("y", y, R.linear(x, w, b, "gelu", r)["y"])
+
+
+def _strided(x, dev):
+    """x on the device with the strides it has."""
+    whole = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=dev)
+    return whole.copy_(x)
+
+
 def test_linear_wide(gpu_device):
     for dtype in R.TYPES:
         x, w, b, r, gy = _inputs(11, 700, 1200, 1100, dtype)
