@@ -117,10 +117,14 @@ unsigned grid_for(int64_t items) {
     return (unsigned)(b < 1 ? 1 : (b > 256 * 16 ? 256 * 16 : b));
 }
 
-// Tiles of 16 rows that k_linear_few works on at a time, 0: the rows are too many for it.
-int few_rows(int64_t rows, int n_sets) {
-    const int64_t mean = n_sets > 1 ? (rows + n_sets - 1) / n_sets : rows;
-    return mean <= 16 ? 1 : mean <= 32 ? 2 : mean <= 64 ? 4 : 0;
+// Tiles of 16 rows that k_linear_few works on at a time, 0: the product is too much for it.  Microseconds, few / tiles: bfloat16
+// 64 rows of 2048 x 2048 10.8 / 16.9, 512 of 512 x 512 7.5 / 7.2, 256 of 2048 x 2048 33 / 17; float 64 of 2048 x 2048 18.8 / 50
+// (two row tiles 16.6), 256 of 2048 x 2048 64 / 51.  One matrix per modality: 64 rows over 200 of 512 x 128 7.9 / 12.3,
+// 2000 rows over 200 of 256 x 96 13.6 / 8.8.
+int few_rows(int64_t rows, int in, int out, bool grouped, bool half) {
+    const int64_t products = rows * in * out;
+    if (rows > 512 || products > (half ? 1ll << 28 : 1ll << 29)) return 0;
+    return !grouped && products >= 1ll << 28 ? 2 : 1;
 }
 
 // rows of a 16-bit operand have to start on 4 bytes; a row distance beyond 2^20 elements would leave the loads' 32-bit offsets
@@ -163,7 +167,7 @@ enum LinTileShape { TILE_32x128, TILE_64x64, TILE_64x128, TILE_96x128, TILE_128x
 
 int64_t tiles_of(int64_t rows, int64_t cols, int bc, int br) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); }
 
-LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, bool grouped) {
+LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, int n_sets) {
     if (mode == MTP_LINEAR_GRAD_WEIGHT) {  // rows, cols: of the gradient
         if (!half) return cols <= 96 ? TILE_32x128 : TILE_64x64;
         if (cols <= 32) return TILE_32x128;
@@ -173,30 +177,34 @@ LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, b
         return tiles_of(rows, cols, 128, 128) >= 64 ? TILE_128x128 : TILE_128x64;
     }
     if (cols <= 32) return TILE_32x128;
-    if (tiles_of(rows, cols, 64, 64) < 512) return rows < 128 ? TILE_64x64 : TILE_32x128;
+    const int64_t least = n_sets > 1 ? (int64_t)n_sets * ((cols + 63) / 64) : 0;  // each set has a tile of its own
+    if (tiles_of(rows, cols, 64, 64) + least < 512) return rows < 128 || n_sets > 1 ? TILE_64x64 : TILE_32x128;
     if (cols <= 64) return TILE_64x128;
     if (cols <= 96) return half ? TILE_96x128 : TILE_32x128;
-    if (half && !grouped && k >= 512 && tiles_of(rows, cols, 256, 256) >= 192) return TILE_256x256;
+    if (half && n_sets == 1 && k >= 512 && tiles_of(rows, cols, 256, 256) >= 192) return TILE_256x256;
     if (half && mode == MTP_LINEAR_GRAD_INPUT) return TILE_128x128;
     return TILE_128x64;
 }
 
 // Rows of x that one workgroup of the weight gradient sums, as a power of two.  One matrix: some 1024 workgroups, 2048 of big
-// tiles (32 768 rows, 2048 x 2048: 374 us with 2048 workgroups, 455 with 1024, 617 with 512).  Many: sets differ in size by a
-// factor of ten, and the longest one is what the others wait for.
+// tiles (32 768 rows, 2048 x 2048 bfloat16: 374 us with 2048 workgroups, 402 with 1024, 503 with 512).  Many: sets differ in size
+// by a factor of ten and the longest one is what the others wait for, but parts have to be written and added (143 760 rows over
+// 400, 96 -> 256: 36 us with parts of 2048, 40 of 1024, 47 of 512; 52 280 rows over 200: 23 us of 1024, 29 of 2048).
 int part_bits_for(int64_t rows, int in, int out, int n_sets, bool half) {
     int64_t tiles;
-    int64_t most = 1024;
-    switch (pick_tile(MTP_LINEAR_GRAD_WEIGHT, half, out, in, rows, n_sets > 1)) {
+    int64_t most = n_sets > 1 ? 160 : 1024;
+    switch (pick_tile(MTP_LINEAR_GRAD_WEIGHT, half, out, in, rows, n_sets)) {
         case TILE_32x128: tiles = tiles_of(out, in, 32, 128); break;
         case TILE_64x64: tiles = tiles_of(out, in, 64, 64); break;
         case TILE_64x128: tiles = tiles_of(out, in, 64, 128); break;
         case TILE_96x128: tiles = tiles_of(out, in, 96, 128); break;
         case TILE_128x64: tiles = tiles_of(out, in, 128, 64); break;
-        default: tiles = tiles_of(out, in, 128, 128), most = 2048;
+        default:
+            tiles = tiles_of(out, in, 128, 128);
+            if (n_sets == 1) most = 2048;
     }
     const int64_t part = rows * tiles / most;
-    int bits = 9;
+    int bits = half ? 10 : 9;
     while (bits < 30 && ((int64_t)1 << bits) < part) ++bits;
     return bits;
 }
@@ -231,7 +239,7 @@ int launch_tile(LinArgs a, hipStream_t s) {
 template <typename T, int MODE>
 int launch_product(const LinArgs &a, hipStream_t s) {
     const bool half = sizeof(T) == 2;
-    switch (pick_tile(MODE, half, MODE == LIN_GRAD_WEIGHT ? a.out_rows : a.rows, a.cols, a.k, a.offsets != nullptr)) {
+    switch (pick_tile(MODE, half, MODE == LIN_GRAD_WEIGHT ? a.out_rows : a.rows, a.cols, a.k, a.n_sets)) {
         case TILE_32x128: return launch_tile<T, MODE, 32, 128, 32, 32>(a, s);
         case TILE_64x64: return launch_tile<T, MODE, 64, 64, 32, 32>(a, s);
         case TILE_64x128: return launch_tile<T, MODE, 64, 128, 32, 64>(a, s);
@@ -273,7 +281,7 @@ template <typename T>
 int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias, int act,
             const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre, char *ws, hipStream_t s) {
     int64_t ldw = in;
-    const int few = few_rows(rows, n_sets);
+    const int few = few_rows(rows, in, out, n_sets > 1, sizeof(T) == 2);
     if (few == 0) {
         int rc = relayout<T>(&x, &ldx, rows, in, &ws, s);
         if (rc == MTP_OK) rc = relayout<T>(&w, &ldw, (int64_t)n_sets * out, in, &ws, s);
@@ -295,7 +303,6 @@ int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int
     a.pre = pre;
     if (few == 1) return launch_few<T, 1>(a, s);
     if (few == 2) return launch_few<T, 2>(a, s);
-    if (few == 4) return launch_few<T, 4>(a, s);
     return launch_product<T, LIN_FORWARD>(a, s);
 }
 
@@ -380,7 +387,7 @@ extern "C" int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows,
                                               int64_t lda, const void *b, int64_t ldb) {
     if (rows < 0 || in < 1 || out < 1 || n_sets < 1) return 0;
     const int64_t w_rows = (int64_t)n_sets * out;
-    if (step == MTP_LINEAR_FORWARD && few_rows(rows, n_sets) != 0) return 0;
+    if (step == MTP_LINEAR_FORWARD && few_rows(rows, in, out, n_sets > 1, elem_size(dtype) == 2) != 0) return 0;
     if (step == MTP_LINEAR_FORWARD) return relayout_bytes(dtype, a, lda, rows, in) + relayout_bytes(dtype, b, in, w_rows, in);
     if (step == MTP_LINEAR_GRAD_INPUT) return relayout_bytes(dtype, a, lda, rows, out) + relayout_bytes(dtype, b, in, w_rows, in);
     int64_t n = relayout_bytes(dtype, a, lda, rows, out) + relayout_bytes(dtype, b, ldb, rows, in);

@@ -456,12 +456,13 @@ constexpr int lin_pass_rows(int room, int rows) {
 
 enum { LIN_FORWARD = 0, LIN_GRAD_INPUT = 1, LIN_GRAD_WEIGHT = 2 };
 
-// A tile's rows on their way out of LDS, N columns a thread; U is the type they leave in.  Four rows are on their way at a time.
+// A tile's rows on their way out of LDS, N columns a thread; U is the type they leave in.  Up to four rows are on their way at a time (two where
+// there are many: 256 x 256 tiles with everything 335 us, 388 with four).
 template <typename T, typename U, int MODE, int BC, int ER, int NT, int N>
 __device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, const float *bias, U *to, int64_t r0, int64_t row_end,
                                           int64_t c0, int tid) {
     constexpr int ITEMS = BC / N, STEP = NT / ITEMS;  // items of a row; rows that the workgroup takes at a time
-    constexpr int PM = lin_twist_mask(BC / 4), AT_ONCE = ER / STEP < 4 ? (ER / STEP < 1 ? 1 : ER / STEP) : 4;
+    constexpr int PM = lin_twist_mask(BC / 4), AT_ONCE = ER / STEP < 1 ? 1 : ER / STEP <= 4 ? ER / STEP : 2;
     const int item = tid % ITEMS;
     const int64_t col = c0 + item * N;
     if (col >= a.cols || tid >= ITEMS * STEP) return;  // (16-byte pieces: cols is a multiple of N)

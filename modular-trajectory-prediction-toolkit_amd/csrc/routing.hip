@@ -27,15 +27,41 @@ struct RouteKey {
     typedef uint32_t type;
     static constexpr type NONE = 0;
     static constexpr uint32_t INF = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
-    static __device__ __forceinline__ type make(T v, int index, bool *bad) {
-        uint32_t b = __builtin_bit_cast(uint16_t, v);
-        if ((b & 0x7fffu) > INF) {
-            *bad = true;
-            b = 0x8000u | INF;  // NaN: as -inf
+    // nothing: NONE, or an index without a score (a place beyond the row; -inf's bits are 0x7f or 0x3ff)
+    static __device__ __forceinline__ bool nothing(type k) { return k < 0x10000u; }
+    // the keys of v[0 .. V), indexes from i0 on; those from e on become nothing.  Two scores at a time; NaN (to become -inf) and -0
+    // (to equal +0) are looked for at the end and put right only where a wave has one.
+    template <int V>
+    static __device__ __forceinline__ void keys(const T (&v)[V], int i0, int e, type (&key)[V], bool *bad) {
+        typedef short s2 __attribute__((ext_vector_type(2)));
+        typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+        u2 o[(V + 1) / 2], odd = {0xffff, 0xffff}, big = {0, 0};
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            u2 x = {__builtin_bit_cast(unsigned short, v[j]), __builtin_bit_cast(unsigned short, v[j + 1 < V ? j + 1 : j])};
+            const u2 neg = (u2)((s2)x >> 15);
+            o[j / 2] = x ^ (neg | (u2){0x8000, 0x8000});
+            odd = __builtin_elementwise_min(odd, (u2)(o[j / 2] - (u2){0x7fff, 0x7fff}));  // -0: 0
+            big = __builtin_elementwise_max(big, (u2)(x & (u2){0x7fff, 0x7fff}));          // NaN: above INF
         }
-        b = b == 0x8000u ? 0u : b;  // -0 equals +0
-        b = (b & 0x8000u) ? (b ^ 0xffffu) : (b | 0x8000u);
-        return (b << 16) | (uint32_t)(0xffff - index);
+        const bool special = odd[0] == 0 || odd[1] == 0 || big[0] > INF || big[1] > INF;
+        if (__ballot(special) != 0) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                uint32_t b = __builtin_bit_cast(uint16_t, v[j]);
+                const bool nan = (b & 0x7fffu) > INF;
+                *bad |= nan && i0 + j < e;
+                b = nan ? 0x8000u | INF : b == 0x8000u ? 0u : b;
+                o[j / 2][j & 1] = (unsigned short)((b & 0x8000u) ? (b ^ 0xffffu) : (b | 0x8000u));
+            }
+        }
+        const uint32_t low = 0xffffu - i0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t w = __builtin_bit_cast(uint32_t, o[j / 2]);
+            const uint32_t k = ((j & 1) ? (w & 0xffff0000u) : (w << 16)) | (low - j);
+            key[j] = i0 + j < e ? k : NONE;
+        }
     }
     static __device__ __forceinline__ float score(type k) {
         uint32_t b = k >> 16;
@@ -55,14 +81,19 @@ template <>
 struct RouteKey<float> {
     typedef double type;
     static constexpr type NONE = 2.0;
-    static __device__ __forceinline__ type make(float v, int index, bool *bad) {
-        if (v != v) {
-            *bad = true;
-            v = -__builtin_inff();
+    static __device__ __forceinline__ bool nothing(type k) { return k == NONE; }
+    template <int V>
+    static __device__ __forceinline__ void keys(const float (&v)[V], int i0, int e, type (&key)[V], bool *bad) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool nan = v[j] != v[j];
+            *bad |= nan && i0 + j < e;
+            uint32_t b = __float_as_uint((nan ? -__builtin_inff() : v[j]) + 0.0f);  // -0 equals +0
+            b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+            const type k = __longlong_as_double(
+                (long long)(0x4000000000000000ull | ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - (i0 + j))));
+            key[j] = i0 + j < e ? k : NONE;
         }
-        uint32_t b = __float_as_uint(v + 0.0f);  // -0 equals +0
-        b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-        return __longlong_as_double((long long)(0x4000000000000000ull | ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - index)));
     }
     static __device__ __forceinline__ float score(type k) {
         const uint32_t b = (uint32_t)((uint64_t)__double_as_longlong(k) >> 12);
@@ -174,14 +205,7 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
     }
     key_t key[V];
     bool bad = false;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int i = sub * V + j;
-        bool is_bad = false;
-        const key_t made = R::make(v[j], i, &is_bad);
-        key[j] = i < e ? made : R::NONE;
-        bad |= is_bad && i < e;
-    }
+    R::keys(v, sub * V, e, key, &bad);
     float total = 0.f, top = 0.f;
     if (!normalize) {  // the softmax over all modalities
         key_t m = key[0];
@@ -190,7 +214,7 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
         top = R::score(group_max<T, L>(m));
         if (top == -__builtin_inff()) top = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) total += key[j] != R::NONE ? expf(R::score(key[j]) - top) : 0.f;
+        for (int j = 0; j < V; ++j) total += !R::nothing(key[j]) ? expf(R::score(key[j]) - top) : 0.f;
         total = group_sum<L>(total);
     }
     const uint64_t any_bad = __ballot(bad);
@@ -209,26 +233,34 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
     for (int b = 0; b < KB; ++b) {
         chosen[b] = R::NONE;
         const int most = k - b * L < L ? k - b * L : L;
-        for (int i = 0; i < most; ++i) {
+        auto take = [&](int i) {
             const key_t best = group_max<T, L>(head);
             if (sub == i) chosen[b] = best;
             // keys differ by their index, so one lane moves on; a lane that has given its last key stays at NONE
             next += head == best && best != R::NONE ? 256 : 0;
             head = *next;
+        };
+        int i = 0;
+        for (; i + 4 <= most; i += 4) {
+            take(i);
+            take(i + 1);
+            take(i + 2);
+            take(i + 3);
         }
+        for (; i < most; ++i) take(i);
     }
     float w[KB];
     if (normalize) {
         // lane 0 of the first batch has the largest score
         const key_t first = __shfl(chosen[0], (tid & 63) / L * L);
-        top = first == R::NONE ? 0.f : R::score(first);
+        top = R::nothing(first) ? 0.f : R::score(first);
         if (top == -__builtin_inff()) top = 0.f;
     }
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
         const float x = R::score(chosen[b]);
-        const bool none = chosen[b] == R::NONE || x == -__builtin_inff();
+        const bool none = R::nothing(chosen[b]) || x == -__builtin_inff();
         if (none) chosen[b] = R::NONE;
         w[b] = none ? 0.f : expf(x - top);
         sum += w[b];

@@ -52,10 +52,10 @@ def test_entry_points_refuse_a_small_workspace():
     assert L.mtp_sort_pairs(ONE, 100000, 200, ONE, ONE, ONE, ONE, need - 1, None) == -3
     assert L.mtp_sort_pairs(ONE, 100000, 200, ONE, ONE, ONE, None, need, None) == -3
     # float rows always start on 4 bytes; a 16-bit row of odd length does not
-    assert L.mtp_linear_workspace_bytes(0, _lib.LINEAR_FORWARD, 500, 97, 40, 1, ONE, 97, ONE, 97) == 0
-    need = L.mtp_linear_workspace_bytes(1, _lib.LINEAR_FORWARD, 500, 97, 40, 1, ONE, 97, ONE, 97)
-    assert need >= (500 + 40) * 104 * 2
-    assert L.mtp_linear(1, ONE, 500, 97, 97, ONE, 40, None, 0, None, 0, None, 1, ONE, None, ONE, need - 1, None) == -3
+    assert L.mtp_linear_workspace_bytes(0, _lib.LINEAR_FORWARD, 600, 97, 40, 1, ONE, 97, ONE, 97) == 0
+    need = L.mtp_linear_workspace_bytes(1, _lib.LINEAR_FORWARD, 600, 97, 40, 1, ONE, 97, ONE, 97)
+    assert need >= (600 + 40) * 104 * 2
+    assert L.mtp_linear(1, ONE, 600, 97, 97, ONE, 40, None, 0, None, 0, None, 1, ONE, None, ONE, need - 1, None) == -3
     need = L.mtp_linear_workspace_bytes(1, _lib.LINEAR_GRAD_WEIGHT, 50000, 96, 40, 1, ONE, 40, ONE, 96)
     assert need > 0 and L.mtp_linear_grad_weight(1, ONE, 50000, 40, 40, ONE, 96, 96, None, 1, ONE, None, ONE, need - 1, None) == -3
 
