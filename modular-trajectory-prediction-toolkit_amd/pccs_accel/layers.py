@@ -31,7 +31,7 @@ class _Linear(torch.autograd.Function):
         x, weight, pre, offsets = ctx.saved_tensors
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
         grad = grad.contiguous()
-        dx, dw, db = K.linear_backward(grad, pre, ctx.activation, x, weight, offsets, want_x, want_w, want_b)
+        dx, dw, db = K.linear_backward(grad, pre, ctx.activation, x, weight, offsets, want_x, want_w, want_b, trusted=True)
         dr = None
         if want_r:  # rows behind the last set have none
             dr = grad if offsets is None else K.linear_mask_rows(grad, offsets)

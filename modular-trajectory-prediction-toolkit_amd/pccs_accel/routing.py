@@ -44,7 +44,7 @@ class _RouteTopk(torch.autograd.Function):
         if grad is None:
             return None, None, None
         scores, ids, weights, stats = ctx.saved_tensors
-        return K.route_topk_grad(scores, ids, weights, stats, grad.contiguous(), ctx.normalize), None, None
+        return K.route_topk_grad(scores, ids, weights, stats, grad.contiguous(), ctx.normalize, trusted=True), None, None
 
 
 def route_topk(scores, k, normalize=True):
@@ -74,7 +74,7 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return K.combine_rows(grad.contiguous(), *ctx.saved_tensors), None, None
+        return K.combine_rows(grad.contiguous(), *ctx.saved_tensors, trusted=True), None, None
 
 
 def dispatch(x, plan):
@@ -99,9 +99,10 @@ class _Combine(torch.autograd.Function):
         rows, weights, position, offsets = ctx.saved_tensors
         grad = grad.contiguous()
         if not ctx.has_weights:
-            return K.dispatch_rows(grad, position, offsets), None, None, None
+            return K.dispatch_rows(grad, position, offsets, trusted=True), None, None, None
         want_rows, want_weights = ctx.needs_input_grad[:2]
-        return K.combine_rows_grad(rows, grad, position, offsets, weights, want_rows, want_weights) + (None, None)
+        return K.combine_rows_grad(rows, grad, position, offsets, weights, want_rows, want_weights,
+                                   trusted=True) + (None, None)
 
 
 def combine(rows, plan, weights=None):
