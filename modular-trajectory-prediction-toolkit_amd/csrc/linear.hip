@@ -34,7 +34,9 @@ __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g
         const int64_t n = rows * (cols / 8);
         const int per = cols / 8;
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-            const t8 gv = reinterpret_cast<const t8 *>(g)[i], zv = reinterpret_cast<const t8 *>(z)[i];
+            // read once more at most, and not soon
+            const t8 gv = __builtin_nontemporal_load(reinterpret_cast<const t8 *>(g) + i);
+            const t8 zv = __builtin_nontemporal_load(reinterpret_cast<const t8 *>(z) + i);
             t8 o;
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(to_f32(gv[e]) * lin_slope(to_f32(zv[e]), act));
@@ -214,6 +216,10 @@ int64_t most_parts(int64_t rows, int n_sets, int bits) {
     return (2 * rows) >> bits;
 }
 
+// Outputs larger than this leave past the caches (what is kept for the backward pass always does): 73 568 x 512 floats with gelu
+// and a residual 139 -> 135 us for what is kept, 119 for both.
+constexpr int64_t AWAY_BYTES = 64ll << 20;
+
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
 int launch_tile(LinArgs a, hipStream_t s) {
     constexpr int NT = 64 * (BC / WC) * (BR / WR);
@@ -227,6 +233,7 @@ int launch_tile(LinArgs a, hipStream_t s) {
         // a set's last tile may be ragged, and so may the one behind the last set
         a.row_tiles = a.offsets == nullptr ? (a.rows + BR - 1) / BR : (a.rows + (int64_t)(a.n_sets + 1) * (BR - 1)) / BR;
         blocks = a.row_tiles * a.col_tiles;
+        a.away = a.rows * a.cols * (int64_t)sizeof(T) > AWAY_BYTES;
     }
     MTP_REQUIRE(blocks <= 0x7fffffff, "mtp_linear: %lld workgroups are too many", (long long)blocks);
     if (blocks == 0) return MTP_OK;

@@ -408,6 +408,7 @@ struct LinArgs {
     float *partial;  // weight gradient: the sums of sets that are cut into parts, [parts][out_rows][cols], ...
     float *partial_bias;  // ... and [parts][out_rows]
     int64_t parts;        // room for so many
+    int away;             // the output is more than the caches hold: past them
 };
 
 // N consecutive elements
@@ -420,6 +421,18 @@ __device__ __forceinline__ void lin_store(T *p, const float *v) {
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = from_f32<T>(v[e]);
         *reinterpret_cast<tn *>(p) = w;
+    }
+}
+// the same past the caches: what is not read again soon
+template <typename T, int N>
+__device__ __forceinline__ void lin_store_away(T *p, const float *v) {
+    if constexpr (N == 1) __builtin_nontemporal_store(from_f32<T>(v[0]), p);
+    else {
+        typedef T tn __attribute__((ext_vector_type(N)));
+        tn w;
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = from_f32<T>(v[e]);
+        __builtin_nontemporal_store(w, reinterpret_cast<tn *>(p));
     }
 }
 template <typename T, int N>
@@ -496,7 +509,7 @@ __device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, cons
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u)
                     if (row0 + u * STEP < rows)
-                        lin_store<T, N>(reinterpret_cast<T *>(a.pre) + (r0 + row0 + u * STEP) * a.cols + col, v[u]);
+                        lin_store_away<T, N>(reinterpret_cast<T *>(a.pre) + (r0 + row0 + u * STEP) * a.cols + col, v[u]);
             }
             auto bend = [&](auto kind) {
 #pragma unroll
@@ -516,7 +529,11 @@ __device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, cons
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u)
-            if (row0 + u * STEP < rows) lin_store<U, N>(to + (r0 + row0 + u * STEP) * a.cols + col, v[u]);
+            if (row0 + u * STEP < rows) {
+                U *at = to + (r0 + row0 + u * STEP) * a.cols + col;
+                if (MODE != LIN_GRAD_WEIGHT && a.away) lin_store_away<U, N>(at, v[u]);
+                else lin_store<U, N>(at, v[u]);
+            }
     }
 }
 // the bias of the columns that lin_leave gives this thread
