@@ -1,0 +1,342 @@
+// Calls of the routing and layer entry points from torch, with their autograd nodes.
+//
+// A small layer takes a few microseconds on the card; a call through Python takes ten, a backward pass through Python nodes some
+// thirty more.  Here the arguments are looked over, the results allocated and the entry points of mtp_accel.h called without
+// Python between them (forward and backward of a 64 x 96 layer with gelu: 45 us against 68).  A call whose arguments are not as they have to be returns
+// None: the Python front end then finds out what is wrong and raises.
+#include <torch/extension.h>
+
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <optional>
+
+#include "mtp_accel.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr int64_t MOST = 0x7fffffff;
+constexpr int64_t MOST_SIZE = 65536, MOST_SETS = 65535, MOST_MODALITIES = 4096, MOST_TOPK = 128;
+enum { NONE = 0, RELU = 1 };
+
+void *stream_of(const Tensor &t) {
+    return static_cast<void *>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream());
+}
+void *at_(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+void check(int rc, const char *what) { TORCH_CHECK(rc == MTP_OK, what, " failed (rc=", rc, "): ", mtp_last_error()); }
+
+int type_code(const Tensor &t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return MTP_FLOAT;
+        case at::kBFloat16: return MTP_BFLOAT16;
+        case at::kHalf: return MTP_HALF;
+        default: return -1;
+    }
+}
+// elements from row to row of a matrix with contiguous rows that do not overlap, -1 otherwise
+int64_t row_distance(const Tensor &t) {
+    const int64_t rows = t.size(0), cols = t.size(1);
+    if (rows <= 1 && (cols <= 1 || t.stride(1) == 1)) return cols > 1 ? cols : 1;
+    if ((cols > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < cols)) return -1;
+    return t.stride(0);
+}
+bool matrix(const Tensor &t) { return t.is_cuda() && t.dim() == 2 && t.layout() == at::kStrided && type_code(t) >= 0; }
+bool like(const Tensor &t, at::ScalarType type, const Tensor &ref, at::IntArrayRef shape) {
+    return t.scalar_type() == type && t.device() == ref.device() && t.sizes() == shape && t.is_contiguous();
+}
+Tensor workspace(int64_t bytes, const Tensor &ref) {
+    return bytes > 0 ? at::empty({bytes}, ref.options().dtype(at::kByte)) : Tensor();
+}
+
+// What a backward pass returns can be differentiated no further: trying to says so.  `from`: what it was computed from.
+variable_list no_further(variable_list out, variable_list from, const char *what) {
+    if (!at::GradMode::is_enabled()) return out;
+    const size_t n = out.size();
+    auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative",
+                                                                (int64_t)(n + from.size()));
+    variable_list in = std::move(out);
+    for (auto &t : from) in.push_back(t);  // the error stands between the result and these
+    variable_list got = (*node)(std::move(in));
+    got.resize(n);
+    return got;
+}
+
+// ---- linear layers ----
+struct Sizes {
+    int code, act;
+    int64_t rows, in, out, sets;
+};
+
+Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, const Tensor &offsets,
+                  Tensor *pre) {
+    Tensor y = at::empty({z.rows, z.out}, x.options());
+    if (pre != nullptr) *pre = at::empty({z.rows, z.out}, x.options());
+    const int64_t ldx = row_distance(x);
+    const int64_t bytes = mtp_linear_workspace_bytes(z.code, MTP_LINEAR_FORWARD, z.rows, (int)z.in, (int)z.out, (int)z.sets, at_(x),
+                                                     ldx, at_(w), z.in);
+    const Tensor ws = workspace(bytes, x);
+    check(mtp_linear(z.code, at_(x), z.rows, (int)z.in, ldx, at_(w), (int)z.out, at_(bias), z.act, at_(residual),
+                     residual.defined() ? row_distance(residual) : 0, static_cast<const int32_t *>(at_(offsets)), (int)z.sets, at_(y),
+                     pre != nullptr ? at_(*pre) : nullptr, at_(ws), (size_t)bytes, stream_of(x)),
+          "mtp_linear");
+    return y;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+    // arguments that are not there have no edge: the residual's follows the bias' or takes its place
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_,
+                          const std::optional<Tensor> &residual_, const std::optional<Tensor> &offsets_, const Sizes &z) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
+        // relu's slope can be read off y where nothing was added to it
+        const bool from_y = z.act == RELU && !residual.defined();
+        Tensor pre;
+        Tensor y = run_linear(z, x, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr);
+        ctx->save_for_backward({x, w, from_y ? y : pre, offsets});
+        ctx->saved_data["sizes"] =
+            std::vector<int64_t>{z.code, z.act, z.rows, z.in, z.out, z.sets, bias.defined(), residual.defined()};
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &pre = saved[2], &offsets = saved[3];
+        const auto v = ctx->saved_data["sizes"].toIntVector();
+        const Sizes z{(int)v[0], (int)v[1], v[2], v[3], v[4], v[5]};
+        Tensor dx, dw, db, dr;
+        {
+            at::NoGradGuard off;
+            const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+            const Tensor g = grads[0].contiguous();
+            const bool want_x = ctx->needs_input_grad(0), want_b = v[6] != 0 && ctx->needs_input_grad(2);
+            const bool want_w = ctx->needs_input_grad(1) || want_b;
+            if (want_x) dx = at::empty({z.rows, z.in}, x.options());
+            if (want_w) dw = at::empty(w.sizes(), w.options());
+            if (want_b) db = at::empty(w.sizes().slice(0, w.dim() - 1), w.options());
+            const int32_t *sets = static_cast<const int32_t *>(at_(offsets));
+            if (want_x || want_w) {
+                const int64_t ldx = row_distance(x);
+                const int64_t bytes = mtp_linear_backward_workspace_bytes(z.code, z.rows, (int)z.in, (int)z.out, (int)z.sets, z.act,
+                                                                          at_(g), at_(w), at_(x), ldx, want_x, want_w);
+                const Tensor ws = workspace(bytes, x);
+                check(mtp_linear_backward(z.code, at_(g), at_(pre), z.act, at_(x), z.rows, (int)z.in, ldx, at_(w), (int)z.out, sets,
+                                          (int)z.sets, at_(dx), at_(dw), at_(db), at_(ws), (size_t)bytes, stream_of(x)),
+                      "mtp_linear_backward");
+            }
+            if (v[7] != 0 && ctx->needs_input_grad(v[6] != 0 ? 3 : 2)) {
+                if (offsets.defined()) {  // rows behind the last set have none
+                    dr = at::empty_like(g);
+                    check(mtp_linear_mask_rows(z.code, at_(g), z.rows, (int)z.out, sets, (int)z.sets, at_(dr), stream_of(x)),
+                          "mtp_linear_mask_rows");
+                } else {
+                    dr = g;
+                }
+            }
+            if (!ctx->needs_input_grad(1)) dw = Tensor();
+        }
+        return no_further({dx, dw, db, dr, Tensor(), Tensor()}, {x, w, grads[0]}, "linear");
+    }
+};
+
+std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_, int act,
+                             const std::optional<Tensor> &residual_, const std::optional<Tensor> &offsets_) {
+    const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
+    const bool many = offsets.defined();
+    if (!matrix(x) || row_distance(x) < 0 || w.dim() != (many ? 3 : 2) || !w.is_contiguous() || w.scalar_type() != x.scalar_type() ||
+        w.device() != x.device())
+        return std::nullopt;
+    const Sizes z{type_code(x), act, x.size(0), x.size(1), w.size(many ? 1 : 0), many ? w.size(0) : 1};
+    if (w.size(many ? 2 : 1) != z.in || z.rows > MOST || z.in < 1 || z.in > MOST_SIZE || z.out < 1 || z.out > MOST_SIZE || z.sets < 1 ||
+        z.sets > MOST_SETS)
+        return std::nullopt;
+    if (many && !like(offsets, at::kInt, x, {z.sets + 1})) return std::nullopt;
+    if (bias.defined() && !like(bias, x.scalar_type(), x, w.sizes().slice(0, w.dim() - 1))) return std::nullopt;
+    if (residual.defined() && (!matrix(residual) || residual.scalar_type() != x.scalar_type() || residual.device() != x.device() ||
+                               residual.size(0) != z.rows || residual.size(1) != z.out || row_distance(residual) < 0))
+        return std::nullopt;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
+                                       (residual.defined() && residual.requires_grad())))
+        return Linear::apply(x, w, bias_, residual_, offsets_, z);
+    return run_linear(z, x, w, bias, residual, offsets, nullptr);
+}
+
+// ---- router ----
+struct Route : torch::autograd::Function<Route> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &scores, int64_t k, bool normalize) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const int64_t n = scores.size(0), e = scores.size(1);
+        Tensor ids = at::empty({n, k}, scores.options().dtype(at::kInt)), weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+        Tensor stats = at::empty({n, 2}, weights.options());
+        check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, row_distance(scores), (int)k, normalize,
+                             static_cast<int32_t *>(at_(ids)), static_cast<float *>(at_(weights)), static_cast<float *>(at_(stats)),
+                             stream_of(scores)),
+              "mtp_route_topk");
+        ctx->save_for_backward({scores, ids, weights, stats});
+        ctx->saved_data["normalize"] = normalize;
+        ctx->mark_non_differentiable({ids});
+        ctx->set_materialize_grads(false);
+        return {ids, weights};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        Tensor out;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &scores = saved[0];
+        if (grads[1].defined()) {
+            at::NoGradGuard off;
+            const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
+            const Tensor g = grads[1].contiguous();
+            out = at::empty(scores.sizes(), scores.options());
+            check(mtp_route_topk_grad(type_code(scores), at_(scores), scores.size(0), (int)scores.size(1), row_distance(scores),
+                                      (int)saved[1].size(1), ctx->saved_data["normalize"].toBool(),
+                                      static_cast<const int32_t *>(at_(saved[1])), static_cast<const float *>(at_(saved[2])),
+                                      static_cast<const float *>(at_(saved[3])), static_cast<const float *>(at_(g)), at_(out),
+                                      stream_of(scores)),
+                  "mtp_route_topk_grad");
+        }
+        return no_further({out, Tensor(), Tensor()}, {scores, grads[1]}, "route_topk");
+    }
+};
+
+std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64_t k, bool normalize) {
+    if (!matrix(scores)) return std::nullopt;
+    const int64_t n = scores.size(0), e = scores.size(1), ld = row_distance(scores);
+    if (ld < 0 || n > MOST || e < 1 || e > MOST_MODALITIES || k < 1 || k > e || k > MOST_TOPK) return std::nullopt;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
+    if (at::GradMode::is_enabled() && scores.requires_grad()) {
+        auto out = Route::apply(scores, k, normalize);
+        return std::make_tuple(out[0], out[1]);
+    }
+    Tensor ids = at::empty({n, k}, scores.options().dtype(at::kInt)), weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+    check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, ld, (int)k, normalize, static_cast<int32_t *>(at_(ids)),
+                         static_cast<float *>(at_(weights)), nullptr, stream_of(scores)),
+          "mtp_route_topk");
+    return std::make_tuple(ids, weights);
+}
+
+// ---- pairs ----
+std::optional<std::tuple<Tensor, Tensor, Tensor>> sort_pairs(const Tensor &ids, int64_t e) {
+    if (!ids.is_cuda() || ids.scalar_type() != at::kInt || ids.dim() != 2 || !ids.is_contiguous() || e < 1 || e > MOST_MODALITIES ||
+        ids.numel() > MOST)
+        return std::nullopt;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ids.device());
+    const int64_t pairs = ids.numel(), bytes = mtp_sort_pairs_workspace_bytes(pairs, (int)e);
+    Tensor offsets = at::empty({e + 1}, ids.options()), order = at::empty({pairs}, ids.options());
+    Tensor position = at::empty(ids.sizes(), ids.options()), ws = workspace(bytes, ids);
+    check(mtp_sort_pairs(static_cast<const int32_t *>(at_(ids)), pairs, (int)e, static_cast<int32_t *>(at_(offsets)),
+                         static_cast<int32_t *>(at_(order)), static_cast<int32_t *>(at_(position)), at_(ws), (size_t)bytes,
+                         stream_of(ids)),
+          "mtp_sort_pairs");
+    return std::make_tuple(offsets, order, position);
+}
+
+// the device's count of pairs that have a modality
+const int32_t *held(const Tensor &offsets) { return static_cast<const int32_t *>(at_(offsets)) + (offsets.numel() - 1); }
+const int32_t *places(const Tensor &position) { return static_cast<const int32_t *>(at_(position)); }
+
+Tensor run_dispatch(const Tensor &x, const Tensor &position, const Tensor &offsets) {
+    const int64_t n = x.size(0), d = x.size(1), k = position.size(1);
+    Tensor rows = at::empty({n * k, d}, x.options());
+    check(mtp_dispatch_rows(type_code(x), at_(x), n, (int)d, row_distance(x), (int)k, places(position), held(offsets), at_(rows),
+                            stream_of(x)),
+          "mtp_dispatch_rows");
+    return rows;
+}
+Tensor run_combine(const Tensor &rows, const Tensor &position, const Tensor &offsets, const Tensor &weights) {
+    const int64_t n = position.size(0), d = rows.size(1), k = position.size(1);
+    Tensor y = at::empty({n, d}, rows.options());
+    check(mtp_combine_rows(type_code(rows), at_(rows), n, (int)d, (int)k, places(position), held(offsets),
+                           static_cast<const float *>(at_(weights)), at_(y), stream_of(rows)),
+          "mtp_combine_rows");
+    return y;
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &position, const Tensor &offsets) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({position, offsets});
+        return run_dispatch(x, position, offsets);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        Tensor dx;
+        {
+            at::NoGradGuard off;
+            const auto saved = ctx->get_saved_variables();
+            const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(grads[0].device());
+            dx = run_combine(grads[0].contiguous(), saved[0], saved[1], Tensor());
+        }
+        return no_further({dx, Tensor(), Tensor()}, {grads[0]}, "dispatch");
+    }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &rows, const std::optional<Tensor> &weights_, const Tensor &position,
+                          const Tensor &offsets) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor weights = weights_.value_or(Tensor());
+        // the rows themselves are needed for the weights' gradient only
+        ctx->save_for_backward({weights.defined() ? rows : Tensor(), weights, position, offsets});
+        return run_combine(rows, position, offsets, weights);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        Tensor dr, dw;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &rows = saved[0], &weights = saved[1], &position = saved[2], &offsets = saved[3];
+        {
+            at::NoGradGuard off;
+            const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(grads[0].device());
+            const Tensor g = grads[0].contiguous();
+            if (!weights.defined()) {
+                dr = run_dispatch(g, position, offsets);
+            } else {
+                if (ctx->needs_input_grad(0)) dr = at::empty_like(rows);
+                if (ctx->needs_input_grad(1)) dw = at::empty_like(weights);
+                check(mtp_combine_rows_grad(type_code(rows), at_(rows), at_(g), g.size(0), (int)g.size(1), (int)position.size(1),
+                                            places(position), held(offsets), static_cast<const float *>(at_(weights)), at_(dr),
+                                            static_cast<float *>(at_(dw)), stream_of(g)),
+                      "mtp_combine_rows_grad");
+            }
+        }
+        return no_further({dr, dw, Tensor(), Tensor()}, {rows, weights, grads[0]}, "combine");
+    }
+};
+
+bool plan_for(const Tensor &t, const Tensor &position, const Tensor &offsets) {
+    return position.dim() == 2 && like(position, at::kInt, t, position.sizes()) && offsets.dim() == 1 && offsets.numel() >= 1 &&
+           like(offsets, at::kInt, t, offsets.sizes());
+}
+
+std::optional<Tensor> dispatch(const Tensor &x, const Tensor &position, const Tensor &offsets) {
+    if (!matrix(x) || row_distance(x) < 0 || !plan_for(x, position, offsets) || position.size(0) != x.size(0) || x.size(1) < 1 ||
+        position.size(1) < 1)
+        return std::nullopt;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, position, offsets);
+    return run_dispatch(x, position, offsets);
+}
+
+std::optional<Tensor> combine(const Tensor &rows, const Tensor &position, const Tensor &offsets, const std::optional<Tensor> &weights_) {
+    const Tensor weights = weights_.value_or(Tensor());
+    if (!matrix(rows) || !rows.is_contiguous() || !plan_for(rows, position, offsets) || rows.size(0) != position.numel() ||
+        rows.size(1) < 1 || position.size(1) < 1)
+        return std::nullopt;
+    if (weights.defined() && !like(weights, at::kFloat, rows, position.sizes())) return std::nullopt;
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(rows.device());
+    if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.defined() && weights.requires_grad())))
+        return Combine::apply(rows, weights_, position, offsets);
+    return run_combine(rows, position, offsets, weights);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("linear", &linear);
+    m.def("route_topk", &route_topk);
+    m.def("sort_pairs", &sort_pairs);
+    m.def("dispatch", &dispatch);
+    m.def("combine", &combine);
+}

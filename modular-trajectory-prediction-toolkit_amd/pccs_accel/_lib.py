@@ -136,6 +136,23 @@ def lib():
     return _LIB
 
 
+_BINDING = None
+
+
+def binding():
+    """The entry points as torch calls them, with autograd nodes (csrc/binding.cpp).  Raises if it has not been built."""
+    global _BINDING
+    if _BINDING is None:
+        lib()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise MtpError(f"{os.path.join(_HERE, '_binding.so')} does not load ({e}): build it with "
+                           "`make -C modular-trajectory-prediction-toolkit_amd/csrc` (or __graft_entry__.build())") from e
+        _BINDING = _binding
+    return _BINDING
+
+
 def check(rc, what):
     if rc != 0:
         raise MtpError(f"{what} failed (rc={rc}): {lib().mtp_last_error().decode(errors='replace')}")

@@ -511,19 +511,16 @@ def route_topk(scores, k, normalize=True, want_stats=False):
     return ids, weights, stats
 
 
-def route_topk_grad(scores, ids, weights, stats, grad, normalize=True, trusted=False):
-    """Gradient of the scores [N, E] from that of the weights [N, k] -- ``mtp_route_topk_grad``.
-
-    ``trusted`` (here and below): the tensors are those of a forward call, which has checked them."""
-    if not trusted:
-        _device_tensor(scores, "scores", 2)
-        _type_code(scores, "scores")
-        _like(ids, "ids", 2, scores, "scores", torch.int32)
-        n, k = scores.shape[0], ids.shape[1]
-        _like(ids, "ids", 2, scores, "scores", torch.int32, (n, k))
-        _like(weights, "weights", 2, scores, "scores", torch.float32, (n, k))
-        _like(stats, "stats", 2, scores, "scores", torch.float32, (n, 2))
-        _like(grad, "grad", 2, scores, "scores", torch.float32, (n, k))
+def route_topk_grad(scores, ids, weights, stats, grad, normalize=True):
+    """Gradient of the scores [N, E] from that of the weights [N, k] -- ``mtp_route_topk_grad``."""
+    _device_tensor(scores, "scores", 2)
+    _type_code(scores, "scores")
+    _like(ids, "ids", 2, scores, "scores", torch.int32)
+    n, k = scores.shape[0], ids.shape[1]
+    _like(ids, "ids", 2, scores, "scores", torch.int32, (n, k))
+    _like(weights, "weights", 2, scores, "scores", torch.float32, (n, k))
+    _like(stats, "stats", 2, scores, "scores", torch.float32, (n, 2))
+    _like(grad, "grad", 2, scores, "scores", torch.float32, (n, k))
     code, (n, e), k = _TYPE_CODE[scores.dtype], scores.shape, ids.shape[1]
     ld = _row_distance(scores, "scores")
     out = torch.empty((n, e), dtype=scores.dtype, device=scores.device)
@@ -556,15 +553,14 @@ def _held(offsets):
     return offsets.data_ptr() + 4 * (offsets.numel() - 1)
 
 
-def dispatch_rows(x, position, offsets, trusted=False):
+def dispatch_rows(x, position, offsets):
     """rows [N * k, D]: x's rows at their pairs' places -- ``mtp_dispatch_rows``."""
-    if not trusted:
-        _device_tensor(x, "x", 2)
-        _type_code(x, "x")
-        _like(position, "position", 2, x, "x", torch.int32)
-        _like(offsets, "offsets", 1, x, "x", torch.int32)
-        if position.shape[0] != x.shape[0]:
-            raise ValueError(f"x has {x.shape[0]} rows, the pairs have {position.shape[0]}")
+    _device_tensor(x, "x", 2)
+    _type_code(x, "x")
+    _like(position, "position", 2, x, "x", torch.int32)
+    _like(offsets, "offsets", 1, x, "x", torch.int32)
+    if position.shape[0] != x.shape[0]:
+        raise ValueError(f"x has {x.shape[0]} rows, the pairs have {position.shape[0]}")
     code, (n, d) = _TYPE_CODE[x.dtype], x.shape
     ld, k = _row_distance(x, "x"), position.shape[1]
     rows = torch.empty((n * k, d), dtype=x.dtype, device=x.device)
@@ -583,21 +579,19 @@ def _check_rows(rows, position, offsets, weights):
         _like(weights, "weights", 2, rows, "rows", torch.float32, (n, k))
 
 
-def combine_rows(rows, position, offsets, weights=None, trusted=False):
+def combine_rows(rows, position, offsets, weights=None):
     """[N, D]: each agent's rows summed with its weights (None: all one) -- ``mtp_combine_rows``."""
-    if not trusted:
-        _check_rows(rows, position, offsets, weights)
+    _check_rows(rows, position, offsets, weights)
     code, (n, k), d = _TYPE_CODE[rows.dtype], position.shape, rows.shape[1]
     y = torch.empty((n, d), dtype=rows.dtype, device=rows.device)
     _call(rows.device, "mtp_combine_rows", code, _at(rows), n, d, k, _at(position), _held(offsets), _at(weights), _at(y))
     return y
 
 
-def combine_rows_grad(rows, grad, position, offsets, weights, want_rows=True, want_weights=True, trusted=False):
+def combine_rows_grad(rows, grad, position, offsets, weights, want_rows=True, want_weights=True):
     """(gradient of rows or None, of weights or None) from that of ``combine_rows``' result -- ``mtp_combine_rows_grad``."""
-    if not trusted:
-        _check_rows(rows, position, offsets, weights)
-        _like(grad, "grad", 2, rows, "rows", shape=(position.shape[0], rows.shape[1]))
+    _check_rows(rows, position, offsets, weights)
+    _like(grad, "grad", 2, rows, "rows", shape=(position.shape[0], rows.shape[1]))
     code, (n, k), d = _TYPE_CODE[rows.dtype], position.shape, rows.shape[1]
     grad_rows = torch.empty_like(rows) if want_rows else None
     grad_weights = torch.empty_like(weights) if want_weights else None
@@ -727,19 +721,17 @@ def linear_grad_weight(dz, x, offsets=None, want_bias=False):
     return dw, db
 
 
-def linear_backward(grad, pre, activation, x, weight, offsets=None, want_x=True, want_weight=True, want_bias=True,
-                    trusted=False):
+def linear_backward(grad, pre, activation, x, weight, offsets=None, want_x=True, want_weight=True, want_bias=True):
     """(dx, dweight, dbias), None for what is not wanted, from the gradient of ``linear``'s result (contiguous) and the
     ``pre`` it gave (None without an activation) -- ``mtp_linear_backward``: one call for the whole backward pass."""
-    if not trusted:
-        _device_tensor(x, "x", 2)
-        _type_code(x, "x")
-        out, i = _sets(weight, x, offsets)[1:]
-        if x.shape[1] != i:
-            raise ValueError(f"x has {x.shape[1]} features, weight takes {i}")
-        _like(grad, "grad", 2, x, "x", shape=(x.shape[0], out))
-        if _act_code(activation):
-            _like(pre, "pre", 2, x, "x", shape=(x.shape[0], out))
+    _device_tensor(x, "x", 2)
+    _type_code(x, "x")
+    out, i = _sets(weight, x, offsets)[1:]
+    if x.shape[1] != i:
+        raise ValueError(f"x has {x.shape[1]} features, weight takes {i}")
+    _like(grad, "grad", 2, x, "x", shape=(x.shape[0], out))
+    if _act_code(activation):
+        _like(pre, "pre", 2, x, "x", shape=(x.shape[0], out))
     code, act, (rows, i) = _TYPE_CODE[x.dtype], _ACT_CODE[activation], x.shape
     s, out = (1, weight.shape[0]) if offsets is None else weight.shape[:2]
     want_weight = want_weight or want_bias

@@ -10,38 +10,18 @@ activation z is kept in the same type (rounded once).  Second derivatives are no
 stream, wait for nothing and can be captured into a graph; sums have a fixed order.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels as K
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, offsets):
-        # relu's slope can be read off y where nothing was added to it
-        from_y = activation == "relu" and residual is None
-        y, pre = K.linear(x, weight, bias, activation, residual, offsets, want_pre=activation not in (None, "none") and not from_y)
-        ctx.save_for_backward(x, weight, y if from_y else pre, offsets)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        x, weight, pre, offsets = ctx.saved_tensors
-        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        grad = grad.contiguous()
-        dx, dw, db = K.linear_backward(grad, pre, ctx.activation, x, weight, offsets, want_x, want_w, want_b, trusted=True)
-        dr = None
-        if want_r:  # rows behind the last set have none
-            dr = grad if offsets is None else K.linear_mask_rows(grad, offsets)
-        return dx, dw if want_w else None, db, dr, None, None
+from ._lib import binding
 
 
 def _apply(x, weight, bias, activation, residual, offsets):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, residual)):
-        return _Linear.apply(x, weight, bias, residual, activation, offsets)
-    return K.linear(x, weight, bias, activation, residual, offsets)[0]
+    try:
+        y = binding().linear(x, weight, bias, K._act_code(activation), residual, offsets)
+    except TypeError:  # not even the right kinds of objects
+        y = None
+    # None: the arguments are not as they have to be, and the front end says what is wrong
+    return y if y is not None else K.linear(x, weight, bias, activation, residual, offsets)[0]
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):

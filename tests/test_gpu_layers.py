@@ -357,3 +357,39 @@ def test_refusals(gpu_device):
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_second_derivatives_are_refused(gpu_device):
+    x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(16, 20, 8, 8, torch.float32))
+    x, w = x.requires_grad_(), w.requires_grad_()
+    y = linear(x, w, b, "gelu")
+    dx, = torch.autograd.grad(y, x, gy, create_graph=True)
+    R.check("dx", dx, R.linear(x.detach().cpu(), w.detach().cpu(), b.cpu(), "gelu", None, gy.cpu())["dx"])
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(dx.sum(), x)
+
+
+def test_changed_inputs_are_noticed_by_the_backward_pass(gpu_device):
+    x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(17, 20, 8, 8, torch.float32))
+    x = x.requires_grad_()
+    y = linear(x, w, b, "relu")
+    y.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, gy)
+    y = linear(x, w, b, "gelu")
+    w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, gy)
+
+
+def test_front_ends_and_nodes_agree_bit_for_bit(gpu_device):
+    """The entry points through ``kernels`` (no autograd) and through the nodes."""
+    for dtype in R.TYPES:
+        x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(18, 1500, 40, 56, dtype))
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        y = linear(leaves[0], leaves[1], leaves[2], "silu", leaves[3])
+        dx, dw, db, dr = torch.autograd.grad(y, leaves, gy)
+        y2, pre = K.linear(x, w, b, "silu", r, want_pre=True)
+        dx2, dw2, db2 = K.linear_backward(gy, pre, "silu", x, w)
+        for a, c in ((y, y2), (dx, dx2), (dw, dw2), (db, db2), (dr, gy)):
+            assert torch.equal(a, c)

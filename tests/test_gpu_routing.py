@@ -348,3 +348,22 @@ def test_refusals(gpu_device):
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_second_derivatives_are_refused(gpu_device):
+    s = _scores(1, 6, 20, torch.float32).to(gpu_device).requires_grad_()
+    ids, w = route_topk(s, 3)
+    ds, = torch.autograd.grad(w[:, 0].sum(), s, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(ds.square().sum(), s)
+    plan = sort_pairs(ids, 20)
+    x = torch.randn(6, 8, device=gpu_device, requires_grad=True)
+    rows = torch.randn(18, 8, device=gpu_device, requires_grad=True)
+    g = torch.randn(18, 8, device=gpu_device, requires_grad=True)
+    dx, = torch.autograd.grad(dispatch(x, plan), x, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(dx.sum(), g)
+    weights = w.detach().requires_grad_()
+    dr, dw = torch.autograd.grad(combine(rows, plan, weights).square().sum(), [rows, weights], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(dr.sum() + dw.sum(), rows)
