@@ -17,6 +17,7 @@ import torch
 
 from . import _lib
 from . import kernels as K
+from .routing import combine, dispatch, route_topk, sort_pairs
 
 MODE_NAMES = {0: "ADE-prioritized", 1: "FDE-prioritized", 2: "Equal-Focus"}
 
@@ -59,6 +60,25 @@ def predict_topk(net, obs_enc, k, all_modalities):
     future_enc = net.synthesizer(expanded, labels=labels, all_modalities=all_modalities)
     out = net.decoder([expanded, future_enc])
     return out.reshape(n, k, out.shape[-2], 2)
+
+
+def predict_mixture(net, obs_enc, k, all_modalities, normalize=True):
+    """``predict_topk`` with the weight of each candidate and their weighted mean, differentiable.
+
+    The classifier's k most probable modalities of each agent, their probabilities as weights (``normalize=True``: summing to
+    one over the k), synthesizer and decoder over the (agent, modality) pairs sorted by modality, so that the pairs of a
+    modality read the same row of ``all_modalities`` one after the other, and the candidates averaged back per agent.
+
+    Returns (displacements [N, k, T, 2], weights float32 [N, k], mean displacements [N, T, 2]).  Equal probabilities go by the
+    lower index.  A modality of probability zero is no candidate: its weight is 0 and its place holds modality 0's."""
+    ids, weights = route_topk(torch.log(net.classifier(obs_enc)), k, normalize=normalize)
+    plan = sort_pairs(ids, all_modalities.shape[0])
+    rows = dispatch(obs_enc.contiguous(), plan)
+    labels = ids.reshape(-1)[plan.order.long()].clamp_min(0).long()
+    out = net.decoder([rows, net.synthesizer(rows, labels=labels, all_modalities=all_modalities)])
+    n, t = obs_enc.shape[0], out.shape[-2]
+    mean = combine(out.reshape(n * k, t * 2).contiguous(), plan, weights)
+    return out[plan.position.long()].reshape(n, k, t, 2), weights, mean.reshape(n, t, 2)
 
 
 def _collect(loader, keys):

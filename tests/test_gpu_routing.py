@@ -367,3 +367,38 @@ def test_second_derivatives_are_refused(gpu_device):
     dr, dw = torch.autograd.grad(combine(rows, plan, weights).square().sum(), [rows, weights], create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(dr.sum() + dw.sum(), rows)
+
+
+def test_predict_mixture_is_predict_topk_with_weights(gpu_device):
+    """Candidates as predict_topk gives them (the toy net's probabilities differ), weights and mean by their formulas, gradients."""
+    from pccs_accel.evaluation import predict_mixture, predict_topk
+    from test_gpu_glue import _ToyNet
+    net = _ToyNet().to(gpu_device)
+    g = torch.Generator().manual_seed(3)
+    obs = torch.randn(29, 16, generator=g).to(gpu_device)
+    mods = torch.randn(12, 32, generator=g).to(gpu_device)
+    for k in (1, 5, 12):
+        with torch.no_grad():
+            want = predict_topk(net, obs, k, mods)
+            disp, weights, mean = predict_mixture(net, obs, k, mods)
+            p = net.classifier(obs).double().sort(dim=1, descending=True).values[:, :k]
+        # the same float32 products over rows in another order: the library may choose another kernel, 32 terms each
+        assert torch.allclose(disp, want, rtol=0, atol=64 * R.U32 * float(want.abs().max()) + 64 * R.U32)
+        w = (p / p.sum(1, keepdim=True)).cpu()
+        R.check("weights", weights, (w, 128 * R.U32 * w))  # log and exp of probabilities down to e^-30
+        exact = (w[:, :, None, None] * disp.cpu().double()).sum(1)
+        size = (w[:, :, None, None] * disp.cpu().double().abs()).sum(1)
+        R.check("mean", mean, (exact, (130 + k) * R.U32 * size))
+    leaf = obs.clone().requires_grad_()
+    params = [leaf] + [q for q in net.parameters()]
+    _, _, mean = predict_mixture(net, leaf, 4, mods)
+    got = torch.autograd.grad(mean.square().sum(), params)
+    ref = _ToyNet().to(gpu_device).double()
+    leaf64 = obs.double().requires_grad_()
+    top = ref.classifier(leaf64).topk(4, dim=1)
+    w = top.values / top.values.sum(1, keepdim=True)
+    many = leaf64.repeat_interleave(4, dim=0)
+    out = ref.decoder([many, ref.synthesizer(many, labels=top.indices.reshape(-1), all_modalities=mods.double())]).reshape(29, 4, 12, 2)
+    want = torch.autograd.grad((w[:, :, None, None] * out).sum(1).square().sum(), [leaf64] + [q for q in ref.parameters()])
+    for a, c in zip(got, want):  # float32 sums of at most 29 * 4 * 24 terms
+        assert float((a.double() - c).norm()) <= 29 * 4 * 24 * R.U32 * float(c.norm()) + 1e-12
