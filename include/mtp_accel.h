@@ -492,6 +492,10 @@ int mtp_combine_rows_grad(int dtype, const void *rows, const void *g, int64_t n,
 #define MTP_LINEAR_GRAD_WEIGHT 2
 int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows, int in, int out, int n_sets, const void *a, int64_t lda,
                                    const void *b, int64_t ldb);
+/* Whether x's rows start where the products want them, and a copy that does (ldo a multiple of 8): a caller that needs the rows for
+ * a forward and a backward call lays them out once. */
+int mtp_linear_rows_aligned(int dtype, const void *x, int64_t ld);
+int mtp_linear_align_rows(int dtype, const void *x, int64_t rows, int cols, int64_t ld, void *to, int64_t ldo, void *stream);
 int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias, int act,
                const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre, void *ws, size_t ws_bytes,
                void *stream);

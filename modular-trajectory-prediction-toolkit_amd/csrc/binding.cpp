@@ -95,9 +95,18 @@ struct Linear : torch::autograd::Function<Linear> {
         const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
         // relu's slope can be read off y where nothing was added to it
         const bool from_y = z.act == RELU && !residual.defined();
+        // rows that do not start where the products want them are laid out once for both passes
+        Tensor rows = x;
+        if (!mtp_linear_rows_aligned(z.code, at_(x), row_distance(x))) {
+            const int64_t ld = (z.in + 7) / 8 * 8;
+            const Tensor all = at::empty({z.rows, ld}, x.options());
+            check(mtp_linear_align_rows(z.code, at_(x), z.rows, (int)z.in, row_distance(x), at_(all), ld, stream_of(x)),
+                  "mtp_linear_align_rows");
+            rows = all.narrow(1, 0, z.in);
+        }
         Tensor pre;
-        Tensor y = run_linear(z, x, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr);
-        ctx->save_for_backward({x, w, from_y ? y : pre, offsets});
+        Tensor y = run_linear(z, rows, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr);
+        ctx->save_for_backward({rows, w, from_y ? y : pre, offsets});
         ctx->saved_data["sizes"] =
             std::vector<int64_t>{z.code, z.act, z.rows, z.in, z.out, z.sets, bias.defined(), residual.defined()};
         return y;

@@ -8,46 +8,80 @@
 // activation: one rounding, half a step of the type relative to z, and act' is taken at that point.
 #include "linear_kernel.h"
 
-// [rows, cols] with leading dimension ld -> the same with leading dimension ldo: operands whose rows do not start on a 4-byte
-// boundary (the LDS loads' unit) are laid out anew first
+// One or two matrices laid out anew with rows that start where the LDS loads want them (a 16-bit row of odd length starts on 2
+// bytes, their unit is 4): rows of `cols` elements, from ld to ldo apart, eight elements a thread.
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_relayout(const T *__restrict__ in, int64_t rows, int cols, int64_t ld,
-                                                         T *__restrict__ out, int64_t ldo) {
-    const int64_t n = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        out[r * ldo + c] = in[r * ld + c];
+struct LinCopy {
+    const T *from;
+    T *to;
+    int64_t rows, ld, ldo;
+    int cols;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_relayout(LinCopy<T> p, LinCopy<T> q, int64_t first_blocks) {
+    const bool second = blockIdx.x >= first_blocks;
+    const LinCopy<T> &m = second ? q : p;
+    const int64_t block = second ? blockIdx.x - first_blocks : blockIdx.x, blocks = second ? gridDim.x - first_blocks : first_blocks;
+    const uint32_t per = (uint32_t)(m.cols + 7) / 8;
+    // a block takes a run of rows, so that the division stays in 32 bits
+    const int64_t run = (m.rows + blocks - 1) / blocks, r0 = block * run;
+    const int64_t mine = m.rows - r0 < run ? m.rows - r0 : run;
+    if (mine <= 0) return;
+    typedef typename LinLoose<T, 8>::type loose;
+    for (uint32_t i = threadIdx.x; i < (uint32_t)mine * per; i += 256) {
+        const uint32_t r = i / per, c = lin_piece_at((i - r * per) * 8, m.cols, 8);
+        const T *from = m.from + (r0 + r) * m.ld + c;
+        T *to = m.to + (r0 + r) * m.ldo + c;
+        if (m.cols >= 8) *reinterpret_cast<loose *>(to) = *reinterpret_cast<const loose *>(from);
+        else
+            for (int e = 0; e < m.cols; ++e) to[e] = from[e];
     }
 }
 
-// dz = g * act'(z), eight columns a thread.  HBM-bound: g and z are read, dz is written.
+// dz = g * act'(z), 16 bytes a thread.  HBM-bound: g and z are read (once, past the caches), dz is written for the products that
+// follow.  Rows of dz may lie further apart than those of g and z (ldo).
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g, const T *__restrict__ z, int64_t rows, int cols,
                                                          int act, const int32_t *offsets, int n_sets, T *__restrict__ dz,
-                                                         int64_t ldo, int vec) {
+                                                         int64_t ldo) {
+    constexpr int N = 16 / (int)sizeof(T);
+    typedef typename LinLoose<T, N>::type loose;
     if (offsets != nullptr) {
         const int64_t end = offsets[n_sets];
         rows = end < rows ? (end < 0 ? 0 : end) : rows;
     }
-    if (vec) {
-        typedef T t8 __attribute__((ext_vector_type(8)));
-        const int64_t n = rows * (cols / 8);
-        const int per = cols / 8;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-            // read once more at most, and not soon
-            const t8 gv = __builtin_nontemporal_load(reinterpret_cast<const t8 *>(g) + i);
-            const t8 zv = __builtin_nontemporal_load(reinterpret_cast<const t8 *>(z) + i);
-            t8 o;
+    auto one = [&](const loose &gv, const loose &zv, T *to) {
+        float v[N];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(to_f32(gv[e]) * lin_slope(to_f32(zv[e]), act));
-            const int64_t r = i / per, c = i - r * per;
-            *reinterpret_cast<t8 *>(dz + r * ldo + c * 8) = o;
-        }
-    } else {
+        for (int e = 0; e < N; ++e) v[e] = to_f32(gv[e]) * lin_slope(to_f32(zv[e]), act);
+        lin_store<T, N>(to, v);
+    };
+    if (ldo == cols) {  // one long row
         const int64_t n = rows * cols;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-            const int64_t r = i / cols, c = i - r * cols;
-            dz[r * ldo + c] = from_f32<T>(to_f32(g[i]) * lin_slope(to_f32(z[i]), act));
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N; i < n; i += (int64_t)gridDim.x * 256 * N) {
+            if (i + N <= n) {
+                one(__builtin_nontemporal_load(reinterpret_cast<const loose *>(g + i)),
+                    __builtin_nontemporal_load(reinterpret_cast<const loose *>(z + i)), dz + i);
+            } else {
+                for (int64_t e = i; e < n; ++e) dz[e] = from_f32<T>(to_f32(g[e]) * lin_slope(to_f32(z[e]), act));
+            }
+        }
+        return;
+    }
+    const uint32_t per = (uint32_t)(cols + N - 1) / N;
+    const int64_t run = (rows + gridDim.x - 1) / gridDim.x, r0 = blockIdx.x * run;
+    const int64_t mine = rows - r0 < run ? rows - r0 : run;
+    if (mine <= 0) return;
+    for (uint32_t i = threadIdx.x; i < (uint32_t)mine * per; i += 256) {
+        const uint32_t r = i / per, c = lin_piece_at((i - r * per) * N, cols, N);
+        const int64_t at = (r0 + r) * cols + c;
+        T *to = dz + (r0 + r) * ldo + c;
+        if (cols >= N) {
+            one(__builtin_nontemporal_load(reinterpret_cast<const loose *>(g + at)),
+                __builtin_nontemporal_load(reinterpret_cast<const loose *>(z + at)), to);
+        } else {
+            for (int e = 0; e < cols; ++e)
+                to[e] = from_f32<T>(to_f32(g[at + e]) * lin_slope(to_f32(z[at + e]), act));
         }
     }
 }
@@ -137,19 +171,32 @@ int64_t relayout_bytes(int dtype, const void *p, int64_t ld, int64_t rows, int64
     return needs_relayout(dtype, p, ld) ? round_up(rows * round_up(cols, 8) * elem_size(dtype), 256) : 0;
 }
 
+// blocks for a copy of rows x cols: some eight pieces of eight elements a thread, a run of rows each
+int64_t copy_blocks(int64_t rows, int cols) {
+    const int64_t b = (rows * ((cols + 7) / 8) + 2047) / 2048;
+    return b < 1 ? 1 : (b > 65536 ? 65536 : (b > rows && rows > 0 ? rows : b));
+}
+// the two operands of a product, where they need it
 template <typename T>
-int relayout(const void **p, int64_t *ld, int64_t rows, int cols, char **ws, hipStream_t s) {
+int relayout(const void **a, int64_t *lda, int64_t a_rows, int a_cols, const void **b, int64_t *ldb, int64_t b_rows, int b_cols,
+             char **ws, hipStream_t s) {
     const int dtype = sizeof(T) == 4 ? MTP_FLOAT : MTP_BFLOAT16;
-    const int64_t bytes = relayout_bytes(dtype, *p, *ld, rows, cols);
-    if (bytes == 0) return MTP_OK;
-    const int64_t ldo = round_up(cols, 8);
-    T *to = reinterpret_cast<T *>(*ws);
-    hipLaunchKernelGGL(k_linear_relayout<T>, dim3(grid_for(rows * cols)), dim3(256), 0, s, reinterpret_cast<const T *>(*p), rows,
-                       cols, *ld, to, ldo);
+    LinCopy<T> c[2];
+    int n = 0;
+    auto take = [&](const void **p, int64_t *ld, int64_t rows, int cols) {
+        const int64_t bytes = relayout_bytes(dtype, *p, *ld, rows, cols);
+        if (bytes == 0) return;
+        c[n++] = LinCopy<T>{reinterpret_cast<const T *>(*p), reinterpret_cast<T *>(*ws), rows, *ld, round_up(cols, 8), cols};
+        *p = *ws;
+        *ld = round_up(cols, 8);
+        *ws += bytes;
+    };
+    take(a, lda, a_rows, a_cols);
+    take(b, ldb, b_rows, b_cols);
+    if (n == 0) return MTP_OK;
+    const int64_t first = copy_blocks(c[0].rows, c[0].cols), second = n == 2 ? copy_blocks(c[1].rows, c[1].cols) : 0;
+    hipLaunchKernelGGL(k_linear_relayout<T>, dim3((unsigned)(first + second)), dim3(256), 0, s, c[0], c[n - 1], first);
     MTP_LAUNCH_CHECK();
-    *p = to;
-    *ld = ldo;
-    *ws += bytes;
     return MTP_OK;
 }
 
@@ -290,8 +337,7 @@ int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int
     int64_t ldw = in;
     const int few = few_rows(rows, in, out, n_sets > 1, sizeof(T) == 2);
     if (few == 0) {
-        int rc = relayout<T>(&x, &ldx, rows, in, &ws, s);
-        if (rc == MTP_OK) rc = relayout<T>(&w, &ldw, (int64_t)n_sets * out, in, &ws, s);
+        const int rc = relayout<T>(&x, &ldx, rows, in, &w, &ldw, (int64_t)n_sets * out, in, &ws, s);
         if (rc != MTP_OK) return rc;
     }
     LinArgs a{};
@@ -335,8 +381,7 @@ template <typename T>
 int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, const int32_t *offsets, int n_sets,
                void *dx, char *ws, hipStream_t s) {
     int64_t ldw = in;
-    int rc = relayout<T>(&dz, &lddz, rows, out, &ws, s);
-    if (rc == MTP_OK) rc = relayout<T>(&w, &ldw, (int64_t)n_sets * out, in, &ws, s);
+    const int rc = relayout<T>(&dz, &lddz, rows, out, &w, &ldw, (int64_t)n_sets * out, in, &ws, s);
     if (rc != MTP_OK) return rc;
     LinArgs a{};
     a.P = LinOperand{w, ldw, (int64_t)out * ldw};
@@ -353,8 +398,7 @@ int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *
 template <typename T>
 int grad_weight(const void *dz, int64_t rows, int out, int64_t lddz, const void *x, int in, int64_t ldx, const int32_t *offsets,
                 int n_sets, void *dw, void *db, char *ws, hipStream_t s) {
-    int rc = relayout<T>(&dz, &lddz, rows, out, &ws, s);
-    if (rc == MTP_OK) rc = relayout<T>(&x, &ldx, rows, in, &ws, s);
+    int rc = relayout<T>(&dz, &lddz, rows, out, &x, &ldx, rows, in, &ws, s);
     if (rc != MTP_OK) return rc;
     LinArgs a{};
     a.P = LinOperand{x, ldx, 0};
@@ -401,6 +445,27 @@ extern "C" int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows,
     return n + most_parts(rows, n_sets, part_bits_for(rows, in, out, n_sets, elem_size(dtype) == 2)) * out * (in + 1) * 4;
 }
 
+extern "C" int mtp_linear_rows_aligned(int dtype, const void *x, int64_t ld) { return !needs_relayout(dtype, x, ld); }
+
+extern "C" int mtp_linear_align_rows(int dtype, const void *x, int64_t rows, int cols, int64_t ld, void *to, int64_t ldo, void *stream) {
+    int rc = check_sizes("mtp_linear_align_rows", dtype, rows, cols, 1, nullptr, 1);
+    if (rc != MTP_OK) return rc;
+    MTP_REQUIRE(ld >= cols && ldo >= cols, "mtp_linear_align_rows: row distance below the row's length");
+    if (rows == 0) return MTP_OK;
+    MTP_REQUIRE(x && to, "mtp_linear_align_rows: null pointer");
+    hipStream_t s = mtp_stream(stream);
+    const int64_t blocks = copy_blocks(rows, cols);
+    if (dtype == MTP_FLOAT) {
+        const LinCopy<float> c{(const float *)x, (float *)to, rows, ld, ldo, cols};
+        hipLaunchKernelGGL(k_linear_relayout<float>, dim3((unsigned)blocks), dim3(256), 0, s, c, c, blocks);
+    } else {  // the other two types are moved as they are
+        const LinCopy<_Float16> c{(const _Float16 *)x, (_Float16 *)to, rows, ld, ldo, cols};
+        hipLaunchKernelGGL(k_linear_relayout<_Float16>, dim3((unsigned)blocks), dim3(256), 0, s, c, c, blocks);
+    }
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
 extern "C" int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias,
                           int act, const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre,
                           void *ws, size_t ws_bytes, void *stream) {
@@ -427,20 +492,19 @@ extern "C" int mtp_linear_act_grad(int dtype, const void *g, const void *pre, in
     MTP_REQUIRE(lddz >= out, "mtp_linear_act_grad: row distance below the row's length");
     if (rows == 0) return MTP_OK;
     MTP_REQUIRE(g && pre && dz, "mtp_linear_act_grad: null pointer");
-    const int sz = elem_size(dtype);
-    const int vec = out % 8 == 0 && lddz % 8 == 0 &&
-                    ((uintptr_t)g | (uintptr_t)pre | (uintptr_t)dz) % (8 * sz) == 0;
     hipStream_t s = mtp_stream(stream);
-    const dim3 grid(grid_for(vec ? rows * (out / 8) : rows * out));
+    int64_t blocks = (rows * out + 256 * 16 - 1) / (256 * 16);
+    if (lddz != out && blocks > rows) blocks = rows;
+    const dim3 grid((unsigned)(blocks < 1 ? 1 : blocks > 65536 ? 65536 : blocks));
     if (dtype == MTP_FLOAT)
         hipLaunchKernelGGL(k_linear_act_grad<float>, grid, dim3(256), 0, s, (const float *)g, (const float *)pre, rows, out, act,
-                           offsets, n_sets, (float *)dz, lddz, vec);
+                           offsets, n_sets, (float *)dz, lddz);
     else if (dtype == MTP_BFLOAT16)
         hipLaunchKernelGGL(k_linear_act_grad<__bf16>, grid, dim3(256), 0, s, (const __bf16 *)g, (const __bf16 *)pre, rows, out,
-                           act, offsets, n_sets, (__bf16 *)dz, lddz, vec);
+                           act, offsets, n_sets, (__bf16 *)dz, lddz);
     else
         hipLaunchKernelGGL(k_linear_act_grad<_Float16>, grid, dim3(256), 0, s, (const _Float16 *)g, (const _Float16 *)pre, rows,
-                           out, act, offsets, n_sets, (_Float16 *)dz, lddz, vec);
+                           out, act, offsets, n_sets, (_Float16 *)dz, lddz);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }

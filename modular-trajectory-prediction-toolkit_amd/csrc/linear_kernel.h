@@ -411,46 +411,51 @@ struct LinArgs {
     int away;             // the output is more than the caches hold: past them
 };
 
-// N consecutive elements
+// N consecutive elements at any address an element can have (the card reads and writes 16 bytes wherever they start)
 template <typename T, int N>
-__device__ __forceinline__ void lin_store(T *p, const float *v) {
-    if constexpr (N == 1) *p = from_f32<T>(v[0]);
+struct LinLoose {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <typename T>
+struct LinLoose<T, 1> {
+    typedef T type;
+};
+// where a row's piece starts: the last one moves back so that it ends with the row, and says some of the one before it again (a
+// thread that went through an incomplete piece by elements would hold its wave up)
+__device__ __forceinline__ uint32_t lin_piece_at(uint32_t c, int cols, int n) {
+    return (int)c + n <= cols ? c : cols >= n ? (uint32_t)(cols - n) : 0;
+}
+template <typename T, int N>
+__device__ __forceinline__ typename LinLoose<T, N>::type lin_pack(const float *v) {
+    typename LinLoose<T, N>::type w;
+    if constexpr (N == 1) w = from_f32<T>(v[0]);
     else {
-        typedef T tn __attribute__((ext_vector_type(N)));
-        tn w;
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = from_f32<T>(v[e]);
-        *reinterpret_cast<tn *>(p) = w;
     }
+    return w;
+}
+template <typename T, int N>
+__device__ __forceinline__ void lin_store(T *p, const float *v) {
+    *reinterpret_cast<typename LinLoose<T, N>::type *>(p) = lin_pack<T, N>(v);
 }
 // the same past the caches: what is not read again soon
 template <typename T, int N>
 __device__ __forceinline__ void lin_store_away(T *p, const float *v) {
-    if constexpr (N == 1) __builtin_nontemporal_store(from_f32<T>(v[0]), p);
-    else {
-        typedef T tn __attribute__((ext_vector_type(N)));
-        tn w;
-#pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = from_f32<T>(v[e]);
-        __builtin_nontemporal_store(w, reinterpret_cast<tn *>(p));
-    }
+    __builtin_nontemporal_store(lin_pack<T, N>(v), reinterpret_cast<typename LinLoose<T, N>::type *>(p));
 }
 template <typename T, int N>
-__device__ __forceinline__ void lin_load(const T *p, float *v) {
-    if constexpr (N == 1) v[0] = to_f32(*p);
+__device__ __forceinline__ void lin_unpack(const typename LinLoose<T, N>::type &w, float *v) {
+    if constexpr (N == 1) v[0] = to_f32(w);
     else {
-        typedef T tn __attribute__((ext_vector_type(N)));
-        const tn w = *reinterpret_cast<const tn *>(p);
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = to_f32(w[e]);
     }
 }
-// 16-byte pieces: the address and the row distance allow them
-template <typename T>
-__device__ __forceinline__ bool lin_aligned16(const void *p, int64_t ld) {
-    return (uintptr_t)p % 16 == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
+template <typename T, int N>
+__device__ __forceinline__ void lin_load(const T *p, float *v) {
+    lin_unpack<T, N>(*reinterpret_cast<const typename LinLoose<T, N>::type *>(p), v);
 }
-
 // Consecutive workgroups go to different XCDs in turn: each XCD gets one contiguous run of tiles, so that the tiles that share
 // an operand meet in one L2.
 __device__ __forceinline__ int64_t lin_xcd_order(int64_t id, int64_t n) {
@@ -469,48 +474,65 @@ constexpr int lin_pass_rows(int room, int rows) {
 
 enum { LIN_FORWARD = 0, LIN_GRAD_INPUT = 1, LIN_GRAD_WEIGHT = 2 };
 
-// A tile's rows on their way out of LDS, N columns a thread; U is the type they leave in.  Up to four rows are on their way at a time (two where
-// there are many: 256 x 256 tiles with everything 335 us, 388 with four).
-template <typename T, typename U, int MODE, int BC, int ER, int NT, int N>
+// A tile's rows on their way out of LDS, N columns (16 bytes) a thread; U is the type they leave in.  Up to four rows are on their
+// way at a time (two where there are many: 256 x 256 tiles with everything 335 us, 388 with four).  The thread that has a row's
+// last, incomplete piece takes it element by element.
+template <typename T, typename U, int MODE, int BC, int ER, int NT>
 __device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, const float *bias, U *to, int64_t r0, int64_t row_end,
                                           int64_t c0, int tid) {
-    constexpr int ITEMS = BC / N, STEP = NT / ITEMS;  // items of a row; rows that the workgroup takes at a time
+    constexpr int N = 16 / (int)sizeof(U), ITEMS = BC / N, STEP = NT / ITEMS;  // STEP: rows that the workgroup takes at a time
     constexpr int PM = lin_twist_mask(BC / 4), AT_ONCE = ER / STEP < 1 ? 1 : ER / STEP <= 4 ? ER / STEP : 2;
     const int item = tid % ITEMS;
     const int64_t col = c0 + item * N;
-    if (col >= a.cols || tid >= ITEMS * STEP) return;  // (16-byte pieces: cols is a multiple of N)
+    if (col >= a.cols || tid >= ITEMS * STEP) return;
+    const int n = (int)(a.cols - col < N ? a.cols - col : N);
     const int rows = (int)(row_end - r0 < ER ? row_end - r0 : ER);
+    const bool away = MODE != LIN_GRAD_WEIGHT && a.away;
     for (int row0 = tid / ITEMS; row0 < rows; row0 += STEP * AT_ONCE) {
         float v[AT_ONCE][N], res[AT_ONCE][N];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
             const int row = row0 + u * STEP < rows ? row0 + u * STEP : row0;
-            if constexpr (N == 1) {
-                v[u][0] = z[row * BC + (((item >> 2) ^ (row & PM)) << 2) + (item & 3)];
-            } else {
 #pragma unroll
-                for (int q = 0; q < N / 4; ++q) {
-                    const f32x4v w = *reinterpret_cast<const f32x4v *>(z + row * BC + (((item * (N / 4) + q) ^ (row & PM)) << 2));
+            for (int q = 0; q < N / 4; ++q) {
+                const f32x4v w = *reinterpret_cast<const f32x4v *>(z + row * BC + (((item * (N / 4) + q) ^ (row & PM)) << 2));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[u][q * 4 + e] = w[e];
-                }
+                for (int e = 0; e < 4; ++e) v[u][q * 4 + e] = w[e];
             }
             if constexpr (MODE == LIN_FORWARD) {
-                if (a.residual != nullptr)
-                    lin_load<T, N>(reinterpret_cast<const T *>(a.residual) + (r0 + row) * a.ld_res + col, res[u]);
+                if (a.residual != nullptr) {
+                    const T *from = reinterpret_cast<const T *>(a.residual) + (r0 + row) * a.ld_res + col;
+                    if (n == N) lin_load<T, N>(from, res[u]);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) res[u][e] = e < n ? to_f32(from[e]) : 0.f;
+                    }
+                }
             }
         }
+        auto leave = [&](auto *first, bool past) {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                if (row0 + u * STEP >= rows) continue;
+                auto *at = first + (r0 + row0 + u * STEP) * a.cols + col;
+                typedef std::remove_reference_t<decltype(*at)> V;
+                if (n < N) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (e < n) at[e] = from_f32<V>(v[u][e]);
+                } else if (past) {
+                    lin_store_away<V, N>(at, v[u]);
+                } else {
+                    lin_store<V, N>(at, v[u]);
+                }
+            }
+        };
         if constexpr (MODE == LIN_FORWARD) {
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
                 for (int e = 0; e < N; ++e) v[u][e] += bias[e];
-            if (a.pre != nullptr) {
-#pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u)
-                    if (row0 + u * STEP < rows)
-                        lin_store_away<T, N>(reinterpret_cast<T *>(a.pre) + (r0 + row0 + u * STEP) * a.cols + col, v[u]);
-            }
+            if (a.pre != nullptr) leave(reinterpret_cast<T *>(a.pre), true);
             auto bend = [&](auto kind) {
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u)
@@ -527,25 +549,21 @@ __device__ __forceinline__ void lin_leave(const LinArgs &a, const float *z, cons
                     for (int e = 0; e < N; ++e) v[u][e] += res[u][e];
             }
         }
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-            if (row0 + u * STEP < rows) {
-                U *at = to + (r0 + row0 + u * STEP) * a.cols + col;
-                if (MODE != LIN_GRAD_WEIGHT && a.away) lin_store_away<U, N>(at, v[u]);
-                else lin_store<U, N>(at, v[u]);
-            }
+        leave(to, away);
     }
 }
 // the bias of the columns that lin_leave gives this thread
-template <typename T, int BC, int N>
+template <typename T, int BC>
 __device__ __forceinline__ void lin_bias(const LinArgs &a, int set, int64_t c0, int tid, float *bias) {
+    constexpr int N = 16 / (int)sizeof(T);
     const int64_t col = c0 + tid % (BC / N) * N;
 #pragma unroll
     for (int e = 0; e < N; ++e) bias[e] = 0.f;
-    if (a.bias == nullptr || col >= a.cols) return;
-    const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols + col;
+    if (a.bias == nullptr) return;
+    const T *b = reinterpret_cast<const T *>(a.bias) + (int64_t)set * a.cols;
 #pragma unroll
-    for (int e = 0; e < N; ++e) bias[e] = to_f32(b[e]);
+    for (int e = 0; e < N; ++e)
+        if (col + e < a.cols) bias[e] = to_f32(b[col + e]);
 }
 
 // waves a SIMD that a tile's 2 * (BC + BR) * 128 bytes of LDS leave room for (160 KB a CU): what the registers have to allow
@@ -725,17 +743,8 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     static_assert(BR % ER == 0 && ER % WR == 0, "a wave's rows are in one pass");
     float *z = reinterpret_cast<float *>(smem);
     const bool to_partial = MODE == LIN_GRAD_WEIGHT && part_at >= 0;
-    bool vec = lin_aligned16<T>(a.out, a.cols);
-    if constexpr (MODE == LIN_FORWARD) {
-        if (a.residual != nullptr) vec = vec && lin_aligned16<T>(a.residual, a.ld_res);
-        if (a.pre != nullptr) vec = vec && lin_aligned16<T>(a.pre, a.cols);
-    }
-    if (to_partial) vec = a.cols % 4 == 0;
     float bias[16 / SZ];
-    if constexpr (MODE == LIN_FORWARD) {
-        if (vec) lin_bias<T, BC, 16 / SZ>(a, set, c0, tid, bias);
-        else lin_bias<T, BC, 1>(a, set, c0, tid, bias);
-    }
+    if constexpr (MODE == LIN_FORWARD) lin_bias<T, BC>(a, set, c0, tid, bias);
     for (int p0 = 0; p0 < BR; p0 += ER) {
         __syncthreads();
         if (wr * WR >= p0 && wr * WR < p0 + ER) {
@@ -757,12 +766,10 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
         const int64_t r0 = row0 + p0;
         if (to_partial) {
             float *part = a.partial + part_at * a.out_rows * a.cols;
-            if (vec) lin_leave<T, float, MODE, BC, ER, NT, 4>(a, z, bias, part, r0, row_end, c0, tid);
-            else lin_leave<T, float, MODE, BC, ER, NT, 1>(a, z, bias, part, r0, row_end, c0, tid);
+            lin_leave<T, float, MODE, BC, ER, NT>(a, z, bias, part, r0, row_end, c0, tid);
         } else {
             T *to = out + (MODE == LIN_GRAD_WEIGHT ? (int64_t)set * a.out_rows * a.cols : 0);
-            if (vec) lin_leave<T, T, MODE, BC, ER, NT, 16 / SZ>(a, z, bias, to, r0, row_end, c0, tid);
-            else lin_leave<T, T, MODE, BC, ER, NT, 1>(a, z, bias, to, r0, row_end, c0, tid);
+            lin_leave<T, T, MODE, BC, ER, NT>(a, z, bias, to, r0, row_end, c0, tid);
         }
     }
     if constexpr (MODE == LIN_GRAD_WEIGHT && SZ == 4) {  // the two halves of a wave hold different k

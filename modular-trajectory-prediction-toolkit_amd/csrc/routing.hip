@@ -29,10 +29,11 @@ struct RouteKey {
     static constexpr uint32_t INF = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
     // nothing: NONE, or an index without a score (a place beyond the row; -inf's bits are 0x7f or 0x3ff)
     static __device__ __forceinline__ bool nothing(type k) { return k < 0x10000u; }
-    // the keys of v[0 .. V), indexes from i0 on; those from e on become nothing.  Two scores at a time; NaN (to become -inf) and -0
+    // the keys of v[0 .. V), pieces of W with the indexes from[q] on, of which those in [first[q], end[q]) count.  Two scores at a time; NaN (to become -inf) and -0
     // (to equal +0) are looked for at the end and put right only where a wave has one.
-    template <int V>
-    static __device__ __forceinline__ void keys(const T (&v)[V], int i0, int e, type (&key)[V], bool *bad) {
+    template <int V, int W>
+    static __device__ __forceinline__ void keys(const T (&v)[V], const int (&from)[V / W], const int (&first)[V / W],
+                                                const int (&end)[V / W], type (&key)[V], bool *bad) {
         typedef short s2 __attribute__((ext_vector_type(2)));
         typedef unsigned short u2 __attribute__((ext_vector_type(2)));
         u2 o[(V + 1) / 2], odd = {0xffff, 0xffff}, big = {0, 0};
@@ -50,17 +51,18 @@ struct RouteKey {
             for (int j = 0; j < V; ++j) {
                 uint32_t b = __builtin_bit_cast(uint16_t, v[j]);
                 const bool nan = (b & 0x7fffu) > INF;
-                *bad |= nan && i0 + j < e;
+                const int i = from[j / W] + j % W;
+                *bad |= nan && i >= first[j / W] && i < end[j / W];
                 b = nan ? 0x8000u | INF : b == 0x8000u ? 0u : b;
                 o[j / 2][j & 1] = (unsigned short)((b & 0x8000u) ? (b ^ 0xffffu) : (b | 0x8000u));
             }
         }
-        const uint32_t low = 0xffffu - i0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+            const int i = from[j / W] + j % W;
             const uint32_t w = __builtin_bit_cast(uint32_t, o[j / 2]);
-            const uint32_t k = ((j & 1) ? (w & 0xffff0000u) : (w << 16)) | (low - j);
-            key[j] = i0 + j < e ? k : NONE;
+            const uint32_t k = ((j & 1) ? (w & 0xffff0000u) : (w << 16)) | (0xffffu - i);
+            key[j] = i >= first[j / W] && i < end[j / W] ? k : NONE;
         }
     }
     static __device__ __forceinline__ float score(type k) {
@@ -75,24 +77,35 @@ struct RouteKey {
     static __device__ __forceinline__ type turn(type v) {
         return (type)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
     }
-    static __device__ __forceinline__ type lane(type v, int l) { return (type)__builtin_amdgcn_readlane((int)v, l); }
+    // the larger of a lane's and that of the lane 16 (32) away: the swap puts the two halves side by side
+    static __device__ __forceinline__ type across16(type v) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return more(s[0], s[1]);
+    }
+    static __device__ __forceinline__ type across32(type v) {
+        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return more(s[0], s[1]);
+    }
 };
 template <>
 struct RouteKey<float> {
     typedef double type;
     static constexpr type NONE = 2.0;
     static __device__ __forceinline__ bool nothing(type k) { return k == NONE; }
-    template <int V>
-    static __device__ __forceinline__ void keys(const float (&v)[V], int i0, int e, type (&key)[V], bool *bad) {
+    template <int V, int W>
+    static __device__ __forceinline__ void keys(const float (&v)[V], const int (&from)[V / W], const int (&first)[V / W],
+                                                const int (&end)[V / W], type (&key)[V], bool *bad) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+            const int i = from[j / W] + j % W;
+            const bool counts = i >= first[j / W] && i < end[j / W];
             const bool nan = v[j] != v[j];
-            *bad |= nan && i0 + j < e;
+            *bad |= nan && counts;
             uint32_t b = __float_as_uint((nan ? -__builtin_inff() : v[j]) + 0.0f);  // -0 equals +0
             b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
             const type k = __longlong_as_double(
-                (long long)(0x4000000000000000ull | ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - (i0 + j))));
-            key[j] = i0 + j < e ? k : NONE;
+                (long long)(0x4000000000000000ull | ((uint64_t)b << 12) | (uint32_t)(ROUTE_MAX_E - 1 - i)));
+            key[j] = counts ? k : NONE;
         }
     }
     static __device__ __forceinline__ float score(type k) {
@@ -111,17 +124,26 @@ struct RouteKey<float> {
         const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
         return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
     }
-    static __device__ __forceinline__ type lane(type v, int l) {
-        const uint64_t b = (uint64_t)__double_as_longlong(v);
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
+    static __device__ __forceinline__ type from_words(uint32_t lo, uint32_t hi) {
         return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+    }
+    static __device__ __forceinline__ type across16(type v) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+        return more(from_words(lo[0], hi[0]), from_words(lo[1], hi[1]));
+    }
+    static __device__ __forceinline__ type across32(type v) {
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+        return more(from_words(lo[0], hi[0]), from_words(lo[1], hi[1]));
     }
 };
 
 constexpr int ROW_ROR = 0x120;  // rotation within 16 lanes
 
-// over the L lanes (16 or 64) that share a row, the same result in each
+// over the L lanes (16, 32 or 64) that share a row, the same result in each
 template <typename T, int L>
 __device__ __forceinline__ typename RouteKey<T>::type group_max(typename RouteKey<T>::type v) {
     typedef RouteKey<T> R;
@@ -129,8 +151,8 @@ __device__ __forceinline__ typename RouteKey<T>::type group_max(typename RouteKe
     v = R::more(v, R::template turn<ROW_ROR + 4>(v));
     v = R::more(v, R::template turn<ROW_ROR + 2>(v));
     v = R::more(v, R::template turn<ROW_ROR + 1>(v));
-    if constexpr (L == 64)
-        v = R::more(R::more(R::lane(v, 0), R::lane(v, 16)), R::more(R::lane(v, 32), R::lane(v, 48)));
+    if constexpr (L >= 32) v = R::across16(v);
+    if constexpr (L == 64) v = R::across32(v);
     return v;
 }
 template <int CTRL>
@@ -143,10 +165,8 @@ __device__ __forceinline__ float group_sum(float v) {
     v += turn_f32<ROW_ROR + 4>(v);
     v += turn_f32<ROW_ROR + 2>(v);
     v += turn_f32<ROW_ROR + 1>(v);
-    if constexpr (L == 64) {
-        v += __shfl_xor(v, 16);
-        v += __shfl_xor(v, 32);
-    }
+    if constexpr (L >= 32) v += __shfl_xor(v, 16);
+    if constexpr (L == 64) v += __shfl_xor(v, 32);
     return v;
 }
 
@@ -172,12 +192,11 @@ __device__ __forceinline__ void sort_registers(typename RouteKey<T>::type (&a)[V
     }
 }
 
-// L lanes share a row, lane `sub` holds the scores sub * V to sub * V + V - 1 (loaded in pieces of up to 16 bytes where the rows
-// allow it).  Each lane sorts its keys and lays them into LDS, as many as could be chosen; k times the largest head is taken (a
+// L lanes share a row, lane `sub` holds the scores sub * V to sub * V + V - 1.  Each lane sorts its keys and lays them into LDS, as many as could be chosen; k times the largest head is taken (a
 // maximum over the L lanes), and the lane it came from moves on to its next key.
 template <typename T, int L, int V, int KB>
 __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores, int64_t n, int e, int64_t ld, int k, int normalize,
-                                                    int pieces, int32_t *__restrict__ ids, float *__restrict__ weights,
+                                                    int32_t *__restrict__ ids, float *__restrict__ weights,
                                                     float *__restrict__ stats) {
     typedef RouteKey<T> R;
     typedef typename R::type key_t;
@@ -189,23 +208,35 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
     const bool live = row < n;
     const T *s = scores + (live ? row : n - 1) * ld;
 
+    // pieces of W elements at any address; the one that would reach beyond the row moves back, and what it says again is left out
     T v[V];
-    if (pieces) {  // e is a multiple of W
-        typedef T piece_t __attribute__((ext_vector_type(W)));
+    int from[V / W];
 #pragma unroll
-        for (int q = 0; q < V / W; ++q) {
-            const int i = sub * V + q * W;
-            const piece_t p = *reinterpret_cast<const piece_t *>(s + (i < e ? i : 0));
+    for (int q = 0; q < V / W; ++q) {
+        const int i = sub * V + q * W;
+        from[q] = i + W <= e ? i : e - W;
+        if (i >= e) from[q] = 0;
+        typedef T piece_t __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+        if (e >= W) {
+            const piece_t p = *reinterpret_cast<const piece_t *>(s + from[q]);
 #pragma unroll
             for (int j = 0; j < W; ++j) v[q * W + j] = p[j];
-        }
-    } else {
+        } else {  // a row shorter than one piece
+            from[q] = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = s[sub * V + j < e ? sub * V + j : 0];
+            for (int j = 0; j < W; ++j) v[q * W + j] = s[j < e ? j : 0];
+        }
     }
     key_t key[V];
     bool bad = false;
-    R::keys(v, sub * V, e, key, &bad);
+    // element j of the lane is score from[j / W] + j % W, and counts where no other piece has it
+    int first[V / W], end[V / W];
+#pragma unroll
+    for (int q = 0; q < V / W; ++q) {
+        first[q] = sub * V + q * W;
+        end[q] = first[q] + W < e ? first[q] + W : e;
+    }
+    R::template keys<V, W>(v, from, first, end, key, &bad);
     float total = 0.f, top = 0.f;
     if (!normalize) {  // the softmax over all modalities
         key_t m = key[0];
@@ -218,7 +249,7 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
         total = group_sum<L>(total);
     }
     const uint64_t any_bad = __ballot(bad);
-    const bool row_bad = ((any_bad >> ((tid & 63) / L * L)) & (L == 64 ? ~0ull : 0xffffull)) != 0;
+    const bool row_bad = ((any_bad >> ((tid & 63) / L * L)) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) != 0;
 
     sort_registers<T, V>(key);
     const int depth = V < k ? V : k;
@@ -310,7 +341,21 @@ __global__ __launch_bounds__(256) void k_route_grad(const T *__restrict__ scores
         __syncthreads();
     } else {
         __syncthreads();
-        for (int r = tid >> 6; r < rows; r += 4) {
+        constexpr int N = 16 / (int)sizeof(T);
+        if (e % N == 0) {
+            typedef T loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+            typedef T whole_t __attribute__((ext_vector_type(N)));
+            const uint32_t per = e / N;
+            for (uint32_t i = tid; i < (uint32_t)rows * per; i += 256) {
+                const uint32_t r = i / per;
+                const float top = stats[(row0 + r) * 2], scale = stats[(row0 + r) * 2 + 1] * -dots[r];
+                const loose v = *reinterpret_cast<const loose *>(scores + (row0 + r) * ld + (i - r * per) * N);
+                whole_t w;
+#pragma unroll
+                for (int j = 0; j < N; ++j) w[j] = (T)(expf(up(v[j]) - top) * scale);
+                reinterpret_cast<whole_t *>(tile)[i] = w;
+            }
+        } else for (int r = tid >> 6; r < rows; r += 4) {
             const float top = stats[(row0 + r) * 2], scale = stats[(row0 + r) * 2 + 1] * -dots[r];
             const T *s = scores + (row0 + r) * ld;
             for (int c = tid & 63; c < e; c += 64) tile[r * e + c] = (T)(expf(up(s[c]) - top) * scale);
@@ -469,9 +514,10 @@ __global__ __launch_bounds__(64 * W) void k_pairs_place(const int32_t *__restric
 }
 
 // ---- rows to their pairs and back ----
+// N elements at any address an element can have (the card reads and writes 16 bytes wherever they start)
 template <typename T, int N>
 struct Pack {
-    typedef T type __attribute__((ext_vector_type(N)));
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 template <typename T>
 struct Pack<T, 1> {
@@ -487,46 +533,51 @@ __device__ __forceinline__ void unpack(const typename Pack<T, N>::type &v, float
 }
 template <typename T, int N>
 __device__ __forceinline__ typename Pack<T, N>::type pack(const float *f) {
-    if constexpr (N == 1) return (T)f[0];
+    typename Pack<T, N>::type v;
+    if constexpr (N == 1) v = (T)f[0];
     else {
-        typename Pack<T, N>::type v;
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = (T)f[e];
-        return v;
     }
+    return v;
 }
+// A row of d >= N elements as ceil(d / N) pieces of N: the last one starts at d - N and says some of the one before it again
+__device__ __forceinline__ int piece_at(int c, int d, int n) { return c * n + n <= d ? c * n : d - n; }
 
 // Rows of pairs are read and written once.  More of them than the 256 MB memory-side cache holds go past the caches (ONCE: there
 // and back with gradients over 1.47 M rows of 384 bytes 637 us, 745 us without); fewer are likely still there for the next kernel
 // (143 760 rows of 192 bytes: the two sums 13 us, 17 us past the caches).
-template <bool ONCE, typename V>
-__device__ __forceinline__ V load_row(const V *p) {
-    if constexpr (ONCE) return __builtin_nontemporal_load(p);
-    else return *p;
+template <bool ONCE, typename T, int N>
+__device__ __forceinline__ typename Pack<T, N>::type load_row(const T *p) {
+    const auto *v = reinterpret_cast<const typename Pack<T, N>::type *>(p);
+    if constexpr (ONCE) return __builtin_nontemporal_load(v);
+    else return *v;
+}
+template <bool ONCE, typename T, int N>
+__device__ __forceinline__ void store_row(T *p, const typename Pack<T, N>::type &v) {
+    auto *to = reinterpret_cast<typename Pack<T, N>::type *>(p);
+    if constexpr (ONCE) __builtin_nontemporal_store(v, to);
+    else *to = v;
 }
 
-template <bool ONCE, typename V>
-__device__ __forceinline__ void store_row(V *p, V v) {
-    if constexpr (ONCE) __builtin_nontemporal_store(v, p);
-    else *p = v;
-}
-
-// rows[position[t][j]] = x[t], zero where the pair has no modality; one thread per N elements of a token
-template <typename T, int N, bool ONCE>
+// rows[position[t][j]] = x[t], zero where the pair has no modality; one thread per N elements of a token.  I: an index that holds
+// the number of threads (divisions of 64 bits cost more than the copy).
+template <typename T, int N, bool ONCE, typename I>
 __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64_t n, int d, int64_t ld, int k,
                                                   const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
                                                   T *__restrict__ rows) {
     typedef typename Pack<T, N>::type vec;
-    const int per = d / N;
-    const int64_t total = n * per;
+    const int per = (d + N - 1) / N;
+    const I total = (I)n * per;
     const int held = *held_at;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t t = i / per, c = i - t * per;
-        const vec v = *reinterpret_cast<const vec *>(x + t * ld + c * N);
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
+        const int64_t t = i / per;
+        const int c = piece_at((int)(i - (I)t * per), d, N);
+        const vec v = *reinterpret_cast<const vec *>(x + t * ld + c);
         const vec zero = {};
         for (int j = 0; j < k; ++j) {
             const int64_t p = position[t * k + j];
-            store_row<ONCE>(reinterpret_cast<vec *>(rows + p * d + c * N), p < held ? v : zero);
+            store_row<ONCE, T, N>(rows + p * d + c, p < held ? v : zero);
         }
     }
 }
@@ -534,16 +585,17 @@ __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64
 // y[t] = sum_j weights[t][j] rows[position[t][j]] (weights NULL: all one), pairs without a modality left out.  One thread per N
 // elements of a token; four rows are in flight at a time (their places are all valid, what does not count is dropped after
 // the load).
-template <typename T, int N, bool ONCE>
+template <typename T, int N, bool ONCE, typename I>
 __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int64_t n, int d, int k,
                                                  const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
                                                  const float *__restrict__ weights, T *__restrict__ y) {
     typedef typename Pack<T, N>::type vec;
-    const int per = d / N;
-    const int64_t total = n * per;
+    const int per = (d + N - 1) / N;
+    const I total = (I)n * per;
     const int held = *held_at;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t t = i / per, c = i - t * per;
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
+        const int64_t t = i / per;
+        const int c = piece_at((int)(i - (I)t * per), d, N);
         const int32_t *at = position + t * k;
         const float *wt = weights + t * k;
         float sum[N];
@@ -558,7 +610,7 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
                 const int j = j0 + q < k ? j0 + q : k - 1;
                 const int64_t p = at[j];
                 in[q] = p < held && j0 + q < k;
-                v[q] = load_row<ONCE>(reinterpret_cast<const vec *>(rows + p * d + c * N));
+                v[q] = load_row<ONCE, T, N>(rows + p * d + c);
                 w[q] = weights != nullptr ? wt[j] : 1.f;
             }
 #pragma unroll
@@ -571,7 +623,7 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
                 }
             }
         }
-        store_row<ONCE>(reinterpret_cast<vec *>(y + t * d + c * N), pack<T, N>(sum));
+        store_row<ONCE, T, N>(y + t * d + c, pack<T, N>(sum));
     }
 }
 
@@ -596,18 +648,19 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                                                       float *__restrict__ grad_weights) {
     typedef typename Pack<T, N>::type vec;
     constexpr int Q = C == 1 ? 4 : 1;
-    const int per = d / N, sub = threadIdx.x % L;
+    const int per = (d + N - 1) / N, sub = threadIdx.x % L;
     const int held = *held_at;
     for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L; t < n; t += (int64_t)gridDim.x * (256 / L)) {
         const int32_t *at = position + t * k;
         for (int c0 = 0; c0 < per; c0 += L * C) {
             float gv[C][N];
+            int from[C], again[C];  // where the lane's pieces start, and how many of their elements another piece has too
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int x = c0 + c * L + sub;
-                vec v = {};
-                if (x < per) v = *reinterpret_cast<const vec *>(g + t * d + (int64_t)x * N);
-                unpack<T, N>(v, gv[c]);
+                from[c] = x < per ? piece_at(x, d, N) : 0;
+                again[c] = x < per ? x * N - from[c] : N;
+                unpack<T, N>(*reinterpret_cast<const vec *>(g + t * d + from[c]), gv[c]);
             }
             for (int j0 = 0; j0 < k; j0 += Q) {
                 int64_t p[Q];
@@ -617,10 +670,8 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                     p[q] = at[j0 + q < k ? j0 + q : k - 1];
                     if (grad_weights != nullptr) {
 #pragma unroll
-                        for (int c = 0; c < C; ++c) {
-                            const int x = c0 + c * L + sub;
-                            v[q][c] = load_row<ONCE>(reinterpret_cast<const vec *>(rows + p[q] * d + (int64_t)(x < per ? x : 0) * N));
-                        }
+                        for (int c = 0; c < C; ++c)
+                            v[q][c] = load_row<ONCE, T, N>(rows + p[q] * d + from[c]);
                     }
                 }
 #pragma unroll
@@ -632,11 +683,11 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                         const float w = in ? weights[t * k + j] : 0.f;
 #pragma unroll
                         for (int c = 0; c < C; ++c) {
-                            const int x = c0 + c * L + sub;
                             float o[N];
 #pragma unroll
                             for (int e = 0; e < N; ++e) o[e] = in ? w * gv[c][e] : 0.f;
-                            if (x < per) store_row<ONCE>(reinterpret_cast<vec *>(grad_rows + p[q] * d + (int64_t)x * N), pack<T, N>(o));
+                            if (c0 + c * L + sub < per)
+                                store_row<ONCE, T, N>(grad_rows + p[q] * d + from[c], pack<T, N>(o));
                         }
                     }
                     if (grad_weights != nullptr) {
@@ -645,9 +696,9 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                         for (int c = 0; c < C; ++c) {
                             float rv[N];
                             unpack<T, N>(v[q][c], rv);
-                            if (in && c0 + c * L + sub < per) {
+                            if (in) {
 #pragma unroll
-                                for (int e = 0; e < N; ++e) dot = fmaf(rv[e], gv[c][e], dot);
+                                for (int e = 0; e < N; ++e) dot = e >= again[c] ? fmaf(rv[e], gv[c][e], dot) : dot;
                             }
                         }
                         dot = lanes_sum<L>(dot);
@@ -668,13 +719,12 @@ unsigned blocks_of(int64_t items, int per_block) {
 template <typename T, int L, int V, int KB>
 int launch_topk(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights, float *stats,
                 hipStream_t s) {
-    constexpr int KEY = (int)sizeof(typename RouteKey<T>::type), W = V * (int)sizeof(T) < 16 ? V : 16 / (int)sizeof(T);
+    constexpr int KEY = (int)sizeof(typename RouteKey<T>::type);
     const int lds = ((V < k ? V : k) + 1) * 256 * KEY;
     const int64_t blocks = (n + 256 / L - 1) / (256 / L);
-    const int pieces = e % W == 0 && ld % W == 0 && (uintptr_t)scores % (W * sizeof(T)) == 0;
     MTP_SET_MAX_LDS_ONCE((k_route_topk<T, L, V, KB>), (V + 1) * 256 * KEY);
     hipLaunchKernelGGL((k_route_topk<T, L, V, KB>), dim3((unsigned)blocks), dim3(256), lds, s, reinterpret_cast<const T *>(scores), n,
-                       e, ld, k, normalize, pieces, ids, weights, stats);
+                       e, ld, k, normalize, ids, weights, stats);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -684,6 +734,7 @@ int route_by_k(const void *scores, int64_t n, int e, int64_t ld, int k, int norm
                hipStream_t s) {
     if (k <= L) return launch_topk<T, L, V, 1>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     if (k <= 2 * L) return launch_topk<T, L, V, 2>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    if constexpr (L == 32) return launch_topk<T, L, V, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     if constexpr (L == 16) return launch_topk<T, L, V, 8>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     mtp_set_error("mtp_route_topk: k=%d", k);
     return MTP_E_ARG;
@@ -692,11 +743,16 @@ int route_by_k(const void *scores, int64_t n, int e, int64_t ld, int k, int norm
 template <typename T>
 int route(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize, int32_t *ids, float *weights, float *stats,
           hipStream_t s) {
-    if (e <= 1024 && n >= 1024) {
+    // More lanes a row: shorter sorts and longer maxima, k of them.  100 000 rows, microseconds for k = 1 / 7 / 20 / 64:
+    //   400 float     16 lanes 67 / 73 / 86 / 160, 32 lanes 51 / 64 / 94 / 189, 64 lanes 51 / 84 / 152 / 415
+    //   900 bfloat16  16 lanes 92 / 100 / 110 / 154, 32 lanes 66 / 75 / 91 / 143, 64 lanes 60 / 77 / 112 / 225
+    // Few rows: one wave a row, since the card is not full anyway.
+    if (n >= 1024 && e <= 1024) {
         if (e <= 64) return route_by_k<T, 16, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
         if (e <= 256) return route_by_k<T, 16, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
-        if (e <= 512) return route_by_k<T, 16, 32>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
-        return route_by_k<T, 16, 64>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 512 && k > 8) return route_by_k<T, 16, 32>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 512) return route_by_k<T, 32, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        return route_by_k<T, 32, 32>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     }
     if (e <= 256) return route_by_k<T, 64, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     if (e <= 1024) return route_by_k<T, 64, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
@@ -714,8 +770,14 @@ constexpr int64_t CACHE_BYTES = 256ll << 20;
 template <typename T, int N, bool ONCE>
 int launch_dispatch(const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held, void *rows,
                     hipStream_t s) {
-    hipLaunchKernelGGL((k_dispatch<T, N, ONCE>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(x),
-                       n, d, ld, k, position, held, reinterpret_cast<T *>(rows));
+    const int64_t threads = n * ((d + N - 1) / N);
+    const dim3 grid(blocks_of(threads, 256));
+    if (threads < 1ll << 31)
+        hipLaunchKernelGGL((k_dispatch<T, N, ONCE, uint32_t>), grid, dim3(256), 0, s, reinterpret_cast<const T *>(x), n, d, ld, k,
+                           position, held, reinterpret_cast<T *>(rows));
+    else
+        hipLaunchKernelGGL((k_dispatch<T, N, ONCE, int64_t>), grid, dim3(256), 0, s, reinterpret_cast<const T *>(x), n, d, ld, k,
+                           position, held, reinterpret_cast<T *>(rows));
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -724,8 +786,7 @@ template <typename T>
 int dispatch(const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held, void *rows,
              hipStream_t s) {
     constexpr int N = 16 / (int)sizeof(T);
-    const bool vec = d % N == 0 && ld % N == 0 && ((uintptr_t)x | (uintptr_t)rows) % 16 == 0;
-    if (!vec) return launch_dispatch<T, 1, false>(x, n, d, ld, k, position, held, rows, s);
+    if (d < N) return launch_dispatch<T, 1, false>(x, n, d, ld, k, position, held, rows, s);
     if (n * k * d * (int64_t)sizeof(T) > CACHE_BYTES) return launch_dispatch<T, N, true>(x, n, d, ld, k, position, held, rows, s);
     return launch_dispatch<T, N, false>(x, n, d, ld, k, position, held, rows, s);
 }
@@ -733,8 +794,14 @@ int dispatch(const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *
 template <typename T, int N, bool ONCE>
 int launch_combine(const void *rows, int64_t n, int d, int k, const int32_t *position, const int32_t *held, const float *weights,
                    void *y, hipStream_t s) {
-    hipLaunchKernelGGL((k_combine<T, N, ONCE>), dim3(blocks_of(n * (d / N), 256)), dim3(256), 0, s, reinterpret_cast<const T *>(rows),
-                       n, d, k, position, held, weights, reinterpret_cast<T *>(y));
+    const int64_t threads = n * ((d + N - 1) / N);
+    const dim3 grid(blocks_of(threads, 256));
+    if (threads < 1ll << 31)
+        hipLaunchKernelGGL((k_combine<T, N, ONCE, uint32_t>), grid, dim3(256), 0, s, reinterpret_cast<const T *>(rows), n, d, k,
+                           position, held, weights, reinterpret_cast<T *>(y));
+    else
+        hipLaunchKernelGGL((k_combine<T, N, ONCE, int64_t>), grid, dim3(256), 0, s, reinterpret_cast<const T *>(rows), n, d, k,
+                           position, held, weights, reinterpret_cast<T *>(y));
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -743,8 +810,7 @@ template <typename T>
 int combine(const void *rows, int64_t n, int d, int k, const int32_t *position, const int32_t *held, const float *weights, void *y,
             hipStream_t s) {
     constexpr int N = 16 / (int)sizeof(T);
-    const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)y) % 16 == 0;
-    if (!vec) return launch_combine<T, 1, false>(rows, n, d, k, position, held, weights, y, s);
+    if (d < N) return launch_combine<T, 1, false>(rows, n, d, k, position, held, weights, y, s);
     if (n * k * d * (int64_t)sizeof(T) > CACHE_BYTES) return launch_combine<T, N, true>(rows, n, d, k, position, held, weights, y, s);
     return launch_combine<T, N, false>(rows, n, d, k, position, held, weights, y, s);
 }
@@ -763,15 +829,15 @@ template <typename T>
 int combine_grad(const void *rows, const void *g, int64_t n, int d, int k, const int32_t *position, const int32_t *held,
                  const float *weights, void *grad_rows, float *grad_weights, hipStream_t s) {
     constexpr int N = 16 / (int)sizeof(T);
-    const bool vec = d % N == 0 && ((uintptr_t)rows | (uintptr_t)g | (uintptr_t)grad_rows) % 16 == 0;
+    const int per = (d + N - 1) / N;
     const bool once = n * k * d * (int64_t)sizeof(T) > CACHE_BYTES;
-    if (!vec) return launch_combine_grad<T, 1, 64, 4>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    if (d / N <= 8) return launch_combine_grad<T, N, 8, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
-    if (d / N <= 16) {
+    if (d < N) return launch_combine_grad<T, 1, 8, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (per <= 8) return launch_combine_grad<T, N, 8, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
+    if (per <= 16) {
         if (once) return launch_combine_grad<T, N, 16, 1, true>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
         return launch_combine_grad<T, N, 16, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
     }
-    if (d / N <= 32) {
+    if (per <= 32) {
         if (once) return launch_combine_grad<T, N, 32, 1, true>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
         return launch_combine_grad<T, N, 32, 1>(rows, g, n, d, k, position, held, weights, grad_rows, grad_weights, s);
     }

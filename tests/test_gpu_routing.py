@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 
 # rows, modalities, k: one agent, every width of the kernel (64, 256, 512, 1024, 4096), few and many rows, k up to all
 ROUTES = [(1, 1, 1), (1, 200, 20), (3, 7, 7), (5, 64, 1), (1030, 5, 3), (1500, 64, 64), (1025, 65, 17), (1200, 200, 20), (900, 256, 128),
-          (1100, 257, 33), (1050, 400, 7), (1040, 1024, 128), (30, 1024, 8), (7, 1025, 5), (2, 4096, 128), (1024, 33, 32), (1026, 999, 16)]
+          (1100, 257, 33), (1050, 400, 7), (1040, 1024, 128), (30, 1024, 8), (7, 1025, 5), (2, 4096, 128), (1024, 33, 32), (1026, 999, 16),
+          (1030, 130, 4), (1040, 300, 8), (1050, 511, 9), (1060, 512, 20), (1030, 513, 70), (1100, 8, 8), (1100, 9, 9)]
 
 
 def _scores(seed, n, e, dtype):
