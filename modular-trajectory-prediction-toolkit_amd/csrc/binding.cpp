@@ -8,7 +8,9 @@
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <optional>
 
@@ -51,6 +53,22 @@ bool like(const Tensor &t, at::ScalarType type, const Tensor &ref, at::IntArrayR
 }
 Tensor workspace(int64_t bytes, const Tensor &ref) {
     return bytes > 0 ? at::empty({bytes}, ref.options().dtype(at::kByte)) : Tensor();
+}
+
+// Under capture a backward pass must not meet a node that was made on another stream: the engine would make that stream wait for
+// the captured one, which fails inside its own thread and ends the process.  Such a node exists where an input is a result
+// from outside the capture, or a leaf that a result from outside still refers to.
+void refuse_foreign_nodes(const char *what, std::initializer_list<const Tensor *> inputs) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor *t : inputs) {
+        if (!t->defined() || !t->requires_grad()) continue;
+        const auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || *stream == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->device().index()).unwrap(), what,
+                    ": an input belongs to an autograd graph that was begun outside this capture; its backward pass cannot be captured "
+                    "(let go of the eager results that refer to it first)");
+    }
 }
 
 // What a backward pass returns can be differentiated no further: trying to says so.  `from`: what it was computed from.
@@ -170,7 +188,10 @@ std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::option
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
                                        (residual.defined() && residual.requires_grad())))
+    {
+        refuse_foreign_nodes("linear", {&x, &w, &bias, &residual});
         return Linear::apply(x, w, bias_, residual_, offsets_, z);
+    }
     return run_linear(z, x, w, bias, residual, offsets, nullptr);
 }
 
@@ -217,6 +238,7 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
     if (ld < 0 || n > MOST || e < 1 || e > MOST_MODALITIES || k < 1 || k > e || k > MOST_TOPK) return std::nullopt;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
     if (at::GradMode::is_enabled() && scores.requires_grad()) {
+        refuse_foreign_nodes("route_topk", {&scores});
         auto out = Route::apply(scores, k, normalize);
         return std::make_tuple(out[0], out[1]);
     }
@@ -324,7 +346,10 @@ std::optional<Tensor> dispatch(const Tensor &x, const Tensor &position, const Te
         position.size(1) < 1)
         return std::nullopt;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
-    if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, position, offsets);
+    if (at::GradMode::is_enabled() && x.requires_grad()) {
+        refuse_foreign_nodes("dispatch", {&x});
+        return Dispatch::apply(x, position, offsets);
+    }
     return run_dispatch(x, position, offsets);
 }
 
@@ -335,8 +360,10 @@ std::optional<Tensor> combine(const Tensor &rows, const Tensor &position, const 
         return std::nullopt;
     if (weights.defined() && !like(weights, at::kFloat, rows, position.sizes())) return std::nullopt;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(rows.device());
-    if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.defined() && weights.requires_grad())))
+    if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.defined() && weights.requires_grad()))) {
+        refuse_foreign_nodes("combine", {&rows, &weights});
         return Combine::apply(rows, weights_, position, offsets);
+    }
     return run_combine(rows, position, offsets, weights);
 }
 

@@ -277,12 +277,13 @@ int launch_tile(LinArgs a, hipStream_t s) {
         a.row_tiles = (a.out_rows + BR - 1) / BR;
         blocks = a.row_tiles * a.col_tiles * ((a.rows >> a.part_bits) + a.n_sets);
     } else {
-        // a set's last tile may be ragged, and so may the one behind the last set
+        // a set's last tile may be ragged, and so may the one behind the last set; each has a row
         a.row_tiles = a.offsets == nullptr ? (a.rows + BR - 1) / BR : (a.rows + (int64_t)(a.n_sets + 1) * (BR - 1)) / BR;
+        if (a.row_tiles > a.rows) a.row_tiles = a.rows;
         blocks = a.row_tiles * a.col_tiles;
         a.away = a.rows * a.cols * (int64_t)sizeof(T) > AWAY_BYTES;
     }
-    MTP_REQUIRE(blocks <= 0x7fffffff, "mtp_linear: %lld workgroups are too many", (long long)blocks);
+    MTP_REQUIRE(blocks * NT <= 0xffffffffll, "mtp_linear: %lld workgroups are too many", (long long)blocks);
     if (blocks == 0) return MTP_OK;
     MTP_SET_MAX_LDS_ONCE((k_linear_tile<T, MODE, BC, BR, WC, WR>), LDS);
     hipLaunchKernelGGL((k_linear_tile<T, MODE, BC, BR, WC, WR>), dim3((unsigned)blocks), dim3(NT), LDS, s, a);
@@ -317,7 +318,7 @@ int launch_few(LinArgs a, hipStream_t s) {
                                        : (a.rows + (int64_t)(a.n_sets + 1) * (16 * RT - 1)) / (16 * RT);
     const int64_t most = a.offsets == nullptr ? a.row_tiles : a.row_tiles < a.rows ? a.row_tiles : a.rows;  // a tile has a row
     const int64_t blocks = most * a.col_tiles;
-    MTP_REQUIRE(blocks <= 0x7fffffff, "mtp_linear: %lld workgroups are too many", (long long)blocks);
+    MTP_REQUIRE(blocks * 256 <= 0xffffffffll, "mtp_linear: %lld workgroups are too many", (long long)blocks);
     hipLaunchKernelGGL((k_linear_few<T, RT>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
@@ -476,8 +477,8 @@ extern "C" int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_
     if (rows == 0) return MTP_OK;
     MTP_REQUIRE(x && w && y, "mtp_linear: null pointer");
     const int64_t need = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_FORWARD, rows, in, out, n_sets, x, ldx, w, in);
-    if ((int64_t)ws_bytes < need || (need > 0 && ws == nullptr)) {
-        mtp_set_error("mtp_linear: workspace of %zu bytes, needs %lld", ws_bytes, (long long)need);
+    if ((int64_t)ws_bytes < need || (need > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0))) {
+        mtp_set_error("mtp_linear: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)need);
         return MTP_E_WORKSPACE;
     }
     return MTP_BY_TYPE(dtype, forward)(x, rows, in, ldx, w, out, bias, act, residual, ldr, offsets, n_sets, y, pre,
@@ -535,8 +536,8 @@ extern "C" int mtp_linear_grad_input(int dtype, const void *dz, int64_t rows, in
     if (rows == 0) return MTP_OK;
     MTP_REQUIRE(dz && w && dx, "mtp_linear_grad_input: null pointer");
     const int64_t need = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_GRAD_INPUT, rows, in, out, n_sets, dz, lddz, w, in);
-    if ((int64_t)ws_bytes < need || (need > 0 && ws == nullptr)) {
-        mtp_set_error("mtp_linear_grad_input: workspace of %zu bytes, needs %lld", ws_bytes, (long long)need);
+    if ((int64_t)ws_bytes < need || (need > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0))) {
+        mtp_set_error("mtp_linear_grad_input: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)need);
         return MTP_E_WORKSPACE;
     }
     return MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, offsets, n_sets, dx, reinterpret_cast<char *>(ws),
@@ -551,8 +552,8 @@ extern "C" int mtp_linear_grad_weight(int dtype, const void *dz, int64_t rows, i
     MTP_REQUIRE(lddz >= out && ldx >= in, "mtp_linear_grad_weight: row distance below the row's length");
     MTP_REQUIRE(dw && (rows == 0 || (dz && x)), "mtp_linear_grad_weight: null pointer");
     const int64_t need = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_GRAD_WEIGHT, rows, in, out, n_sets, dz, lddz, x, ldx);
-    if ((int64_t)ws_bytes < need || (need > 0 && ws == nullptr)) {
-        mtp_set_error("mtp_linear_grad_weight: workspace of %zu bytes, needs %lld", ws_bytes, (long long)need);
+    if ((int64_t)ws_bytes < need || (need > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0))) {
+        mtp_set_error("mtp_linear_grad_weight: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)need);
         return MTP_E_WORKSPACE;
     }
     return MTP_BY_TYPE(dtype, grad_weight)(dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db,
@@ -573,8 +574,8 @@ extern "C" int mtp_linear_backward(int dtype, const void *g, const void *pre, in
     MTP_REQUIRE(dx || dw, "mtp_linear_backward: nothing is asked for");
     MTP_REQUIRE(db == nullptr || dw != nullptr, "mtp_linear_backward: the bias' gradient comes with the weight's");
     const BackwardPlan p = plan_backward(dtype, rows, in, out, n_sets, act, g, w, x, ldx, dx != nullptr, dw != nullptr);
-    if ((int64_t)ws_bytes < p.total() || (p.total() > 0 && ws == nullptr)) {
-        mtp_set_error("mtp_linear_backward: workspace of %zu bytes, needs %lld", ws_bytes, (long long)p.total());
+    if ((int64_t)ws_bytes < p.total() || (p.total() > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0))) {
+        mtp_set_error("mtp_linear_backward: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)p.total());
         return MTP_E_WORKSPACE;
     }
     char *rest = reinterpret_cast<char *>(ws) + p.dz_bytes;

@@ -721,11 +721,15 @@ int launch_topk(const void *scores, int64_t n, int e, int64_t ld, int k, int nor
                 hipStream_t s) {
     constexpr int KEY = (int)sizeof(typename RouteKey<T>::type);
     const int lds = ((V < k ? V : k) + 1) * 256 * KEY;
-    const int64_t blocks = (n + 256 / L - 1) / (256 / L);
+    constexpr int64_t ROWS = (int64_t)(256 / L) << 22;  // rows of a launch: a grid holds less than 2^32 threads
     MTP_SET_MAX_LDS_ONCE((k_route_topk<T, L, V, KB>), (V + 1) * 256 * KEY);
-    hipLaunchKernelGGL((k_route_topk<T, L, V, KB>), dim3((unsigned)blocks), dim3(256), lds, s, reinterpret_cast<const T *>(scores), n,
-                       e, ld, k, normalize, ids, weights, stats);
-    MTP_LAUNCH_CHECK();
+    for (int64_t r = 0; r < n; r += ROWS) {
+        const int64_t m = n - r < ROWS ? n - r : ROWS;
+        hipLaunchKernelGGL((k_route_topk<T, L, V, KB>), dim3((unsigned)((m + 256 / L - 1) / (256 / L))), dim3(256), lds, s,
+                           reinterpret_cast<const T *>(scores) + r * ld, m, e, ld, k, normalize, ids + r * k, weights + r * k,
+                           stats == nullptr ? nullptr : stats + r * 2);
+        MTP_LAUNCH_CHECK();
+    }
     return MTP_OK;
 }
 
@@ -876,18 +880,23 @@ extern "C" int mtp_route_topk_grad(int dtype, const void *scores, int64_t n, int
     if (rows_per > 64) rows_per = 64;
     const int pieces = (uintptr_t)out % 16 == 0 && (int64_t)rows_per * e * sz % 16 == 0;
     const int lds = (rows_per * 4 + 15) / 16 * 16 + (rows_per * e * sz + 15) / 16 * 16;
-    const dim3 grid((unsigned)((n + rows_per - 1) / rows_per));
     hipStream_t s = mtp_stream(stream);
-    if (dtype == MTP_FLOAT)
-        hipLaunchKernelGGL(k_route_grad<float>, grid, dim3(256), lds, s, (const float *)scores, n, e, ld, k, normalize, ids, weights,
-                           stats, g, (float *)out, rows_per, pieces);
-    else if (dtype == MTP_BFLOAT16)
-        hipLaunchKernelGGL(k_route_grad<__bf16>, grid, dim3(256), lds, s, (const __bf16 *)scores, n, e, ld, k, normalize, ids,
-                           weights, stats, g, (__bf16 *)out, rows_per, pieces);
-    else
-        hipLaunchKernelGGL(k_route_grad<_Float16>, grid, dim3(256), lds, s, (const _Float16 *)scores, n, e, ld, k, normalize, ids,
-                           weights, stats, g, (_Float16 *)out, rows_per, pieces);
-    MTP_LAUNCH_CHECK();
+    const int64_t most = (int64_t)rows_per << 22;  // rows of a launch: a grid holds less than 2^32 threads
+    for (int64_t r = 0; r < n; r += most) {
+        const int64_t m = n - r < most ? n - r : most;
+        const int64_t at = r * ld * sz, to = r * e * sz;
+        const void *x = reinterpret_cast<const char *>(scores) + at;
+        void *o = reinterpret_cast<char *>(out) + to;
+        const dim3 grid((unsigned)((m + rows_per - 1) / rows_per));
+#define ROUTE_GRAD(T)                                                                                                          \
+    hipLaunchKernelGGL(k_route_grad<T>, grid, dim3(256), lds, s, (const T *)x, m, e, ld, k, normalize, ids + r * k, weights + r * k, \
+                       stats + r * 2, g + r * k, (T *)o, rows_per, pieces)
+        if (dtype == MTP_FLOAT) ROUTE_GRAD(float);
+        else if (dtype == MTP_BFLOAT16) ROUTE_GRAD(__bf16);
+        else ROUTE_GRAD(_Float16);
+#undef ROUTE_GRAD
+        MTP_LAUNCH_CHECK();
+    }
     return MTP_OK;
 }
 

@@ -7,7 +7,8 @@
 
 Types float32, bfloat16, float16, all tensors of a call alike; sums are float32, y is rounded once.  For the backward pass of an
 activation z is kept in the same type (rounded once).  Second derivatives are not offered.  All calls enqueue on the current
-stream, wait for nothing and can be captured into a graph; sums have a fixed order.
+stream, wait for nothing and can be captured into a graph (a backward pass together with its forward pass, see ``routing``);
+sums have a fixed order.
 """
 import torch
 
@@ -20,8 +21,10 @@ def _apply(x, weight, bias, activation, residual, offsets):
         y = binding().linear(x, weight, bias, K._act_code(activation), residual, offsets)
     except TypeError:  # not even the right kinds of objects
         y = None
-    # None: the arguments are not as they have to be, and the front end says what is wrong
-    return y if y is not None else K.linear(x, weight, bias, activation, residual, offsets)[0]
+    if y is None:  # the front end says what is wrong; it has no autograd node, so its result is not used
+        K.linear(x, weight, bias, activation, residual, offsets)
+        raise TypeError("linear: arguments of another kind than described")
+    return y
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):

@@ -8,7 +8,9 @@ layer with one weight matrix per modality that runs over the sorted rows.
 
 Types float32, bfloat16, float16; softmax statistics, weights and sums are float32.  Gradients go to the scores, the rows
 and the weights; second derivatives are not offered.  All calls enqueue on the current stream, wait for nothing and can be
-captured into a graph; sums have a fixed order.
+captured into a graph; sums have a fixed order.  A backward pass is captured with its forward pass: a call under capture whose
+inputs belong to a graph of autograd that was begun outside (a leaf that an eager result still refers to) is refused, since its
+backward pass would end the process.
 """
 from typing import NamedTuple
 
@@ -18,13 +20,17 @@ from . import kernels as K
 from ._lib import binding
 
 
-def _call(name, *args):
-    """The operator with its autograd node; None where the arguments are not as they have to be (the front end in ``kernels``
-    then says what is wrong)."""
+def _call(name, explain, *args):
+    """The operator with its autograd node.  Where the arguments are not as they have to be, the front end in ``kernels`` says
+    what is wrong; it has no node, so its result is not used."""
     try:
-        return getattr(binding(), name)(*args)
+        got = getattr(binding(), name)(*args)
     except TypeError:  # not even the right kinds of objects
-        return None
+        got = None
+    if got is None:
+        explain()
+        raise TypeError(f"{name}: arguments of another kind than described")
+    return got
 
 
 class PairPlan(NamedTuple):
@@ -43,28 +49,25 @@ def route_topk(scores, k, normalize=True):
 
     scores [N, E], E <= 4096, k <= min(E, 128).  A score of -inf forbids the modality: where fewer than k are left, ids are -1
     and weights 0.  A NaN is never chosen before another score and makes its row's weights NaN."""
-    got = _call("route_topk", scores, k, bool(normalize))
-    return got if got is not None else K.route_topk(scores, k, normalize)[:2]
+    return _call("route_topk", lambda: K.route_topk(scores, k, normalize), scores, k, bool(normalize))
 
 
 def sort_pairs(ids, n_modalities):
     """The pairs of ids int32 [N, k] sorted by modality (stable): a ``PairPlan``.  n_modalities <= 4096."""
-    got = _call("sort_pairs", ids, n_modalities)
-    if got is None:
+    def explain():
         if isinstance(ids, torch.Tensor) and ids.dim() != 2:
             raise ValueError(f"ids: expected [N, k], got shape {tuple(ids.shape)}")
-        got = K.sort_pairs(ids, n_modalities)
-    return PairPlan(*got)
+        K.sort_pairs(ids, n_modalities)
+    return PairPlan(*_call("sort_pairs", explain, ids, n_modalities))
 
 
 def dispatch(x, plan):
     """rows [N * k, D]: agent t's row of x [N, D] at each of its pairs' places; zeros behind the last modality's rows."""
-    got = _call("dispatch", x, plan.position, plan.offsets)
-    return got if got is not None else K.dispatch_rows(x, plan.position, plan.offsets)
+    return _call("dispatch", lambda: K.dispatch_rows(x, plan.position, plan.offsets), x, plan.position, plan.offsets)
 
 
 def combine(rows, plan, weights=None):
     """[N, D]: for each agent the sum of its pairs' rows [N * k, D], times weights float32 [N, k] if given.  Pairs without a
     modality are left out."""
-    got = _call("combine", rows, plan.position, plan.offsets, weights)
-    return got if got is not None else K.combine_rows(rows, plan.position, plan.offsets, weights)
+    return _call("combine", lambda: K.combine_rows(rows, plan.position, plan.offsets, weights), rows, plan.position, plan.offsets,
+                 weights)

@@ -393,3 +393,59 @@ def test_front_ends_and_nodes_agree_bit_for_bit(gpu_device):
         dx2, dw2, db2 = K.linear_backward(gy, pre, "silu", x, w)
         for a, c in ((y, y2), (dx, dx2), (dw, dw2), (db, db2), (dr, gy)):
             assert torch.equal(a, c)
+
+
+def test_no_rows_still_have_gradients(gpu_device):
+    for dtype in R.TYPES:
+        x, w, b, r, gy = _inputs(19, 0, 9, 7, dtype)
+        got = _run(gpu_device, x, w, b, r, gy, "gelu")
+        assert got["y"].shape == (0, 7) and got["dx"].shape == (0, 9)
+        assert not got["dw"].any() and not got["db"].any() and got["dw"].shape == (7, 9)
+        x, w, b, r, gy = _inputs(19, 0, 9, 7, dtype, lead=(3,))
+        got = _run(gpu_device, x, w, b, r, gy, "relu", torch.zeros(4, dtype=torch.int32))
+        assert not got["dw"].any() and not got["db"].any() and got["dw"].shape == (3, 7, 9)
+
+
+def test_more_than_32_bits_of_elements(gpu_device):
+    """1.1 M rows of 2048: the last rows' elements lie beyond 2^31, their bytes beyond 2^32."""
+    n, i, o, tail = 1_100_000, 2048, 8, 40
+    g = torch.Generator(device=gpu_device).manual_seed(1)
+    x = torch.empty(n, i, dtype=torch.bfloat16, device=gpu_device).normal_(generator=g).requires_grad_()
+    w = (torch.randn(o, i, generator=g, device=gpu_device) / 45).to(torch.bfloat16).requires_grad_()
+    gy = torch.zeros(n, o, dtype=torch.bfloat16, device=gpu_device)
+    gy[-tail:] = torch.randn(tail, o, generator=g, device=gpu_device).to(torch.bfloat16)
+    y = linear(x, w, activation="gelu")
+    dx, dw = torch.autograd.grad(y, [x, w], gy)
+    want = R.linear(x[-tail:].detach().cpu(), w.detach().cpu(), None, "gelu", None, gy[-tail:].cpu())
+    R.check("y", y[-tail:], want["y"])
+    R.check("dx", dx[-tail:], want["dx"])
+    R.check("dw", dw, want["dw"])
+    assert not dx[:-tail].any()
+    # the same the other way round: a wide output
+    x2, w2 = gy[:, :8].contiguous(), x[:2048, :8].detach().contiguous()
+    y2 = linear(x2, w2)
+    R.check("y2", y2[-tail:], R.linear(x2[-tail:].cpu(), w2.cpu(), None, None, None)["y"])
+    assert not y2[:-tail].any()
+
+
+def test_capture_refuses_inputs_of_an_eager_graph(gpu_device):
+    x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(20, 40, 16, 8, torch.float32))
+    w = w.requires_grad_()
+    eager = linear(x, w, b, "gelu")  # alive: w's node belongs to the current stream
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep = x * 2  # something to capture
+        with pytest.raises(RuntimeError, match="begun outside this capture"):
+            linear(x, w, b, "gelu")
+        with torch.no_grad():
+            inner = linear(x, w, b, "gelu")  # no backward pass: fine
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(inner, eager) and torch.equal(keep, x * 2)
+
+
+def test_arguments_of_another_kind_are_never_taken_without_gradient(gpu_device):
+    x = torch.randn(4, 8, device=gpu_device, requires_grad=True)
+    for call in (lambda: linear(x, [1.0]), lambda: linear(x, 3), lambda: linear(x, x, bias="b")):
+        with pytest.raises((TypeError, ValueError)):
+            call()

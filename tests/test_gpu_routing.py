@@ -403,3 +403,67 @@ def test_predict_mixture_is_predict_topk_with_weights(gpu_device):
     want = torch.autograd.grad((w[:, :, None, None] * out).sum(1).square().sum(), [leaf64] + [q for q in ref.parameters()])
     for a, c in zip(got, want):  # float32 sums of at most 29 * 4 * 24 terms
         assert float((a.double() - c).norm()) <= 29 * 4 * 24 * R.U32 * float(c.norm()) + 1e-12
+
+
+def test_more_than_32_bits_of_scores(gpu_device):
+    """2.2 M rows of 1000 scores: the last rows' elements lie beyond 2^31."""
+    g = torch.Generator(device=gpu_device).manual_seed(1)
+    s = torch.empty(2_200_000, 1000, dtype=torch.bfloat16, device=gpu_device).normal_(generator=g).requires_grad_()
+    gw = torch.randn(2_200_000, 3, generator=g, device=gpu_device)
+    ids, w = route_topk(s, 3, normalize=False)
+    ds, = torch.autograd.grad(w, s, gw)
+    want = R.route(s[-300:].detach().cpu(), 3, False, gw[-300:].cpu())
+    assert torch.equal(ids[-300:].cpu(), want["ids"])
+    R.check("w", w[-300:], want["w"])
+    R.check("ds", ds[-300:], want["ds"])
+
+
+def test_more_than_32_bits_of_rows(gpu_device):
+    """4.4 M pairs of 512 elements there and back: places beyond 2^31 elements."""
+    n, k, d = 220_000, 20, 512
+    g = torch.Generator(device=gpu_device).manual_seed(2)
+    plan = sort_pairs(torch.randint(0, 150, (n, k), generator=g, device=gpu_device, dtype=torch.int32), 150)
+    x = torch.empty(n, d, dtype=torch.bfloat16, device=gpu_device).normal_(generator=g)
+    rows = dispatch(x, plan)
+    last = plan.order[-200:].long() // k
+    assert torch.equal(rows[-200:], x[last])
+    w = torch.rand(n, k, generator=g, device=gpu_device).requires_grad_()
+    leaf = rows.requires_grad_()
+    y = combine(leaf, plan, w)
+    t = torch.unique(last)[:50].cpu()
+    terms = rows.detach()[plan.position[t.to(gpu_device)].long()].cpu().double() * w.detach()[t.to(gpu_device)].cpu().double()[:, :, None]
+    v, e32 = terms.sum(1), (k + 2) * R.U32 * terms.abs().sum(1)
+    R.check("y", y[t.to(gpu_device)], (v, e32 + R.half_step(torch.bfloat16) * (v.abs() + e32)))
+    gy = torch.empty(n, d, dtype=torch.bfloat16, device=gpu_device).normal_(generator=g)
+    dr, dw = torch.autograd.grad(y, [leaf, w], gy)
+    wl = w.detach().reshape(-1)[plan.order[-200:].long()].cpu().double()
+    back = wl[:, None] * gy[last].cpu().double()
+    R.check("drows", dr[-200:], (back, (R.half_step(torch.bfloat16) + 2 * R.U32) * back.abs()))
+    prod = rows.detach()[-200:].cpu().double() * gy[last].cpu().double()
+    R.check("dw", dw.reshape(-1)[plan.order[-200:].long()], (prod.sum(1), (d + 2) * R.U32 * prod.abs().sum(1)))
+
+
+def test_capture_refuses_inputs_of_an_eager_graph(gpu_device):
+    s = _scores(1, 40, 20, torch.float32).to(gpu_device).requires_grad_()
+    x = torch.randn(40, 8, device=gpu_device, requires_grad=True)
+    rows = torch.randn(120, 8, device=gpu_device, requires_grad=True)
+    ids, w = route_topk(s, 3)  # alive, as are the next two: the leaves' nodes belong to the current stream
+    plan = sort_pairs(ids, 20)
+    alive = dispatch(x, plan), combine(rows, plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep = s.detach() * 2
+        for call in (lambda: route_topk(s, 3), lambda: dispatch(x, plan), lambda: combine(rows, plan), lambda: combine(rows.detach(), plan, w)):
+            with pytest.raises(RuntimeError, match="begun outside this capture"):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(keep, s.detach() * 2) and len(alive) == 2
+
+
+def test_arguments_of_another_kind_are_never_taken_without_gradient(gpu_device):
+    s = torch.randn(4, 8, device=gpu_device, requires_grad=True)
+    plan = sort_pairs(torch.zeros(4, 1, dtype=torch.int32, device=gpu_device), 2)
+    for call in (lambda: route_topk(s, 2.0), lambda: route_topk(s, "2"), lambda: combine(s, plan, [1.0]), lambda: dispatch([s], plan)):
+        with pytest.raises((TypeError, ValueError)):
+            call()
