@@ -236,12 +236,13 @@ LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, i
 }
 
 // Rows of x that one workgroup of the weight gradient sums, as a power of two.  One matrix: some 1024 workgroups, 2048 of big
-// tiles (32 768 rows, 2048 x 2048 bfloat16: 374 us with 2048 workgroups, 402 with 1024, 503 with 512).  Many: sets differ in size
+// tiles and of float, whose products are longer (32 768 rows, 2048 x 2048 bfloat16: 374 us with 2048 workgroups, 402 with 1024, 503
+// with 512; 8192 rows, 512 x 512 float 60 us with 1024, 65 with 512).  Many: sets differ in size
 // by a factor of ten and the longest one is what the others wait for, but parts have to be written and added (143 760 rows over
 // 400, 96 -> 256: 36 us with parts of 2048, 40 of 1024, 47 of 512; 52 280 rows over 200: 23 us of 1024, 29 of 2048).
 int part_bits_for(int64_t rows, int in, int out, int n_sets, bool half) {
     int64_t tiles;
-    int64_t most = n_sets > 1 ? 160 : 1024;
+    int64_t most = n_sets > 1 ? 160 : half ? 1024 : 2048;
     switch (pick_tile(MTP_LINEAR_GRAD_WEIGHT, half, out, in, rows, n_sets)) {
         case TILE_32x128: tiles = tiles_of(out, in, 32, 128); break;
         case TILE_64x64: tiles = tiles_of(out, in, 64, 64); break;
