@@ -287,6 +287,14 @@ int launch_tile(LinArgs a, hipStream_t s) {
     MTP_REQUIRE(blocks * NT <= 0xffffffffll, "mtp_linear: %lld workgroups are too many", (long long)blocks);
     if (blocks == 0) return MTP_OK;
     MTP_SET_MAX_LDS_ONCE((k_linear_tile<T, MODE, BC, BR, WC, WR>), LDS);
+    a.tiles = (uint32_t)blocks;
+    if (MODE != LIN_GRAD_WEIGHT && a.offsets != nullptr && a.n_sets < 512) {  // as many workgroups as have a place
+        int cus = 0;
+        const int rc = mtp_device_cu_count(&cus);
+        if (rc != MTP_OK) return rc;
+        const int64_t places = (int64_t)cus * lin_waves(BC, BR, NT) * 256 / NT;
+        if (blocks > places) blocks = places;
+    }
     hipLaunchKernelGGL((k_linear_tile<T, MODE, BC, BR, WC, WR>), dim3((unsigned)blocks), dim3(NT), LDS, s, a);
     MTP_LAUNCH_CHECK();
     return MTP_OK;

@@ -287,46 +287,77 @@ __device__ __forceinline__ void lin_count(const int32_t *offsets, int n_sets, in
     }
 }
 
-// Piece number `piece`, counted set after set (`last`: number of the last set; the rows behind the sets are "set" n_sets).  Every
-// wave finds it for itself: a prefix sum over the lanes finds the eight sets, and their counts are read across.
+// The sets as a wave sees them, 512 at a time: each lane its eight and the pieces up to and in them.
 template <bool CUT>
-__device__ __forceinline__ bool lin_find(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least, int64_t piece,
-                                         LinPiece *out) {
-    int64_t before = 0, split_before = 0;
-    for (int e0 = 0; e0 <= last; e0 += 512) {
-        int lo[8], len[8], n[8], mine = 0, many = 0;
+struct LinSets {
+    int lo[8], len[8], n[8], mine, upto, many, many_upto;
+
+    __device__ __forceinline__ void look(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least, int e0) {
         lin_count(offsets, n_sets, last, rows, part_bits, least, e0, lo, len, n);
+        mine = many = 0;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             mine += n[u];
             if (CUT) many += n[u] > 1 ? n[u] : 0;
         }
-        const int upto = lin_scan(mine), many_upto = CUT ? lin_scan(many) : 0;
-        const int64_t want = piece - before;
+        upto = lin_scan(mine);
+        many_upto = CUT ? lin_scan(many) : 0;
+    }
+    // piece `want` of these 512 (e0: the first of them): the lane that has it, then its counts one by one
+    __device__ __forceinline__ bool find(int64_t want, int e0, int64_t split_before, LinPiece *out) const {
         const uint64_t hit = __ballot(want >= upto - mine && want < upto);
-        if (hit != 0) {
-            const int src = __builtin_ctzll(hit);
-            int at = __builtin_amdgcn_readlane(upto - mine, src), split_at = __builtin_amdgcn_readlane(many_upto - many, src);
+        if (hit == 0) return false;
+        const int src = __builtin_ctzll(hit);
+        int at = __builtin_amdgcn_readlane(upto - mine, src), split_at = CUT ? __builtin_amdgcn_readlane(many_upto - many, src) : 0;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int c = __builtin_amdgcn_readlane(n[u], src);
-                if (want < at + c) {
-                    out->set = e0 + src * 8 + u;
-                    out->count = c;
-                    out->index = want - at;
-                    out->lo = __builtin_amdgcn_readlane(lo[u], src);
-                    out->hi = out->lo + __builtin_amdgcn_readlane(len[u], src);
-                    out->split_at = split_before + split_at;
-                    return true;
-                }
-                at += c;
-                split_at += c > 1 ? c : 0;
+        for (int u = 0; u < 8; ++u) {
+            const int c = __builtin_amdgcn_readlane(n[u], src);
+            if (want < at + c) {
+                out->set = e0 + src * 8 + u;
+                out->count = c;
+                out->index = want - at;
+                out->lo = __builtin_amdgcn_readlane(lo[u], src);
+                out->hi = out->lo + __builtin_amdgcn_readlane(len[u], src);
+                out->split_at = split_before + split_at;
+                return true;
             }
+            at += c;
+            if (CUT) split_at += c > 1 ? c : 0;
         }
-        before += __builtin_amdgcn_readlane(upto, 63);
-        split_before += __builtin_amdgcn_readlane(many_upto, 63);
+        return false;
+    }
+};
+
+// Piece number `piece`, counted set after set (`last`: number of the last set; the rows behind the sets are "set" n_sets).  Every
+// wave finds it for itself.
+template <bool CUT>
+__device__ __forceinline__ bool lin_find(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least, int64_t piece,
+                                         LinPiece *out) {
+    int64_t before = 0, split_before = 0;
+    for (int e0 = 0; e0 <= last; e0 += 512) {
+        LinSets<CUT> sets;
+        sets.look(offsets, n_sets, last, rows, part_bits, least, e0);
+        if (sets.find(piece - before, e0, split_before, out)) return true;
+        before += __builtin_amdgcn_readlane(sets.upto, 63);
+        if (CUT) split_before += __builtin_amdgcn_readlane(sets.many_upto, 63);
     }
     return false;
+}
+
+// The piece behind `p`: the next of its set, or the first of the next set that has rows (the rows behind the sets are "set" n_sets).
+__device__ __forceinline__ void lin_next(const int32_t *offsets, int n_sets, int64_t rows, int part_bits, LinPiece *p) {
+    if (++p->index < p->count) return;
+    p->index = 0;
+    const int top = (int)rows;
+    do {
+        ++p->set;
+        if (p->set > n_sets) return;  // not while pieces are left
+        const int lo = min(max(offsets[p->set], 0), top);
+        const int hi = p->set < n_sets ? min(max(offsets[p->set + 1], lo), top) : top;
+        p->lo = lo;
+        p->hi = hi;
+        p->count = lin_pieces(hi - lo, part_bits, 0);
+    } while (p->count == 0);
 }
 
 // parts of the sets before `set` that are cut into more than one
@@ -396,6 +427,7 @@ struct LinArgs {
     const int32_t *offsets;  // [n_sets + 1] or NULL
     int n_sets;
     int64_t row_tiles;
+    uint32_t tiles;    // workgroups' worth of work in all, at most
     int col_tiles;
     int out_rows, part_bits;  // weight gradient: rows of the output; a workgroup sums 1 << part_bits rows of x
     const void *bias;
@@ -458,8 +490,8 @@ __device__ __forceinline__ void lin_load(const T *p, float *v) {
 }
 // Consecutive workgroups go to different XCDs in turn: each XCD gets one contiguous run of tiles, so that the tiles that share
 // an operand meet in one L2.
-__device__ __forceinline__ int64_t lin_xcd_order(int64_t id, int64_t n) {
-    const int64_t per = n / 8;
+__device__ __forceinline__ uint32_t lin_xcd_order(uint32_t id, uint32_t n) {
+    const uint32_t per = n / 8;
     return id < per * 8 ? (id % 8) * per + id / 8 : id;
 }
 
@@ -581,39 +613,66 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     constexpr int FC = WC / 32, FR = WR / 32;
     constexpr int P_BYTES = BC * 128, STAGE = (BC + BR) * 128;
     extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 * STAGE
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wc = wave % (BC / WC), wr = wave / (BC / WC);
 
-    int64_t id = lin_xcd_order(blockIdx.x, gridDim.x);
+    // Tiles of sets: a workgroup takes several that follow each other, so that it looks the sets up once (143 760 rows over 400,
+    // 96 -> 256: 1.5 of the 6 us that a tile took were that).
+    uint32_t left = 1, id = lin_xcd_order(blockIdx.x, gridDim.x);
+    int ct = 0;
+    LinPiece p{0, 1, 0, 0, a.rows, 0};
+    const bool walk = MODE != LIN_GRAD_WEIGHT && a.offsets != nullptr && a.n_sets < 512;
+    if (walk) {
+        LinSets<false> sets;
+        sets.look(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, 0);
+        const uint32_t most = (uint32_t)__builtin_amdgcn_readlane(sets.upto, 63) * (uint32_t)a.col_tiles;
+        const uint32_t tiles = most < a.tiles ? most : a.tiles;
+        const uint32_t per = tiles / gridDim.x, more = tiles % gridDim.x;
+        const uint32_t first = id * per + (id < more ? id : more);
+        left = per + (id < more ? 1 : 0);
+        if (left == 0 || !sets.find(first / (uint32_t)a.col_tiles, 0, 0, &p)) return;
+        ct = (int)(first % (uint32_t)a.col_tiles);
+    } else {
+        ct = (int)(id % (uint32_t)a.col_tiles);
+        id /= (uint32_t)a.col_tiles;
+        if (MODE != LIN_GRAD_WEIGHT && a.offsets != nullptr && !lin_find<false>(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, id, &p))
+            return;
+        if (MODE != LIN_GRAD_WEIGHT && a.offsets == nullptr) p.index = id;
+    }
+    for (bool again = false; left > 0; --left, again = true) {
+    int tid_here = tid;
+    asm volatile("" : "+v"(tid_here));  // what follows from it is found anew for each tile: there are no registers to keep it in
+    if (again) {
+        __syncthreads();  // the last tile has left LDS
+        if (++ct == (int)a.col_tiles) {
+            ct = 0;
+            lin_next(a.offsets, a.n_sets, a.rows, lin_log2(BR), &p);
+            if (p.set > a.n_sets) return;
+        }
+    }
     int64_t row0 = 0, row_end = 0, k_lo = 0, k_len = a.k, part_at = -1;
-    int set = 0;
-    const int ct = (int)(id % a.col_tiles);
-    id /= a.col_tiles;
     const int64_t c0 = (int64_t)ct * BC;
     if constexpr (MODE == LIN_GRAD_WEIGHT) {
-        row0 = (int64_t)(id % a.row_tiles) * BR;
-        id /= a.row_tiles;
+        row0 = (int64_t)(id % (uint32_t)a.row_tiles) * BR;
+        id /= (uint32_t)a.row_tiles;
         row_end = a.out_rows;
-        LinPiece p{0, lin_pieces(a.rows, a.part_bits, 1), id, 0, a.rows, 0};
-        if (a.offsets == nullptr ? id >= p.count : !lin_find<true>(a.offsets, a.n_sets, a.n_sets - 1, a.rows, a.part_bits, 1, id, &p)) return;
-        set = p.set;
+        p.count = lin_pieces(a.rows, a.part_bits, 1);
+        p.index = id;
+        if (a.offsets == nullptr ? id >= (uint32_t)p.count
+                                 : !lin_find<true>(a.offsets, a.n_sets, a.n_sets - 1, a.rows, a.part_bits, 1, id, &p))
+            return;
         k_lo = p.lo + (p.index << a.part_bits);
         k_len = p.hi - k_lo < (1 << a.part_bits) ? p.hi - k_lo : (int64_t)1 << a.part_bits;
         if (p.count > 1) {
             part_at = p.split_at + p.index;
             if (part_at >= a.parts) return;  // offsets that overlap: more parts than there can be
         }
-    } else if (a.offsets != nullptr) {
-        LinPiece p;
-        if (!lin_find<false>(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, id, &p)) return;
-        set = p.set;
+    } else {
         row0 = p.lo + p.index * BR;
         row_end = p.hi;
-    } else {
-        row0 = id * BR;
-        row_end = a.rows;
     }
+    const int set = p.set;
     T *out = reinterpret_cast<T *>(a.out);
     if (MODE != LIN_GRAD_WEIGHT && set == a.n_sets) {  // rows behind the last set
         for (int i = tid; i < BR * BC; i += NT) {
@@ -623,7 +682,7 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
                 if (MODE == LIN_FORWARD && a.pre != nullptr) reinterpret_cast<T *>(a.pre)[r * a.cols + c] = (T)0.f;
             }
         }
-        return;
+        continue;
     }
 
     // operand windows: first element, bytes to the last element that counts, bytes per step along k
@@ -652,13 +711,12 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     }
     LinTile<T, PKC, BC, NT> tp;
     LinTile<T, QKC, BR, NT> tq;
-    tp.init(a.P.ld, tid);
-    tq.init(a.Q.ld, tid);
+    tp.init(a.P.ld, tid_here);
+    tq.init(a.Q.ld, tid_here);
     LinReader<T, PKC, BC> rp;
     LinReader<T, QKC, BR> rq;
-    rp.init(wc * WC, lane);
-    rq.init(wr * WR, lane);
-
+    rp.init(wc * WC, tid_here & 63);
+    rq.init(wr * WR, tid_here & 63);
     f32x16v acc[FC][FR];
     f32x16v acc_ones[MODE == LIN_GRAD_WEIGHT ? FR : 1];
 #pragma unroll
@@ -737,14 +795,15 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     // lane (i, h) holds row i of a fragment, columns 8 g + 4 h + 0..3 for g = 0..3: stored from there a wave would touch 32 rows
     // with 16 bytes each.  The sums go through LDS (as floats, pieces of 16 bytes placed at p ^ row so that neither side
     // conflicts), and whole rows of the tile leave in 16-byte pieces; bias, activation and residual are applied on the way.
-    const int i = lane & 31, h = lane >> 5;
+    asm volatile("" : "+v"(tid_here));
+    const int lane_here = tid_here & 63, i = lane_here & 31, h = lane_here >> 5;
     constexpr int ER = lin_pass_rows(2 * STAGE / (BC * 4), BR);  // rows per pass
     constexpr int PM = lin_twist_mask(BC / 4);
     static_assert(BR % ER == 0 && ER % WR == 0, "a wave's rows are in one pass");
     float *z = reinterpret_cast<float *>(smem);
     const bool to_partial = MODE == LIN_GRAD_WEIGHT && part_at >= 0;
     float bias[16 / SZ];
-    if constexpr (MODE == LIN_FORWARD) lin_bias<T, BC>(a, set, c0, tid, bias);
+    if constexpr (MODE == LIN_FORWARD) lin_bias<T, BC>(a, set, c0, tid_here, bias);
     for (int p0 = 0; p0 < BR; p0 += ER) {
         __syncthreads();
         if (wr * WR >= p0 && wr * WR < p0 + ER) {
@@ -766,10 +825,10 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
         const int64_t r0 = row0 + p0;
         if (to_partial) {
             float *part = a.partial + part_at * a.out_rows * a.cols;
-            lin_leave<T, float, MODE, BC, ER, NT>(a, z, bias, part, r0, row_end, c0, tid);
+            lin_leave<T, float, MODE, BC, ER, NT>(a, z, bias, part, r0, row_end, c0, tid_here);
         } else {
             T *to = out + (MODE == LIN_GRAD_WEIGHT ? (int64_t)set * a.out_rows * a.cols : 0);
-            lin_leave<T, T, MODE, BC, ER, NT>(a, z, bias, to, r0, row_end, c0, tid);
+            lin_leave<T, T, MODE, BC, ER, NT>(a, z, bias, to, r0, row_end, c0, tid_here);
         }
     }
     if constexpr (MODE == LIN_GRAD_WEIGHT && SZ == 4) {  // the two halves of a wave hold different k
@@ -789,6 +848,7 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
                 }
             }
         }
+    }
     }
 }
 
@@ -844,8 +904,8 @@ __global__ __launch_bounds__(256) void k_linear_few(LinArgs a) {
     __shared__ f32x4v sums[3][RT][64];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int ct = (int)(blockIdx.x % a.col_tiles);
-    const int64_t c0 = (int64_t)ct * 16, id = blockIdx.x / a.col_tiles;
+    const uint32_t ct = blockIdx.x % (uint32_t)a.col_tiles, id = blockIdx.x / (uint32_t)a.col_tiles;
+    const int64_t c0 = (int64_t)ct * 16;
     int64_t row0 = 0, row_end = a.rows;
     int set = 0;
     if (a.offsets != nullptr) {
@@ -855,7 +915,7 @@ __global__ __launch_bounds__(256) void k_linear_few(LinArgs a) {
         row0 = p.lo + p.index * (16 * RT);
         row_end = p.hi;
     } else {
-        row0 = id * (16 * RT);
+        row0 = (int64_t)id * (16 * RT);
     }
     T *out = reinterpret_cast<T *>(a.out);
     if (set == a.n_sets) {  // rows behind the last set
