@@ -211,7 +211,9 @@ int relayout(const void **a, int64_t *lda, int64_t a_rows, int a_cols, const voi
 //   TILE_128x128  input and weight gradients of 16-bit types, whose products are longer than their way out (143 760 rows,
 //                 24 -> 256: 33, 37 with 128x64)
 //   TILE_256x256  long sums of 16-bit types that fill the card with such tiles (32 768 rows, 2048 -> 2048: 276, 337 with
-//                 128x128): half the LDS traffic a product
+//                 128x128): half the LDS traffic a product; weight gradients of 64 such tiles or more
+//                 (32 768 rows, 2048 x 2048: 340, 375 with 128x128; 8192 rows, 4096 x 4096: 370, 470; but 32 768 rows,
+//                 1024 x 1024: 116, 108)
 enum LinTileShape { TILE_32x128, TILE_64x64, TILE_64x128, TILE_96x128, TILE_128x64, TILE_128x128, TILE_256x256 };
 
 int64_t tiles_of(int64_t rows, int64_t cols, int bc, int br) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); }
@@ -223,6 +225,8 @@ LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, i
         if (rows <= 64) return cols <= 64 ? TILE_64x64 : TILE_128x64;
         if (cols <= 64) return TILE_64x128;
         if (cols <= 96) return TILE_96x128;
+        const int64_t big = tiles_of(rows, cols, 256, 256);
+        if (n_sets == 1 && big >= 64 && k * big >= 512 * 1024) return TILE_256x256;
         return tiles_of(rows, cols, 128, 128) >= 64 ? TILE_128x128 : TILE_128x64;
     }
     if (cols <= 32) return TILE_32x128;
@@ -249,6 +253,10 @@ int part_bits_for(int64_t rows, int in, int out, int n_sets, bool half) {
         case TILE_64x128: tiles = tiles_of(out, in, 64, 128); break;
         case TILE_96x128: tiles = tiles_of(out, in, 96, 128); break;
         case TILE_128x64: tiles = tiles_of(out, in, 128, 64); break;
+        case TILE_256x256:
+            tiles = tiles_of(out, in, 256, 256);
+            most = 512;
+            break;
         default:
             tiles = tiles_of(out, in, 128, 128);
             if (n_sets == 1) most = 2048;
@@ -313,7 +321,7 @@ int launch_product(const LinArgs &a, hipStream_t s) {
         case TILE_128x128:
             if constexpr (sizeof(T) == 2 && MODE != LIN_FORWARD) return launch_tile<T, MODE, 128, 128, 64, 64>(a, s);
         case TILE_256x256:
-            if constexpr (sizeof(T) == 2 && MODE != LIN_GRAD_WEIGHT) return launch_tile<T, MODE, 256, 256, 128, 64>(a, s);
+            if constexpr (sizeof(T) == 2) return launch_tile<T, MODE, 256, 256, 128, 64>(a, s);
     }
     mtp_set_error("mtp_linear: no kernel of this shape");
     return MTP_E_ARG;

@@ -95,6 +95,13 @@ def test_linear_wide(gpu_device):
         _compare(_run(gpu_device, x, w, b, r, gy, "silu"), R.linear(x, w, b, "silu", r, gy), dtype)
 
 
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "gelu"), (torch.float16, "silu")], ids=str)
+def test_linear_that_fills_the_card(gpu_device, dtype, act):
+    """The largest tiles in all three products, ragged on every side."""
+    x, w, b, r, gy = _inputs(15, 8200, 1801, 1797, dtype)
+    _compare(_run(gpu_device, x, w, b, r, gy, act), R.linear(x, w, b, act, r, gy), dtype)
+
+
 @pytest.mark.parametrize("dtype", R.TYPES, ids=str)
 def test_linear_takes_slices_and_odd_addresses(gpu_device, dtype):
     """The observation half of a memory [N, obs + pred] is a slice of columns; an odd column start is no multiple of 4 bytes."""
