@@ -492,10 +492,10 @@ int mtp_combine_rows_grad(int dtype, const void *rows, const void *g, int64_t n,
 #define MTP_LINEAR_GRAD_WEIGHT 2
 int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows, int in, int out, int n_sets, const void *a, int64_t lda,
                                    const void *b, int64_t ldb);
-/* Whether x's rows start where the products want them, and a copy that does (ldo a multiple of 8): a caller that needs the rows for
- * a forward and a backward call lays them out once. */
+/* Whether x's rows start where the products want them.  Where they do not, mtp_linear lays them out in its workspace, if that has a
+ * size at all (few rows are read as they are): from the workspace's start x, then w (each if it needs it), with a row distance ld of
+ * in rounded up to 8 and rows * ld elements rounded up to 256 bytes.  A caller that goes on to mtp_linear_backward can keep them. */
 int mtp_linear_rows_aligned(int dtype, const void *x, int64_t ld);
-int mtp_linear_align_rows(int dtype, const void *x, int64_t rows, int cols, int64_t ld, void *to, int64_t ldo, void *stream);
 int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias, int act,
                const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre, void *ws, size_t ws_bytes,
                void *stream);
@@ -513,10 +513,10 @@ int mtp_linear_grad_weight(int dtype, const void *dz, int64_t rows, int out, int
 /* The whole backward pass of mtp_linear in one call: dz = g * act'(pre) (act 0: dz = g, pre is not read), then dx and / or dw
  * (with db) as above; what is NULL is not computed.  g [rows][out] contiguous.  want_x, want_w: dx, dw are not NULL. */
 int64_t mtp_linear_backward_workspace_bytes(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g,
-                                            const void *w, const void *x, int64_t ldx, int want_x, int want_w);
+                                            const void *w, int64_t ldw, const void *x, int64_t ldx, int want_x, int want_w);
 int mtp_linear_backward(int dtype, const void *g, const void *pre, int act, const void *x, int64_t rows, int in, int64_t ldx,
-                        const void *w, int out, const int32_t *offsets, int n_sets, void *dx, void *dw, void *db, void *ws,
-                        size_t ws_bytes, void *stream);
+                        const void *w, int out, int64_t ldw, const int32_t *offsets, int n_sets, void *dx, void *dw, void *db,
+                        void *ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -91,7 +91,7 @@ struct Sizes {
 };
 
 Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, const Tensor &offsets,
-                  Tensor *pre) {
+                  Tensor *pre, Tensor *laid_out = nullptr) {
     Tensor y = at::empty({z.rows, z.out}, x.options());
     if (pre != nullptr) *pre = at::empty({z.rows, z.out}, x.options());
     const int64_t ldx = row_distance(x);
@@ -102,6 +102,7 @@ Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor
                      residual.defined() ? row_distance(residual) : 0, static_cast<const int32_t *>(at_(offsets)), (int)z.sets, at_(y),
                      pre != nullptr ? at_(*pre) : nullptr, at_(ws), (size_t)bytes, stream_of(x)),
           "mtp_linear");
+    if (laid_out != nullptr) *laid_out = ws;
     return y;
 }
 
@@ -113,18 +114,24 @@ struct Linear : torch::autograd::Function<Linear> {
         const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
         // relu's slope can be read off y where nothing was added to it
         const bool from_y = z.act == RELU && !residual.defined();
-        // rows that do not start where the products want them are laid out once for both passes
-        Tensor rows = x;
-        if (!mtp_linear_rows_aligned(z.code, at_(x), row_distance(x))) {
-            const int64_t ld = (z.in + 7) / 8 * 8;
-            const Tensor all = at::empty({z.rows, ld}, x.options());
-            check(mtp_linear_align_rows(z.code, at_(x), z.rows, (int)z.in, row_distance(x), at_(all), ld, stream_of(x)),
-                  "mtp_linear_align_rows");
-            rows = all.narrow(1, 0, z.in);
+        Tensor pre, ws;
+        Tensor y = run_linear(z, x, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr, &ws);
+        // rows that do not start where the products want them have been laid out there: once for both passes
+        Tensor rows, weights;
+        const int64_t ld = (z.in + 7) / 8 * 8;
+        if (ws.defined()) {
+            const Tensor all = ws.view(x.scalar_type());
+            int64_t at = 0;
+            auto take = [&](const Tensor &t, int64_t n, int64_t distance) {
+                if (mtp_linear_rows_aligned(z.code, at_(t), distance)) return Tensor();
+                const int64_t from = at;
+                at += (n * ld * x.element_size() + 255) / 256 * 256 / x.element_size();
+                return all.as_strided({n, z.in}, {ld, 1}, from);
+            };
+            rows = take(x, z.rows, row_distance(x));
+            weights = take(w, z.sets * z.out, z.in);
         }
-        Tensor pre;
-        Tensor y = run_linear(z, rows, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr);
-        ctx->save_for_backward({rows, w, from_y ? y : pre, offsets});
+        ctx->save_for_backward({x, w, from_y ? y : pre, offsets, rows, weights});
         ctx->saved_data["sizes"] =
             std::vector<int64_t>{z.code, z.act, z.rows, z.in, z.out, z.sets, bias.defined(), residual.defined()};
         return y;
@@ -142,16 +149,17 @@ struct Linear : torch::autograd::Function<Linear> {
             const bool want_x = ctx->needs_input_grad(0), want_b = v[6] != 0 && ctx->needs_input_grad(2);
             const bool want_w = ctx->needs_input_grad(1) || want_b;
             if (want_x) dx = at::empty({z.rows, z.in}, x.options());
-            if (want_w) dw = at::empty(w.sizes(), w.options());
-            if (want_b) db = at::empty(w.sizes().slice(0, w.dim() - 1), w.options());
+            if (want_w) dw = offsets.defined() ? at::empty({z.sets, z.out, z.in}, x.options()) : at::empty({z.out, z.in}, x.options());
+            if (want_b) db = offsets.defined() ? at::empty({z.sets, z.out}, x.options()) : at::empty({z.out}, x.options());
             const int32_t *sets = static_cast<const int32_t *>(at_(offsets));
             if (want_x || want_w) {
-                const int64_t ldx = row_distance(x);
+                const Tensor &xs = saved[4].defined() ? saved[4] : x, &wt = saved[5].defined() ? saved[5] : w;
+                const int64_t ldx = row_distance(xs), ldw = saved[5].defined() ? (z.in + 7) / 8 * 8 : z.in;
                 const int64_t bytes = mtp_linear_backward_workspace_bytes(z.code, z.rows, (int)z.in, (int)z.out, (int)z.sets, z.act,
-                                                                          at_(g), at_(w), at_(x), ldx, want_x, want_w);
+                                                                          at_(g), at_(wt), ldw, at_(xs), ldx, want_x, want_w);
                 const Tensor ws = workspace(bytes, x);
-                check(mtp_linear_backward(z.code, at_(g), at_(pre), z.act, at_(x), z.rows, (int)z.in, ldx, at_(w), (int)z.out, sets,
-                                          (int)z.sets, at_(dx), at_(dw), at_(db), at_(ws), (size_t)bytes, stream_of(x)),
+                check(mtp_linear_backward(z.code, at_(g), at_(pre), z.act, at_(xs), z.rows, (int)z.in, ldx, at_(wt), (int)z.out,
+                                          ldw, sets, (int)z.sets, at_(dx), at_(dw), at_(db), at_(ws), (size_t)bytes, stream_of(x)),
                       "mtp_linear_backward");
             }
             if (v[7] != 0 && ctx->needs_input_grad(v[6] != 0 ? 3 : 2)) {

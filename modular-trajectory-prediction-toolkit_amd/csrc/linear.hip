@@ -377,28 +377,33 @@ int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int
     return launch_product<T, LIN_FORWARD>(a, s);
 }
 
-// where the parts of a backward pass lie in the workspace: dz, then what the products need one after the other
+// where the parts of a backward pass lie in the workspace, one behind the other: dz, the weights and x with rows as the products
+// load them, the weight gradient's parts
 struct BackwardPlan {
-    int64_t lddz, dz_bytes, input_bytes, weight_bytes;
-    int64_t total() const { return dz_bytes + (input_bytes > weight_bytes ? input_bytes : weight_bytes); }
+    int64_t lddz, dz_bytes, w_bytes, x_bytes, parts_bytes;
+    int64_t total() const { return dz_bytes + w_bytes + x_bytes + parts_bytes; }
 };
-BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g, const void *w, const void *x,
-                           int64_t ldx, bool want_x, bool want_w) {
+BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g, const void *w,
+                           int64_t ldw, const void *x, int64_t ldx, bool want_x, bool want_w) {
     BackwardPlan p{};
-    // dz has rows of its own, so they can start where the loads want them
-    const bool own = act != LIN_NONE;
-    p.lddz = own && elem_size(dtype) == 2 && out % 2 != 0 ? round_up(out, 8) : out;
-    p.dz_bytes = own ? round_up(rows * p.lddz * elem_size(dtype), 256) : 0;
-    const void *dz = own ? nullptr : g;
-    if (want_x) p.input_bytes = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_GRAD_INPUT, rows, in, out, n_sets, dz, p.lddz, w, in);
-    if (want_w) p.weight_bytes = mtp_linear_workspace_bytes(dtype, MTP_LINEAR_GRAD_WEIGHT, rows, in, out, n_sets, dz, p.lddz, x, ldx);
+    if (act == LIN_NONE) {
+        p.lddz = out;
+        p.dz_bytes = relayout_bytes(dtype, g, out, rows, out);
+    } else {  // dz has rows of its own, so they can start where the loads want them
+        p.lddz = elem_size(dtype) == 2 && out % 2 != 0 ? round_up(out, 8) : out;
+        p.dz_bytes = round_up(rows * p.lddz * elem_size(dtype), 256);
+    }
+    if (want_x) p.w_bytes = relayout_bytes(dtype, w, ldw, (int64_t)n_sets * out, in);
+    if (want_w) {
+        p.x_bytes = relayout_bytes(dtype, x, ldx, rows, in);
+        p.parts_bytes = most_parts(rows, n_sets, part_bits_for(rows, in, out, n_sets, elem_size(dtype) == 2)) * out * (in + 1) * 4;
+    }
     return p;
 }
 
 template <typename T>
-int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, const int32_t *offsets, int n_sets,
-               void *dx, char *ws, hipStream_t s) {
-    int64_t ldw = in;
+int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, int64_t ldw, const int32_t *offsets,
+               int n_sets, void *dx, char *ws, hipStream_t s) {
     const int rc = relayout<T>(&dz, &lddz, rows, out, &w, &ldw, (int64_t)n_sets * out, in, &ws, s);
     if (rc != MTP_OK) return rc;
     LinArgs a{};
@@ -464,25 +469,6 @@ extern "C" int64_t mtp_linear_workspace_bytes(int dtype, int step, int64_t rows,
 }
 
 extern "C" int mtp_linear_rows_aligned(int dtype, const void *x, int64_t ld) { return !needs_relayout(dtype, x, ld); }
-
-extern "C" int mtp_linear_align_rows(int dtype, const void *x, int64_t rows, int cols, int64_t ld, void *to, int64_t ldo, void *stream) {
-    int rc = check_sizes("mtp_linear_align_rows", dtype, rows, cols, 1, nullptr, 1);
-    if (rc != MTP_OK) return rc;
-    MTP_REQUIRE(ld >= cols && ldo >= cols, "mtp_linear_align_rows: row distance below the row's length");
-    if (rows == 0) return MTP_OK;
-    MTP_REQUIRE(x && to, "mtp_linear_align_rows: null pointer");
-    hipStream_t s = mtp_stream(stream);
-    const int64_t blocks = copy_blocks(rows, cols);
-    if (dtype == MTP_FLOAT) {
-        const LinCopy<float> c{(const float *)x, (float *)to, rows, ld, ldo, cols};
-        hipLaunchKernelGGL(k_linear_relayout<float>, dim3((unsigned)blocks), dim3(256), 0, s, c, c, blocks);
-    } else {  // the other two types are moved as they are
-        const LinCopy<_Float16> c{(const _Float16 *)x, (_Float16 *)to, rows, ld, ldo, cols};
-        hipLaunchKernelGGL(k_linear_relayout<_Float16>, dim3((unsigned)blocks), dim3(256), 0, s, c, c, blocks);
-    }
-    MTP_LAUNCH_CHECK();
-    return MTP_OK;
-}
 
 extern "C" int mtp_linear(int dtype, const void *x, int64_t rows, int in, int64_t ldx, const void *w, int out, const void *bias,
                           int act, const void *residual, int64_t ldr, const int32_t *offsets, int n_sets, void *y, void *pre,
@@ -557,7 +543,7 @@ extern "C" int mtp_linear_grad_input(int dtype, const void *dz, int64_t rows, in
         mtp_set_error("mtp_linear_grad_input: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)need);
         return MTP_E_WORKSPACE;
     }
-    return MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, offsets, n_sets, dx, reinterpret_cast<char *>(ws),
+    return MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, in, offsets, n_sets, dx, reinterpret_cast<char *>(ws),
                                           mtp_stream(stream));
 }
 
@@ -578,36 +564,51 @@ extern "C" int mtp_linear_grad_weight(int dtype, const void *dz, int64_t rows, i
 }
 
 extern "C" int64_t mtp_linear_backward_workspace_bytes(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g,
-                                                       const void *w, const void *x, int64_t ldx, int want_x, int want_w) {
+                                                       const void *w, int64_t ldw, const void *x, int64_t ldx, int want_x,
+                                                       int want_w) {
     if (rows < 0 || in < 1 || out < 1 || n_sets < 1) return 0;
-    return plan_backward(dtype, rows, in, out, n_sets, act, g, w, x, ldx, want_x != 0, want_w != 0).total();
+    return plan_backward(dtype, rows, in, out, n_sets, act, g, w, ldw, x, ldx, want_x != 0, want_w != 0).total();
 }
 
 extern "C" int mtp_linear_backward(int dtype, const void *g, const void *pre, int act, const void *x, int64_t rows, int in,
-                                   int64_t ldx, const void *w, int out, const int32_t *offsets, int n_sets, void *dx, void *dw,
-                                   void *db, void *ws, size_t ws_bytes, void *stream) {
+                                   int64_t ldx, const void *w, int out, int64_t ldw, const int32_t *offsets, int n_sets, void *dx,
+                                   void *dw, void *db, void *ws, size_t ws_bytes, void *stream) {
     int rc = check_sizes("mtp_linear_backward", dtype, rows, in, out, offsets, n_sets);
     if (rc != MTP_OK) return rc;
     MTP_REQUIRE(dx || dw, "mtp_linear_backward: nothing is asked for");
     MTP_REQUIRE(db == nullptr || dw != nullptr, "mtp_linear_backward: the bias' gradient comes with the weight's");
-    const BackwardPlan p = plan_backward(dtype, rows, in, out, n_sets, act, g, w, x, ldx, dx != nullptr, dw != nullptr);
+    const BackwardPlan p = plan_backward(dtype, rows, in, out, n_sets, act, g, w, ldw, x, ldx, dx != nullptr, dw != nullptr);
     if ((int64_t)ws_bytes < p.total() || (p.total() > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0))) {
         mtp_set_error("mtp_linear_backward: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)p.total());
         return MTP_E_WORKSPACE;
     }
-    char *rest = reinterpret_cast<char *>(ws) + p.dz_bytes;
+    MTP_REQUIRE(rows == 0 || (g && (act == LIN_NONE || pre) && (dx == nullptr || w) && (dw == nullptr || x)),
+                "mtp_linear_backward: null pointer");
+    MTP_REQUIRE(ldx >= in && ldw >= in, "mtp_linear_backward: row distance below the row's length");
+    char *at = reinterpret_cast<char *>(ws);
     const void *dz = g;
+    int64_t lddz = p.lddz;
+    hipStream_t s = mtp_stream(stream);
     if (act != LIN_NONE) {
-        rc = mtp_linear_act_grad(dtype, g, pre, rows, out, act, offsets, n_sets, ws, p.lddz, stream);
+        rc = mtp_linear_act_grad(dtype, g, pre, rows, out, act, offsets, n_sets, ws, lddz, stream);
         if (rc != MTP_OK) return rc;
         dz = ws;
-    }
-    if (dx != nullptr) {
-        rc = mtp_linear_grad_input(dtype, dz, rows, out, p.lddz, w, in, offsets, n_sets, dx, rest, (size_t)p.input_bytes, stream);
+        at += p.dz_bytes;
+    } else if (p.dz_bytes > 0) {  // both products read it
+        const void *none = nullptr;
+        int64_t ld = 0;
+        rc = MTP_BY_TYPE(dtype, relayout)(&dz, &lddz, rows, out, &none, &ld, 0, 0, &at, s);
         if (rc != MTP_OK) return rc;
     }
-    if (dw != nullptr)
-        rc = mtp_linear_grad_weight(dtype, dz, rows, out, p.lddz, x, in, ldx, offsets, n_sets, dw, db, rest, (size_t)p.weight_bytes,
-                                    stream);
+    if (p.w_bytes + p.x_bytes > 0) {  // in one launch
+        rc = MTP_BY_TYPE(dtype, relayout)(&w, &ldw, p.w_bytes > 0 ? (int64_t)n_sets * out : 0, in, &x, &ldx, p.x_bytes > 0 ? rows : 0, in,
+                                          &at, s);
+        if (rc != MTP_OK) return rc;
+    }
+    if (dx != nullptr && rows > 0) {
+        rc = MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, ldw, offsets, n_sets, dx, at, s);
+        if (rc != MTP_OK) return rc;
+    }
+    if (dw != nullptr) rc = MTP_BY_TYPE(dtype, grad_weight)(dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db, at, s);
     return rc;
 }

@@ -99,11 +99,10 @@ SIGNATURES = {
     "mtp_combine_rows_grad": (_i32, [_i32, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mtp_linear_workspace_bytes": (_i64, [_i32, _i32, _i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64]),
     "mtp_linear_rows_aligned": (_i32, [_i32, _vp, _i64]),
-    "mtp_linear_align_rows": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _i64, _vp]),
     "mtp_linear": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _i32, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
-    "mtp_linear_backward_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _i32]),
-    "mtp_linear_backward": (_i32, [_i32, _vp, _vp, _i32, _vp, _i64, _i32, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _sz,
-                                   _vp]),
+    "mtp_linear_backward_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp, _i64, _i32, _i32]),
+    "mtp_linear_backward": (_i32, [_i32, _vp, _vp, _i32, _vp, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _vp, _vp,
+                                   _sz, _vp]),
     "mtp_linear_act_grad": (_i32, [_i32, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp, _i64, _vp]),
     "mtp_linear_mask_rows": (_i32, [_i32, _vp, _i64, _i32, _vp, _i32, _vp, _vp]),
     "mtp_linear_grad_input": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _sz, _vp]),

@@ -620,18 +620,6 @@ def _workspace(n_bytes, device):
     return torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
 
 
-def linear_align_rows(x):
-    """x, or a copy with rows padded to 16 bytes where x's rows do not start where the products want them (16-bit rows of odd
-    length): what uses x twice has them laid out once -- ``mtp_linear_align_rows``."""
-    _device_tensor(x, "x", 2)
-    code, (rows, cols), ld = _type_code(x, "x"), x.shape, _row_distance(x, "x")
-    if cols == 0 or lib().mtp_linear_rows_aligned(code, _at(x), ld):
-        return x
-    to = torch.empty((rows, -(-cols // 8) * 8), dtype=x.dtype, device=x.device)
-    _call(x.device, "mtp_linear_align_rows", code, _at(x), rows, cols, ld, _at(to), to.shape[1])
-    return to[:, :cols]
-
-
 def linear(x, weight, bias=None, activation=None, residual=None, offsets=None, want_pre=False):
     """(act(x weight^T + bias) + residual, x weight^T + bias or None) -- ``mtp_linear``."""
     _device_tensor(x, "x", 2)
@@ -754,8 +742,8 @@ def linear_backward(grad, pre, activation, x, weight, offsets=None, want_x=True,
     dw = torch.empty_like(weight) if want_weight else None
     db = torch.empty(weight.shape[:-1], dtype=x.dtype, device=dev) if want_bias else None
     pg, px, pw = grad.data_ptr(), x.data_ptr(), weight.data_ptr()
-    ws_bytes = lib().mtp_linear_backward_workspace_bytes(code, rows, i, out, s, act, pg, pw, px, ldx, want_x, want_weight)
+    ws_bytes = lib().mtp_linear_backward_workspace_bytes(code, rows, i, out, s, act, pg, pw, i, px, ldx, want_x, want_weight)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "mtp_linear_backward", code, pg, _at(pre) if act else None, act, px, rows, i, ldx, pw, out, _at(offsets), s,
+    _call(dev, "mtp_linear_backward", code, pg, _at(pre) if act else None, act, px, rows, i, ldx, pw, out, i, _at(offsets), s,
           _at(dx), _at(dw), _at(db), _at(ws), ws_bytes)
     return dx, dw, db

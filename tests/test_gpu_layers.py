@@ -95,6 +95,26 @@ def test_linear_wide(gpu_device):
         _compare(_run(gpu_device, x, w, b, r, gy, "silu"), R.linear(x, w, b, "silu", r, gy), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_which_rows_are_laid_out_anew(gpu_device, dtype):
+    """x, the weights, the gradient or none of them start where the products want them; one row of output; with and without sets."""
+    for i, o, slice_x, act in ((64, 41, True, None), (97, 40, False, None), (97, 41, True, "silu"), (33, 1, False, None), (32, 1, True, "relu")):
+        x, w, b, r, gy = _inputs(i + o, 300, i, o, dtype, residual=False)
+        if slice_x:
+            x = torch.cat([x[:, :1], x], 1)[:, 1:]  # rows i + 1 apart, from the second element on
+        leaves = [_strided(x, gpu_device) if slice_x else x.to(gpu_device), w.to(gpu_device), b.to(gpu_device)]
+        if o == 1:  # contiguous, whatever distance its only row names
+            leaves[1] = torch.cat([leaves[1], leaves[1]], 1)[:, :i]
+            assert leaves[1].is_contiguous() and leaves[1].stride(0) == 2 * i
+        got = [t.requires_grad_() for t in leaves]
+        y = linear(*got, activation=act)
+        grads = torch.autograd.grad(y, got, gy.to(gpu_device))
+        _compare(dict(zip(("y", "dx", "dw", "db"), (y,) + grads)), R.linear(x, w, b, act, None, gy), dtype)
+        offsets = torch.tensor([0, 100, 100, 290], dtype=torch.int32)
+        x, w, b, r, gy = _inputs(i + o + 1, 300, i, o, dtype, residual=False, lead=(3,))
+        _compare(_run(gpu_device, x, w, b, None, gy, act, offsets), R.modality_linear(x, offsets, w, b, act, None, gy), dtype)
+
+
 @pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "gelu"), (torch.float16, "silu")], ids=str)
 def test_linear_that_fills_the_card(gpu_device, dtype, act):
     """The largest tiles in all three products, ragged on every side."""
@@ -374,6 +394,23 @@ def test_second_derivatives_are_refused(gpu_device):
     R.check("dx", dx, R.linear(x.detach().cpu(), w.detach().cpu(), b.cpu(), "gelu", None, gy.cpu())["dx"])
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(dx.sum(), x)
+
+
+def test_rows_laid_out_anew_keep_the_inputs_history(gpu_device):
+    """Odd 16-bit rows: both passes use a copy of x and of the weights, and the node still knows where they came from."""
+    x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(18, 600, 97, 41, torch.float16))
+    x, w = x.requires_grad_(), w.requires_grad_()
+    y = linear(x, w, b, "gelu")
+    dx, = torch.autograd.grad(y, x, gy, create_graph=True)
+    R.check("dx", dx, R.linear(x.detach().cpu(), w.detach().cpu(), b.cpu(), "gelu", None, gy.cpu())["dx"])
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(dx.float().sum(), w)
+    for t in (x, w):
+        y = linear(x, w, b, "gelu")
+        with torch.no_grad():
+            t.mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, x, gy)
 
 
 def test_changed_inputs_are_noticed_by_the_backward_pass(gpu_device):
