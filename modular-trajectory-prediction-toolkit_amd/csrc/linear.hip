@@ -9,7 +9,8 @@
 #include "linear_kernel.h"
 
 // One or two matrices laid out anew with rows that start where the LDS loads want them (a 16-bit row of odd length starts on 2
-// bytes, their unit is 4): rows of `cols` elements, from ld to ldo apart, eight elements a thread.
+// bytes, their unit is 4): rows of `cols` elements, from ld to ldo apart, eight elements a thread.  Short of large ones a launch
+// (2614 x 97 and 201 x 97 halves: 4.9 us).
 template <typename T>
 struct LinCopy {
     const T *from;
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(256) void k_linear_relayout(LinCopy<T> p, LinCopy<T
 }
 
 // dz = g * act'(z), 16 bytes a thread.  HBM-bound: g and z are read (once, past the caches), dz is written for the products that
-// follow.  Rows of dz may lie further apart than those of g and z (ldo).
+// follow (73 568 x 512 floats 68 us, 6.6 TB/s).  Rows of dz may lie further apart than those of g and z (ldo).
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g, const T *__restrict__ z, int64_t rows, int cols,
                                                          int act, const int32_t *offsets, int n_sets, T *__restrict__ dz,
@@ -209,11 +210,11 @@ int relayout(const void **a, int64_t *lda, int64_t a_rows, int a_cols, const voi
 //   TILE_96x128   up to 96 columns of 16-bit types (143 760 rows, 256 -> 96: 30, 31 with 128x64, 37 with 32x128)
 //   TILE_128x64   most others: three workgroups a CU (143 760 rows, 96 -> 256 with gelu: 62, 67 with 128x128)
 //   TILE_128x128  input and weight gradients of 16-bit types, whose products are longer than their way out (143 760 rows,
-//                 24 -> 256: 33, 37 with 128x64)
-//   TILE_256x256  long sums of 16-bit types that fill the card with such tiles (32 768 rows, 2048 -> 2048: 276, 337 with
-//                 128x128): half the LDS traffic a product; weight gradients of 64 such tiles or more
-//                 (32 768 rows, 2048 x 2048: 340, 375 with 128x128; 8192 rows, 4096 x 4096: 370, 470; but 32 768 rows,
-//                 1024 x 1024: 116, 108)
+//                 24 -> 256: 33, 37 with 128x64); long sums forward that give each CU two (2048 rows, 4096 -> 4096: 75, 126;
+//                 8192 rows, 1024 -> 1024 with gelu: 28, 34; but 2048 rows, 2048 -> 2048: 31, 29; 8192 rows, 512 -> 512: 16.1, 15.6)
+//   TILE_256x256  long sums of 16-bit types that fill the card with such tiles (32 768 rows, 2048 -> 2048: 247, 318 with
+//                 128x128): half the LDS traffic a product; weight gradients with 2048 rows for each of 256 workgroups (32 768 rows,
+//                 2048 x 2048: 256, 299 with 128x128; 1024 x 1024: 82, 84; 4096 rows, 2048 x 2048: 54, 51)
 enum LinTileShape { TILE_32x128, TILE_64x64, TILE_64x128, TILE_96x128, TILE_128x64, TILE_128x128, TILE_256x256 };
 
 int64_t tiles_of(int64_t rows, int64_t cols, int bc, int br) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); }
@@ -226,7 +227,7 @@ LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, i
         if (cols <= 64) return TILE_64x128;
         if (cols <= 96) return TILE_96x128;
         const int64_t big = tiles_of(rows, cols, 256, 256);
-        if (n_sets == 1 && big >= 64 && k * big >= 512 * 1024) return TILE_256x256;
+        if (n_sets == 1 && k * big >= 512 * 1024 && 4ll * rows * cols >= 3 * big * 256 * 256) return TILE_256x256;
         return tiles_of(rows, cols, 128, 128) >= 64 ? TILE_128x128 : TILE_128x64;
     }
     if (cols <= 32) return TILE_32x128;
@@ -235,40 +236,36 @@ LinTileShape pick_tile(int mode, bool half, int64_t rows, int cols, int64_t k, i
     if (cols <= 64) return TILE_64x128;
     if (cols <= 96) return half ? TILE_96x128 : TILE_32x128;
     if (half && n_sets == 1 && k >= 512 && tiles_of(rows, cols, 256, 256) >= 192) return TILE_256x256;
-    if (half && mode == MTP_LINEAR_GRAD_INPUT) return TILE_128x128;
+    if (half && (mode == MTP_LINEAR_GRAD_INPUT || (k >= 512 && tiles_of(rows, cols, 128, 128) >= 512))) return TILE_128x128;
     return TILE_128x64;
 }
 
-// Rows of x that one workgroup of the weight gradient sums, as a power of two.  One matrix: some 1024 workgroups, 2048 of big
-// tiles and of float, whose products are longer (32 768 rows, 2048 x 2048 bfloat16: 374 us with 2048 workgroups, 402 with 1024, 503
-// with 512; 8192 rows, 512 x 512 float 60 us with 1024, 65 with 512).  Many: sets differ in size
-// by a factor of ten and the longest one is what the others wait for, but parts have to be written and added (143 760 rows over
-// 400, 96 -> 256: 36 us with parts of 2048, 40 of 1024, 47 of 512; 52 280 rows over 200: 23 us of 1024, 29 of 2048).
+// Rows of x that one workgroup of the weight gradient sums, as a power of two.
+// One matrix: a part of L rows takes about 8 ns a row (23 in float), and rows / L parts of in x out floats are written and read again at
+// some 5 bytes a picosecond; the sum of both is least around L^2 = rows in out / 5000 (/ 15 000), and flat towards longer parts, of
+// which fewer share the card.  2614 rows, 96 x 200 fp16: 9.4 us with parts of 256 rows, 14.4 of 1024; 20 000 rows, 512 x 512 bfloat16:
+// 29 of 1024, 44 of 256; 73 568 rows, 512 x 512 float 327 of 2048, 363 of 512, 353 of 4096.  256 x 256 tiles, one a CU: one part for
+// each (32 768 rows, 2048 x 2048: 256 us, 282 with two, 2048 rows, 4096 x 4096: 65 us, 102 with two).
+// Many: sets differ in size by a factor of ten and the longest one is what the others wait for, but parts have to be written and added
+// (143 760 rows over 400, 96 -> 256: 36 us with parts of 2048, 40 of 1024, 47 of 512; 52 280 rows over 200: 23 us of 1024, 29 of 2048).
 int part_bits_for(int64_t rows, int in, int out, int n_sets, bool half) {
-    int64_t tiles;
-    int64_t most = n_sets > 1 ? 160 : half ? 1024 : 2048;
-    switch (pick_tile(MTP_LINEAR_GRAD_WEIGHT, half, out, in, rows, n_sets)) {
-        case TILE_32x128: tiles = tiles_of(out, in, 32, 128); break;
-        case TILE_64x64: tiles = tiles_of(out, in, 64, 64); break;
-        case TILE_64x128: tiles = tiles_of(out, in, 64, 128); break;
-        case TILE_96x128: tiles = tiles_of(out, in, 96, 128); break;
-        case TILE_128x64: tiles = tiles_of(out, in, 128, 64); break;
-        case TILE_256x256:
-            tiles = tiles_of(out, in, 256, 256);
-            most = 512;
-            break;
-        default:
-            tiles = tiles_of(out, in, 128, 128);
-            if (n_sets == 1) most = 2048;
+    int bits = 6;
+    if (n_sets == 1) {
+        if (pick_tile(MTP_LINEAR_GRAD_WEIGHT, half, out, in, rows, 1) == TILE_256x256) {
+            while (bits < 30 && ((int64_t)256 << bits) < rows * tiles_of(out, in, 256, 256)) ++bits;
+            return bits;
+        }
+        const double least = (double)rows * in * out / (half ? 2500 : 6700);
+        while ((double)((int64_t)1 << bits) * (double)((int64_t)1 << bits) < least) ++bits;
+        return bits;
     }
-    const int64_t part = rows * tiles / most;
-    int bits = half ? 10 : 9;
-    while (bits < 30 && ((int64_t)1 << bits) < part) ++bits;
+    bits = half ? 10 : 9;
+    while (bits < 30 && ((int64_t)160 << bits) < rows * tiles_of(out, in, in <= 64 ? 64 : 128, out <= 64 ? 64 : 128)) ++bits;
     return bits;
 }
 // parts of the sets that have more than one: such a set has more rows than `part`, so fewer parts than twice its rows / part
 int64_t most_parts(int64_t rows, int n_sets, int bits) {
-    if (n_sets == 1) return (rows >> bits) == 0 ? 0 : (rows + ((int64_t)1 << bits) - 1) >> bits;
+    if (n_sets == 1) return rows <= (int64_t)1 << bits ? 0 : (rows + ((int64_t)1 << bits) - 1) >> bits;
     return (2 * rows) >> bits;
 }
 
@@ -284,7 +281,9 @@ int launch_tile(LinArgs a, hipStream_t s) {
     int64_t blocks;
     if (MODE == LIN_GRAD_WEIGHT) {
         a.row_tiles = (a.out_rows + BR - 1) / BR;
-        blocks = a.row_tiles * a.col_tiles * ((a.rows >> a.part_bits) + a.n_sets);
+        // of sets at most so many
+        const int64_t pieces = a.offsets == nullptr ? lin_pieces(a.rows, a.part_bits, 1) : (a.rows >> a.part_bits) + a.n_sets;
+        blocks = a.row_tiles * a.col_tiles * pieces;
     } else {
         // a set's last tile may be ragged, and so may the one behind the last set; each has a row
         a.row_tiles = a.offsets == nullptr ? (a.rows + BR - 1) / BR : (a.rows + (int64_t)(a.n_sets + 1) * (BR - 1)) / BR;
@@ -319,7 +318,7 @@ int launch_product(const LinArgs &a, hipStream_t s) {
         case TILE_96x128:
             if constexpr (sizeof(T) == 2) return launch_tile<T, MODE, 96, 128, 96, 32>(a, s);
         case TILE_128x128:
-            if constexpr (sizeof(T) == 2 && MODE != LIN_FORWARD) return launch_tile<T, MODE, 128, 128, 64, 64>(a, s);
+            if constexpr (sizeof(T) == 2) return launch_tile<T, MODE, 128, 128, 64, 64>(a, s);
         case TILE_256x256:
             if constexpr (sizeof(T) == 2) return launch_tile<T, MODE, 256, 256, 128, 64>(a, s);
     }

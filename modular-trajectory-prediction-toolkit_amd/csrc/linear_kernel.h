@@ -254,10 +254,9 @@ __device__ __forceinline__ int lin_scan(int v) {
     return v;
 }
 
-// What a set's rows are cut into: row tiles of BR rows, or for the weight gradient parts of `part` rows, one at least (a set
+// What a set's rows are cut into, pieces of 1 << part_bits rows: row tiles, or the weight gradient's parts, one at least (a set
 // without rows has a gradient of zero).
-// What a piece is: 1 << part_bits rows.
-__device__ __forceinline__ int lin_pieces(int64_t len, int part_bits, int least) {
+__host__ __device__ __forceinline__ int lin_pieces(int64_t len, int part_bits, int least) {
     const int n = (int)(((uint32_t)len + (1u << part_bits) - 1) >> part_bits);
     return n < least ? least : n;
 }
@@ -605,6 +604,13 @@ constexpr int lin_waves(int bc, int br, int threads) {
     return waves < 1 ? 1 : waves > 4 ? 4 : waves;
 }
 
+// A wave owns WC x WR of the BC x BR tile as 32 x 32 fragments: 32x32x16 matrix instructions for the 16-bit types, 32x32x2 for float.
+// What bounds it depends on the sizes.  Long sums, bfloat16, 32 768 rows of 2048 -> 2048 in 256 x 256 tiles: input gradient 250 us,
+// 1.10 PFLOP/s (a library product 1.28 to 1.46), of which 30 us are the LDS loads' share (222 us with the loads left out); forward
+// 290 us, 350 with gelu, the kept z and a residual, as nothing covers a single workgroup's way out; weight gradient 314 us, as the
+// transposing reads run at half the rate of the others.  Fragments read one step ahead changed none of these.  Short sums: the way
+// out (143 760 rows over 400 sets, 96 -> 256 bfloat16: 46 us, 68 with gelu and the kept z, which are 16 vector instructions an
+// element and 74 MB).  float: the matrix cores (73 568 rows, 512 -> 96: 75 us, 96 TFLOP/s; 153 in a large library product).
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
 __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * (BC / WC) * (BR / WR))) void k_linear_tile(LinArgs a) {
     constexpr int NT = 64 * (BC / WC) * (BR / WR);
@@ -617,28 +623,48 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wc = wave % (BC / WC), wr = wave / (BC / WC);
 
-    // Tiles of sets: a workgroup takes several that follow each other, so that it looks the sets up once (143 760 rows over 400,
-    // 96 -> 256: 1.5 of the 6 us that a tile took were that).
-    uint32_t left = 1, id = lin_xcd_order(blockIdx.x, gridDim.x);
+    // How many tiles there are of up to 511 sets is known here only.  Forward and input gradient: a workgroup takes several that follow
+    // each other, so that it looks the sets up once (143 760 rows over 400, 96 -> 256: 1.5 of the 6 us that a tile took were that).
+    // Weight gradient: a run of them for each XCD (numbered over the whole grid the last XCD would have the empty ones).
+    uint32_t left = 1, id = blockIdx.x;
     int ct = 0;
     LinPiece p{0, 1, 0, 0, a.rows, 0};
-    const bool walk = MODE != LIN_GRAD_WEIGHT && a.offsets != nullptr && a.n_sets < 512;
-    if (walk) {
-        LinSets<false> sets;
-        sets.look(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, 0);
-        const uint32_t most = (uint32_t)__builtin_amdgcn_readlane(sets.upto, 63) * (uint32_t)a.col_tiles;
+    if (a.offsets != nullptr && a.n_sets < 512) {
+        constexpr bool WEIGHT = MODE == LIN_GRAD_WEIGHT;
+        LinSets<WEIGHT> sets;
+        sets.look(a.offsets, a.n_sets, WEIGHT ? a.n_sets - 1 : a.n_sets, a.rows, WEIGHT ? a.part_bits : lin_log2(BR), WEIGHT ? 1 : 0, 0);
+        const uint32_t most = (uint32_t)__builtin_amdgcn_readlane(sets.upto, 63) * (uint32_t)a.col_tiles *
+                              (WEIGHT ? (uint32_t)a.row_tiles : 1u);
         const uint32_t tiles = most < a.tiles ? most : a.tiles;
-        const uint32_t per = tiles / gridDim.x, more = tiles % gridDim.x;
-        const uint32_t first = id * per + (id < more ? id : more);
-        left = per + (id < more ? 1 : 0);
-        if (left == 0 || !sets.find(first / (uint32_t)a.col_tiles, 0, 0, &p)) return;
-        ct = (int)(first % (uint32_t)a.col_tiles);
-    } else {
+        if (WEIGHT) {
+            if (id >= tiles) return;
+            id = lin_xcd_order(id, tiles);
+        } else {
+            id = lin_xcd_order(id, gridDim.x);
+            const uint32_t per = tiles / gridDim.x, more = tiles % gridDim.x;
+            const uint32_t first = id * per + id * more / gridDim.x;
+            left = (id + 1) * per + (id + 1) * more / gridDim.x - first;
+            id = first;
+        }
         ct = (int)(id % (uint32_t)a.col_tiles);
         id /= (uint32_t)a.col_tiles;
-        if (MODE != LIN_GRAD_WEIGHT && a.offsets != nullptr && !lin_find<false>(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, id, &p))
+        const uint32_t at = WEIGHT ? id / (uint32_t)a.row_tiles : id;
+        if (left == 0 || !sets.find(at, 0, 0, &p)) return;
+    } else {
+        if (a.offsets == nullptr) id = lin_xcd_order(id, a.tiles);
+        ct = (int)(id % (uint32_t)a.col_tiles);
+        id /= (uint32_t)a.col_tiles;
+        if (a.offsets == nullptr) {
+            if (MODE != LIN_GRAD_WEIGHT) p.index = id;
+            else {
+                p.count = lin_pieces(a.rows, a.part_bits, 1);
+                p.index = id / (uint32_t)a.row_tiles;
+            }
+        } else if (MODE == LIN_GRAD_WEIGHT ? !lin_find<true>(a.offsets, a.n_sets, a.n_sets - 1, a.rows, a.part_bits, 1,
+                                                             id / (uint32_t)a.row_tiles, &p)
+                                           : !lin_find<false>(a.offsets, a.n_sets, a.n_sets, a.rows, lin_log2(BR), 0, id, &p)) {
             return;
-        if (MODE != LIN_GRAD_WEIGHT && a.offsets == nullptr) p.index = id;
+        }
     }
     for (bool again = false; left > 0; --left, again = true) {
     int tid_here = tid;
@@ -655,13 +681,7 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     const int64_t c0 = (int64_t)ct * BC;
     if constexpr (MODE == LIN_GRAD_WEIGHT) {
         row0 = (int64_t)(id % (uint32_t)a.row_tiles) * BR;
-        id /= (uint32_t)a.row_tiles;
         row_end = a.out_rows;
-        p.count = lin_pieces(a.rows, a.part_bits, 1);
-        p.index = id;
-        if (a.offsets == nullptr ? id >= (uint32_t)p.count
-                                 : !lin_find<true>(a.offsets, a.n_sets, a.n_sets - 1, a.rows, a.part_bits, 1, id, &p))
-            return;
         k_lo = p.lo + (p.index << a.part_bits);
         k_len = p.hi - k_lo < (1 << a.part_bits) ? p.hi - k_lo : (int64_t)1 << a.part_bits;
         if (p.count > 1) {
@@ -871,7 +891,8 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
 // ---- few rows ----
 // Up to 16 * RT rows of x against 16 columns of the output: W is read once, straight from memory into the operands of the 16 x 16
 // matrix instructions (a lane holds 16 bytes of k of one row of W and of x), the four waves share the sum over k and are
-// added through LDS.  What bounds it is reading W: each wave has UNROLL pieces of it in flight.
+// added through LDS.  What bounds it is reading W: each wave has UNROLL pieces of it in flight (64 rows of 2048 x 2048 bfloat16
+// 10.8 us; one row of 1024 x 1024 is a launch, 4.7 us).
 template <typename T>
 struct LinMfma16;
 template <>
