@@ -605,12 +605,13 @@ constexpr int lin_waves(int bc, int br, int threads) {
 }
 
 // A wave owns WC x WR of the BC x BR tile as 32 x 32 fragments: 32x32x16 matrix instructions for the 16-bit types, 32x32x2 for float.
-// What bounds it depends on the sizes.  Long sums, bfloat16, 32 768 rows of 2048 -> 2048 in 256 x 256 tiles: input gradient 250 us,
-// 1.10 PFLOP/s (a library product 1.28 to 1.46), of which 30 us are the LDS loads' share (222 us with the loads left out); forward
-// 290 us, 350 with gelu, the kept z and a residual, as nothing covers a single workgroup's way out; weight gradient 314 us, as the
-// transposing reads run at half the rate of the others.  Fragments read one step ahead changed none of these.  Short sums: the way
-// out (143 760 rows over 400 sets, 96 -> 256 bfloat16: 46 us, 68 with gelu and the kept z, which are 16 vector instructions an
-// element and 74 MB).  float: the matrix cores (73 568 rows, 512 -> 96: 75 us, 96 TFLOP/s; 153 in a large library product).
+// What bounds it depends on the sizes.  Long sums, bfloat16, 32 768 rows of 2048 -> 2048 in 256 x 256 tiles: forward 247 us
+// (1.11 PFLOP/s; a library product 1.13 to 1.46), 328 with gelu, the kept z and a residual, as nothing covers a single workgroup's
+// way out; input gradient 234; weight gradient 256 with its join, as the transposing reads run at half the rate of the others.  The
+// matrix cores are busy for half of the time; leaving the LDS loads out would take a fifth off, fragments read one step ahead
+// nothing.  Short sums: the way out (143 760 rows over 400 sets, 96 -> 256 bfloat16: 46 us, 68 with gelu and the kept z, which are
+// some 25 vector instructions an element and 74 MB).  float: the matrix cores (73 568 rows, 512 -> 96: 75 us, 96 TFLOP/s; 153 in a
+// large library product).
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
 __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * (BC / WC) * (BR / WR))) void k_linear_tile(LinArgs a) {
     constexpr int NT = 64 * (BC / WC) * (BR / WR);
@@ -774,7 +775,7 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
         fetch_q(buf);
     };
     // Big tiles have one workgroup a CU: its loads are sent in two halves, between products, as eight in a row keep a wave from
-    // its products until they have been taken (32 768 rows, 2048 -> 2048: weight gradient 365 -> 340 us, input gradient 257 -> 250;
+    // its products until they have been taken (32 768 rows, 2048 -> 2048: input gradient 257 -> 250 us, weight gradient 365 -> 340;
     // 128x128 tiles, two a CU, 314 -> 326).
     constexpr bool HALVES = BC == 256;
     // both buffers are on their way before the first is used; later tiles are fetched one ahead
