@@ -392,7 +392,7 @@ BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets,
         p.lddz = elem_size(dtype) == 2 && out % 2 != 0 ? round_up(out, 8) : out;
         p.dz_bytes = round_up(rows * p.lddz * elem_size(dtype), 256);
     }
-    if (want_x) p.w_bytes = relayout_bytes(dtype, w, ldw, (int64_t)n_sets * out, in);
+    if (want_x && rows > 0) p.w_bytes = relayout_bytes(dtype, w, ldw, (int64_t)n_sets * out, in);
     if (want_w) {
         p.x_bytes = relayout_bytes(dtype, x, ldx, rows, in);
         p.parts_bytes = most_parts(rows, n_sets, part_bits_for(rows, in, out, n_sets, elem_size(dtype) == 2)) * out * (in + 1) * 4;

@@ -57,6 +57,9 @@ def test_entry_points_refuse_a_small_workspace():
     assert need >= (600 + 40) * 104 * 2
     assert L.mtp_linear(1, ONE, 600, 97, 97, ONE, 40, None, 0, None, 0, None, 1, ONE, None, ONE, need - 1, None) == -3
     assert L.mtp_linear(1, ONE, 600, 97, 97, ONE, 40, None, 0, None, 0, None, 1, ONE, None, ONE + 8, need, None) == -3
+    # without rows the weights are not read, so they are not laid out anew either
+    assert L.mtp_linear_backward_workspace_bytes(1, 0, 97, 41, 1, 0, None, None, 97, None, 97, 1, 1) == 0
+    assert L.mtp_linear_backward_workspace_bytes(1, 4, 97, 41, 1, 0, ONE, ONE, 97, ONE, 97, 1, 0) > 0
     need = L.mtp_linear_workspace_bytes(1, _lib.LINEAR_GRAD_WEIGHT, 50000, 96, 40, 1, ONE, 40, ONE, 96)
     assert need > 0 and L.mtp_linear_grad_weight(1, ONE, 50000, 40, 40, ONE, 96, 96, None, 1, ONE, None, ONE, need - 1, None) == -3
 
