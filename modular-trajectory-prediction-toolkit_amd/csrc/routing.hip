@@ -142,11 +142,17 @@ struct RouteKey<float> {
 };
 
 constexpr int ROW_ROR = 0x120;  // rotation within 16 lanes
+constexpr int HALF_MIRROR = 0x141, QUAD_XOR1 = 0xb1, QUAD_XOR2 = 0x4e;  // lane 7 - i of eight; the neighbour, the next but one of four
 
-// over the L lanes (16, 32 or 64) that share a row, the same result in each
+// over the L lanes (8, 16, 32 or 64) that share a row, the same result in each
 template <typename T, int L>
 __device__ __forceinline__ typename RouteKey<T>::type group_max(typename RouteKey<T>::type v) {
     typedef RouteKey<T> R;
+    if constexpr (L == 8) {
+        v = R::more(v, R::template turn<HALF_MIRROR>(v));
+        v = R::more(v, R::template turn<QUAD_XOR1>(v));
+        return R::more(v, R::template turn<QUAD_XOR2>(v));
+    }
     v = R::more(v, R::template turn<ROW_ROR + 8>(v));
     v = R::more(v, R::template turn<ROW_ROR + 4>(v));
     v = R::more(v, R::template turn<ROW_ROR + 2>(v));
@@ -161,6 +167,11 @@ __device__ __forceinline__ float turn_f32(float v) {
 }
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
+    if constexpr (L == 8) {
+        v += turn_f32<HALF_MIRROR>(v);
+        v += turn_f32<QUAD_XOR1>(v);
+        return v + turn_f32<QUAD_XOR2>(v);
+    }
     v += turn_f32<ROW_ROR + 8>(v);
     v += turn_f32<ROW_ROR + 4>(v);
     v += turn_f32<ROW_ROR + 2>(v);
@@ -196,7 +207,7 @@ __device__ __forceinline__ void sort_registers(typename RouteKey<T>::type (&a)[V
 // the scores sub * V to sub * V + V - 1.  Each lane sorts its keys and lays them into LDS, as many as could be chosen; k times the
 // largest head is taken (a maximum over the L lanes), and the lane it came from moves on to its next key.  Scores are read once.
 // Bound by its vector instructions: for 16 keys a lane 63 pairs of the sort, then some twelve for each of the k.  1 M rows of
-// 200 bfloat16, top 20: 270 us for 0.57 GB (2.1 TB/s, 44 % of the rate of a copy); 17 970 rows of 400, top 8: 13 us.
+// 200 bfloat16, top 20: 230 us for 0.57 GB (2.5 TB/s, half the rate of a copy); 17 970 rows of 400, top 8: 13 us.
 template <typename T, int L, int V, int KB>
 __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores, int64_t n, int e, int64_t ld, int k, int normalize,
                                                     int32_t *__restrict__ ids, float *__restrict__ weights,
@@ -270,8 +281,8 @@ __global__ __launch_bounds__(256) void k_route_topk(const T *__restrict__ scores
         auto take = [&](int i) {
             const key_t best = group_max<T, L>(head);
             if (sub == i) chosen[b] = best;
-            // keys differ by their index, so one lane moves on; a lane that has given its last key stays at NONE
-            next += head == best && best != R::NONE ? 256 : 0;
+            // keys differ by their index, so one lane moves on; there are k keys at least, so the largest is never NONE
+            next += head == best ? 256 : 0;
             head = *next;
         };
         int i = 0;
@@ -748,6 +759,10 @@ int route_by_k(const void *scores, int64_t n, int e, int64_t ld, int k, int norm
     if (k <= 2 * L) return launch_topk<T, L, V, 2>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     if constexpr (L == 32) return launch_topk<T, L, V, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
     if constexpr (L == 16) return launch_topk<T, L, V, 8>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    if constexpr (L == 8) {
+        if (k <= 4 * L) return launch_topk<T, L, V, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        return launch_topk<T, L, V, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+    }
     mtp_set_error("mtp_route_topk: k=%d", k);
     return MTP_E_ARG;
 }
@@ -758,9 +773,16 @@ int route(const void *scores, int64_t n, int e, int64_t ld, int k, int normalize
     // More lanes a row: shorter sorts and longer maxima, k of them.  100 000 rows, microseconds for k = 1 / 7 / 20 / 64:
     //   400 float     16 lanes 67 / 73 / 86 / 160, 32 lanes 51 / 64 / 94 / 189, 64 lanes 51 / 84 / 152 / 415
     //   900 bfloat16  16 lanes 92 / 100 / 110 / 154, 32 lanes 66 / 75 / 91 / 143, 64 lanes 60 / 77 / 112 / 225
+    // 400 000 rows, k = 4 / 20 / 40 / 100:
+    //   50 bfloat16   8 lanes 22 / 39 / 71, 16 lanes 29 / 57 / 103;  float 30 / 56 / 101, 39 / 90 / 176
+    //   100 bfloat16  8 lanes 35 / 52 / 83 / 130, 16 lanes 65 / 92 / 136 / 227;  float 54 / 81 / 129 / 217, 101 / 152 / 228 / 409
+    //   200 bfloat16  8 lanes 67 / 89 / 123 / 172, 16 lanes 63 / 92 / 139 / 226;  float 127 / 157 / 260 / 377, 107 / 159 / 233 / 419
     // Few rows: one wave a row, since the card is not full anyway.
     if (n >= 1024 && e <= 1024) {
-        if (e <= 64) return route_by_k<T, 16, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 32) return route_by_k<T, 8, 4>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 64) return route_by_k<T, 8, 8>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 128) return route_by_k<T, 8, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
+        if (e <= 256 && sizeof(T) == 2 && k > 32) return route_by_k<T, 8, 32>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
         if (e <= 256) return route_by_k<T, 16, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
         if (e <= 512 && k > 8) return route_by_k<T, 16, 32>(scores, n, e, ld, k, normalize, ids, weights, stats, s);
         if (e <= 512) return route_by_k<T, 32, 16>(scores, n, e, ld, k, normalize, ids, weights, stats, s);

@@ -130,7 +130,11 @@ def route(scores, k, normalize, g=None):
         weight = mine if normalize else p
         v = back - weight * dot
         err = (2 * rel + (k + 4) * U32) * (back.abs() + weight * size)
-        out["ds"] = (v, err + u * (v.abs() + err) + floor_of(scores.dtype))
+        # below the smallest normal float a rounding costs up to half of 2^-149 whatever the value: one in exp(s - top), one in the
+        # weight made of it (the scale 1 / mass is at most 1, as the largest term is exp(0)), both then multiplied by g - dot or
+        # dot, and one in that product
+        low = floor_of(torch.float32) * (1 + 2 * (G.abs().max(1, keepdim=True).values + size))
+        out["ds"] = (v, err + low + u * (v.abs() + err + low) + floor_of(scores.dtype))
     return out
 
 

@@ -1,4 +1,5 @@
 """``pccs_accel.routing`` on the GPU against float64 formulas (routing_reference.py), and the routed layers as they run together."""
+import io
 import math
 
 import pytest
@@ -15,6 +16,9 @@ pytestmark = pytest.mark.gpu
 ROUTES = [(1, 1, 1), (1, 200, 20), (3, 7, 7), (5, 64, 1), (1030, 5, 3), (1500, 64, 64), (1025, 65, 17), (1200, 200, 20), (900, 256, 128),
           (1100, 257, 33), (1050, 400, 7), (1040, 1024, 128), (30, 1024, 8), (7, 1025, 5), (2, 4096, 128), (1024, 33, 32), (1026, 999, 16),
           (1030, 130, 4), (1040, 300, 8), (1050, 511, 9), (1060, 512, 20), (1030, 513, 70), (1100, 8, 8), (1100, 9, 9)]
+# eight lanes a row: every width and batch of choices, their borders, rows that end inside a piece
+ROUTES += [(1024, 1, 1), (1031, 7, 2), (1024, 31, 31), (1057, 32, 9), (1033, 40, 17), (1039, 64, 33), (1025, 100, 8), (1041, 127, 100),
+           (1029, 128, 128), (1030, 129, 33), (1037, 201, 70), (1026, 256, 128), (1027, 256, 32)]
 
 
 def _scores(seed, n, e, dtype):
@@ -60,6 +64,26 @@ def test_route_ties_go_to_the_lowest_index(gpu_device, n):
         scores[1, 1::2] = 0.0
         _check_route(gpu_device, scores, 40, True)
         _check_route(gpu_device, scores, 40, False)
+
+
+@pytest.mark.parametrize("e,k", [(20, 12), (50, 30), (110, 50), (250, 60)])
+def test_route_eight_lanes_masks_and_ties(gpu_device, e, k):
+    """Rows with fewer than k scores left, rows of equal scores, NaN: lanes run out of keys at different times."""
+    for dtype in R.TYPES:
+        scores = _scores(e, 1033, e, dtype)
+        scores[0] = -math.inf
+        scores[1, 3:] = -math.inf
+        scores[2] = 1.0
+        scores[3] = torch.arange(e).to(dtype)          # the best in the last lanes
+        scores[4] = -torch.arange(e).to(dtype)         # and in the first
+        scores[5, ::3] = -math.inf
+        scores[1032, 1:] = -math.inf                   # the last row, which fills the rest of its workgroup
+        for normalize in (False, True):
+            _check_route(gpu_device, scores, k, normalize)
+        scores[6, e // 2] = math.nan
+        ids, w = route_topk(scores.to(gpu_device), k)
+        assert torch.isnan(w[6]).all() and not torch.isnan(w[5]).any() and not torch.isnan(w[7]).any()
+        assert int(ids[6].max()) < e
 
 
 @pytest.mark.parametrize("n", [6, 1200])
@@ -467,3 +491,35 @@ def test_arguments_of_another_kind_are_never_taken_without_gradient(gpu_device):
     for call in (lambda: route_topk(s, 2.0), lambda: route_topk(s, "2"), lambda: combine(s, plan, [1.0]), lambda: dispatch([s], plan)):
         with pytest.raises((TypeError, ValueError)):
             call()
+
+
+def test_results_of_small_calls_are_tensors_of_their_own(gpu_device):
+    """They share an allocation; writing one, saving it, inference mode and gradients are as with any other tensor."""
+    s = _scores(5, 12, 40, torch.float32).to(gpu_device)
+    ids, w = route_topk(s, 4)
+    plan = sort_pairs(ids, 40)
+    kept = [t.clone() for t in (ids, w) + tuple(plan)]
+    for t in (ids, w) + tuple(plan):
+        assert t.is_contiguous() and t.data_ptr() % 16 == 0 and not t._is_view() and t._version == 0
+        t.fill_(7)
+    again = route_topk(s, 4)
+    for t, k in zip(again + tuple(sort_pairs(again[0], 40)), kept):
+        assert torch.equal(t, k)
+    for k, t in enumerate((ids, w) + tuple(plan)):
+        assert (t == 7).all(), k
+    w2 = again[1].requires_grad_()
+    (w2 * 2).sum().backward()
+    assert (w2.grad == 2).all()
+    again[0].add_(1)  # another tensor's version does not move
+    assert again[1]._version == 0
+    buffer = io.BytesIO()
+    torch.save(again[0], buffer)
+    buffer.seek(0)
+    assert torch.equal(torch.load(buffer, weights_only=True), again[0])
+    with torch.inference_mode():
+        ids, w = route_topk(s, 4)
+        assert ids.is_inference() and w.is_inference() and torch.equal(ids, kept[0]) and torch.equal(w, kept[1])
+        assert torch.equal(sort_pairs(ids, 40).order, kept[3])
+    rows = dispatch(torch.ones(12, 3, device=gpu_device), sort_pairs(kept[0], 40)).requires_grad_()
+    combine(rows, sort_pairs(kept[0], 40), kept[1]).sum().backward()
+    assert rows.grad is not None
