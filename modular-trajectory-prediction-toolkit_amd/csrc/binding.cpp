@@ -2,7 +2,7 @@
 //
 // A small layer takes a few microseconds on the card; a call through Python takes ten, a backward pass through Python nodes some
 // thirty more.  Here the arguments are looked over, the results allocated and the entry points of mtp_accel.h called without
-// Python between them (forward and backward of a 64 x 96 layer with gelu: 45 us against 68).  A call whose arguments are not as
+// Python between them (forward and backward of a 64 x 96 layer with gelu: 45 us against 68 on one host, 57 on a slower one).  A call whose arguments are not as
 // they have to be returns None: the Python front end then finds out what is wrong and raises.
 #include <torch/extension.h>
 
@@ -10,8 +10,11 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <array>
 #include <optional>
 
 #include "mtp_accel.h"
@@ -19,7 +22,8 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 constexpr int64_t MOST = 0x7fffffff;
@@ -57,7 +61,7 @@ Tensor workspace(int64_t bytes, const Tensor &ref) {
 
 // Results of a scene's size share one allocation (each takes the host a microsecond, a sixth of such a call: sort_pairs 6.0 -> 4.8 us,
 // route_topk 5.2 -> 4.5); large ones have their own, so that each can go when it is not needed.
-constexpr int64_t TOGETHER_BYTES = 64 << 10, PLACE_BYTES = 256;
+constexpr int64_t TOGETHER_BYTES = 256 << 10, PLACE_BYTES = 256;
 int64_t place(int64_t bytes) { return (bytes + PLACE_BYTES - 1) / PLACE_BYTES * PLACE_BYTES; }
 Tensor part_of(const Tensor &all, int64_t at, at::ScalarType type, at::IntArrayRef sizes) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
@@ -81,6 +85,21 @@ void refuse_foreign_nodes(const char *what, std::initializer_list<const Tensor *
                     ": an input belongs to an autograd graph that was begun outside this capture; its backward pass cannot be captured "
                     "(let go of the eager results that refer to it first)");
     }
+}
+
+// no derivative in forward mode: a tangent must not get lost in silence
+void refuse_tangents(const char *what, std::initializer_list<const Tensor *> inputs) {
+    for (const Tensor *t : inputs)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no derivative in forward mode");
+}
+
+// A node of the operators below with an edge to each of its inputs.  (Nodes of their own rather than torch::autograd::Function: its
+// bookkeeping takes the host some 5 us of a forward and a backward pass.)
+template <typename N, typename... Inputs>
+std::shared_ptr<N> node_with_edges(const Inputs &...inputs) {
+    std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    return node;
 }
 
 // What a backward pass returns can be differentiated no further: trying to says so.  `from`: what it was computed from.
@@ -118,63 +137,62 @@ Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor
     return y;
 }
 
-struct Linear : torch::autograd::Function<Linear> {
-    // arguments that are not there have no edge: the residual's follows the bias' or takes its place
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_,
-                          const std::optional<Tensor> &residual_, const std::optional<Tensor> &offsets_, const Sizes &z) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
-        // relu's slope can be read off y where nothing was added to it
-        const bool from_y = z.act == RELU && !residual.defined();
-        Tensor pre, ws;
-        Tensor y = run_linear(z, x, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr, &ws);
-        // rows that do not start where the products want them have been laid out there: once for both passes
-        Tensor rows, weights;
-        const int64_t ld = (z.in + 7) / 8 * 8;
-        if (ws.defined()) {
-            const Tensor all = ws.view(x.scalar_type());
-            int64_t at = 0;
-            auto take = [&](const Tensor &t, int64_t n, int64_t distance) {
-                if (mtp_linear_rows_aligned(z.code, at_(t), distance)) return Tensor();
-                const int64_t from = at;
-                at += (n * ld * x.element_size() + 255) / 256 * 256 / x.element_size();
-                return all.as_strided({n, z.in}, {ld, 1}, from);
-            };
-            rows = take(x, z.rows, row_distance(x));
-            weights = take(w, z.sets * z.out, z.in);
-        }
-        ctx->save_for_backward({x, w, from_y ? y : pre, offsets, rows, weights});
-        ctx->saved_data["sizes"] =
-            std::vector<int64_t>{z.code, z.act, z.rows, z.in, z.out, z.sets, bias.defined(), residual.defined()};
-        return y;
+struct LinearNode : Node {
+    Sizes z;
+    bool has_bias, has_residual;
+    SavedVariable x_, w_, pre_, offsets_, rows_, weights_;
+
+    std::string name() const override { return "LinearBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&x_, &w_, &pre_, &offsets_, &rows_, &weights_}) v->reset_data();
     }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &pre = saved[2], &offsets = saved[3];
-        const auto v = ctx->saved_data["sizes"].toIntVector();
-        const Sizes z{(int)v[0], (int)v[1], v[2], v[3], v[4], v[5]};
+    // edges: x, weight, bias, residual
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return variable_list(4);
+        const Tensor x = x_.unpack(), w = w_.unpack(), pre = pre_.unpack(getptr()), offsets = offsets_.unpack();
+        const Tensor rows = rows_.unpack(), weights = weights_.unpack();
         Tensor dx, dw, db, dr;
         {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
             const Tensor g = grads[0].contiguous();
-            const bool want_x = ctx->needs_input_grad(0), want_b = v[6] != 0 && ctx->needs_input_grad(2);
-            const bool want_w = ctx->needs_input_grad(1) || want_b;
-            if (want_x) dx = at::empty({z.rows, z.in}, x.options());
-            if (want_w) dw = offsets.defined() ? at::empty({z.sets, z.out, z.in}, x.options()) : at::empty({z.out, z.in}, x.options());
-            if (want_b) db = offsets.defined() ? at::empty({z.sets, z.out}, x.options()) : at::empty({z.out}, x.options());
+            const bool want_x = task_should_compute_output(0), want_b = has_bias && task_should_compute_output(2);
+            const bool want_w = task_should_compute_output(1) || want_b;
             const int32_t *sets = static_cast<const int32_t *>(at_(offsets));
             if (want_x || want_w) {
-                const Tensor &xs = saved[4].defined() ? saved[4] : x, &wt = saved[5].defined() ? saved[5] : w;
-                const int64_t ldx = row_distance(xs), ldw = saved[5].defined() ? (z.in + 7) / 8 * 8 : z.in;
-                const int64_t bytes = mtp_linear_backward_workspace_bytes(z.code, z.rows, (int)z.in, (int)z.out, (int)z.sets, z.act,
-                                                                          at_(g), at_(wt), ldw, at_(xs), ldx, want_x, want_w);
-                const Tensor ws = workspace(bytes, x);
-                check(mtp_linear_backward(z.code, at_(g), at_(pre), z.act, at_(xs), z.rows, (int)z.in, ldx, at_(wt), (int)z.out,
-                                          ldw, sets, (int)z.sets, at_(dx), at_(dw), at_(db), at_(ws), (size_t)bytes, stream_of(x)),
-                      "mtp_linear_backward");
+                const Tensor &xs = rows.defined() ? rows : x, &wt = weights.defined() ? weights : w;
+                const int64_t ldx = row_distance(xs), ldw = weights.defined() ? (z.in + 7) / 8 * 8 : z.in;
+                const int64_t ws_bytes = mtp_linear_backward_workspace_bytes(z.code, z.rows, (int)z.in, (int)z.out, (int)z.sets, z.act,
+                                                                             at_(g), at_(wt), ldw, at_(xs), ldx, want_x, want_w);
+                const bool many = offsets.defined();
+                const std::array<int64_t, 2> x_size{z.rows, z.in};
+                const std::array<int64_t, 3> w_size{z.sets, z.out, z.in};
+                const auto w_sizes = at::IntArrayRef(w_size).slice(many ? 0 : 1), b_sizes = w_sizes.slice(0, w_sizes.size() - 1);
+                const int64_t size = x.element_size(), x_bytes = want_x ? place(z.rows * z.in * size) : 0,
+                              w_bytes = want_w ? place(z.sets * z.out * z.in * size) : 0, b_bytes = want_b ? place(z.sets * z.out * size) : 0;
+                Tensor all;
+                char *ws = nullptr;
+                if (x_bytes + w_bytes + b_bytes + ws_bytes <= TOGETHER_BYTES) {
+                    all = at::empty({x_bytes + w_bytes + b_bytes + ws_bytes}, x.options().dtype(at::kByte));
+                    if (want_x) dx = part_of(all, 0, x.scalar_type(), x_size);
+                    if (want_w) dw = part_of(all, x_bytes, x.scalar_type(), w_sizes);
+                    if (want_b) db = part_of(all, x_bytes + w_bytes, x.scalar_type(), b_sizes);
+                    ws = static_cast<char *>(all.data_ptr()) + x_bytes + w_bytes + b_bytes;
+                } else {
+                    if (want_x) dx = at::empty(x_size, x.options());
+                    if (want_w) dw = at::empty(w_sizes, x.options());
+                    if (want_b) db = at::empty(b_sizes, x.options());
+                    all = workspace(ws_bytes, x);
+                    ws = static_cast<char *>(at_(all));
+                }
+                if (want_w || z.rows > 0)  // else dx has no elements
+                    check(mtp_linear_backward(z.code, at_(g), at_(pre), z.act, at_(xs), z.rows, (int)z.in, ldx, at_(wt), (int)z.out,
+                                              ldw, sets, (int)z.sets, at_(dx), at_(dw), at_(db), ws, (size_t)ws_bytes, stream_of(x)),
+                          "mtp_linear_backward");
             }
-            if (v[7] != 0 && ctx->needs_input_grad(v[6] != 0 ? 3 : 2)) {
+            if (has_residual && task_should_compute_output(3)) {
                 if (offsets.defined()) {  // rows behind the last set have none
                     dr = at::empty_like(g);
                     check(mtp_linear_mask_rows(z.code, at_(g), z.rows, (int)z.out, sets, (int)z.sets, at_(dr), stream_of(x)),
@@ -183,11 +201,49 @@ struct Linear : torch::autograd::Function<Linear> {
                     dr = g;
                 }
             }
-            if (!ctx->needs_input_grad(1)) dw = Tensor();
+            if (!task_should_compute_output(1)) dw = Tensor();
         }
-        return no_further({dx, dw, db, dr, Tensor(), Tensor()}, {x, w, grads[0]}, "linear");
+        return no_further({dx, dw, db, dr}, {x, w, grads[0]}, "linear");
     }
 };
+
+Tensor linear_with_node(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, const Tensor &offsets,
+                        const Sizes &z) {
+    const auto node = node_with_edges<LinearNode>(x, w, bias, residual);
+    // relu's slope can be read off y where nothing was added to it
+    const bool from_y = z.act == RELU && !residual.defined();
+    Tensor pre, ws, y, rows, weights;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = run_linear(z, x, w, bias, residual, offsets, z.act != NONE && !from_y ? &pre : nullptr, &ws);
+        // rows that do not start where the products want them have been laid out there: once for both passes
+        const int64_t ld = (z.in + 7) / 8 * 8;
+        if (ws.defined()) {
+            const Tensor all = ws.view(x.scalar_type());
+            int64_t at = 0;
+            auto take = [&](const Tensor &t, int64_t n, int64_t distance) {
+                if (mtp_linear_rows_aligned(z.code, at_(t), distance)) return Tensor();
+                const int64_t from = at;
+                at += place(n * ld * x.element_size()) / x.element_size();
+                return all.as_strided({n, z.in}, {ld, 1}, from);
+            };
+            rows = take(x, z.rows, row_distance(x));
+            weights = take(w, z.sets * z.out, z.in);
+        }
+    }
+    torch::autograd::set_history(y, node);
+    node->z = z;
+    node->has_bias = bias.defined();
+    node->has_residual = residual.defined();
+    node->x_ = SavedVariable(x, false);
+    node->w_ = SavedVariable(w, false);
+    if (from_y) node->pre_ = SavedVariable(y, true);
+    else if (pre.defined()) node->pre_ = SavedVariable(pre, false);
+    if (offsets.defined()) node->offsets_ = SavedVariable(offsets, false);
+    if (rows.defined()) node->rows_ = SavedVariable(rows, false);
+    if (weights.defined()) node->weights_ = SavedVariable(weights, false);
+    return y;
+}
 
 std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_, int act,
                              const std::optional<Tensor> &residual_, const std::optional<Tensor> &offsets_) {
@@ -205,50 +261,44 @@ std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::option
     if (residual.defined() && (!matrix(residual) || residual.scalar_type() != x.scalar_type() || residual.device() != x.device() ||
                                residual.size(0) != z.rows || residual.size(1) != z.out || row_distance(residual) < 0))
         return std::nullopt;
+    refuse_tangents("linear", {&x, &w, &bias, &residual});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
                                        (residual.defined() && residual.requires_grad())))
     {
         refuse_foreign_nodes("linear", {&x, &w, &bias, &residual});
-        return Linear::apply(x, w, bias_, residual_, offsets_, z);
+        return linear_with_node(x, w, bias, residual, offsets, z);
     }
     return run_linear(z, x, w, bias, residual, offsets, nullptr);
 }
 
 // ---- router ----
-struct Route : torch::autograd::Function<Route> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &scores, int64_t k, bool normalize) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        const int64_t n = scores.size(0), e = scores.size(1);
-        Tensor ids = at::empty({n, k}, scores.options().dtype(at::kInt)), weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
-        Tensor stats = at::empty({n, 2}, weights.options());
-        check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, row_distance(scores), (int)k, normalize,
-                             static_cast<int32_t *>(at_(ids)), static_cast<float *>(at_(weights)), static_cast<float *>(at_(stats)),
-                             stream_of(scores)),
-              "mtp_route_topk");
-        ctx->save_for_backward({scores, ids, weights, stats});
-        ctx->saved_data["normalize"] = normalize;
-        ctx->mark_non_differentiable({ids});
-        ctx->set_materialize_grads(false);
-        return {ids, weights};
+struct RouteNode : Node {
+    bool normalize;
+    SavedVariable scores_, ids_, weights_, stats_;
+
+    std::string name() const override { return "RouteTopkBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&scores_, &ids_, &weights_, &stats_}) v->reset_data();
     }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return variable_list(1);
+        const Tensor scores = scores_.unpack(), ids = ids_.unpack(), weights = weights_.unpack(getptr()), stats = stats_.unpack();
         Tensor out;
-        const auto saved = ctx->get_saved_variables();
-        const Tensor &scores = saved[0];
-        if (grads[1].defined()) {
+        {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
-            const Tensor g = grads[1].contiguous();
+            const Tensor g = grads[0].contiguous();
             out = at::empty(scores.sizes(), scores.options());
             check(mtp_route_topk_grad(type_code(scores), at_(scores), scores.size(0), (int)scores.size(1), row_distance(scores),
-                                      (int)saved[1].size(1), ctx->saved_data["normalize"].toBool(),
-                                      static_cast<const int32_t *>(at_(saved[1])), static_cast<const float *>(at_(saved[2])),
-                                      static_cast<const float *>(at_(saved[3])), static_cast<const float *>(at_(g)), at_(out),
-                                      stream_of(scores)),
+                                      (int)ids.size(1), normalize, static_cast<const int32_t *>(at_(ids)),
+                                      static_cast<const float *>(at_(weights)), static_cast<const float *>(at_(stats)),
+                                      static_cast<const float *>(at_(g)), at_(out), stream_of(scores)),
                   "mtp_route_topk_grad");
         }
-        return no_further({out, Tensor(), Tensor()}, {scores, grads[1]}, "route_topk");
+        return no_further({out}, {scores, grads[0]}, "route_topk");
     }
 };
 
@@ -256,25 +306,36 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
     if (!matrix(scores)) return std::nullopt;
     const int64_t n = scores.size(0), e = scores.size(1), ld = row_distance(scores);
     if (ld < 0 || n > MOST || e < 1 || e > MOST_MODALITIES || k < 1 || k > e || k > MOST_TOPK) return std::nullopt;
+    refuse_tangents("route_topk", {&scores});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
-    if (at::GradMode::is_enabled() && scores.requires_grad()) {
-        refuse_foreign_nodes("route_topk", {&scores});
-        auto out = Route::apply(scores, k, normalize);
-        return std::make_tuple(out[0], out[1]);
+    const bool train = at::GradMode::is_enabled() && scores.requires_grad();
+    if (train) refuse_foreign_nodes("route_topk", {&scores});
+    Tensor ids, weights, stats;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const int64_t bytes = n * k * 4;
+        if (bytes > 0 && bytes <= TOGETHER_BYTES) {
+            const Tensor all = at::empty({place(bytes) + bytes}, scores.options().dtype(at::kByte));
+            ids = part_of(all, 0, at::kInt, {n, k});
+            weights = part_of(all, place(bytes), at::kFloat, {n, k});
+        } else {
+            ids = at::empty({n, k}, scores.options().dtype(at::kInt));
+            weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+        }
+        if (train) stats = at::empty({n, 2}, scores.options().dtype(at::kFloat));
+        check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, ld, (int)k, normalize, static_cast<int32_t *>(at_(ids)),
+                             static_cast<float *>(at_(weights)), static_cast<float *>(at_(stats)), stream_of(scores)),
+              "mtp_route_topk");
     }
-    Tensor ids, weights;
-    const int64_t bytes = n * k * 4;
-    if (bytes > 0 && bytes <= TOGETHER_BYTES) {
-        const Tensor all = at::empty({place(bytes) + bytes}, scores.options().dtype(at::kByte));
-        ids = part_of(all, 0, at::kInt, {n, k});
-        weights = part_of(all, place(bytes), at::kFloat, {n, k});
-    } else {
-        ids = at::empty({n, k}, scores.options().dtype(at::kInt));
-        weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+    if (train) {
+        const auto node = node_with_edges<RouteNode>(scores);
+        torch::autograd::set_history(weights, node);
+        node->normalize = normalize;
+        node->scores_ = SavedVariable(scores, false);
+        node->ids_ = SavedVariable(ids, false);
+        node->weights_ = SavedVariable(weights, true);
+        node->stats_ = SavedVariable(stats, false);
     }
-    check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, ld, (int)k, normalize, static_cast<int32_t *>(at_(ids)),
-                         static_cast<float *>(at_(weights)), nullptr, stream_of(scores)),
-          "mtp_route_topk");
     return std::make_tuple(ids, weights);
 }
 
@@ -326,53 +387,60 @@ Tensor run_combine(const Tensor &rows, const Tensor &position, const Tensor &off
     return y;
 }
 
-struct Dispatch : torch::autograd::Function<Dispatch> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &position, const Tensor &offsets) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        ctx->save_for_backward({position, offsets});
-        return run_dispatch(x, position, offsets);
+struct DispatchNode : Node {
+    SavedVariable position_, offsets_;
+
+    std::string name() const override { return "DispatchBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        position_.reset_data();
+        offsets_.reset_data();
     }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return variable_list(1);
+        const Tensor position = position_.unpack(), offsets = offsets_.unpack();
         Tensor dx;
         {
             at::NoGradGuard off;
-            const auto saved = ctx->get_saved_variables();
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(grads[0].device());
-            dx = run_combine(grads[0].contiguous(), saved[0], saved[1], Tensor());
+            dx = run_combine(grads[0].contiguous(), position, offsets, Tensor());
         }
-        return no_further({dx, Tensor(), Tensor()}, {grads[0]}, "dispatch");
+        return no_further({dx}, {grads[0]}, "dispatch");
     }
 };
 
-struct Combine : torch::autograd::Function<Combine> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &rows, const std::optional<Tensor> &weights_, const Tensor &position,
-                          const Tensor &offsets) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor weights = weights_.value_or(Tensor());
-        // the rows themselves are needed for the weights' gradient only
-        ctx->save_for_backward({weights.defined() ? rows : Tensor(), weights, position, offsets});
-        return run_combine(rows, position, offsets, weights);
+struct CombineNode : Node {
+    SavedVariable rows_, weights_, position_, offsets_;
+    bool weighted;
+
+    std::string name() const override { return "CombineBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&rows_, &weights_, &position_, &offsets_}) v->reset_data();
     }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    // edges: rows, weights
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return variable_list(2);
+        const Tensor rows = rows_.unpack(), weights = weights_.unpack(), position = position_.unpack(), offsets = offsets_.unpack();
         Tensor dr, dw;
-        const auto saved = ctx->get_saved_variables();
-        const Tensor &rows = saved[0], &weights = saved[1], &position = saved[2], &offsets = saved[3];
         {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(grads[0].device());
             const Tensor g = grads[0].contiguous();
-            if (!weights.defined()) {
+            if (!weighted) {
                 dr = run_dispatch(g, position, offsets);
             } else {
-                if (ctx->needs_input_grad(0)) dr = at::empty_like(rows);
-                if (ctx->needs_input_grad(1)) dw = at::empty_like(weights);
+                if (task_should_compute_output(0)) dr = at::empty_like(rows);
+                if (task_should_compute_output(1)) dw = at::empty_like(weights);
                 check(mtp_combine_rows_grad(type_code(rows), at_(rows), at_(g), g.size(0), (int)g.size(1), (int)position.size(1),
                                             places(position), held(offsets), static_cast<const float *>(at_(weights)), at_(dr),
                                             static_cast<float *>(at_(dw)), stream_of(g)),
                       "mtp_combine_rows_grad");
             }
         }
-        return no_further({dr, dw, Tensor(), Tensor()}, {rows, weights, grads[0]}, "combine");
+        return no_further({dr, dw}, {rows, weights, grads[0]}, "combine");
     }
 };
 
@@ -385,12 +453,18 @@ std::optional<Tensor> dispatch(const Tensor &x, const Tensor &position, const Te
     if (!matrix(x) || row_distance(x) < 0 || !plan_for(x, position, offsets) || position.size(0) != x.size(0) || x.size(1) < 1 ||
         position.size(1) < 1)
         return std::nullopt;
+    refuse_tangents("dispatch", {&x});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
-    if (at::GradMode::is_enabled() && x.requires_grad()) {
-        refuse_foreign_nodes("dispatch", {&x});
-        return Dispatch::apply(x, position, offsets);
+    const bool train = at::GradMode::is_enabled() && x.requires_grad();
+    if (train) refuse_foreign_nodes("dispatch", {&x});
+    const Tensor rows = run_dispatch(x, position, offsets);
+    if (train) {
+        const auto node = node_with_edges<DispatchNode>(x);
+        torch::autograd::set_history(rows, node);
+        node->position_ = SavedVariable(position, false);
+        node->offsets_ = SavedVariable(offsets, false);
     }
-    return run_dispatch(x, position, offsets);
+    return rows;
 }
 
 std::optional<Tensor> combine(const Tensor &rows, const Tensor &position, const Tensor &offsets, const std::optional<Tensor> &weights_) {
@@ -399,12 +473,23 @@ std::optional<Tensor> combine(const Tensor &rows, const Tensor &position, const 
         rows.size(1) < 1 || position.size(1) < 1)
         return std::nullopt;
     if (weights.defined() && !like(weights, at::kFloat, rows, position.sizes())) return std::nullopt;
+    refuse_tangents("combine", {&rows, &weights});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(rows.device());
-    if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.defined() && weights.requires_grad()))) {
-        refuse_foreign_nodes("combine", {&rows, &weights});
-        return Combine::apply(rows, weights_, position, offsets);
+    const bool train = at::GradMode::is_enabled() && (rows.requires_grad() || (weights.defined() && weights.requires_grad()));
+    if (train) refuse_foreign_nodes("combine", {&rows, &weights});
+    const Tensor y = run_combine(rows, position, offsets, weights);
+    if (train) {
+        const auto node = node_with_edges<CombineNode>(rows, weights);
+        torch::autograd::set_history(y, node);
+        node->weighted = weights.defined();
+        if (weights.defined()) {  // the rows themselves are needed for the weights' gradient only
+            node->rows_ = SavedVariable(rows, false);
+            node->weights_ = SavedVariable(weights, false);
+        }
+        node->position_ = SavedVariable(position, false);
+        node->offsets_ = SavedVariable(offsets, false);
     }
-    return run_combine(rows, position, offsets, weights);
+    return y;
 }
 
 }  // namespace

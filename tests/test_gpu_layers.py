@@ -493,3 +493,41 @@ def test_arguments_of_another_kind_are_never_taken_without_gradient(gpu_device):
     for call in (lambda: linear(x, [1.0]), lambda: linear(x, 3), lambda: linear(x, x, bias="b")):
         with pytest.raises((TypeError, ValueError)):
             call()
+
+
+def test_no_rows_and_only_the_inputs_gradient(gpu_device):
+    x = torch.zeros(0, 8, device=gpu_device, requires_grad=True)
+    w = torch.randn(5, 8, device=gpu_device)
+    dx, = torch.autograd.grad(linear(x, w, activation="gelu"), x, torch.zeros(0, 5, device=gpu_device))
+    assert dx.shape == (0, 8)
+
+
+def test_nodes_behave_like_torchs(gpu_device):
+    """Twice through a graph, kept or not; hooks; a leaf's .grad; undefined gradients; forward mode is refused, not forgotten."""
+    x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(30, 50, 12, 9, torch.float32))
+    for act in (None, "relu", "silu"):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        y = linear(leaves[0], leaves[1], leaves[2], act, leaves[3])
+        assert y.grad_fn is not None and "Linear" in y.grad_fn.name()
+        once = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+        again = torch.autograd.grad(y, leaves, gy)
+        assert all(torch.equal(p, q) for p, q in zip(once, again))
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, leaves, gy)
+        seen = []
+        leaves[1].register_hook(lambda g: seen.append(g.clone()))
+        (linear(leaves[0], leaves[1], leaves[2], act, leaves[3]) * gy).sum().backward()
+        assert len(seen) == 1 and torch.equal(seen[0], leaves[1].grad)
+        assert all(torch.equal(t.grad, g) for t, g in zip(leaves, once))
+        (linear(leaves[0], leaves[1], leaves[2], act, leaves[3]) * gy).sum().backward()  # added to what is there
+        assert all(torch.equal(t.grad, 2 * g) for t, g in zip(leaves, once))
+    y = linear(leaves[0], leaves[1].detach())
+    z = linear(y, torch.ones(4, 9, device=gpu_device))
+    assert leaves[0].grad.add_(1)._version  # small gradients share an allocation: the others are left as they are
+    assert torch.equal(leaves[1].grad, 2 * once[1]) and torch.equal(leaves[2].grad, 2 * once[2])
+    del y
+    z.sum().backward()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            linear(dual, w)
