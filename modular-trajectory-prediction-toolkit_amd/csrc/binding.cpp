@@ -2,8 +2,9 @@
 //
 // A small layer takes a few microseconds on the card; a call through Python takes ten, a backward pass through Python nodes some
 // thirty more.  Here the arguments are looked over, the results allocated and the entry points of mtp_accel.h called without
-// Python between them (forward and backward of a 64 x 96 layer with gelu: 45 us against 68 on one host, 57 on a slower one).  A call whose arguments are not as
-// they have to be returns None: the Python front end then finds out what is wrong and raises.
+// Python between them: a forward and a backward pass of a 64 x 96 layer with gelu take the host 57 us, 35 of which the engine takes
+// for a node that does nothing.  A call whose arguments are not as they have to be returns None: the Python front end then finds
+// out what is wrong and raises.
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
