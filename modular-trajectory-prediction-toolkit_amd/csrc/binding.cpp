@@ -103,6 +103,12 @@ std::shared_ptr<N> node_with_edges(const Inputs &...inputs) {
     return node;
 }
 
+// hooks on saved tensors may give back what they like
+void refuse_other_layouts(const char *what, std::initializer_list<const Tensor *> saved) {
+    for (const Tensor *t : saved)
+        TORCH_CHECK(!t->defined() || t->is_contiguous(), what, ": a saved tensor has come back from its hook with another layout");
+}
+
 // What a backward pass returns can be differentiated no further: trying to says so.  `from`: what it was computed from.
 variable_list no_further(variable_list out, variable_list from, const char *what) {
     if (!at::GradMode::is_enabled()) return out;
@@ -154,6 +160,7 @@ struct LinearNode : Node {
         if (!grads[0].defined()) return variable_list(4);
         const Tensor x = x_.unpack(), w = w_.unpack(), pre = pre_.unpack(getptr()), offsets = offsets_.unpack();
         const Tensor rows = rows_.unpack(), weights = weights_.unpack();
+        refuse_other_layouts("linear", {&w, &pre, &offsets});
         Tensor dx, dw, db, dr;
         {
             at::NoGradGuard off;
@@ -164,7 +171,8 @@ struct LinearNode : Node {
             const int32_t *sets = static_cast<const int32_t *>(at_(offsets));
             if (want_x || want_w) {
                 const Tensor &xs = rows.defined() ? rows : x, &wt = weights.defined() ? weights : w;
-                const int64_t ldx = row_distance(xs), ldw = weights.defined() ? (z.in + 7) / 8 * 8 : z.in;
+                // hooks on saved tensors may have given the copies other distances
+                const int64_t ldx = row_distance(xs), ldw = weights.defined() ? row_distance(weights) : z.in;
                 const int64_t ws_bytes = mtp_linear_backward_workspace_bytes(z.code, z.rows, (int)z.in, (int)z.out, (int)z.sets, z.act,
                                                                              at_(g), at_(wt), ldw, at_(xs), ldx, want_x, want_w);
                 const bool many = offsets.defined();
@@ -287,6 +295,7 @@ struct RouteNode : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
         const Tensor scores = scores_.unpack(), ids = ids_.unpack(), weights = weights_.unpack(getptr()), stats = stats_.unpack();
+        refuse_other_layouts("route_topk", {&ids, &weights, &stats});
         Tensor out;
         {
             at::NoGradGuard off;
@@ -401,6 +410,7 @@ struct DispatchNode : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
         const Tensor position = position_.unpack(), offsets = offsets_.unpack();
+        refuse_other_layouts("dispatch", {&position, &offsets});
         Tensor dx;
         {
             at::NoGradGuard off;
@@ -425,6 +435,7 @@ struct CombineNode : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(2);
         const Tensor rows = rows_.unpack(), weights = weights_.unpack(), position = position_.unpack(), offsets = offsets_.unpack();
+        refuse_other_layouts("combine", {&rows, &weights, &position, &offsets});
         Tensor dr, dw;
         {
             at::NoGradGuard off;

@@ -6,8 +6,8 @@
 //
 // Types float, bfloat16, half; sums are float.  z is kept for the backward pass in the layers' type when there is an
 // activation: one rounding, half a step of the type relative to z, and act' is taken at that point.  dz is rounded once to that type,
-// the one the matrix cores multiply; db is the sum of the same dz.  (In 32 bits each would move twice the bytes: 55 and 80 us of the
-// 890 of 32 768 rows of 2048 -> 2048.)
+// the one the matrix cores multiply; db is the sum of the same dz.  (In 32 bits z would move 270 MB more and dz 400, of the 1.9 GB that
+// 32 768 rows of 2048 -> 2048 move forward and back.)
 #include "linear_kernel.h"
 
 // One or two matrices laid out anew with rows that start where the LDS loads want them (a 16-bit row of odd length starts on 2

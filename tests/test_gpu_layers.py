@@ -3,6 +3,7 @@ import itertools
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import routing_reference as R
 from pccs_accel import kernels as K
@@ -531,3 +532,29 @@ def test_nodes_behave_like_torchs(gpu_device):
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises(RuntimeError, match="forward mode"):
             linear(dual, w)
+
+
+@pytest.mark.parametrize("sizes", [(300, 97, 41), (300, 96, 40), (20, 33, 7)], ids=str)
+def test_hooks_on_saved_tensors(gpu_device, sizes):
+    """Saved tensors that go to the host and come back have other strides than those that went; recomputed ones are new."""
+    for dtype, act in ((torch.float16, "gelu"), (torch.bfloat16, "relu"), (torch.float32, "silu")):
+        x, w, b, r, gy = _inputs(sum(sizes), *sizes, dtype, residual=False)
+        wide = torch.cat([x, x], 1).to(gpu_device)
+        leaves = [wide[:, :sizes[1]].requires_grad_(), w.to(gpu_device).requires_grad_(), b.to(gpu_device).requires_grad_()]
+        want = torch.autograd.grad(linear(*leaves, activation=act), leaves, gy.to(gpu_device))
+        with torch.autograd.graph.save_on_cpu():
+            y = linear(*leaves, activation=act)
+        for got, expected in zip(torch.autograd.grad(y, leaves, gy.to(gpu_device)), want):
+            assert torch.equal(got, expected)
+        y = torch.utils.checkpoint.checkpoint(lambda *a: linear(*a, activation=act), *leaves, use_reentrant=False)
+        for got, expected in zip(torch.autograd.grad(y, leaves, gy.to(gpu_device)), want):
+            assert torch.equal(got, expected)
+
+
+def test_hooks_that_change_a_layout_are_refused(gpu_device):
+    x, w, b, r, gy = (t.to(gpu_device) for t in _inputs(31, 40, 16, 12, torch.float32))
+    w.requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+        y = linear(x, w, b, "gelu")
+    with pytest.raises(RuntimeError, match="another layout"):
+        torch.autograd.grad(y, w, gy)
