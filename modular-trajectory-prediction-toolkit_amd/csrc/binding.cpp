@@ -130,8 +130,16 @@ struct Sizes {
 
 Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, const Tensor &offsets,
                   Tensor *pre, Tensor *laid_out = nullptr) {
-    Tensor y = at::empty({z.rows, z.out}, x.options());
-    if (pre != nullptr) *pre = at::empty({z.rows, z.out}, x.options());
+    Tensor y;
+    const int64_t y_bytes = z.rows * z.out * x.element_size();
+    if (pre != nullptr && y_bytes > 0 && place(y_bytes) + y_bytes <= TOGETHER_BYTES) {
+        const Tensor all = at::empty({place(y_bytes) + y_bytes}, x.options().dtype(at::kByte));
+        y = part_of(all, 0, x.scalar_type(), {z.rows, z.out});
+        *pre = part_of(all, place(y_bytes), x.scalar_type(), {z.rows, z.out});
+    } else {
+        y = at::empty({z.rows, z.out}, x.options());
+        if (pre != nullptr) *pre = at::empty({z.rows, z.out}, x.options());
+    }
     const int64_t ldx = row_distance(x);
     const int64_t bytes = mtp_linear_workspace_bytes(z.code, MTP_LINEAR_FORWARD, z.rows, (int)z.in, (int)z.out, (int)z.sets, at_(x),
                                                      ldx, at_(w), z.in);
@@ -323,16 +331,17 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
     Tensor ids, weights, stats;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        const int64_t bytes = n * k * 4;
-        if (bytes > 0 && bytes <= TOGETHER_BYTES) {
-            const Tensor all = at::empty({place(bytes) + bytes}, scores.options().dtype(at::kByte));
+        const int64_t each = place(n * k * 4), all_bytes = 2 * each + (train ? n * 2 * 4 : 0);
+        if (n > 0 && all_bytes <= TOGETHER_BYTES) {
+            const Tensor all = at::empty({all_bytes}, scores.options().dtype(at::kByte));
             ids = part_of(all, 0, at::kInt, {n, k});
-            weights = part_of(all, place(bytes), at::kFloat, {n, k});
+            weights = part_of(all, each, at::kFloat, {n, k});
+            if (train) stats = part_of(all, 2 * each, at::kFloat, {n, 2});
         } else {
             ids = at::empty({n, k}, scores.options().dtype(at::kInt));
             weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
+            if (train) stats = at::empty({n, 2}, scores.options().dtype(at::kFloat));
         }
-        if (train) stats = at::empty({n, 2}, scores.options().dtype(at::kFloat));
         check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, ld, (int)k, normalize, static_cast<int32_t *>(at_(ids)),
                              static_cast<float *>(at_(weights)), static_cast<float *>(at_(stats)), stream_of(scores)),
               "mtp_route_topk");
@@ -444,8 +453,16 @@ struct CombineNode : Node {
             if (!weighted) {
                 dr = run_dispatch(g, position, offsets);
             } else {
-                if (task_should_compute_output(0)) dr = at::empty_like(rows);
-                if (task_should_compute_output(1)) dw = at::empty_like(weights);
+                const bool want_r = task_should_compute_output(0), want_w = task_should_compute_output(1);
+                const int64_t r_bytes = place(rows.numel() * rows.element_size()), w_bytes = weights.numel() * 4;
+                if (want_r && want_w && w_bytes > 0 && r_bytes + w_bytes <= TOGETHER_BYTES) {
+                    const Tensor all = at::empty({r_bytes + w_bytes}, rows.options().dtype(at::kByte));
+                    dr = part_of(all, 0, rows.scalar_type(), rows.sizes());
+                    dw = part_of(all, r_bytes, at::kFloat, weights.sizes());
+                } else {
+                    if (want_r) dr = at::empty_like(rows);
+                    if (want_w) dw = at::empty_like(weights);
+                }
                 check(mtp_combine_rows_grad(type_code(rows), at_(rows), at_(g), g.size(0), (int)g.size(1), (int)position.size(1),
                                             places(position), held(offsets), static_cast<const float *>(at_(weights)), at_(dr),
                                             static_cast<float *>(at_(dw)), stream_of(g)),
