@@ -271,40 +271,71 @@ int64_t most_parts(int64_t rows, int n_sets, int bits) {
     return (2 * rows) >> bits;
 }
 
+// Up to so many workgroups the two products of a backward pass share a launch, in tiles that leave room for each other on a CU; in
+// launches of their own they have tiles of their own size.  Both products, microseconds in one launch / in two:
+//   bfloat16 2614 rows, 96 -> 200 8.4 / 13.7, 20 000 rows, 96 -> 200 15.7 / 19.9, 4096 rows, 1024 -> 1024 42 / 46; 30 000 rows,
+//   200 -> 200 32.2 / 32.5 (over the limit)
+//   float 2614 rows, 96 -> 200 13.5 / 19.1, 40 000 rows, 64 -> 64 22 / 31, 20 000 rows, 96 -> 96 24 / 23, 8000 rows, 512 -> 512 88 / 85
+//   sets, of whose tiles many are empty: bfloat16 5000 rows over 100, 200 -> 200 15.5 / 19.3, 52 280 over 200, 96 -> 256 29 / 28
+int64_t both_blocks(int n_sets, bool half) { return n_sets > 1 ? 4096 : half ? 2048 : 1024; }
+
 // Outputs larger than this leave past the caches (what is kept for the backward pass always does): 73 568 x 512 floats with gelu
 // and a residual 139 -> 135 us for what is kept, 119 for both.
 constexpr int64_t AWAY_BYTES = 64ll << 20;
+
+// a's tiles of BC columns x BR rows, and the workgroups of NT threads for them
+template <typename T, int MODE, int BC, int BR, int NT>
+int set_tiles(LinArgs *a, int64_t *blocks) {
+    a->col_tiles = (a->cols + BC - 1) / BC;
+    if (MODE == LIN_GRAD_WEIGHT) {
+        a->row_tiles = (a->out_rows + BR - 1) / BR;
+        // of sets at most so many
+        const int64_t pieces = a->offsets == nullptr ? lin_pieces(a->rows, a->part_bits, 1) : (a->rows >> a->part_bits) + a->n_sets;
+        *blocks = a->row_tiles * a->col_tiles * pieces;
+    } else {
+        // a set's last tile may be ragged, and so may the one behind the last set; each has a row
+        a->row_tiles = a->offsets == nullptr ? (a->rows + BR - 1) / BR : (a->rows + (int64_t)(a->n_sets + 1) * (BR - 1)) / BR;
+        if (a->row_tiles > a->rows) a->row_tiles = a->rows;
+        *blocks = a->row_tiles * a->col_tiles;
+        a->away = a->rows * a->cols * (int64_t)sizeof(T) > AWAY_BYTES;
+    }
+    MTP_REQUIRE(*blocks * NT <= 0xffffffffll, "mtp_linear: %lld workgroups are too many", (long long)*blocks);
+    a->tiles = (uint32_t)*blocks;
+    if (MODE != LIN_GRAD_WEIGHT && a->offsets != nullptr && a->n_sets < 512) {  // as many workgroups as have a place
+        int cus = 0;
+        const int rc = mtp_device_cu_count(&cus);
+        if (rc != MTP_OK) return rc;
+        const int64_t places = (int64_t)cus * lin_waves(BC, BR, NT) * 256 / NT;
+        if (*blocks > places) *blocks = places;
+    }
+    return MTP_OK;
+}
 
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
 int launch_tile(LinArgs a, hipStream_t s) {
     constexpr int NT = 64 * (BC / WC) * (BR / WR);
     constexpr int LDS = 2 * (BC + BR) * 128;
-    a.col_tiles = (a.cols + BC - 1) / BC;
     int64_t blocks;
-    if (MODE == LIN_GRAD_WEIGHT) {
-        a.row_tiles = (a.out_rows + BR - 1) / BR;
-        // of sets at most so many
-        const int64_t pieces = a.offsets == nullptr ? lin_pieces(a.rows, a.part_bits, 1) : (a.rows >> a.part_bits) + a.n_sets;
-        blocks = a.row_tiles * a.col_tiles * pieces;
-    } else {
-        // a set's last tile may be ragged, and so may the one behind the last set; each has a row
-        a.row_tiles = a.offsets == nullptr ? (a.rows + BR - 1) / BR : (a.rows + (int64_t)(a.n_sets + 1) * (BR - 1)) / BR;
-        if (a.row_tiles > a.rows) a.row_tiles = a.rows;
-        blocks = a.row_tiles * a.col_tiles;
-        a.away = a.rows * a.cols * (int64_t)sizeof(T) > AWAY_BYTES;
-    }
-    MTP_REQUIRE(blocks * NT <= 0xffffffffll, "mtp_linear: %lld workgroups are too many", (long long)blocks);
-    if (blocks == 0) return MTP_OK;
+    const int rc = set_tiles<T, MODE, BC, BR, NT>(&a, &blocks);
+    if (rc != MTP_OK || blocks == 0) return rc;
     MTP_SET_MAX_LDS_ONCE((k_linear_tile<T, MODE, BC, BR, WC, WR>), LDS);
-    a.tiles = (uint32_t)blocks;
-    if (MODE != LIN_GRAD_WEIGHT && a.offsets != nullptr && a.n_sets < 512) {  // as many workgroups as have a place
-        int cus = 0;
-        const int rc = mtp_device_cu_count(&cus);
-        if (rc != MTP_OK) return rc;
-        const int64_t places = (int64_t)cus * lin_waves(BC, BR, NT) * 256 / NT;
-        if (blocks > places) blocks = places;
-    }
     hipLaunchKernelGGL((k_linear_tile<T, MODE, BC, BR, WC, WR>), dim3((unsigned)blocks), dim3(NT), LDS, s, a);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
+}
+
+// Both products of a backward pass in one launch, if they are small; *done says whether.
+template <typename T, int BC, int BR>
+int launch_both(LinArgs input, LinArgs weight, bool *done, hipStream_t s) {
+    constexpr int LDS = 2 * (BC + BR > 128 ? BC + BR : 128) * 128;
+    int64_t input_blocks, weight_blocks;
+    int rc = set_tiles<T, LIN_GRAD_INPUT, BC, BR, 256>(&input, &input_blocks);
+    if (rc == MTP_OK) rc = set_tiles<T, LIN_GRAD_WEIGHT, 64, 64, 256>(&weight, &weight_blocks);
+    *done = rc == MTP_OK && input_blocks + weight_blocks <= both_blocks(input.n_sets, sizeof(T) == 2);
+    if (!*done) return rc;
+    MTP_SET_MAX_LDS_ONCE((k_linear_both<T, BC, BR>), LDS);
+    hipLaunchKernelGGL((k_linear_both<T, BC, BR>), dim3((unsigned)(input_blocks + weight_blocks)), dim3(256), LDS, s, input, weight,
+                       (uint32_t)input_blocks);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -402,11 +433,8 @@ BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets,
     return p;
 }
 
-template <typename T>
-int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, int64_t ldw, const int32_t *offsets,
-               int n_sets, void *dx, char *ws, hipStream_t s) {
-    const int rc = relayout<T>(&dz, &lddz, rows, out, &w, &ldw, (int64_t)n_sets * out, in, &ws, s);
-    if (rc != MTP_OK) return rc;
+LinArgs input_args(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, int64_t ldw, const int32_t *offsets,
+                   int n_sets, void *dx) {
     LinArgs a{};
     a.P = LinOperand{w, ldw, (int64_t)out * ldw};
     a.Q = LinOperand{dz, lddz, 0};
@@ -416,14 +444,10 @@ int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *
     a.offsets = offsets;
     a.n_sets = n_sets;
     a.out = dx;
-    return launch_product<T, LIN_GRAD_INPUT>(a, s);
+    return a;
 }
-
-template <typename T>
-int grad_weight(const void *dz, int64_t rows, int out, int64_t lddz, const void *x, int in, int64_t ldx, const int32_t *offsets,
-                int n_sets, void *dw, void *db, char *ws, hipStream_t s) {
-    int rc = relayout<T>(&dz, &lddz, rows, out, &x, &ldx, rows, in, &ws, s);
-    if (rc != MTP_OK) return rc;
+LinArgs weight_args(bool half, const void *dz, int64_t rows, int out, int64_t lddz, const void *x, int in, int64_t ldx,
+                    const int32_t *offsets, int n_sets, void *dw, void *db, char *ws) {
     LinArgs a{};
     a.P = LinOperand{x, ldx, 0};
     a.Q = LinOperand{dz, lddz, 0};
@@ -433,24 +457,66 @@ int grad_weight(const void *dz, int64_t rows, int out, int64_t lddz, const void 
     a.offsets = offsets;
     a.n_sets = n_sets;
     a.k = (int)rows;
-    a.part_bits = part_bits_for(rows, in, out, n_sets, sizeof(T) == 2);
-    const int64_t parts = most_parts(rows, n_sets, a.part_bits);
+    a.part_bits = part_bits_for(rows, in, out, n_sets, half);
+    a.parts = most_parts(rows, n_sets, a.part_bits);
     a.out = dw;
     a.bias_out = db;
     a.partial = reinterpret_cast<float *>(ws);
-    a.partial_bias = a.partial + parts * out * in;
-    a.parts = parts;
-    rc = launch_product<T, LIN_GRAD_WEIGHT>(a, s);
-    if (rc != MTP_OK || parts == 0) return rc;
-    const int64_t all = (int64_t)out * (in + 1);
-    if (n_sets == 1 && parts >= 32)
+    a.partial_bias = a.partial + a.parts * out * in;
+    return a;
+}
+// the weight gradient's parts, if it has any
+template <typename T>
+int join_parts(const LinArgs &a, hipStream_t s) {
+    if (a.parts == 0) return MTP_OK;
+    const int64_t all = (int64_t)a.out_rows * (a.cols + 1);
+    if (a.n_sets == 1 && a.parts >= 32)
         hipLaunchKernelGGL((k_linear_join<T, 16>), dim3((unsigned)((all + 63) / 64), 1), dim3(256), 0, s, a);
-    else if (n_sets == 1 && parts >= 8)
+    else if (a.n_sets == 1 && a.parts >= 8)
         hipLaunchKernelGGL((k_linear_join<T, 4>), dim3((unsigned)((all + 255) / 256), 1), dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((k_linear_join<T, 1>), dim3((unsigned)((all + 1023) / 1024), (unsigned)n_sets), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_linear_join<T, 1>), dim3((unsigned)((all + 1023) / 1024), (unsigned)a.n_sets), dim3(256), 0, s, a);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
+}
+
+template <typename T>
+int grad_input(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int in, const int32_t *offsets, int n_sets,
+               void *dx, char *ws, hipStream_t s) {
+    int64_t ldw = in;
+    const int rc = relayout<T>(&dz, &lddz, rows, out, &w, &ldw, (int64_t)n_sets * out, in, &ws, s);
+    if (rc != MTP_OK) return rc;
+    return launch_product<T, LIN_GRAD_INPUT>(input_args(dz, rows, out, lddz, w, in, ldw, offsets, n_sets, dx), s);
+}
+
+template <typename T>
+int grad_weight(const void *dz, int64_t rows, int out, int64_t lddz, const void *x, int in, int64_t ldx, const int32_t *offsets,
+                int n_sets, void *dw, void *db, char *ws, hipStream_t s) {
+    int rc = relayout<T>(&dz, &lddz, rows, out, &x, &ldx, rows, in, &ws, s);
+    if (rc != MTP_OK) return rc;
+    const LinArgs a = weight_args(sizeof(T) == 2, dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db, ws);
+    rc = launch_product<T, LIN_GRAD_WEIGHT>(a, s);
+    return rc != MTP_OK ? rc : join_parts<T>(a, s);
+}
+
+// both from operands that need no new layout
+template <typename T>
+int grad_both(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int64_t ldw, const void *x, int in, int64_t ldx,
+              const int32_t *offsets, int n_sets, void *dx, void *dw, void *db, char *ws, hipStream_t s) {
+    const LinArgs input = input_args(dz, rows, out, lddz, w, in, ldw, offsets, n_sets, dx);
+    const LinArgs weight = weight_args(sizeof(T) == 2, dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db, ws);
+    bool done = false;
+    int rc = MTP_OK;
+    if (dx != nullptr && dw != nullptr && rows > 0) {
+        rc = n_sets > 1 || rows < 128 ? launch_both<T, 64, 64>(input, weight, &done, s) : launch_both<T, 32, 128>(input, weight, &done, s);
+        if (rc != MTP_OK) return rc;
+    }
+    if (!done) {
+        if (dx != nullptr && rows > 0) rc = launch_product<T, LIN_GRAD_INPUT>(input, s);
+        if (rc == MTP_OK && dw != nullptr) rc = launch_product<T, LIN_GRAD_WEIGHT>(weight, s);
+        if (rc != MTP_OK) return rc;
+    }
+    return dw != nullptr ? join_parts<T>(weight, s) : rc;
 }
 
 }  // namespace
@@ -544,7 +610,7 @@ extern "C" int mtp_linear_grad_input(int dtype, const void *dz, int64_t rows, in
         mtp_set_error("mtp_linear_grad_input: workspace of %zu bytes, needs %lld on a 16-byte boundary", ws_bytes, (long long)need);
         return MTP_E_WORKSPACE;
     }
-    return MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, in, offsets, n_sets, dx, reinterpret_cast<char *>(ws),
+    return MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, offsets, n_sets, dx, reinterpret_cast<char *>(ws),
                                           mtp_stream(stream));
 }
 
@@ -606,10 +672,5 @@ extern "C" int mtp_linear_backward(int dtype, const void *g, const void *pre, in
                                           &at, s);
         if (rc != MTP_OK) return rc;
     }
-    if (dx != nullptr && rows > 0) {
-        rc = MTP_BY_TYPE(dtype, grad_input)(dz, rows, out, lddz, w, in, ldw, offsets, n_sets, dx, at, s);
-        if (rc != MTP_OK) return rc;
-    }
-    if (dw != nullptr) rc = MTP_BY_TYPE(dtype, grad_weight)(dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db, at, s);
-    return rc;
+    return MTP_BY_TYPE(dtype, grad_both)(dz, rows, out, lddz, w, ldw, x, in, ldx, offsets, n_sets, dx, dw, db, at, s);
 }

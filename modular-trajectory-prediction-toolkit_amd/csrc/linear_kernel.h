@@ -613,13 +613,12 @@ constexpr int lin_waves(int bc, int br, int threads) {
 // some 25 vector instructions an element and 74 MB).  float: the matrix cores (73 568 rows, 512 -> 96: 75 us, 96 TFLOP/s; 153 in a
 // large library product).
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
-__global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * (BC / WC) * (BR / WR))) void k_linear_tile(LinArgs a) {
+__device__ __forceinline__ void lin_tile(const LinArgs &a, uint32_t block, uint32_t blocks, char *smem) {
     constexpr int NT = 64 * (BC / WC) * (BR / WR);
     constexpr bool PKC = MODE == LIN_FORWARD, QKC = MODE != LIN_GRAD_WEIGHT;
     constexpr int SZ = sizeof(T), BK = 128 / SZ;
     constexpr int FC = WC / 32, FR = WR / 32;
     constexpr int P_BYTES = BC * 128, STAGE = (BC + BR) * 128;
-    extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 * STAGE
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wc = wave % (BC / WC), wr = wave / (BC / WC);
@@ -627,7 +626,7 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
     // How many tiles there are of up to 511 sets is known here only.  Forward and input gradient: a workgroup takes several that follow
     // each other, so that it looks the sets up once (143 760 rows over 400, 96 -> 256: 1.5 of the 6 us that a tile took were that).
     // Weight gradient: a run of them for each XCD (numbered over the whole grid the last XCD would have the empty ones).
-    uint32_t left = 1, id = blockIdx.x;
+    uint32_t left = 1, id = block;
     int ct = 0;
     LinPiece p{0, 1, 0, 0, a.rows, 0};
     if (a.offsets != nullptr && a.n_sets < 512) {
@@ -641,10 +640,10 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
             if (id >= tiles) return;
             id = lin_xcd_order(id, tiles);
         } else {
-            id = lin_xcd_order(id, gridDim.x);
-            const uint32_t per = tiles / gridDim.x, more = tiles % gridDim.x;
-            const uint32_t first = id * per + id * more / gridDim.x;
-            left = (id + 1) * per + (id + 1) * more / gridDim.x - first;
+            id = lin_xcd_order(id, blocks);
+            const uint32_t per = tiles / blocks, more = tiles % blocks;
+            const uint32_t first = id * per + id * more / blocks;
+            left = (id + 1) * per + (id + 1) * more / blocks - first;
             id = first;
         }
         ct = (int)(id % (uint32_t)a.col_tiles);
@@ -887,6 +886,22 @@ __global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * 
         }
     }
     }
+}
+
+template <typename T, int MODE, int BC, int BR, int WC, int WR>
+__global__ __launch_bounds__(64 * (BC / WC) * (BR / WR), lin_waves(BC, BR, 64 * (BC / WC) * (BR / WR))) void k_linear_tile(LinArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char tile_lds[];  // 2 * (BC + BR) * 128
+    lin_tile<T, MODE, BC, BR, WC, WR>(a, blockIdx.x, gridDim.x, tile_lds);
+}
+
+// Both products of a small backward pass side by side: `input_blocks` workgroups for the input gradient (BC x BR tiles), the others for
+// the weight gradient (64 x 64).
+template <typename T, int BC, int BR>
+__global__ __launch_bounds__(256, 4) void k_linear_both(LinArgs input, LinArgs weight, uint32_t input_blocks) {
+    extern __shared__ __attribute__((aligned(16))) char both_lds[];
+    static_assert((BC / 32) * (BR / 32) == 4, "four waves");
+    if (blockIdx.x < input_blocks) lin_tile<T, LIN_GRAD_INPUT, BC, BR, 32, 32>(input, blockIdx.x, input_blocks, both_lds);
+    else lin_tile<T, LIN_GRAD_WEIGHT, 64, 64, 32, 32>(weight, blockIdx.x - input_blocks, gridDim.x - input_blocks, both_lds);
 }
 
 // ---- few rows ----
