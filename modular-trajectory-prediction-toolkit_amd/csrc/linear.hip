@@ -276,8 +276,9 @@ int64_t most_parts(int64_t rows, int n_sets, int bits) {
 //   bfloat16 2614 rows, 96 -> 200 8.4 / 13.7, 20 000 rows, 96 -> 200 15.7 / 19.9, 4096 rows, 1024 -> 1024 42 / 46; 30 000 rows,
 //   200 -> 200 32.2 / 32.5 (over the limit)
 //   float 2614 rows, 96 -> 200 13.5 / 19.1, 40 000 rows, 64 -> 64 22 / 31, 20 000 rows, 96 -> 96 24 / 23, 8000 rows, 512 -> 512 88 / 85
-//   sets, of whose tiles many are empty: bfloat16 5000 rows over 100, 200 -> 200 15.5 / 19.3, 52 280 over 200, 96 -> 256 29 / 28
-int64_t both_blocks(int n_sets, bool half) { return n_sets > 1 ? 4096 : half ? 2048 : 1024; }
+//   sets, of whose tiles many are empty: bfloat16 5000 rows over 100, 200 -> 200 15.5 / 19.3 (2372 workgroups), 20 000 over 300,
+//   256 -> 24 17.8 / 19.6 (2300), 52 280 over 200, 96 -> 256 29.3 / 28.1 (3032)
+int64_t both_blocks(int n_sets, bool half) { return n_sets > 1 ? 2560 : half ? 2048 : 1024; }
 
 // Outputs larger than this leave past the caches (what is kept for the backward pass always does): 73 568 x 512 floats with gelu
 // and a residual 139 -> 135 us for what is kept, 119 for both.
