@@ -330,8 +330,8 @@ struct LinSets {
 // Piece number `piece`, counted set after set (`last`: number of the last set; the rows behind the sets are "set" n_sets).  Every
 // wave finds it for itself.
 template <bool CUT>
-__device__ __forceinline__ bool lin_find(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least, int64_t piece,
-                                         LinPiece *out) {
+__device__ __forceinline__ bool lin_find(const int32_t *offsets, int n_sets, int last, int64_t rows, int part_bits, int least,
+                                         int64_t piece, LinPiece *out) {
     int64_t before = 0, split_before = 0;
     for (int e0 = 0; e0 <= last; e0 += 512) {
         LinSets<CUT> sets;
@@ -667,224 +667,224 @@ __device__ __forceinline__ void lin_tile(const LinArgs &a, uint32_t block, uint3
         }
     }
     for (bool again = false; left > 0; --left, again = true) {
-    int tid_here = tid;
-    asm volatile("" : "+v"(tid_here));  // what follows from it is found anew for each tile: there are no registers to keep it in
-    if (again) {
-        __syncthreads();  // the last tile has left LDS
-        if (++ct == (int)a.col_tiles) {
-            ct = 0;
-            lin_next(a.offsets, a.n_sets, a.rows, lin_log2(BR), &p);
-            if (p.set > a.n_sets) return;
-        }
-    }
-    int64_t row0 = 0, row_end = 0, k_lo = 0, k_len = a.k, part_at = -1;
-    const int64_t c0 = (int64_t)ct * BC;
-    if constexpr (MODE == LIN_GRAD_WEIGHT) {
-        row0 = (int64_t)(id % (uint32_t)a.row_tiles) * BR;
-        row_end = a.out_rows;
-        k_lo = p.lo + (p.index << a.part_bits);
-        k_len = p.hi - k_lo < (1 << a.part_bits) ? p.hi - k_lo : (int64_t)1 << a.part_bits;
-        if (p.count > 1) {
-            part_at = p.split_at + p.index;
-            if (part_at >= a.parts) return;  // offsets that overlap: more parts than there can be
-        }
-    } else {
-        row0 = p.lo + p.index * BR;
-        row_end = p.hi;
-    }
-    const int set = p.set;
-    T *out = reinterpret_cast<T *>(a.out);
-    if (MODE != LIN_GRAD_WEIGHT && set == a.n_sets) {  // rows behind the last set
-        for (int i = tid; i < BR * BC; i += NT) {
-            const int64_t r = row0 + i / BC, c = c0 + i % BC;
-            if (r < row_end && c < a.cols) {
-                out[r * a.cols + c] = (T)0.f;
-                if (MODE == LIN_FORWARD && a.pre != nullptr) reinterpret_cast<T *>(a.pre)[r * a.cols + c] = (T)0.f;
+        int tid_here = tid;
+        asm volatile("" : "+v"(tid_here));  // what follows from it is found anew for each tile: there are no registers to keep it in
+        if (again) {
+            __syncthreads();  // the last tile has left LDS
+            if (++ct == (int)a.col_tiles) {
+                ct = 0;
+                lin_next(a.offsets, a.n_sets, a.rows, lin_log2(BR), &p);
+                if (p.set > a.n_sets) return;
             }
         }
-        continue;
-    }
-
-    // operand windows: first element, bytes to the last element that counts, bytes per step along k
-    const T *p_at = reinterpret_cast<const T *>(a.P.base) + set * a.P.group;
-    const T *q_at = reinterpret_cast<const T *>(a.Q.base) + set * a.Q.group;
-    int64_t p_left, q_left, p_step, q_step;
-    if constexpr (PKC) {
-        const int64_t n = a.cols - c0 < BC ? a.cols - c0 : BC;
-        p_at += c0 * a.P.ld;
-        p_left = ((n - 1) * a.P.ld + k_len) * SZ;
-        p_step = 128;
-    } else {
-        p_at += k_lo * a.P.ld + c0;
-        p_left = k_len > 0 ? ((k_len - 1) * a.P.ld + a.cols - c0) * SZ : 0;
-        p_step = (int64_t)BK * a.P.ld * SZ;
-    }
-    const int64_t n_rows = row_end - row0 < BR ? row_end - row0 : BR;
-    if constexpr (QKC) {
-        q_at += row0 * a.Q.ld;
-        q_left = ((n_rows - 1) * a.Q.ld + k_len) * SZ;
-        q_step = 128;
-    } else {
-        q_at += k_lo * a.Q.ld + row0;
-        q_left = k_len > 0 ? ((k_len - 1) * a.Q.ld + row_end - row0) * SZ : 0;
-        q_step = (int64_t)BK * a.Q.ld * SZ;
-    }
-    LinTile<T, PKC, BC, NT> tp;
-    LinTile<T, QKC, BR, NT> tq;
-    tp.init(a.P.ld, tid_here);
-    tq.init(a.Q.ld, tid_here);
-    LinReader<T, PKC, BC> rp;
-    LinReader<T, QKC, BR> rq;
-    rp.init(wc * WC, tid_here & 63);
-    rq.init(wr * WR, tid_here & 63);
-    f32x16v acc[FC][FR];
-    f32x16v acc_ones[MODE == LIN_GRAD_WEIGHT ? FR : 1];
-#pragma unroll
-    for (int c = 0; c < FC; ++c)
-#pragma unroll
-        for (int r = 0; r < FR; ++r)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[c][r][e] = 0.f;
-    const bool sum_q = MODE == LIN_GRAD_WEIGHT && a.bias_out != nullptr && ct == 0 && wc == 0;
-    if constexpr (MODE == LIN_GRAD_WEIGHT) {
-#pragma unroll
-        for (int r = 0; r < FR; ++r)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc_ones[r][e] = 0.f;
-    }
-
-    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-    const int64_t n_steps = (k_len + BK - 1) / BK;
-    int64_t k_left = k_len;
-    auto fetch_p = [&](int buf) {
-        const unsigned l = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(buf * STAGE));
-        tp.load(make_rsrc(p_at, p_left), k_left, l, wave);
-        p_at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(p_at) + p_step);
-        p_left -= p_step;
-    };
-    auto fetch_q = [&](int buf) {
-        const unsigned l = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(buf * STAGE));
-        tq.load(make_rsrc(q_at, q_left), k_left, l + P_BYTES, wave);
-        q_at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(q_at) + q_step);
-        q_left -= q_step;
-        k_left -= BK;
-    };
-    auto fetch = [&](int buf) {
-        fetch_p(buf);
-        fetch_q(buf);
-    };
-    // Big tiles have one workgroup a CU: its loads are sent in two halves, between products, as eight in a row keep a wave from
-    // its products until they have been taken (32 768 rows, 2048 -> 2048: input gradient 257 -> 250 us, weight gradient 365 -> 340;
-    // 128x128 tiles, two a CU, 314 -> 326).
-    constexpr bool HALVES = BC == 256;
-    // both buffers are on their way before the first is used; later tiles are fetched one ahead
-    constexpr int IN_FLIGHT = LinTile<T, PKC, BC, NT>::PER + LinTile<T, QKC, BR, NT>::PER;
-    if (n_steps > 0) fetch(0);
-    if (n_steps > 1) fetch(1);
-    for (int64_t t = 0; t < n_steps; ++t) {
-        if (t == 0 && n_steps > 1) dma_wait<IN_FLIGHT>();
-        else dma_wait_all();
-        __syncthreads();  // tile t has landed for every wave, and nobody reads the other buffer any more
-        const bool more = t > 0 && t + 1 < n_steps;
-        if (more) {
-            if constexpr (HALVES) fetch_p((int)((t + 1) & 1));
-            else fetch((int)((t + 1) & 1));
-        }
-        char *buf = smem + (t & 1) * STAGE;
-        const int64_t left = k_len - t * BK;
-        if constexpr (PKC || QKC) {
-            if (left < BK && left % (16 / SZ) != 0) {
-                if constexpr (PKC) LinTile<T, true, BC, NT>::clear_tail(buf, (int)left, tid);
-                if constexpr (QKC) LinTile<T, true, BR, NT>::clear_tail(buf + P_BYTES, (int)left, tid);
-                __syncthreads();
+        int64_t row0 = 0, row_end = 0, k_lo = 0, k_len = a.k, part_at = -1;
+        const int64_t c0 = (int64_t)ct * BC;
+        if constexpr (MODE == LIN_GRAD_WEIGHT) {
+            row0 = (int64_t)(id % (uint32_t)a.row_tiles) * BR;
+            row_end = a.out_rows;
+            k_lo = p.lo + (p.index << a.part_bits);
+            k_len = p.hi - k_lo < (1 << a.part_bits) ? p.hi - k_lo : (int64_t)1 << a.part_bits;
+            if (p.count > 1) {
+                part_at = p.split_at + p.index;
+                if (part_at >= a.parts) return;  // offsets that overlap: more parts than there can be
             }
+        } else {
+            row0 = p.lo + p.index * BR;
+            row_end = p.hi;
         }
+        const int set = p.set;
+        T *out = reinterpret_cast<T *>(a.out);
+        if (MODE != LIN_GRAD_WEIGHT && set == a.n_sets) {  // rows behind the last set
+            for (int i = tid; i < BR * BC; i += NT) {
+                const int64_t r = row0 + i / BC, c = c0 + i % BC;
+                if (r < row_end && c < a.cols) {
+                    out[r * a.cols + c] = (T)0.f;
+                    if (MODE == LIN_FORWARD && a.pre != nullptr) reinterpret_cast<T *>(a.pre)[r * a.cols + c] = (T)0.f;
+                }
+            }
+            continue;
+        }
+
+        // operand windows: first element, bytes to the last element that counts, bytes per step along k
+        const T *p_at = reinterpret_cast<const T *>(a.P.base) + set * a.P.group;
+        const T *q_at = reinterpret_cast<const T *>(a.Q.base) + set * a.Q.group;
+        int64_t p_left, q_left, p_step, q_step;
+        if constexpr (PKC) {
+            const int64_t n = a.cols - c0 < BC ? a.cols - c0 : BC;
+            p_at += c0 * a.P.ld;
+            p_left = ((n - 1) * a.P.ld + k_len) * SZ;
+            p_step = 128;
+        } else {
+            p_at += k_lo * a.P.ld + c0;
+            p_left = k_len > 0 ? ((k_len - 1) * a.P.ld + a.cols - c0) * SZ : 0;
+            p_step = (int64_t)BK * a.P.ld * SZ;
+        }
+        const int64_t n_rows = row_end - row0 < BR ? row_end - row0 : BR;
+        if constexpr (QKC) {
+            q_at += row0 * a.Q.ld;
+            q_left = ((n_rows - 1) * a.Q.ld + k_len) * SZ;
+            q_step = 128;
+        } else {
+            q_at += k_lo * a.Q.ld + row0;
+            q_left = k_len > 0 ? ((k_len - 1) * a.Q.ld + row_end - row0) * SZ : 0;
+            q_step = (int64_t)BK * a.Q.ld * SZ;
+        }
+        LinTile<T, PKC, BC, NT> tp;
+        LinTile<T, QKC, BR, NT> tq;
+        tp.init(a.P.ld, tid_here);
+        tq.init(a.Q.ld, tid_here);
+        LinReader<T, PKC, BC> rp;
+        LinReader<T, QKC, BR> rq;
+        rp.init(wc * WC, tid_here & 63);
+        rq.init(wr * WR, tid_here & 63);
+        f32x16v acc[FC][FR];
+        f32x16v acc_ones[MODE == LIN_GRAD_WEIGHT ? FR : 1];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (HALVES && s == 1 && more) fetch_q((int)((t + 1) & 1));
-            typename LinMfma<T>::frag fp[FC], fq[FR];
+        for (int c = 0; c < FC; ++c)
 #pragma unroll
-            for (int c = 0; c < FC; ++c) fp[c] = rp.read(buf, c, s);
+            for (int r = 0; r < FR; ++r)
 #pragma unroll
-            for (int r = 0; r < FR; ++r) fq[r] = rq.read(buf + P_BYTES, r, s);
+                for (int e = 0; e < 16; ++e) acc[c][r][e] = 0.f;
+        const bool sum_q = MODE == LIN_GRAD_WEIGHT && a.bias_out != nullptr && ct == 0 && wc == 0;
+        if constexpr (MODE == LIN_GRAD_WEIGHT) {
 #pragma unroll
-            for (int c = 0; c < FC; ++c)
+            for (int r = 0; r < FR; ++r)
 #pragma unroll
-                for (int r = 0; r < FR; ++r) acc[c][r] = LinMfma<T>::mul(fp[c], fq[r], acc[c][r]);
-            if constexpr (MODE == LIN_GRAD_WEIGHT) {
-                if (sum_q) {
+                for (int e = 0; e < 16; ++e) acc_ones[r][e] = 0.f;
+        }
+
+        const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+        const int64_t n_steps = (k_len + BK - 1) / BK;
+        int64_t k_left = k_len;
+        auto fetch_p = [&](int buf) {
+            const unsigned l = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(buf * STAGE));
+            tp.load(make_rsrc(p_at, p_left), k_left, l, wave);
+            p_at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(p_at) + p_step);
+            p_left -= p_step;
+        };
+        auto fetch_q = [&](int buf) {
+            const unsigned l = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(buf * STAGE));
+            tq.load(make_rsrc(q_at, q_left), k_left, l + P_BYTES, wave);
+            q_at = reinterpret_cast<const T *>(reinterpret_cast<const char *>(q_at) + q_step);
+            q_left -= q_step;
+            k_left -= BK;
+        };
+        auto fetch = [&](int buf) {
+            fetch_p(buf);
+            fetch_q(buf);
+        };
+        // Big tiles have one workgroup a CU: its loads are sent in two halves, between products, as eight in a row keep a wave from
+        // its products until they have been taken (32 768 rows, 2048 -> 2048: input gradient 257 -> 250 us, weight gradient 365 -> 340;
+        // 128x128 tiles, two a CU, 314 -> 326).
+        constexpr bool HALVES = BC == 256;
+        // both buffers are on their way before the first is used; later tiles are fetched one ahead
+        constexpr int IN_FLIGHT = LinTile<T, PKC, BC, NT>::PER + LinTile<T, QKC, BR, NT>::PER;
+        if (n_steps > 0) fetch(0);
+        if (n_steps > 1) fetch(1);
+        for (int64_t t = 0; t < n_steps; ++t) {
+            if (t == 0 && n_steps > 1) dma_wait<IN_FLIGHT>();
+            else dma_wait_all();
+            __syncthreads();  // tile t has landed for every wave, and nobody reads the other buffer any more
+            const bool more = t > 0 && t + 1 < n_steps;
+            if (more) {
+                if constexpr (HALVES) fetch_p((int)((t + 1) & 1));
+                else fetch((int)((t + 1) & 1));
+            }
+            char *buf = smem + (t & 1) * STAGE;
+            const int64_t left = k_len - t * BK;
+            if constexpr (PKC || QKC) {
+                if (left < BK && left % (16 / SZ) != 0) {
+                    if constexpr (PKC) LinTile<T, true, BC, NT>::clear_tail(buf, (int)left, tid);
+                    if constexpr (QKC) LinTile<T, true, BR, NT>::clear_tail(buf + P_BYTES, (int)left, tid);
+                    __syncthreads();
+                }
+            }
 #pragma unroll
-                    for (int r = 0; r < FR; ++r) {
-                        if constexpr (SZ == 4) {  // a matrix instruction would cost as much as one of the product's
+            for (int s = 0; s < 4; ++s) {
+                if (HALVES && s == 1 && more) fetch_q((int)((t + 1) & 1));
+                typename LinMfma<T>::frag fp[FC], fq[FR];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc_ones[r][0] += fq[r][e];
-                        } else {
-                            acc_ones[r] = LinMfma<T>::mul(LinMfma<T>::ones(), fq[r], acc_ones[r]);
+                for (int c = 0; c < FC; ++c) fp[c] = rp.read(buf, c, s);
+#pragma unroll
+                for (int r = 0; r < FR; ++r) fq[r] = rq.read(buf + P_BYTES, r, s);
+#pragma unroll
+                for (int c = 0; c < FC; ++c)
+#pragma unroll
+                    for (int r = 0; r < FR; ++r) acc[c][r] = LinMfma<T>::mul(fp[c], fq[r], acc[c][r]);
+                if constexpr (MODE == LIN_GRAD_WEIGHT) {
+                    if (sum_q) {
+#pragma unroll
+                        for (int r = 0; r < FR; ++r) {
+                            if constexpr (SZ == 4) {  // a matrix instruction would cost as much as one of the product's
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc_ones[r][0] += fq[r][e];
+                            } else {
+                                acc_ones[r] = LinMfma<T>::mul(LinMfma<T>::ones(), fq[r], acc_ones[r]);
+                            }
                         }
                     }
                 }
             }
         }
-    }
 
-    // ---- epilogue ----
-    // lane (i, h) holds row i of a fragment, columns 8 g + 4 h + 0..3 for g = 0..3: stored from there a wave would touch 32 rows
-    // with 16 bytes each.  The sums go through LDS (as floats, pieces of 16 bytes placed at p ^ row so that neither side
-    // conflicts), and whole rows of the tile leave in 16-byte pieces; bias, activation and residual are applied on the way.
-    asm volatile("" : "+v"(tid_here));
-    const int lane_here = tid_here & 63, i = lane_here & 31, h = lane_here >> 5;
-    constexpr int ER = lin_pass_rows(2 * STAGE / (BC * 4), BR);  // rows per pass
-    constexpr int PM = lin_twist_mask(BC / 4);
-    static_assert(BR % ER == 0 && ER % WR == 0, "a wave's rows are in one pass");
-    float *z = reinterpret_cast<float *>(smem);
-    const bool to_partial = MODE == LIN_GRAD_WEIGHT && part_at >= 0;
-    float bias[16 / SZ];
-    if constexpr (MODE == LIN_FORWARD) lin_bias<T, BC>(a, set, c0, tid_here, bias);
-    for (int p0 = 0; p0 < BR; p0 += ER) {
-        __syncthreads();
-        if (wr * WR >= p0 && wr * WR < p0 + ER) {
+        // ---- epilogue ----
+        // lane (i, h) holds row i of a fragment, columns 8 g + 4 h + 0..3 for g = 0..3: stored from there a wave would touch 32 rows
+        // with 16 bytes each.  The sums go through LDS (as floats, pieces of 16 bytes placed at p ^ row so that neither side
+        // conflicts), and whole rows of the tile leave in 16-byte pieces; bias, activation and residual are applied on the way.
+        asm volatile("" : "+v"(tid_here));
+        const int lane_here = tid_here & 63, i = lane_here & 31, h = lane_here >> 5;
+        constexpr int ER = lin_pass_rows(2 * STAGE / (BC * 4), BR);  // rows per pass
+        constexpr int PM = lin_twist_mask(BC / 4);
+        static_assert(BR % ER == 0 && ER % WR == 0, "a wave's rows are in one pass");
+        float *z = reinterpret_cast<float *>(smem);
+        const bool to_partial = MODE == LIN_GRAD_WEIGHT && part_at >= 0;
+        float bias[16 / SZ];
+        if constexpr (MODE == LIN_FORWARD) lin_bias<T, BC>(a, set, c0, tid_here, bias);
+        for (int p0 = 0; p0 < BR; p0 += ER) {
+            __syncthreads();
+            if (wr * WR >= p0 && wr * WR < p0 + ER) {
 #pragma unroll
-            for (int c = 0; c < FC; ++c)
+                for (int c = 0; c < FC; ++c)
 #pragma unroll
-                for (int r = 0; r < FR; ++r)
+                    for (int r = 0; r < FR; ++r)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int row = wr * WR - p0 + r * 32 + i;
-                        const int piece = (wc * WC + c * 32 + 8 * g + 4 * h) >> 2;
-                        f32x4v v;
+                        for (int g = 0; g < 4; ++g) {
+                            const int row = wr * WR - p0 + r * 32 + i;
+                            const int piece = (wc * WC + c * 32 + 8 * g + 4 * h) >> 2;
+                            f32x4v v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = acc[c][r][4 * g + e];
-                        *reinterpret_cast<f32x4v *>(z + row * BC + ((piece ^ (row & PM)) << 2)) = v;
+                            for (int e = 0; e < 4; ++e) v[e] = acc[c][r][4 * g + e];
+                            *reinterpret_cast<f32x4v *>(z + row * BC + ((piece ^ (row & PM)) << 2)) = v;
+                        }
+            }
+            __syncthreads();
+            const int64_t r0 = row0 + p0;
+            if (to_partial) {
+                float *part = a.partial + part_at * a.out_rows * a.cols;
+                lin_leave<T, float, MODE, BC, ER, NT>(a, z, bias, part, r0, row_end, c0, tid_here);
+            } else {
+                T *to = out + (MODE == LIN_GRAD_WEIGHT ? (int64_t)set * a.out_rows * a.cols : 0);
+                lin_leave<T, T, MODE, BC, ER, NT>(a, z, bias, to, r0, row_end, c0, tid_here);
+            }
+        }
+        if constexpr (MODE == LIN_GRAD_WEIGHT && SZ == 4) {  // the two halves of a wave hold different k
+            if (sum_q) {
+#pragma unroll
+                for (int r = 0; r < FR; ++r) acc_ones[r][0] += __shfl_xor(acc_ones[r][0], 32);
+            }
+        }
+        if constexpr (MODE == LIN_GRAD_WEIGHT) {
+            if (sum_q && h == 0) {
+#pragma unroll
+                for (int r = 0; r < FR; ++r) {
+                    const int64_t row = row0 + wr * WR + r * 32 + i;
+                    if (row < row_end) {
+                        if (part_at >= 0) a.partial_bias[part_at * a.out_rows + row] = acc_ones[r][0];
+                        else reinterpret_cast<T *>(a.bias_out)[(int64_t)set * a.out_rows + row] = from_f32<T>(acc_ones[r][0]);
                     }
-        }
-        __syncthreads();
-        const int64_t r0 = row0 + p0;
-        if (to_partial) {
-            float *part = a.partial + part_at * a.out_rows * a.cols;
-            lin_leave<T, float, MODE, BC, ER, NT>(a, z, bias, part, r0, row_end, c0, tid_here);
-        } else {
-            T *to = out + (MODE == LIN_GRAD_WEIGHT ? (int64_t)set * a.out_rows * a.cols : 0);
-            lin_leave<T, T, MODE, BC, ER, NT>(a, z, bias, to, r0, row_end, c0, tid_here);
-        }
-    }
-    if constexpr (MODE == LIN_GRAD_WEIGHT && SZ == 4) {  // the two halves of a wave hold different k
-        if (sum_q) {
-#pragma unroll
-            for (int r = 0; r < FR; ++r) acc_ones[r][0] += __shfl_xor(acc_ones[r][0], 32);
-        }
-    }
-    if constexpr (MODE == LIN_GRAD_WEIGHT) {
-        if (sum_q && h == 0) {
-#pragma unroll
-            for (int r = 0; r < FR; ++r) {
-                const int64_t row = row0 + wr * WR + r * 32 + i;
-                if (row < row_end) {
-                    if (part_at >= 0) a.partial_bias[part_at * a.out_rows + row] = acc_ones[r][0];
-                    else reinterpret_cast<T *>(a.bias_out)[(int64_t)set * a.out_rows + row] = from_f32<T>(acc_ones[r][0]);
                 }
             }
         }
-    }
     }
 }
 

@@ -399,8 +399,9 @@ __global__ __launch_bounds__(256) void k_route_grad(const T *__restrict__ scores
 // ---- pairs sorted by modality ----
 // Stable counting sort in three launches, or in one where a single workgroup has all pairs: pairs of each modality per run, prefix
 // over the runs, places.  The ids are read twice, order and position written once (1.47 M pairs over 200: 24 MB, 5 + 9 + 16 us;
-// bound by the way of each round's counts through LDS, not by bytes).  A wave owns a run of pairs and goes through it 64 at a time; lanes with the same modality find each
-// other by ballots over the modality's bits, so a pair's place is (pairs of its modality before this round) + (lanes below).
+// bound by the way of the counts through LDS, not by bytes).  A wave owns a run of pairs and goes through it 64 at a time; lanes
+// with the same modality find each other by ballots over the modality's bits, so a pair's place is (pairs of its modality before
+// these 64) + (lanes below).
 __device__ __forceinline__ int pair_key(int id, int e) { return id >= 0 && id < e ? id : e; }
 
 __device__ __forceinline__ uint64_t same_key_lanes(int key, int bits, bool valid) {
