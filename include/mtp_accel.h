@@ -511,7 +511,8 @@ int mtp_linear_grad_input(int dtype, const void *dz, int64_t rows, int out, int6
 int mtp_linear_grad_weight(int dtype, const void *dz, int64_t rows, int out, int64_t lddz, const void *x, int in, int64_t ldx,
                            const int32_t *offsets, int n_sets, void *dw, void *db, void *ws, size_t ws_bytes, void *stream);
 /* The whole backward pass of mtp_linear in one call: dz = g * act'(pre) (act 0: dz = g, pre is not read), then dx and / or dw
- * (with db) as above; what is NULL is not computed.  g [rows][out] contiguous.  want_x, want_w: dx, dw are not NULL. */
+ * (with db) as above; what is NULL is not computed.  db is the sum of g * act'(pre) before it is rounded to dz.  g [rows][out]
+ * contiguous.  want_x, want_w: dx, dw are not NULL. */
 int64_t mtp_linear_backward_workspace_bytes(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g,
                                             const void *w, int64_t ldw, const void *x, int64_t ldx, int want_x, int want_w);
 int mtp_linear_backward(int dtype, const void *g, const void *pre, int act, const void *x, int64_t rows, int in, int64_t ldx,

@@ -5,9 +5,10 @@
 //   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz
 //
 // Types float, bfloat16, half; sums are float.  z is kept for the backward pass in the layers' type when there is an
-// activation: one rounding, half a step of the type relative to z, and act' is taken at that point.  dz is rounded once to that type,
-// the one the matrix cores multiply; db is the sum of the same dz.  (In 32 bits z would move 270 MB more and dz 400, of the 1.9 GB that
-// 32 768 rows of 2048 -> 2048 move forward and back.)
+// activation: one rounding, half a step of the type relative to z, and act' is taken at that point (it adds 3 % to the error of dx and
+// dW).  dz is rounded once to that type, the one the matrix cores multiply (dx and dW are off by sqrt 2 times their own rounding); db
+// is the sum of dz before that rounding.  (In 32 bits z would move 270 MB more and dz 400, of the 1.9 GB that 32 768 rows of
+// 2048 -> 2048 move forward and back.)
 #include "linear_kernel.h"
 
 // One or two matrices laid out anew with rows that start where the LDS loads want them (a 16-bit row of odd length starts on 2
@@ -89,51 +90,155 @@ __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g
     }
 }
 
-// The parts of a cut weight gradient, added in a fixed order: G groups of parts side by side, then the groups.  A workgroup takes
-// 1024 / G elements of one set; sets in one part are done already.
+// The same with db: a workgroup has 1 << bits rows of a set (of the matrix, if there is one) and 64 pieces of columns at most; a thread
+// keeps one piece's eight columns and goes down its rows, the threads of a piece are added through LDS in a fixed order.  16-bit types
+// with gelu or silu only: elsewhere dz is exact in its type and the weight gradient sums it by the way.  Bound like the above, and by
+// the search for the set: 32 768 x 2048 bfloat16 74 us (65 without db), 143 760 x 256 over 400 sets 49 (37).
+struct LinSums {
+    float *partial;  // [parts][cols rounded up to 4]: the sums of sets that have more than one piece
+    void *out;       // db [n_sets][cols]
+    int bits;
+    int64_t parts;   // room for so many
+};
+constexpr int SUMS_PIECES = 64;
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void k_linear_act_grad_sums(const T *__restrict__ g, const T *__restrict__ z, int64_t rows, int cols,
+                                                              const int32_t *offsets, int n_sets, T *__restrict__ dz, int64_t ldo,
+                                                              LinSums b) {
+    constexpr int N = 16 / (int)sizeof(T), AT_ONCE = 4;
+    typedef typename LinLoose<T, N>::type loose;
+    __shared__ f32x4v sums[2][256];
+    const int tid = threadIdx.x;
+    LinPiece p{0, lin_pieces(rows, b.bits, 1), (int64_t)blockIdx.x, 0, rows, 0};
+    if (offsets != nullptr) {
+        if (!lin_find<true>(offsets, n_sets, n_sets - 1, rows, b.bits, 1, blockIdx.x, &p)) return;
+    } else if (p.index >= p.count) {
+        return;
+    }
+    const int per = (cols + N - 1) / N, first = (int)blockIdx.y * SUMS_PIECES, pieces = per - first < SUMS_PIECES ? per - first : SUMS_PIECES;
+    const int groups = 256 / pieces, group = tid / pieces, x = first + tid % pieces;
+    const int c = (int)lin_piece_at((uint32_t)x * N, cols, N);
+    const int n = cols < N ? cols : N, again = x * N - c;  // what the piece before has too
+    const int64_t lo = p.lo + (p.index << b.bits), end = p.hi - lo < (1ll << b.bits) ? p.hi : lo + (1ll << b.bits);
+    float sum[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = 0.f;
+    if (group < groups) {
+        for (int64_t r0 = lo + group; r0 < end; r0 += groups * AT_ONCE) {
+            loose gv[AT_ONCE], zv[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int64_t r = r0 + u * groups < end ? r0 + u * groups : r0, at = r * cols + c;
+                if (n == N) {
+                    gv[u] = __builtin_nontemporal_load(reinterpret_cast<const loose *>(g + at));
+                    zv[u] = __builtin_nontemporal_load(reinterpret_cast<const loose *>(z + at));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        gv[u][e] = e < n ? g[at + e] : (T)0.f;
+                        zv[u][e] = e < n ? z[at + e] : (T)0.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int64_t r = r0 + u * groups;
+                if (r >= end) break;
+                float v[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    v[e] = to_f32(gv[u][e]) * lin_slope(to_f32(zv[u][e]), ACT);
+                    sum[e] += v[e];
+                }
+                T *to = dz + r * ldo + c;
+                if (n == N) lin_store<T, N>(to, v);
+                else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (e < n) to[e] = from_f32<T>(v[e]);
+                }
+            }
+        }
+    }
+    static_assert(N == 8, "two quads a piece");
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[q][tid][e] = sum[q * 4 + e];
+    int most = 1;
+    while (most < groups) most *= 2;
+    for (int half = most / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (group < half && group + half < groups) {
+            sums[0][tid] += sums[0][tid + half * pieces];
+            sums[1][tid] += sums[1][tid + half * pieces];
+        }
+    }
+    if (group != 0) return;
+    const int64_t part = p.split_at + p.index, ld = (cols + 3) / 4 * 4;
+    if (p.count > 1 && part >= b.parts) return;  // offsets that overlap: more parts than there can be
+    for (int e = again; e < n; ++e) {
+        const float v = sums[e >> 2][tid][e & 3];
+        if (p.count > 1) b.partial[part * ld + c + e] = v;
+        else reinterpret_cast<T *>(b.out)[(int64_t)p.set * cols + c + e] = from_f32<T>(v);
+    }
+}
+
+// The parts of a cut weight gradient, or of a bias gradient, added in a fixed order: G groups of parts side by side, then the groups.
+// A workgroup takes 1024 / G of a set's n elements; sets in one part are done already.
+struct LinJoin {
+    const float *partial;  // [parts][ld]
+    void *out;             // [n_sets][n]
+    int64_t n, ld;
+    int bits;
+    int64_t parts;
+};
 template <typename T, int G>
-__global__ __launch_bounds__(256) void k_linear_join(LinArgs a) {
+__device__ __forceinline__ void lin_join(const LinJoin &j, const int32_t *offsets, int n_sets, int64_t rows, unsigned block, f32x4v *sums) {
     constexpr int E = 256 / G;  // threads of a group, four elements each
-    __shared__ f32x4v sums[256];
     const int mine = threadIdx.x % E, group = threadIdx.x / E, set = blockIdx.y;
     int64_t first = 0;
-    int count = lin_pieces(a.rows, a.part_bits, 1);
-    if (a.offsets != nullptr) {
+    int count = lin_pieces(rows, j.bits, 1);
+    if (offsets != nullptr) {
         int64_t lo, hi;
-        lin_bounds(a.offsets, set, a.n_sets, a.rows, &lo, &hi);
-        count = lin_pieces(hi - lo, a.part_bits, 1);
+        lin_bounds(offsets, set, n_sets, rows, &lo, &hi);
+        count = lin_pieces(hi - lo, j.bits, 1);
         if (count <= 1) return;
-        first = lin_parts_before(a.offsets, a.n_sets, set, a.rows, a.part_bits);
+        first = lin_parts_before(offsets, n_sets, set, rows, j.bits);
     }
-    if (count <= 1 || first + count > a.parts) return;
-    const int64_t weights = (int64_t)a.out_rows * a.cols, all = weights + (a.bias_out != nullptr ? a.out_rows : 0);
-    // the weights' sums, then the bias', are one row of `all` elements; four neighbours may span the border
-    const int64_t i0 = ((int64_t)blockIdx.x * E + mine) * 4;
+    if (count <= 1 || first + count > j.parts) return;
+    const int64_t i0 = ((int64_t)block * E + mine) * 4;
     f32x4v s = {0.f, 0.f, 0.f, 0.f};
-    if (i0 + 4 <= weights && weights % 4 == 0) {
-        const float *at = a.partial + first * weights + i0;
+    if (i0 + 4 <= j.ld && j.ld % 4 == 0) {
+        const float *at = j.partial + first * j.ld + i0;
 #pragma unroll 4
-        for (int p = group; p < count; p += G) s += *reinterpret_cast<const f32x4v *>(at + p * weights);
+        for (int p = group; p < count; p += G) s += *reinterpret_cast<const f32x4v *>(at + p * j.ld);
     } else {
         for (int e = 0; e < 4; ++e) {
-            const int64_t i = i0 + e;
-            if (i >= all) break;
-            const float *at = i < weights ? a.partial + first * weights + i : a.partial_bias + first * a.out_rows + (i - weights);
-            const int64_t step = i < weights ? weights : a.out_rows;
-            for (int p = group; p < count; p += G) s[e] += at[p * step];
+            if (i0 + e >= j.n) break;
+            const float *at = j.partial + first * j.ld + i0 + e;
+            for (int p = group; p < count; p += G) s[e] += at[p * j.ld];
         }
     }
     if constexpr (G > 1) {
         sums[threadIdx.x] = s;
-        __syncthreads();
+        for (int half = G / 2; half > 0; half /= 2) {
+            __syncthreads();
+            if (group < half) sums[threadIdx.x] += sums[threadIdx.x + half * E];
+        }
         if (group != 0) return;
-        for (int g = 1; g < G; ++g) s += sums[g * E + mine];
+        s = sums[mine];
     }
-    for (int e = 0; e < 4; ++e) {
-        const int64_t i = i0 + e;
-        if (i < weights) reinterpret_cast<T *>(a.out)[set * weights + i] = from_f32<T>(s[e]);
-        else if (i < all) reinterpret_cast<T *>(a.bias_out)[(int64_t)set * a.out_rows + (i - weights)] = from_f32<T>(s[e]);
-    }
+    for (int e = 0; e < 4; ++e)
+        if (i0 + e < j.n) reinterpret_cast<T *>(j.out)[set * j.n + i0 + e] = from_f32<T>(s[e]);
+}
+// the weight gradient's workgroups, then the bias gradient's (BG groups)
+template <typename T, int G, int BG>
+__global__ __launch_bounds__(256) void k_linear_join(LinJoin weight, LinJoin bias, const int32_t *offsets, int n_sets, int64_t rows,
+                                                     unsigned weight_blocks) {
+    __shared__ f32x4v sums[256];
+    if (blockIdx.x < weight_blocks) lin_join<T, G>(weight, offsets, n_sets, rows, blockIdx.x, sums);
+    else lin_join<T, BG>(bias, offsets, n_sets, rows, blockIdx.x - weight_blocks, sums);
 }
 
 // rows behind the last set have no gradient: out = g there is none, g elsewhere
@@ -269,6 +374,34 @@ int part_bits_for(int64_t rows, int in, int out, int n_sets, bool half) {
 int64_t most_parts(int64_t rows, int n_sets, int bits) {
     if (n_sets == 1) return rows <= (int64_t)1 << bits ? 0 : (rows + ((int64_t)1 << bits) - 1) >> bits;
     return (2 * rows) >> bits;
+}
+
+// db summed beside dz: 16-bit types whose slope is not 0 or 1
+bool sums_beside(int dtype, int act) { return elem_size(dtype) == 2 && (act == LIN_GELU || act == LIN_SILU); }
+int sums_tiles(int out) { return ((out + 7) / 8 + SUMS_PIECES - 1) / SUMS_PIECES; }  // of columns
+// rows of one workgroup there, as a power of two: two rows a thread at least, and some 2000 workgroups (143 760 x 256 over 400 sets: up
+// to 2560 of them 49 us, 1280 52, 640 63, 5120 52; 32 768 x 2048 with its join 91, 90, 96, 99)
+int sum_bits_for(int64_t rows, int out) {
+    const int per = (out + 7) / 8, pieces = per < SUMS_PIECES ? per : SUMS_PIECES;
+    int bits = 4;
+    while ((1 << bits) < 2 * (256 / pieces)) ++bits;
+    while (bits < 30 && (rows >> bits) * sums_tiles(out) > 2560) ++bits;
+    return bits;
+}
+int64_t sums_bytes(int64_t rows, int out, int n_sets) { return most_parts(rows, n_sets, sum_bits_for(rows, out)) * round_up(out, 4) * 4; }
+template <typename T>
+int launch_sums(const void *g, const void *pre, int64_t rows, int out, int act, const int32_t *offsets, int n_sets, void *dz, int64_t lddz,
+                const LinSums &b, hipStream_t s) {
+    const int64_t pieces = offsets == nullptr ? lin_pieces(rows, b.bits, 1) : (rows >> b.bits) + n_sets;
+    const dim3 grid((unsigned)pieces, (unsigned)sums_tiles(out));
+    if (act == LIN_GELU)
+        hipLaunchKernelGGL((k_linear_act_grad_sums<T, LIN_GELU>), grid, dim3(256), 0, s, reinterpret_cast<const T *>(g),
+                           reinterpret_cast<const T *>(pre), rows, out, offsets, n_sets, reinterpret_cast<T *>(dz), lddz, b);
+    else
+        hipLaunchKernelGGL((k_linear_act_grad_sums<T, LIN_SILU>), grid, dim3(256), 0, s, reinterpret_cast<const T *>(g),
+                           reinterpret_cast<const T *>(pre), rows, out, offsets, n_sets, reinterpret_cast<T *>(dz), lddz, b);
+    MTP_LAUNCH_CHECK();
+    return MTP_OK;
 }
 
 // Up to so many workgroups the two products of a backward pass share a launch, in tiles that leave room for each other on a CU; in
@@ -410,11 +543,11 @@ int forward(const void *x, int64_t rows, int in, int64_t ldx, const void *w, int
     return launch_product<T, LIN_FORWARD>(a, s);
 }
 
-// where the parts of a backward pass lie in the workspace, one behind the other: dz, the weights and x with rows as the products
-// load them, the weight gradient's parts
+// where the parts of a backward pass lie in the workspace, one behind the other: dz, the bias gradient's parts where it is summed beside
+// dz, the weights and x with rows as the products load them, the weight gradient's parts
 struct BackwardPlan {
-    int64_t lddz, dz_bytes, w_bytes, x_bytes, parts_bytes;
-    int64_t total() const { return dz_bytes + w_bytes + x_bytes + parts_bytes; }
+    int64_t lddz, dz_bytes, w_bytes, x_bytes, parts_bytes, sums_bytes;
+    int64_t total() const { return dz_bytes + w_bytes + x_bytes + parts_bytes + sums_bytes; }
 };
 BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets, int act, const void *g, const void *w,
                            int64_t ldw, const void *x, int64_t ldx, bool want_x, bool want_w) {
@@ -430,6 +563,7 @@ BackwardPlan plan_backward(int dtype, int64_t rows, int in, int out, int n_sets,
     if (want_w) {
         p.x_bytes = relayout_bytes(dtype, x, ldx, rows, in);
         p.parts_bytes = most_parts(rows, n_sets, part_bits_for(rows, in, out, n_sets, elem_size(dtype) == 2)) * out * (in + 1) * 4;
+        if (sums_beside(dtype, act)) p.sums_bytes = round_up(sums_bytes(rows, out, n_sets), 256);
     }
     return p;
 }
@@ -466,17 +600,24 @@ LinArgs weight_args(bool half, const void *dz, int64_t rows, int out, int64_t ld
     a.partial_bias = a.partial + a.parts * out * in;
     return a;
 }
-// the weight gradient's parts, if it has any
+// the parts of the weight gradient and of the bias gradient (`b`, where it was summed beside dz), if there are any
 template <typename T>
-int join_parts(const LinArgs &a, hipStream_t s) {
-    if (a.parts == 0) return MTP_OK;
-    const int64_t all = (int64_t)a.out_rows * (a.cols + 1);
-    if (a.n_sets == 1 && a.parts >= 32)
-        hipLaunchKernelGGL((k_linear_join<T, 16>), dim3((unsigned)((all + 63) / 64), 1), dim3(256), 0, s, a);
-    else if (a.n_sets == 1 && a.parts >= 8)
-        hipLaunchKernelGGL((k_linear_join<T, 4>), dim3((unsigned)((all + 255) / 256), 1), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((k_linear_join<T, 1>), dim3((unsigned)((all + 1023) / 1024), (unsigned)a.n_sets), dim3(256), 0, s, a);
+int join_parts(const LinArgs &a, const LinSums &b, hipStream_t s) {
+    const int64_t n = (int64_t)a.out_rows * a.cols;
+    const LinJoin weight{a.partial, a.out, n, n, a.part_bits, a.parts};
+    const LinJoin bias = a.bias_out != nullptr ? LinJoin{a.partial_bias, a.bias_out, a.out_rows, a.out_rows, a.part_bits, a.parts}
+                                               : LinJoin{b.partial, b.out, a.out_rows, round_up(a.out_rows, 4), b.bits, b.parts};
+    // a matrix has few biases and many parts of them, a set has few
+    const int bias_each = a.n_sets > 1 ? 256 : 32, each = a.n_sets > 1 || a.parts < 8 ? 1024 : a.parts < 32 ? 256 : 64;  // of a workgroup
+    const unsigned bias_blocks = bias.out != nullptr && bias.parts > 0 ? (unsigned)((bias.n + bias_each - 1) / bias_each) : 0;
+    const unsigned blocks = weight.parts == 0 ? 0 : (unsigned)((weight.n + each - 1) / each);
+    if (blocks + bias_blocks == 0) return MTP_OK;
+    const dim3 grid(blocks + bias_blocks, (unsigned)a.n_sets);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, weight, bias, a.offsets, a.n_sets, a.rows, blocks); };
+    if (a.n_sets > 1) launch(k_linear_join<T, 1, 4>);
+    else if (each == 64) launch(k_linear_join<T, 16, 32>);
+    else if (each == 256) launch(k_linear_join<T, 4, 32>);
+    else launch(k_linear_join<T, 1, 32>);
     MTP_LAUNCH_CHECK();
     return MTP_OK;
 }
@@ -497,13 +638,13 @@ int grad_weight(const void *dz, int64_t rows, int out, int64_t lddz, const void 
     if (rc != MTP_OK) return rc;
     const LinArgs a = weight_args(sizeof(T) == 2, dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db, ws);
     rc = launch_product<T, LIN_GRAD_WEIGHT>(a, s);
-    return rc != MTP_OK ? rc : join_parts<T>(a, s);
+    return rc != MTP_OK ? rc : join_parts<T>(a, LinSums{}, s);
 }
 
-// both from operands that need no new layout
+// both from operands that need no new layout; db NULL: not wanted, or summed beside dz (`sums`)
 template <typename T>
 int grad_both(const void *dz, int64_t rows, int out, int64_t lddz, const void *w, int64_t ldw, const void *x, int in, int64_t ldx,
-              const int32_t *offsets, int n_sets, void *dx, void *dw, void *db, char *ws, hipStream_t s) {
+              const int32_t *offsets, int n_sets, void *dx, void *dw, void *db, const LinSums &sums, char *ws, hipStream_t s) {
     const LinArgs input = input_args(dz, rows, out, lddz, w, in, ldw, offsets, n_sets, dx);
     const LinArgs weight = weight_args(sizeof(T) == 2, dz, rows, out, lddz, x, in, ldx, offsets, n_sets, dw, db, ws);
     bool done = false;
@@ -517,7 +658,7 @@ int grad_both(const void *dz, int64_t rows, int out, int64_t lddz, const void *w
         if (rc == MTP_OK && dw != nullptr) rc = launch_product<T, LIN_GRAD_WEIGHT>(weight, s);
         if (rc != MTP_OK) return rc;
     }
-    return dw != nullptr ? join_parts<T>(weight, s) : rc;
+    return dw != nullptr ? join_parts<T>(weight, sums, s) : rc;
 }
 
 }  // namespace
@@ -657,11 +798,20 @@ extern "C" int mtp_linear_backward(int dtype, const void *g, const void *pre, in
     const void *dz = g;
     int64_t lddz = p.lddz;
     hipStream_t s = mtp_stream(stream);
+    LinSums sums{};
     if (act != LIN_NONE) {
-        rc = mtp_linear_act_grad(dtype, g, pre, rows, out, act, offsets, n_sets, ws, lddz, stream);
+        if (db != nullptr && rows > 0 && sums_beside(dtype, act)) {
+            const int bits = sum_bits_for(rows, out);
+            sums = LinSums{reinterpret_cast<float *>(at + p.dz_bytes), db, bits, most_parts(rows, n_sets, bits)};
+            db = nullptr;
+            rc = dtype == MTP_BFLOAT16 ? launch_sums<__bf16>(g, pre, rows, out, act, offsets, n_sets, ws, lddz, sums, s)
+                                       : launch_sums<_Float16>(g, pre, rows, out, act, offsets, n_sets, ws, lddz, sums, s);
+        } else {
+            rc = mtp_linear_act_grad(dtype, g, pre, rows, out, act, offsets, n_sets, ws, lddz, stream);
+        }
         if (rc != MTP_OK) return rc;
         dz = ws;
-        at += p.dz_bytes;
+        at += p.dz_bytes + p.sums_bytes;
     } else if (p.dz_bytes > 0) {  // both products read it
         const void *none = nullptr;
         int64_t ld = 0;
@@ -673,5 +823,5 @@ extern "C" int mtp_linear_backward(int dtype, const void *g, const void *pre, in
                                           &at, s);
         if (rc != MTP_OK) return rc;
     }
-    return MTP_BY_TYPE(dtype, grad_both)(dz, rows, out, lddz, w, ldw, x, in, ldx, offsets, n_sets, dx, dw, db, at, s);
+    return MTP_BY_TYPE(dtype, grad_both)(dz, rows, out, lddz, w, ldw, x, in, ldx, offsets, n_sets, dx, dw, db, sums, at, s);
 }
