@@ -62,6 +62,17 @@ def predict_topk(net, obs_enc, k, all_modalities):
     return out.reshape(n, k, out.shape[-2], 2)
 
 
+def _chosen(probs, ids, normalize):
+    """float32 [N, k]: the probabilities of the chosen modalities (0 where there is none), summing to one if ``normalize``."""
+    p = probs.gather(1, ids.long().clamp_min(0)).float().masked_fill(ids < 0, 0.0)
+    if not normalize:
+        return p
+    # the slope (g_j - sum g w) / sum p from the quotient w itself: what cancels in it (all of it for one modality) does so exactly
+    total = p.sum(1, keepdim=True)
+    w = (p / total).detach()
+    return w + (p - w * total) / total.detach()
+
+
 def predict_mixture(net, obs_enc, k, all_modalities, normalize=True):
     """``predict_topk`` with the weight of each candidate and their weighted mean, differentiable.
 
@@ -71,7 +82,10 @@ def predict_mixture(net, obs_enc, k, all_modalities, normalize=True):
 
     Returns (displacements [N, k, T, 2], weights float32 [N, k], mean displacements [N, T, 2]).  Equal probabilities go by the
     lower index.  A modality of probability zero is no candidate: its weight is 0 and its place holds modality 0's."""
-    ids, weights = route_topk(torch.log(net.classifier(obs_enc)), k, normalize=normalize)
+    probs = net.classifier(obs_enc)
+    ids, weights = route_topk(torch.log(probs.detach()), k, normalize=normalize)
+    if probs.requires_grad:  # not through the logarithm, whose slope has no value at zero
+        weights = _chosen(probs, ids, normalize)
     plan = sort_pairs(ids, all_modalities.shape[0])
     rows = dispatch(obs_enc.contiguous(), plan)
     labels = ids.reshape(-1)[plan.order.long()].clamp_min(0).long()
