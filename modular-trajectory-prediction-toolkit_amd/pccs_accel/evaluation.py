@@ -63,14 +63,15 @@ def predict_topk(net, obs_enc, k, all_modalities):
 
 
 def _chosen(probs, ids, normalize):
-    """float32 [N, k]: the probabilities of the chosen modalities (0 where there is none), summing to one if ``normalize``."""
-    p = probs.gather(1, ids.long().clamp_min(0)).float().masked_fill(ids < 0, 0.0)
+    """float32 [N, k]: the probabilities of the chosen modalities, summing to one if ``normalize``."""
+    p = probs.gather(1, ids.long().clamp_min(0)).float()
     if not normalize:
         return p
     # the slope (g_j - sum g w) / sum p from the quotient w itself: what cancels in it (all of it for one modality) does so exactly
     total = p.sum(1, keepdim=True)
-    w = (p / total).detach()
-    return w + (p - w * total) / total.detach()
+    by = torch.where(total > 0, total, torch.ones_like(total)).detach()  # nothing but zeros: weights of 0
+    w = (p / by).detach()
+    return w + (p - w * total) / by
 
 
 def predict_mixture(net, obs_enc, k, all_modalities, normalize=True):
@@ -81,11 +82,11 @@ def predict_mixture(net, obs_enc, k, all_modalities, normalize=True):
     modality read the same row of ``all_modalities`` one after the other, and the candidates averaged back per agent.
 
     Returns (displacements [N, k, T, 2], weights float32 [N, k], mean displacements [N, T, 2]).  Equal probabilities go by the
-    lower index.  A modality of probability zero is no candidate: its weight is 0 and its place holds modality 0's."""
+    lower index, those of zero too: such a candidate is the agent's like any other, with weight 0."""
     probs = net.classifier(obs_enc)
-    ids, weights = route_topk(torch.log(probs.detach()), k, normalize=normalize)
-    if probs.requires_grad:  # not through the logarithm, whose slope has no value at zero
-        weights = _chosen(probs, ids, normalize)
+    ids, routed = route_topk(probs.detach(), k)
+    # a probability that is NaN is never chosen before another and makes its agent's weights NaN
+    weights = torch.where(routed.isnan(), routed, _chosen(probs, ids, normalize))
     plan = sort_pairs(ids, all_modalities.shape[0])
     rows = dispatch(obs_enc.contiguous(), plan)
     labels = ids.reshape(-1)[plan.order.long()].clamp_min(0).long()
