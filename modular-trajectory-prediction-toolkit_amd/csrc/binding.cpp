@@ -103,10 +103,12 @@ std::shared_ptr<N> node_with_edges(const Inputs &...inputs) {
     return node;
 }
 
-// hooks on saved tensors may give back what they like
-void refuse_other_layouts(const char *what, std::initializer_list<const Tensor *> saved) {
-    for (const Tensor *t : saved)
-        TORCH_CHECK(!t->defined() || t->is_contiguous(), what, ": a saved tensor has come back from its hook with another layout");
+// Hooks on saved tensors may give back what they like: what the kernels read has to be what the node kept.  `rows`: rows at any
+// distance will do.
+void refuse_changed(const char *what, const Tensor &t, at::ScalarType type, c10::Device device, at::IntArrayRef sizes, bool rows = false) {
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == type && t.device() == device && t.sizes() == sizes &&
+                    (rows ? row_distance(t) >= 0 : t.is_contiguous()),
+                what, ": a saved tensor has come back from its hook with another layout, type, size or device");
 }
 
 // What a backward pass returns can be differentiated no further: trying to says so.  `from`: what it was computed from.
@@ -154,7 +156,7 @@ Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor
 
 struct LinearNode : Node {
     Sizes z;
-    bool has_bias, has_residual;
+    bool has_bias, has_residual, pre_kept, offsets_kept, rows_kept, weights_kept;
     SavedVariable x_, w_, pre_, offsets_, rows_, weights_;
 
     std::string name() const override { return "LinearBackward"; }
@@ -168,7 +170,18 @@ struct LinearNode : Node {
         if (!grads[0].defined()) return variable_list(4);
         const Tensor x = x_.unpack(), w = w_.unpack(), pre = pre_.unpack(getptr()), offsets = offsets_.unpack();
         const Tensor rows = rows_.unpack(), weights = weights_.unpack();
-        refuse_other_layouts("linear", {&w, &pre, &offsets});
+        const auto type = grads[0].scalar_type();
+        const auto device = grads[0].device();
+        refuse_changed("linear", x, type, device, {z.rows, z.in}, true);
+        if (offsets_kept) {
+            refuse_changed("linear", w, type, device, {z.sets, z.out, z.in});
+            refuse_changed("linear", offsets, at::kInt, device, {z.sets + 1});
+        } else {
+            refuse_changed("linear", w, type, device, {z.out, z.in});
+        }
+        if (pre_kept) refuse_changed("linear", pre, type, device, {z.rows, z.out});
+        if (rows_kept) refuse_changed("linear", rows, type, device, {z.rows, z.in}, true);
+        if (weights_kept) refuse_changed("linear", weights, type, device, {z.sets * z.out, z.in}, true);
         Tensor dx, dw, db, dr;
         {
             at::NoGradGuard off;
@@ -254,6 +267,10 @@ Tensor linear_with_node(const Tensor &x, const Tensor &w, const Tensor &bias, co
     node->has_residual = residual.defined();
     node->x_ = SavedVariable(x, false);
     node->w_ = SavedVariable(w, false);
+    node->pre_kept = from_y || pre.defined();
+    node->offsets_kept = offsets.defined();
+    node->rows_kept = rows.defined();
+    node->weights_kept = weights.defined();
     if (from_y) node->pre_ = SavedVariable(y, true);
     else if (pre.defined()) node->pre_ = SavedVariable(pre, false);
     if (offsets.defined()) node->offsets_ = SavedVariable(offsets, false);
@@ -292,6 +309,8 @@ std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::option
 // ---- router ----
 struct RouteNode : Node {
     bool normalize;
+    int64_t modalities;
+    at::ScalarType type;
     SavedVariable scores_, ids_, weights_, stats_;
 
     std::string name() const override { return "RouteTopkBackward"; }
@@ -303,7 +322,12 @@ struct RouteNode : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
         const Tensor scores = scores_.unpack(), ids = ids_.unpack(), weights = weights_.unpack(getptr()), stats = stats_.unpack();
-        refuse_other_layouts("route_topk", {&ids, &weights, &stats});
+        const auto device = grads[0].device();
+        const int64_t n = grads[0].size(0), k = grads[0].size(1);
+        refuse_changed("route_topk", scores, type, device, {n, modalities}, true);
+        refuse_changed("route_topk", ids, at::kInt, device, {n, k});
+        refuse_changed("route_topk", weights, at::kFloat, device, {n, k});
+        refuse_changed("route_topk", stats, at::kFloat, device, {n, 2});
         Tensor out;
         {
             at::NoGradGuard off;
@@ -350,6 +374,8 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
         const auto node = node_with_edges<RouteNode>(scores);
         torch::autograd::set_history(weights, node);
         node->normalize = normalize;
+        node->modalities = e;
+        node->type = scores.scalar_type();
         node->scores_ = SavedVariable(scores, false);
         node->ids_ = SavedVariable(ids, false);
         node->weights_ = SavedVariable(weights, true);
@@ -407,6 +433,7 @@ Tensor run_combine(const Tensor &rows, const Tensor &position, const Tensor &off
 }
 
 struct DispatchNode : Node {
+    int64_t agents, choices, modalities;  // the plan's sizes
     SavedVariable position_, offsets_;
 
     std::string name() const override { return "DispatchBackward"; }
@@ -419,7 +446,8 @@ struct DispatchNode : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
         const Tensor position = position_.unpack(), offsets = offsets_.unpack();
-        refuse_other_layouts("dispatch", {&position, &offsets});
+        refuse_changed("dispatch", position, at::kInt, grads[0].device(), {agents, choices});
+        refuse_changed("dispatch", offsets, at::kInt, grads[0].device(), {modalities + 1});
         Tensor dx;
         {
             at::NoGradGuard off;
@@ -431,6 +459,7 @@ struct DispatchNode : Node {
 };
 
 struct CombineNode : Node {
+    int64_t choices, modalities;
     SavedVariable rows_, weights_, position_, offsets_;
     bool weighted;
 
@@ -444,7 +473,14 @@ struct CombineNode : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(2);
         const Tensor rows = rows_.unpack(), weights = weights_.unpack(), position = position_.unpack(), offsets = offsets_.unpack();
-        refuse_other_layouts("combine", {&rows, &weights, &position, &offsets});
+        const auto device = grads[0].device();
+        const int64_t n = grads[0].size(0), d = grads[0].size(1);
+        if (weighted) {
+            refuse_changed("combine", rows, grads[0].scalar_type(), device, {n * choices, d});
+            refuse_changed("combine", weights, at::kFloat, device, {n, choices});
+        }
+        refuse_changed("combine", position, at::kInt, device, {n, choices});
+        refuse_changed("combine", offsets, at::kInt, device, {modalities + 1});
         Tensor dr, dw;
         {
             at::NoGradGuard off;
@@ -490,6 +526,9 @@ std::optional<Tensor> dispatch(const Tensor &x, const Tensor &position, const Te
     if (train) {
         const auto node = node_with_edges<DispatchNode>(x);
         torch::autograd::set_history(rows, node);
+        node->agents = position.size(0);
+        node->choices = position.size(1);
+        node->modalities = offsets.numel() - 1;
         node->position_ = SavedVariable(position, false);
         node->offsets_ = SavedVariable(offsets, false);
     }
@@ -511,6 +550,8 @@ std::optional<Tensor> combine(const Tensor &rows, const Tensor &position, const 
         const auto node = node_with_edges<CombineNode>(rows, weights);
         torch::autograd::set_history(y, node);
         node->weighted = weights.defined();
+        node->choices = position.size(1);
+        node->modalities = offsets.numel() - 1;
         if (weights.defined()) {  // the rows themselves are needed for the weights' gradient only
             node->rows_ = SavedVariable(rows, false);
             node->weights_ = SavedVariable(weights, false);

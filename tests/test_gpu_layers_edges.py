@@ -55,3 +55,61 @@ def test_bias_gradients_of_modalities_are_sums_of_what_is_not_rounded(gpu_device
         at = offsets.tolist()
         want = [_bias_gradient(x[at[e]:at[e + 1]], w[e], gy[at[e]:at[e + 1]], "gelu") for e in range(sets)]
         R.check("db", db, (torch.stack([v for v, _ in want]), torch.stack([e for _, e in want])))
+
+
+def _calls(dev):
+    """name -> a call of each operator that has a node, its inputs' gradients to be asked for, and the gradient of its result."""
+    from pccs_accel.routing import combine, dispatch, route_topk, sort_pairs
+    g = torch.Generator().manual_seed(1)
+
+    def leaf(*shape, dtype=torch.float16):
+        return torch.randn(*shape, generator=g).to(dtype).to(dev).requires_grad_()
+    x, w, b, w3, b3 = leaf(40, 24), leaf(16, 24), leaf(16), leaf(5, 16, 24), leaf(5, 16)
+    odd_x, odd_w = leaf(700, 97), leaf(41, 97)
+    scores, rows, weights = leaf(40, 30), leaf(120, 24), leaf(40, 3, dtype=torch.float32)
+    plan = sort_pairs(torch.randint(0, 30, (40, 3), generator=g, dtype=torch.int32).to(dev), 30)
+    offsets = torch.tensor([0, 9, 9, 20, 30, 38], dtype=torch.int32, device=dev)
+    return {
+        "linear": (lambda: linear(x, w, b, "gelu"), [x, w, b]),
+        "linear relu": (lambda: linear(x, w, b, "relu"), [x, w]),
+        "linear odd": (lambda: linear(odd_x, odd_w, None, "silu"), [odd_x, odd_w]),
+        "modality_linear": (lambda: modality_linear(x, offsets, w3, b3, "silu"), [x, w3, b3]),
+        "route_topk": (lambda: route_topk(scores, 4)[1], [scores]),
+        "dispatch": (lambda: dispatch(x, plan), [x]),
+        "combine": (lambda: combine(rows, plan, weights), [rows, weights]),
+        "combine unweighted": (lambda: combine(rows, plan), [rows]),
+    }
+
+
+def _backwards(t):
+    """t's values in the order of a matrix stored by columns (of a vector: every other element of a longer one)."""
+    return t.t().contiguous().t() if t.dim() == 2 else torch.stack((t, t), -1)[..., 0]
+
+
+# what a hook may make of a tensor: another type, fewer elements, other dimensions, the host's copy, nothing, strides of its own
+CHANGES = {"wider": lambda t: t.double(), "narrower": lambda t: t.to(torch.int8), "fewer rows": lambda t: t[:-1].contiguous(),
+           "fewer columns": lambda t: t[..., :-1].contiguous(), "flat": lambda t: t.reshape(1, 1, 1, -1), "on the host": lambda t: t.cpu(),
+           "another 16-bit type": lambda t: t.to(torch.bfloat16), "empty": lambda t: t[:0], "by columns": _backwards}
+
+
+@pytest.mark.parametrize("change", list(CHANGES))
+def test_saved_tensors_that_come_back_changed_are_refused(gpu_device, change):
+    for name, (call, leaves) in _calls(gpu_device).items():
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(0) or t, lambda t: t):
+            y = call()
+            g = torch.ones_like(y)
+            want = torch.autograd.grad(y, leaves, g)
+        assert kept, name
+        for which in range(len(kept)):  # each of the saved tensors in turn
+            seen = []
+
+            def unpack(t):
+                seen.append(0)
+                return CHANGES[change](t) if len(seen) - 1 == which else t
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = call()
+            with pytest.raises(RuntimeError, match="come back from its hook|can require gradients"):  # the latter is torch's own
+                torch.autograd.grad(y, leaves, g)
+        for a, c in zip(torch.autograd.grad(call(), leaves, g), want):
+            assert torch.equal(a, c)
