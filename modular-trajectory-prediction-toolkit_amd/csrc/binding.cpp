@@ -9,11 +9,13 @@
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <array>
 #include <optional>
@@ -86,6 +88,14 @@ void refuse_foreign_nodes(const char *what, std::initializer_list<const Tensor *
                     ": an input belongs to an autograd graph that was begun outside this capture; its backward pass cannot be captured "
                     "(let go of the eager results that refer to it first)");
     }
+}
+
+// A tracer records what goes through the dispatcher.  The kernels do not: a trace would hold the results' allocation without what fills
+// it, or their values as constants.
+void refuse_tracing(const char *what) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                what, " cannot be traced: its kernels are not seen by a tracer");
 }
 
 // no derivative in forward mode: a tangent must not get lost in silence
@@ -281,6 +291,7 @@ Tensor linear_with_node(const Tensor &x, const Tensor &w, const Tensor &bias, co
 
 std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_, int act,
                              const std::optional<Tensor> &residual_, const std::optional<Tensor> &offsets_) {
+    refuse_tracing("linear");
     const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
     const bool many = offsets.defined();
     if (!matrix(x) || row_distance(x) < 0 || w.dim() != (many ? 3 : 2) || !w.is_contiguous() || w.scalar_type() != x.scalar_type() ||
@@ -345,6 +356,7 @@ struct RouteNode : Node {
 };
 
 std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64_t k, bool normalize) {
+    refuse_tracing("route_topk");
     if (!matrix(scores)) return std::nullopt;
     const int64_t n = scores.size(0), e = scores.size(1), ld = row_distance(scores);
     if (ld < 0 || n > MOST || e < 1 || e > MOST_MODALITIES || k < 1 || k > e || k > MOST_TOPK) return std::nullopt;
@@ -386,6 +398,7 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
 
 // ---- pairs ----
 std::optional<std::tuple<Tensor, Tensor, Tensor>> sort_pairs(const Tensor &ids, int64_t e) {
+    refuse_tracing("sort_pairs");
     if (!ids.is_cuda() || ids.scalar_type() != at::kInt || ids.dim() != 2 || !ids.is_contiguous() || e < 1 || e > MOST_MODALITIES ||
         ids.numel() > MOST)
         return std::nullopt;
@@ -515,6 +528,7 @@ bool plan_for(const Tensor &t, const Tensor &position, const Tensor &offsets) {
 }
 
 std::optional<Tensor> dispatch(const Tensor &x, const Tensor &position, const Tensor &offsets) {
+    refuse_tracing("dispatch");
     if (!matrix(x) || row_distance(x) < 0 || !plan_for(x, position, offsets) || position.size(0) != x.size(0) || x.size(1) < 1 ||
         position.size(1) < 1)
         return std::nullopt;
@@ -536,6 +550,7 @@ std::optional<Tensor> dispatch(const Tensor &x, const Tensor &position, const Te
 }
 
 std::optional<Tensor> combine(const Tensor &rows, const Tensor &position, const Tensor &offsets, const std::optional<Tensor> &weights_) {
+    refuse_tracing("combine");
     const Tensor weights = weights_.value_or(Tensor());
     if (!matrix(rows) || !rows.is_contiguous() || !plan_for(rows, position, offsets) || rows.size(0) != position.numel() ||
         rows.size(1) < 1 || position.size(1) < 1)

@@ -431,6 +431,8 @@ _ENTRY = {}
 def _call(device, name, *args):
     """Entry point ``name`` on ``device``'s current stream; raises on an error code."""
     fn, i = _ENTRY.get(name), device.index
+    if torch.jit.is_tracing():
+        raise _lib.MtpError(f"{name} cannot be traced: its kernels are not seen by a tracer")
     if fn is None:
         fn = _ENTRY[name] = getattr(lib(), name)
     if i == torch.cuda.current_device():
