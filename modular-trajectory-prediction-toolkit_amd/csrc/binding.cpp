@@ -54,9 +54,10 @@ int64_t row_distance(const Tensor &t) {
     if ((cols > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < cols)) return -1;
     return t.stride(0);
 }
-bool matrix(const Tensor &t) { return t.is_cuda() && t.dim() == 2 && t.layout() == at::kStrided && type_code(t) >= 0; }
+// (a tensor with the negative bit holds the negatives of its values)
+bool matrix(const Tensor &t) { return t.is_cuda() && t.dim() == 2 && t.layout() == at::kStrided && type_code(t) >= 0 && !t.is_neg(); }
 bool like(const Tensor &t, at::ScalarType type, const Tensor &ref, at::IntArrayRef shape) {
-    return t.scalar_type() == type && t.device() == ref.device() && t.sizes() == shape && t.is_contiguous();
+    return t.scalar_type() == type && t.device() == ref.device() && t.sizes() == shape && t.is_contiguous() && !t.is_neg();
 }
 Tensor workspace(int64_t bytes, const Tensor &ref) {
     return bytes > 0 ? at::empty({bytes}, ref.options().dtype(at::kByte)) : Tensor();
@@ -116,7 +117,7 @@ std::shared_ptr<N> node_with_edges(const Inputs &...inputs) {
 // Hooks on saved tensors may give back what they like: what the kernels read has to be what the node kept.  `rows`: rows at any
 // distance will do.
 void refuse_changed(const char *what, const Tensor &t, at::ScalarType type, c10::Device device, at::IntArrayRef sizes, bool rows = false) {
-    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == type && t.device() == device && t.sizes() == sizes &&
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == type && t.device() == device && t.sizes() == sizes && !t.is_neg() &&
                     (rows ? row_distance(t) >= 0 : t.is_contiguous()),
                 what, ": a saved tensor has come back from its hook with another layout, type, size or device");
 }
@@ -196,7 +197,7 @@ struct LinearNode : Node {
         {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
-            const Tensor g = grads[0].contiguous();
+            const Tensor g = grads[0].resolve_neg().contiguous();
             const bool want_x = task_should_compute_output(0), want_b = has_bias && task_should_compute_output(2);
             const bool want_w = task_should_compute_output(1) || want_b;
             const int32_t *sets = static_cast<const int32_t *>(at_(offsets));
@@ -294,7 +295,7 @@ std::optional<Tensor> linear(const Tensor &x, const Tensor &w, const std::option
     refuse_tracing("linear");
     const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
     const bool many = offsets.defined();
-    if (!matrix(x) || row_distance(x) < 0 || w.dim() != (many ? 3 : 2) || !w.is_contiguous() || w.scalar_type() != x.scalar_type() ||
+    if (!matrix(x) || row_distance(x) < 0 || w.dim() != (many ? 3 : 2) || !w.is_contiguous() || w.is_neg() || w.scalar_type() != x.scalar_type() ||
         w.device() != x.device())
         return std::nullopt;
     const Sizes z{type_code(x), act, x.size(0), x.size(1), w.size(many ? 1 : 0), many ? w.size(0) : 1};
@@ -343,7 +344,7 @@ struct RouteNode : Node {
         {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
-            const Tensor g = grads[0].contiguous();
+            const Tensor g = grads[0].resolve_neg().contiguous();
             out = at::empty(scores.sizes(), scores.options());
             check(mtp_route_topk_grad(type_code(scores), at_(scores), scores.size(0), (int)scores.size(1), row_distance(scores),
                                       (int)ids.size(1), normalize, static_cast<const int32_t *>(at_(ids)),
@@ -399,7 +400,7 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
 // ---- pairs ----
 std::optional<std::tuple<Tensor, Tensor, Tensor>> sort_pairs(const Tensor &ids, int64_t e) {
     refuse_tracing("sort_pairs");
-    if (!ids.is_cuda() || ids.scalar_type() != at::kInt || ids.dim() != 2 || !ids.is_contiguous() || e < 1 || e > MOST_MODALITIES ||
+    if (!ids.is_cuda() || ids.scalar_type() != at::kInt || ids.dim() != 2 || !ids.is_contiguous() || ids.is_neg() || e < 1 || e > MOST_MODALITIES ||
         ids.numel() > MOST)
         return std::nullopt;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ids.device());
@@ -465,7 +466,7 @@ struct DispatchNode : Node {
         {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(grads[0].device());
-            dx = run_combine(grads[0].contiguous(), position, offsets, Tensor());
+            dx = run_combine(grads[0].resolve_neg().contiguous(), position, offsets, Tensor());
         }
         return no_further({dx}, {grads[0]}, "dispatch");
     }
@@ -498,7 +499,7 @@ struct CombineNode : Node {
         {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(grads[0].device());
-            const Tensor g = grads[0].contiguous();
+            const Tensor g = grads[0].resolve_neg().contiguous();
             if (!weighted) {
                 dr = run_dispatch(g, position, offsets);
             } else {

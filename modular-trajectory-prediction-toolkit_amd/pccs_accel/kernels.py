@@ -456,6 +456,8 @@ def _device_tensor(t, name, ndim):
                             "there is no CPU path")
     if t.dim() != ndim:
         raise ValueError(f"{name}: expected {ndim} dimensions, got shape {tuple(t.shape)}")
+    if t.is_neg():
+        raise ValueError(f"{name}: a view of the negative of its memory (resolve_neg() gives a tensor that is not)")
     return t
 
 
@@ -470,7 +472,7 @@ def _like(t, name, ndim, ref, ref_name, dtype=None, shape=None):
     """A contiguous tensor on ref's device, of ref's type (or ``dtype``) and of ``shape``."""
     want = ref.dtype if dtype is None else dtype
     if (isinstance(t, torch.Tensor) and t.dtype == want and t.dim() == ndim and (shape is None or t.shape == shape)
-            and t.device == ref.device and t.is_cuda and t.is_contiguous()):
+            and t.device == ref.device and t.is_cuda and t.is_contiguous() and not t.is_neg()):
         return t
     _device_tensor(t, name, ndim)
     if t.dtype != want:
@@ -536,6 +538,7 @@ def sort_pairs(ids, n_modalities):
     if not isinstance(ids, torch.Tensor):
         raise TypeError(f"ids: expected a torch.Tensor, got {type(ids).__name__}")
     _req(ids, "ids", torch.int32, align=4)
+    _device_tensor(ids, "ids", ids.dim())
     e = int(n_modalities)
     if not 1 <= e <= MAX_MODALITIES:
         raise ValueError(f"n_modalities={e} must be in [1, {MAX_MODALITIES}]")

@@ -113,3 +113,26 @@ def test_saved_tensors_that_come_back_changed_are_refused(gpu_device, change):
                 torch.autograd.grad(y, leaves, g)
         for a, c in zip(torch.autograd.grad(call(), leaves, g), want):
             assert torch.equal(a, c)
+
+
+def test_views_of_negatives_are_refused_and_such_gradients_taken(gpu_device):
+    """A tensor with the negative bit holds the negatives of its values; torch gives such gradients to whoever asks."""
+    from pccs_accel.routing import PairPlan, combine, dispatch, route_topk, sort_pairs
+    g = torch.Generator().manual_seed(2)
+    x, w, b, r = (torch.randn(*s, generator=g).to(gpu_device) for s in ((40, 24), (16, 24), (16,), (40, 16)))
+    ids = torch.randint(0, 9, (40, 3), generator=g, dtype=torch.int32).to(gpu_device)
+    plan, weights = sort_pairs(ids, 9), torch.rand(40, 3, generator=g).to(gpu_device)
+    rows = dispatch(x, plan)
+    n = torch._neg_view
+    for call in (lambda: linear(n(x), w), lambda: linear(x, n(w)), lambda: linear(x, w, n(b)), lambda: linear(x, w, b, None, n(r)),
+                 lambda: linear(n(x[0]), w), lambda: route_topk(n(x), 3), lambda: sort_pairs(n(ids), 9), lambda: dispatch(n(x), plan),
+                 lambda: combine(n(rows), plan, weights), lambda: combine(rows, plan, n(weights)),
+                 lambda: dispatch(x, PairPlan(plan.offsets, plan.order, n(plan.position)))):
+        with pytest.raises(ValueError, match="negative"):
+            call()
+    for name, (call, leaves) in _calls(gpu_device).items():
+        y = call()
+        gy = torch.randn(y.shape, generator=g).to(gpu_device).to(y.dtype)
+        want = torch.autograd.grad(call(), leaves, -gy)
+        for a, c in zip(torch.autograd.grad(y, leaves, n(gy)), want):
+            assert torch.equal(a, c), name
