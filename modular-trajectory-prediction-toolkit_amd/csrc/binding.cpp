@@ -2,11 +2,12 @@
 //
 // A small layer takes a few microseconds on the card; a call through Python takes ten, a backward pass through Python nodes some
 // thirty more.  Here the arguments are looked over, the results allocated and the entry points of mtp_accel.h called without
-// Python between them: a forward and a backward pass of a 64 x 96 layer with gelu take the host 57 us, 35 of which the engine takes
+// Python between them: a forward and a backward pass of a 64 x 96 layer with gelu take the host 62 us, 35 of which the engine takes
 // for a node that does nothing.  A call whose arguments are not as they have to be returns None: the Python front end then finds
 // out what is wrong and raises.
 #include <torch/extension.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -59,21 +60,12 @@ bool matrix(const Tensor &t) { return t.is_cuda() && t.dim() == 2 && t.layout() 
 bool like(const Tensor &t, at::ScalarType type, const Tensor &ref, at::IntArrayRef shape) {
     return t.scalar_type() == type && t.device() == ref.device() && t.sizes() == shape && t.is_contiguous() && !t.is_neg();
 }
-Tensor workspace(int64_t bytes, const Tensor &ref) {
-    return bytes > 0 ? at::empty({bytes}, ref.options().dtype(at::kByte)) : Tensor();
+// A result or a workspace on ref's device.  Past the dispatcher, which would take the host as long again as the allocation; each has a
+// storage of its own, so that it can grow, move to another stream and go by itself.
+Tensor fresh(const Tensor &ref, at::ScalarType type, at::IntArrayRef sizes) {
+    return Tensor(at::detail::empty_cuda(sizes, type, ref.device(), std::nullopt));
 }
-
-// Results of a scene's size share one allocation (each takes the host a microsecond, a sixth of such a call: sort_pairs 6.0 -> 4.8 us,
-// route_topk 5.2 -> 4.5); large ones have their own, so that each can go when it is not needed.
-constexpr int64_t TOGETHER_BYTES = 256 << 10, PLACE_BYTES = 256;
-int64_t place(int64_t bytes) { return (bytes + PLACE_BYTES - 1) / PLACE_BYTES * PLACE_BYTES; }
-Tensor part_of(const Tensor &all, int64_t at, at::ScalarType type, at::IntArrayRef sizes) {
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                        c10::scalarTypeToTypeMeta(type));
-    t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    return t;
-}
+Tensor workspace(int64_t bytes, const Tensor &ref) { return bytes > 0 ? fresh(ref, at::kByte, {bytes}) : Tensor(); }
 
 // Under capture a backward pass must not meet a node that was made on another stream: the engine would make that stream wait for
 // the captured one, which fails inside its own thread and ends the process.  Such a node exists where an input is a result
@@ -143,16 +135,8 @@ struct Sizes {
 
 Tensor run_linear(const Sizes &z, const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, const Tensor &offsets,
                   Tensor *pre, Tensor *laid_out = nullptr) {
-    Tensor y;
-    const int64_t y_bytes = z.rows * z.out * x.element_size();
-    if (pre != nullptr && y_bytes > 0 && place(y_bytes) + y_bytes <= TOGETHER_BYTES) {
-        const Tensor all = at::empty({place(y_bytes) + y_bytes}, x.options().dtype(at::kByte));
-        y = part_of(all, 0, x.scalar_type(), {z.rows, z.out});
-        *pre = part_of(all, place(y_bytes), x.scalar_type(), {z.rows, z.out});
-    } else {
-        y = at::empty({z.rows, z.out}, x.options());
-        if (pre != nullptr) *pre = at::empty({z.rows, z.out}, x.options());
-    }
+    const Tensor y = fresh(x, x.scalar_type(), {z.rows, z.out});
+    if (pre != nullptr) *pre = fresh(x, x.scalar_type(), {z.rows, z.out});
     const int64_t ldx = row_distance(x);
     const int64_t bytes = mtp_linear_workspace_bytes(z.code, MTP_LINEAR_FORWARD, z.rows, (int)z.in, (int)z.out, (int)z.sets, at_(x),
                                                      ldx, at_(w), z.in);
@@ -211,31 +195,18 @@ struct LinearNode : Node {
                 const std::array<int64_t, 2> x_size{z.rows, z.in};
                 const std::array<int64_t, 3> w_size{z.sets, z.out, z.in};
                 const auto w_sizes = at::IntArrayRef(w_size).slice(many ? 0 : 1), b_sizes = w_sizes.slice(0, w_sizes.size() - 1);
-                const int64_t size = x.element_size(), x_bytes = want_x ? place(z.rows * z.in * size) : 0,
-                              w_bytes = want_w ? place(z.sets * z.out * z.in * size) : 0, b_bytes = want_b ? place(z.sets * z.out * size) : 0;
-                Tensor all;
-                char *ws = nullptr;
-                if (x_bytes + w_bytes + b_bytes + ws_bytes <= TOGETHER_BYTES) {
-                    all = at::empty({x_bytes + w_bytes + b_bytes + ws_bytes}, x.options().dtype(at::kByte));
-                    if (want_x) dx = part_of(all, 0, x.scalar_type(), x_size);
-                    if (want_w) dw = part_of(all, x_bytes, x.scalar_type(), w_sizes);
-                    if (want_b) db = part_of(all, x_bytes + w_bytes, x.scalar_type(), b_sizes);
-                    ws = static_cast<char *>(all.data_ptr()) + x_bytes + w_bytes + b_bytes;
-                } else {
-                    if (want_x) dx = at::empty(x_size, x.options());
-                    if (want_w) dw = at::empty(w_sizes, x.options());
-                    if (want_b) db = at::empty(b_sizes, x.options());
-                    all = workspace(ws_bytes, x);
-                    ws = static_cast<char *>(at_(all));
-                }
+                if (want_x) dx = fresh(x, type, x_size);
+                if (want_w) dw = fresh(x, type, w_sizes);
+                if (want_b) db = fresh(x, type, b_sizes);
+                const Tensor ws = workspace(ws_bytes, x);
                 if (want_w || z.rows > 0)  // else dx has no elements
                     check(mtp_linear_backward(z.code, at_(g), at_(pre), z.act, at_(xs), z.rows, (int)z.in, ldx, at_(wt), (int)z.out,
-                                              ldw, sets, (int)z.sets, at_(dx), at_(dw), at_(db), ws, (size_t)ws_bytes, stream_of(x)),
+                                              ldw, sets, (int)z.sets, at_(dx), at_(dw), at_(db), at_(ws), (size_t)ws_bytes, stream_of(x)),
                           "mtp_linear_backward");
             }
             if (has_residual && task_should_compute_output(3)) {
                 if (offsets.defined()) {  // rows behind the last set have none
-                    dr = at::empty_like(g);
+                    dr = fresh(g, type, g.sizes());
                     check(mtp_linear_mask_rows(z.code, at_(g), z.rows, (int)z.out, sets, (int)z.sets, at_(dr), stream_of(x)),
                           "mtp_linear_mask_rows");
                 } else {
@@ -265,7 +236,7 @@ Tensor linear_with_node(const Tensor &x, const Tensor &w, const Tensor &bias, co
             auto take = [&](const Tensor &t, int64_t n, int64_t distance) {
                 if (mtp_linear_rows_aligned(z.code, at_(t), distance)) return Tensor();
                 const int64_t from = at;
-                at += place(n * ld * x.element_size()) / x.element_size();
+                at += (n * ld * x.element_size() + 255) / 256 * 256 / x.element_size();
                 return all.as_strided({n, z.in}, {ld, 1}, from);
             };
             rows = take(x, z.rows, row_distance(x));
@@ -345,7 +316,7 @@ struct RouteNode : Node {
             at::NoGradGuard off;
             const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scores.device());
             const Tensor g = grads[0].resolve_neg().contiguous();
-            out = at::empty(scores.sizes(), scores.options());
+            out = fresh(scores, type, {n, modalities});
             check(mtp_route_topk_grad(type_code(scores), at_(scores), scores.size(0), (int)scores.size(1), row_distance(scores),
                                       (int)ids.size(1), normalize, static_cast<const int32_t *>(at_(ids)),
                                       static_cast<const float *>(at_(weights)), static_cast<const float *>(at_(stats)),
@@ -368,17 +339,9 @@ std::optional<std::tuple<Tensor, Tensor>> route_topk(const Tensor &scores, int64
     Tensor ids, weights, stats;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        const int64_t each = place(n * k * 4), all_bytes = 2 * each + (train ? n * 2 * 4 : 0);
-        if (n > 0 && all_bytes <= TOGETHER_BYTES) {
-            const Tensor all = at::empty({all_bytes}, scores.options().dtype(at::kByte));
-            ids = part_of(all, 0, at::kInt, {n, k});
-            weights = part_of(all, each, at::kFloat, {n, k});
-            if (train) stats = part_of(all, 2 * each, at::kFloat, {n, 2});
-        } else {
-            ids = at::empty({n, k}, scores.options().dtype(at::kInt));
-            weights = at::empty({n, k}, scores.options().dtype(at::kFloat));
-            if (train) stats = at::empty({n, 2}, scores.options().dtype(at::kFloat));
-        }
+        ids = fresh(scores, at::kInt, {n, k});
+        weights = fresh(scores, at::kFloat, {n, k});
+        if (train) stats = fresh(scores, at::kFloat, {n, 2});
         check(mtp_route_topk(type_code(scores), at_(scores), n, (int)e, ld, (int)k, normalize, static_cast<int32_t *>(at_(ids)),
                              static_cast<float *>(at_(weights)), static_cast<float *>(at_(stats)), stream_of(scores)),
               "mtp_route_topk");
@@ -405,19 +368,8 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> sort_pairs(const Tensor &ids, 
         return std::nullopt;
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ids.device());
     const int64_t pairs = ids.numel(), bytes = mtp_sort_pairs_workspace_bytes(pairs, (int)e);
-    Tensor offsets, order, position, ws;
-    if (pairs > 0 && bytes == 0 && pairs * 4 <= TOGETHER_BYTES) {
-        const int64_t first = place((e + 1) * 4), each = place(pairs * 4);
-        const Tensor all = at::empty({first + 2 * each}, ids.options().dtype(at::kByte));
-        offsets = part_of(all, 0, at::kInt, {e + 1});
-        order = part_of(all, first, at::kInt, {pairs});
-        position = part_of(all, first + each, at::kInt, ids.sizes());
-    } else {
-        offsets = at::empty({e + 1}, ids.options());
-        order = at::empty({pairs}, ids.options());
-        position = at::empty(ids.sizes(), ids.options());
-        ws = workspace(bytes, ids);
-    }
+    const Tensor offsets = fresh(ids, at::kInt, {e + 1}), order = fresh(ids, at::kInt, {pairs});
+    const Tensor position = fresh(ids, at::kInt, ids.sizes()), ws = workspace(bytes, ids);
     check(mtp_sort_pairs(static_cast<const int32_t *>(at_(ids)), pairs, (int)e, static_cast<int32_t *>(at_(offsets)),
                          static_cast<int32_t *>(at_(order)), static_cast<int32_t *>(at_(position)), at_(ws), (size_t)bytes,
                          stream_of(ids)),
@@ -431,7 +383,7 @@ const int32_t *places(const Tensor &position) { return static_cast<const int32_t
 
 Tensor run_dispatch(const Tensor &x, const Tensor &position, const Tensor &offsets) {
     const int64_t n = x.size(0), d = x.size(1), k = position.size(1);
-    Tensor rows = at::empty({n * k, d}, x.options());
+    Tensor rows = fresh(x, x.scalar_type(), {n * k, d});
     check(mtp_dispatch_rows(type_code(x), at_(x), n, (int)d, row_distance(x), (int)k, places(position), held(offsets), at_(rows),
                             stream_of(x)),
           "mtp_dispatch_rows");
@@ -439,7 +391,7 @@ Tensor run_dispatch(const Tensor &x, const Tensor &position, const Tensor &offse
 }
 Tensor run_combine(const Tensor &rows, const Tensor &position, const Tensor &offsets, const Tensor &weights) {
     const int64_t n = position.size(0), d = rows.size(1), k = position.size(1);
-    Tensor y = at::empty({n, d}, rows.options());
+    Tensor y = fresh(rows, rows.scalar_type(), {n, d});
     check(mtp_combine_rows(type_code(rows), at_(rows), n, (int)d, (int)k, places(position), held(offsets),
                            static_cast<const float *>(at_(weights)), at_(y), stream_of(rows)),
           "mtp_combine_rows");
@@ -504,15 +456,8 @@ struct CombineNode : Node {
                 dr = run_dispatch(g, position, offsets);
             } else {
                 const bool want_r = task_should_compute_output(0), want_w = task_should_compute_output(1);
-                const int64_t r_bytes = place(rows.numel() * rows.element_size()), w_bytes = weights.numel() * 4;
-                if (want_r && want_w && w_bytes > 0 && r_bytes + w_bytes <= TOGETHER_BYTES) {
-                    const Tensor all = at::empty({r_bytes + w_bytes}, rows.options().dtype(at::kByte));
-                    dr = part_of(all, 0, rows.scalar_type(), rows.sizes());
-                    dw = part_of(all, r_bytes, at::kFloat, weights.sizes());
-                } else {
-                    if (want_r) dr = at::empty_like(rows);
-                    if (want_w) dw = at::empty_like(weights);
-                }
+                if (want_r) dr = fresh(rows, rows.scalar_type(), rows.sizes());
+                if (want_w) dw = fresh(rows, at::kFloat, weights.sizes());
                 check(mtp_combine_rows_grad(type_code(rows), at_(rows), at_(g), g.size(0), (int)g.size(1), (int)position.size(1),
                                             places(position), held(offsets), static_cast<const float *>(at_(weights)), at_(dr),
                                             static_cast<float *>(at_(dw)), stream_of(g)),

@@ -136,3 +136,35 @@ def test_views_of_negatives_are_refused_and_such_gradients_taken(gpu_device):
         want = torch.autograd.grad(call(), leaves, -gy)
         for a, c in zip(torch.autograd.grad(y, leaves, n(gy)), want):
             assert torch.equal(a, c), name
+
+
+def _has_its_own_storage(tensors):
+    for t in tensors:
+        assert t.storage_offset() == 0 and t.untyped_storage().nbytes() == t.numel() * t.element_size()
+    assert len({t.untyped_storage().data_ptr() for t in tensors}) == len(tensors)
+
+
+def test_results_and_gradients_grow_and_go_by_themselves(gpu_device):
+    """resize_ (and out= with another shape) of one result leaves the others as they are."""
+    from pccs_accel.routing import combine, dispatch, route_topk, sort_pairs
+    g = torch.Generator().manual_seed(4)
+    scores = torch.randn(12, 40, generator=g).to(gpu_device).requires_grad_()
+    x = torch.randn(12, 8, generator=g).to(gpu_device).requires_grad_()
+    w = torch.randn(6, 8, generator=g).to(gpu_device).requires_grad_()
+    b = torch.randn(6, generator=g).to(gpu_device).requires_grad_()
+    ids, weights = route_topk(scores, 4)
+    plan = sort_pairs(ids, 40)
+    rows = dispatch(x, plan)
+    y = linear(x, w, b, "gelu")
+    rows2 = rows.detach().requires_grad_()
+    mean = combine(rows2, plan, weights)
+    results = [ids, weights, *plan, rows, y, mean]
+    grads = list(torch.autograd.grad([y, mean], [x, w, b, rows2, scores], [torch.ones_like(y), torch.ones_like(mean)]))
+    every = [t.detach() for t in results + grads]
+    _has_its_own_storage(every)
+    kept = [t.clone() for t in every]
+    for i, t in enumerate(every):
+        t.resize_(t.numel() + 4096).fill_(-7)
+        for other, value in list(zip(every, kept))[i + 1:]:
+            assert torch.equal(other, value)
+        t.untyped_storage().resize_(0)
