@@ -346,7 +346,10 @@ __global__ __launch_bounds__(256) void k_route_grad(const T *__restrict__ scores
     for (int r = tid >> 4; r < rows; r += 16) {
         const int64_t at = (row0 + r) * k;
         float dot = 0.f;
-        for (int j = sub; j < k; j += 16) dot += weights[at + j] * g[at + j];
+        for (int j = sub; j < k; j += 16) {
+            const float w = weights[at + j];
+            dot += ids[at + j] >= 0 || w != w ? w * g[at + j] : 0.f;  // where there is no choice g may be anything
+        }
         dot = group_sum<16>(dot);
         if (sub == 0) dots[r] = dot;
     }
