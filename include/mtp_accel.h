@@ -470,7 +470,8 @@ int64_t mtp_sort_pairs_workspace_bytes(int64_t pairs, int e);
 int mtp_sort_pairs(const int32_t *ids, int64_t pairs, int e, int32_t *offsets, int32_t *order, int32_t *position, void *ws,
                    size_t ws_bytes, void *stream);
 
-/* rows[position[t * k + j]] = x[t], zero for rows >= *held (a device int32: offsets + e).  rows [n * k][d]. */
+/* rows[position[t * k + j]] = x[t], zero for rows >= *held (a device int32: offsets + e).  rows [n * k][d].  Here and below a place
+ * outside [0, n * k) is left out: nothing is read or written there. */
 int mtp_dispatch_rows(int dtype, const void *x, int64_t n, int d, int64_t ld, int k, const int32_t *position, const int32_t *held,
                       void *rows, void *stream);
 /* y[t] = sum_j weights[t][j] rows[position[t * k + j]] over rows < *held, in the order of j; weights NULL: all one. */

@@ -581,6 +581,10 @@ __device__ __forceinline__ void store_row(T *p, const typename Pack<T, N>::type 
     else *to = v;
 }
 
+// Places come from the caller, and a plan may be another's: one that is none of the n * k rows (below 2^31) is left out, neither read
+// nor written.
+__device__ __forceinline__ bool is_place(int32_t p, uint32_t rows) { return (uint32_t)p < rows; }
+
 // rows[position[t][j]] = x[t], zero where the pair has no modality; one thread per N elements of a token, which it reads once and
 // writes k times.  I: an index that holds the number of threads (divisions of 64 bits cost more than the copy).  HBM-bound: 73 568
 // rows of 96 floats to 1.47 M places 112 us, 5.3 TB/s.
@@ -592,21 +596,22 @@ __global__ __launch_bounds__(256) void k_dispatch(const T *__restrict__ x, int64
     const int per = (d + N - 1) / N;
     const I total = (I)n * per;
     const int held = *held_at;
+    const uint32_t places = (uint32_t)n * (uint32_t)k;
     for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
         const int64_t t = i / per;
         const int c = piece_at((int)(i - (I)t * per), d, N);
         const vec v = *reinterpret_cast<const vec *>(x + t * ld + c);
         const vec zero = {};
         for (int j = 0; j < k; ++j) {
-            const int64_t p = position[t * k + j];
-            store_row<ONCE, T, N>(rows + p * d + c, p < held ? v : zero);
+            const int32_t p = position[t * k + j];
+            if (is_place(p, places)) store_row<ONCE, T, N>(rows + (int64_t)p * d + c, p < held ? v : zero);
         }
     }
 }
 
 // y[t] = sum_j weights[t][j] rows[position[t][j]] (weights NULL: all one), pairs without a modality left out.  One thread per N
-// elements of a token; four rows are in flight at a time (their places are all valid, what does not count is dropped after
-// the load).  HBM-bound: the same sizes back 100 us, 5.9 TB/s.
+// elements of a token; four rows are in flight at a time (what does not count is dropped after the load).  HBM-bound: the same sizes
+// back 100 us, 5.9 TB/s.
 template <typename T, int N, bool ONCE, typename I>
 __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int64_t n, int d, int k,
                                                  const int32_t *__restrict__ position, const int32_t *__restrict__ held_at,
@@ -615,6 +620,7 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
     const int per = (d + N - 1) / N;
     const I total = (I)n * per;
     const int held = *held_at;
+    const uint32_t places = (uint32_t)n * (uint32_t)k;
     for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
         const int64_t t = i / per;
         const int c = piece_at((int)(i - (I)t * per), d, N);
@@ -630,9 +636,10 @@ __global__ __launch_bounds__(256) void k_combine(const T *__restrict__ rows, int
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int j = j0 + q < k ? j0 + q : k - 1;
-                const int64_t p = at[j];
-                in[q] = p < held && j0 + q < k;
-                v[q] = load_row<ONCE, T, N>(rows + p * d + c);
+                const int32_t p = at[j];
+                const bool there = is_place(p, places);
+                in[q] = there && p < held && j0 + q < k;
+                v[q] = load_row<ONCE, T, N>(rows + (int64_t)(there ? p : 0) * d + c);
                 w[q] = weights != nullptr ? wt[j] : 1.f;
             }
 #pragma unroll
@@ -673,6 +680,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
     constexpr int Q = C == 1 ? 4 : 1;
     const int per = (d + N - 1) / N, sub = threadIdx.x % L;
     const int held = *held_at;
+    const uint32_t places = (uint32_t)n * (uint32_t)k, live = held < 0 ? 0 : min((uint32_t)held, places);
     for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L; t < n; t += (int64_t)gridDim.x * (256 / L)) {
         const int32_t *at = position + t * k;
         for (int c0 = 0; c0 < per; c0 += L * C) {
@@ -686,7 +694,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                 unpack<T, N>(*reinterpret_cast<const vec *>(g + t * d + from[c]), gv[c]);
             }
             for (int j0 = 0; j0 < k; j0 += Q) {
-                int64_t p[Q];
+                int32_t p[Q];
                 vec v[Q][C];
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
@@ -694,14 +702,14 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                     if (grad_weights != nullptr) {
 #pragma unroll
                         for (int c = 0; c < C; ++c)
-                            v[q][c] = load_row<ONCE, T, N>(rows + p[q] * d + from[c]);
+                            v[q][c] = load_row<ONCE, T, N>(rows + (int64_t)(is_place(p[q], places) ? p[q] : 0) * d + from[c]);
                     }
                 }
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
                     const int j = j0 + q;
                     if (j >= k) break;
-                    const bool in = p[q] < held;
+                    const bool in = is_place(p[q], live);
                     if (grad_rows != nullptr) {
                         const float w = in ? weights[t * k + j] : 0.f;
 #pragma unroll
@@ -709,8 +717,8 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T *__restrict__ rows
                             float o[N];
 #pragma unroll
                             for (int e = 0; e < N; ++e) o[e] = in ? w * gv[c][e] : 0.f;
-                            if (c0 + c * L + sub < per)
-                                store_row<ONCE, T, N>(grad_rows + p[q] * d + from[c], pack<T, N>(o));
+                            if (c0 + c * L + sub < per && is_place(p[q], places))
+                                store_row<ONCE, T, N>(grad_rows + (int64_t)p[q] * d + from[c], pack<T, N>(o));
                         }
                     }
                     if (grad_weights != nullptr) {

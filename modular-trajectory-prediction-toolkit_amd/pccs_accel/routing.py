@@ -37,7 +37,8 @@ class PairPlan(NamedTuple):
     """The (agent, modality) pairs sorted by modality; all tensors int32 on the device.
 
     offsets [E + 1]: modality e has the rows offsets[e] to offsets[e + 1]; pairs without a modality (id outside [0, E)) are
-    behind offsets[E].  order [N * k]: the pair (agent * k + choice) of each row.  position [N, k]: the row of each pair."""
+    behind offsets[E].  order [N * k]: the pair (agent * k + choice) of each row.  position [N, k]: the row of each pair; one
+    outside [0, N * k), which no sort gives, is left out."""
     offsets: torch.Tensor
     order: torch.Tensor
     position: torch.Tensor

@@ -29,3 +29,33 @@ def test_gradients_where_there_is_no_choice_may_hold_anything(gpu_device, normal
             ds, = torch.autograd.grad(w, leaf, gw.to(gpu_device))
             assert torch.equal(ids.cpu(), want["ids"])
             R.check("ds", ds, want["ds"])
+
+
+@pytest.mark.parametrize("d", [3, 8, 24, 40, 136, 600])
+def test_places_that_are_none_are_left_out(gpu_device, d):
+    """Places below 0 and behind the last row: the pair is not copied, not summed, and has no gradient."""
+    n, k = 50, 5
+    g = torch.Generator().manual_seed(d)
+    plan = sort_pairs(torch.randint(0, 7, (n, k), generator=g, dtype=torch.int32).to(gpu_device), 7)
+    wrong = torch.rand(n, k, generator=g) < 0.3
+    there = (~wrong).double()
+    here = plan.position.cpu().long()
+    values = torch.tensor([-1, n * k, n * k + 1, -2 ** 31, 2 ** 31 - 1, -n * k], dtype=torch.int32)
+    position = torch.where(wrong, values[torch.arange(n * k).view(n, k) % 6], plan.position.cpu())
+    bad = PairPlan(plan.offsets, plan.order, position.to(gpu_device))
+    for dtype in R.TYPES:
+        u = R.half_step(dtype)
+        x, rows, gy = (torch.randn(m, d, generator=g).to(dtype) for m in (n, n * k, n))
+        w = torch.rand(n, k, generator=g)
+        out = dispatch(x.to(gpu_device), bad).cpu()
+        assert torch.equal(out[here[~wrong]], x[:, None].expand(n, k, d)[~wrong])
+        leaves = rows.to(gpu_device).requires_grad_(), w.to(gpu_device).requires_grad_()
+        y = combine(leaves[0], bad, leaves[1])
+        terms = rows.double()[here] * (w.double() * there)[:, :, None]
+        v, e = terms.sum(1), (k + 2) * R.U32 * terms.abs().sum(1)
+        R.check("y", y, (v, e + u * (v.abs() + e) + R.floor_of(dtype)))
+        dr, dw = torch.autograd.grad(y, leaves, gy.to(gpu_device))
+        back = w.double()[:, :, None] * gy.double()[:, None]
+        R.check("drows", dr[here[~wrong].to(gpu_device)], (back[~wrong], (u + 2 * R.U32) * back[~wrong].abs() + R.floor_of(dtype)))
+        prod = rows.double()[here] * gy.double()[:, None] * there[:, :, None]
+        R.check("dw", dw, (prod.sum(2), (d + 2) * R.U32 * prod.abs().sum(2)))
