@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256) void k_route_grad(const T *__restrict__ scores
         float dot = 0.f;
         for (int j = sub; j < k; j += 16) {
             const float w = weights[at + j];
-            dot += ids[at + j] >= 0 || w != w ? w * g[at + j] : 0.f;  // where there is no choice g may be anything
+            dot += w != 0.f ? w * g[at + j] : 0.f;  // where there is no choice (weight 0) g may be anything
         }
         dot = group_sum<16>(dot);
         if (sub == 0) dots[r] = dot;
