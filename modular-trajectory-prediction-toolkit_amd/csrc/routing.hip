@@ -812,8 +812,15 @@ constexpr int PAIRS_ALONE = 8192;
 bool pairs_alone(int64_t pairs, int e) { return pairs <= PAIRS_ALONE && (int64_t)17 * (e + 1) * 4 + 64 <= 128 * 1024; }
 // Pairs of a workgroup: short runs end sooner, long ones have fewer counts to add (143 760 pairs over 200: 15.2 us with runs of 512,
 // 18.4 of 2048; 600 000: 21.3 of 1024, 25.9 of 512; 1 471 360: 30.3 of 2048, 37.6 of 1024).
-int pairs_run(int64_t pairs) { return pairs < 256 * 1024 ? 512 : pairs < 1024 * 1024 ? 1024 : 2048; }
-int64_t pairs_blocks(int64_t pairs) { return (pairs + pairs_run(pairs) - 1) / pairs_run(pairs); }
+// The runs' counts take no more room than the ids, or than COUNTS_BYTES: longer ones where there are many modalities.
+constexpr int64_t COUNTS_BYTES = 64ll << 20;
+int64_t pairs_blocks(int64_t pairs, int run) { return (pairs + run - 1) / run; }
+int pairs_run(int64_t pairs, int e) {
+    int run = pairs < 256 * 1024 ? 512 : pairs < 1024 * 1024 ? 1024 : 2048;
+    const int64_t most = pairs * 4 > COUNTS_BYTES ? pairs * 4 : COUNTS_BYTES;
+    while ((pairs_blocks(pairs, run) + 1) * (int64_t)(e + 1) * 4 > most) run *= 2;
+    return run;
+}
 
 constexpr int64_t CACHE_BYTES = 256ll << 20;
 
@@ -948,7 +955,7 @@ extern "C" int mtp_route_topk_grad(int dtype, const void *scores, int64_t n, int
 
 extern "C" int64_t mtp_sort_pairs_workspace_bytes(int64_t pairs, int e) {
     if (pairs < 0 || e < 1 || pairs_alone(pairs, e)) return 0;
-    return (pairs_blocks(pairs) + 1) * (int64_t)(e + 1) * 4;
+    return (pairs_blocks(pairs, pairs_run(pairs, e)) + 1) * (int64_t)(e + 1) * 4;
 }
 
 extern "C" int mtp_sort_pairs(const int32_t *ids, int64_t pairs, int e, int32_t *offsets, int32_t *order, int32_t *position, void *ws,
@@ -973,7 +980,7 @@ extern "C" int mtp_sort_pairs(const int32_t *ids, int64_t pairs, int e, int32_t 
                       (long long)mtp_sort_pairs_workspace_bytes(pairs, e));
         return MTP_E_WORKSPACE;
     }
-    const int blocks = (int)pairs_blocks(pairs), run = pairs_run(pairs);
+    const int run = pairs_run(pairs, e), blocks = (int)pairs_blocks(pairs, run);
     int32_t *counts = reinterpret_cast<int32_t *>(ws), *totals = counts + (int64_t)blocks * (e + 1);
     hipLaunchKernelGGL(k_pairs_count, dim3(blocks), dim3(256), (e + 1) * 4, s, ids, pairs, e, run, counts);
     MTP_LAUNCH_CHECK();

@@ -24,3 +24,13 @@ def test_tracing_is_refused(which):
     for mode in ("real", "fake"):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             make_fx(call, tracing_mode=mode)(given)
+
+
+def test_the_sorts_workspace_is_no_larger_than_its_pairs():
+    """Counts of 4096 modalities for each short run of 2^31 pairs would be 17 GB."""
+    from pccs_accel import _lib
+    bytes_for = _lib.lib().mtp_sort_pairs_workspace_bytes
+    for pairs in (8193, 100_000, 1_471_360, 9_400_000, 2 ** 28, 2 ** 31 - 1):
+        for e in (1, 200, 1024, 4096):
+            assert 0 < bytes_for(pairs, e) <= max(4 * pairs, 64 << 20), (pairs, e)
+    assert bytes_for(143_760, 200) == (281 + 1) * 201 * 4  # runs of 512, as ever

@@ -59,3 +59,17 @@ def test_places_that_are_none_are_left_out(gpu_device, d):
         R.check("drows", dr[here[~wrong].to(gpu_device)], (back[~wrong], (u + 2 * R.U32) * back[~wrong].abs() + R.floor_of(dtype)))
         prod = rows.double()[here] * gy.double()[:, None] * there[:, :, None]
         R.check("dw", dw, (prod.sum(2), (d + 2) * R.U32 * prod.abs().sum(2)))
+
+
+def test_sort_of_many_pairs_over_many_modalities(gpu_device):
+    """Runs longer than usual, so that their counts do not outgrow the pairs."""
+    n, k, e = 4_700_000, 2, 4096
+    g = torch.Generator(device=gpu_device).manual_seed(1)
+    ids = torch.randint(-1, e, (n, k), generator=g, dtype=torch.int32, device=gpu_device)
+    plan = sort_pairs(ids, e)
+    key = ids.reshape(-1).long()
+    key = torch.where(key < 0, e, key)
+    order = torch.sort(key, stable=True).indices
+    assert torch.equal(plan.order.long(), order)
+    assert torch.equal(plan.position.reshape(-1)[order].long(), torch.arange(n * k, device=gpu_device))
+    assert torch.equal(plan.offsets.long(), torch.searchsorted(key[order], torch.arange(e + 1, device=gpu_device)))
