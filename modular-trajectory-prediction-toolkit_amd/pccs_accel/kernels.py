@@ -5,6 +5,7 @@ hand-written HIP kernel reached through ctypes.  Shapes, dtypes, devices and con
 checked on the host before a kernel sees a pointer.
 """
 import ctypes
+import operator
 
 import torch
 
@@ -498,10 +499,10 @@ def _row_distance(t, name):
 
 def route_topk(scores, k, normalize=True, want_stats=False):
     """(ids int32 [N, k], weights float32 [N, k], stats float32 [N, 2] or None) -- ``mtp_route_topk``."""
+    k = operator.index(k)
     _device_tensor(scores, "scores", 2)
     code = _type_code(scores, "scores")
     n, e = scores.shape
-    k = int(k)
     if not 1 <= e <= MAX_MODALITIES:
         raise ValueError(f"scores: {e} modalities, expected 1 to {MAX_MODALITIES}")
     if not 1 <= k <= min(e, MAX_TOPK):
@@ -535,11 +536,11 @@ def route_topk_grad(scores, ids, weights, stats, grad, normalize=True):
 
 def sort_pairs(ids, n_modalities):
     """(offsets int32 [E + 1], order int32 [P], position int32 of ids' shape) -- ``mtp_sort_pairs``."""
+    e = operator.index(n_modalities)
     if not isinstance(ids, torch.Tensor):
         raise TypeError(f"ids: expected a torch.Tensor, got {type(ids).__name__}")
     _req(ids, "ids", torch.int32, align=4)
     _device_tensor(ids, "ids", ids.dim())
-    e = int(n_modalities)
     if not 1 <= e <= MAX_MODALITIES:
         raise ValueError(f"n_modalities={e} must be in [1, {MAX_MODALITIES}]")
     pairs, dev = ids.numel(), ids.device

@@ -34,3 +34,13 @@ def test_the_sorts_workspace_is_no_larger_than_its_pairs():
         for e in (1, 200, 1024, 4096):
             assert 0 < bytes_for(pairs, e) <= max(4 * pairs, 64 << 20), (pairs, e)
     assert bytes_for(143_760, 200) == (281 + 1) * 201 * 4  # runs of 512, as ever
+
+
+@pytest.mark.parametrize("count", [2.0, "2", None], ids=repr)
+def test_counts_that_are_no_whole_numbers_are_refused_before_anything_runs(count):
+    """The front end that explains a refusal used to round such a count and to run the kernel first."""
+    from pccs_accel import kernels as K
+    x, ids = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    for call in (lambda: route_topk(x, count), lambda: K.route_topk(x, count), lambda: sort_pairs(ids, count), lambda: K.sort_pairs(ids, count)):
+        with pytest.raises(TypeError):
+            call()
