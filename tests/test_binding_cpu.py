@@ -1,4 +1,7 @@
 """Calls of the routing and layer operators that are refused before they look at a device: these run without one."""
+import os
+import subprocess
+
 import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
@@ -44,3 +47,15 @@ def test_counts_that_are_no_whole_numbers_are_refused_before_anything_runs(count
     for call in (lambda: route_topk(x, count), lambda: K.route_topk(x, count), lambda: sort_pairs(ids, count), lambda: K.sort_pairs(ids, count)):
         with pytest.raises(TypeError):
             call()
+
+
+def test_the_library_builds_without_torch(tmp_path):
+    """A python without torch: the default target ends well, with the library and its check and without the calls from torch."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "modular-trajectory-prediction-toolkit_amd", "csrc")
+    binding = tmp_path / "_binding.so"
+    built = ["-o", "../pccs_accel/libmtp_accel.so", "-o", ".assign_asm_checked"]  # taken as they are
+    got = subprocess.run(["make", "-C", csrc, *built, "PYTHON=/bin/false", f"BINDING={binding}"], capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout + got.stderr
+    assert "has no torch" in got.stdout and not binding.exists()
+    steps = subprocess.run(["make", "-C", csrc, "-n", "-B", "lib", "PYTHON=/bin/false"], capture_output=True, text=True)
+    assert steps.returncode == 0 and "check_assign_asm.py" in steps.stdout and "binding.cpp" not in steps.stdout
