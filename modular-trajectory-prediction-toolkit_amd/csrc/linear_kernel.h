@@ -605,12 +605,12 @@ constexpr int lin_waves(int bc, int br, int threads) {
 }
 
 // A wave owns WC x WR of the BC x BR tile as 32 x 32 fragments: 32x32x16 matrix instructions for the 16-bit types, 32x32x2 for float.
-// What bounds it depends on the sizes.  Long sums, bfloat16, 32 768 rows of 2048 -> 2048 in 256 x 256 tiles: forward 247 us
-// (1.11 PFLOP/s; a library product 1.13 to 1.46), 328 with gelu, the kept z and a residual, as nothing covers a single workgroup's
-// way out; input gradient 234; weight gradient 256 with its join, as the transposing reads run at half the rate of the others.  The
+// What bounds it depends on the sizes.  Long sums, bfloat16, 32 768 rows of 2048 -> 2048 in 256 x 256 tiles: forward 248 us
+// (1.11 PFLOP/s; a library product 1.13 to 1.46), 330 with gelu, the kept z and a residual, as nothing covers a single workgroup's
+// way out; input gradient 235; weight gradient 245 with its join, as the transposing reads run at half the rate of the others.  The
 // matrix cores are busy for half of the time; leaving the LDS loads out would take a fifth off, fragments read one step ahead
 // nothing.  Short sums: the way out (143 760 rows over 400 sets, 96 -> 256 bfloat16: 46 us, 68 with gelu and the kept z, which are
-// some 25 vector instructions an element and 74 MB).  float: the matrix cores (73 568 rows, 512 -> 96: 75 us, 96 TFLOP/s; 153 in a
+// some 25 vector instructions an element and 74 MB).  float: the matrix cores (73 568 rows, 512 -> 96: 71 us, 102 TFLOP/s; 153 in a
 // large library product).
 template <typename T, int MODE, int BC, int BR, int WC, int WR>
 __device__ __forceinline__ void lin_tile(const LinArgs &a, uint32_t block, uint32_t blocks, char *smem) {

@@ -6,9 +6,9 @@
     z = x weight^T + bias,   y = activation(z) + residual
 
 Types float32, bfloat16, float16, all tensors of a call alike; sums are float32, y is rounded once.  For the backward pass of an
-activation z is kept in the same type (rounded once).  Second derivatives are not offered.  All calls enqueue on the current
-stream, wait for nothing and can be captured into a graph (a backward pass together with its forward pass, see ``routing``);
-sums have a fixed order.
+activation z is kept in the same type (rounded once), and z's gradient is rounded to it for the products with weight and x; the bias'
+gradient is summed before that.  Second derivatives are not offered.  All calls enqueue on the current stream, wait for nothing and
+can be captured into a graph (a backward pass together with its forward pass, see ``routing``); sums have a fixed order.
 """
 import torch
 

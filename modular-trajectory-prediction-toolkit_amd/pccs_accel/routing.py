@@ -10,7 +10,8 @@ Types float32, bfloat16, float16; softmax statistics, weights and sums are float
 and the weights; second derivatives are not offered.  All calls enqueue on the current stream, wait for nothing and can be
 captured into a graph; sums have a fixed order.  A backward pass is captured with its forward pass: a call under capture whose
 inputs belong to a graph of autograd that was begun outside (a leaf that an eager result still refers to) is refused, since its
-backward pass would end the process.
+backward pass would end the process.  Refused as well: tracing, which does not see the kernels, forward mode, and views with the negative
+bit.
 """
 from typing import NamedTuple
 
